@@ -529,6 +529,53 @@ int pgb_decode_flow_step_fwd(const void *layer_table, int L, const void *E, cons
  * ------------------------------------------------------------------------------------------------------- */
 int pgb_linear_act(const void *x, const void *W, const void *bias, void *y, long long M, int N, int K, int act, void *stream);
 
+/* ---------------------------------------------------------------------------------------------------------
+ * Losses over the vocabulary straight from the hidden states and the (tied) head's weight, s_nv = h_n . w_v, without the
+ * N x V logits in memory: softmax cross entropy against a word per row, and distillation from a teacher's top logits at a
+ * temperature. The reference's loss is torch's cross entropy on the logits (src/train.py:49, src/model.py:837).
+ *   h [N][d], W [V][d]: dtype (fp32 or bf16), contiguous, 16-byte aligned, d a multiple of 8. Sums in fp32, losses fp32.
+ *   reduction 0: a loss per row (row_loss [N]); 1: their sum; 2: their mean over the rows that count (loss, count: one fp32 each;
+ *   row_loss may be NULL; 0 / 0 where no row counts). L [N][2] fp32: log2 of a row's sum of exponentials in two parts, which the
+ *   backward pass reads.
+ *   grad: the gradient of row_loss [N] (reduction 0) or of loss (one fp32). dh [N][d], dW [V][d]: dtype; either may be NULL.
+ *   scratch: 256-byte aligned, at least what the _scratch_bytes call of the same sizes says (0: bad sizes; k 0: cross entropy).
+ * Cross entropy: rows whose target is ignore_index lose 0 and have no gradient (h must be finite there all the same if dW is
+ * wanted); any other target outside 0 .. V-1 gives NaN, as loss and as gradients of its row and of W.
+ * Distillation: pgb_teacher_lists makes of a teacher's k entries per row (ids in any order; an entry with id < 0 or logit -inf is
+ * absent) their probabilities p at the temperature, sorted by id, and ent, the sum of p log p. A row's loss is
+ * temperature^2 KL(p || softmax(s / temperature)), 0 without gradient for rows without an entry; the same id twice counts twice; an id >= V gives NaN.
+ * N, V up to 2^30, d up to 65536, k 1 .. 1024. Bounded waits as in the prefill kernels (pgb_tc_error_flag: 91-95). The same call gives
+ * the same bits.
+ * ------------------------------------------------------------------------------------------------------- */
+long long pgb_head_loss_fwd_scratch_bytes(long long N, int V, int d, int dtype, int k);
+long long pgb_head_loss_bwd_scratch_bytes(long long N, int V, int d, int dtype, int want_dh, int want_dW);
+int pgb_linear_xent_fwd(const void *h, const void *W, int dtype, const long long *target, long long ignore_index, float *row_loss,
+                        float *loss, float *count, float *L, void *scratch, long long scratch_bytes, int reduction, long long N,
+                        int V, int d, void *stream);
+int pgb_linear_xent_bwd(const void *h, const void *W, int dtype, const long long *target, long long ignore_index, const float *L,
+                        const float *count, const float *grad, void *dh, void *dW, void *scratch, long long scratch_bytes,
+                        int reduction, long long N, int V, int d, void *stream);
+int pgb_teacher_lists(const long long *teacher_ids, const float *teacher_logits, float temperature, int *ids, float *p, float *ent,
+                      long long N, int V, int k, void *stream);
+int pgb_linear_distill_fwd(const void *h, const void *W, int dtype, const int *ids, const float *p, const float *ent, int k,
+                           float temperature, float *row_loss, float *loss, float *count, float *L, void *scratch,
+                           long long scratch_bytes, int reduction, long long N, int V, int d, void *stream);
+int pgb_linear_distill_bwd(const void *h, const void *W, int dtype, const int *ids, const float *p, const float *ent, int k,
+                           float temperature, const float *L, const float *count, const float *grad, void *dh, void *dW,
+                           void *scratch, long long scratch_bytes, int reduction, long long N, int V, int d, void *stream);
+
+/* ---------------------------------------------------------------------------------------------------------
+ * Embedding lookup with scaling and its gradient by sorted tokens (the nn.Embedding of src/model.py:859).
+ *   y[n] = scale W[ids[n]];  dW[v] = scale * sum over ids[n] == v of grad[n], n ascending, added in fp32 and rounded once.
+ *   ids [N] int64; W, dW [V][d], y, grad [N][d]: dtype, contiguous, aligned to their element (to 16 bytes, with d a multiple of
+ *   16 bytes, rows move 16 bytes at a time). An id outside 0 .. V-1 gives a row of NaN and adds nothing to dW; nor does padding_idx (-1: none).
+ *   scratch: 16-byte aligned, pgb_embedding_bwd_scratch_bytes. N, V up to 2^30. The same call gives the same bits.
+ * ------------------------------------------------------------------------------------------------------- */
+int pgb_embedding_fwd(const long long *ids, const void *W, int dtype, float scale, void *y, long long N, int V, int d, void *stream);
+long long pgb_embedding_bwd_scratch_bytes(long long N, int V, int d);
+int pgb_embedding_bwd(const long long *ids, const void *grad, int dtype, float scale, long long padding_idx, void *dW, void *scratch,
+                      long long scratch_bytes, long long N, int V, int d, void *stream);
+
 /* Which kernel pgb_linear_act uses. Bit 0: 0 (default) = one CTA per 128-row tile; 1 = pairs of SMs share one 256-row tile
  * (tcgen05.mma.cta_group::2: each CTA of a two-CTA cluster loads half of either operand, no multicast) whenever the
  * problem has more than 128 rows. Bits 1-2: the tile's width, 0 or 1 = 256 columns (default), 2 = 192. variant in 0..5.

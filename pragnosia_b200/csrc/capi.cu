@@ -84,6 +84,15 @@ int decode_linear_launch(const void *, const void *, const void *, const float *
 int decode_linear_error_flag(int *);
 int decode_sample_launch(const void *, int, float, float, unsigned long long, long long *, long long *, int, long long *, long long *, float *,
                          unsigned int *, int, int, int, cudaStream_t);
+long long head_loss_fwd_bytes(long long, int, int, int, int);
+long long head_loss_bwd_bytes(long long, int, int, int, int, int);
+int head_teacher_launch(const long long *, const float *, int *, float *, float *, long long, int, int, float, cudaStream_t);
+int head_loss_fwd_launch(const HeadLossArgs &, float *, float *, float *, float *, void *, cudaStream_t);
+int head_loss_bwd_launch(const HeadLossArgs &, const float *, const float *, const float *, void *, void *, void *, cudaStream_t);
+int head_loss_error_flag(int *);
+int embedding_fwd_launch(const long long *, const void *, int, float, void *, long long, int, int, cudaStream_t);
+long long embedding_bwd_bytes(long long, int, int);
+int embedding_bwd_launch(const long long *, const void *, int, float, long long, void *, void *, long long, int, int, cudaStream_t);
 int linear_gelu_launch(const void *, const void *, const void *, void *, long long, int, int, int, cudaStream_t);
 int linear_gelu_error_flag(int *);
 int linear_gelu_set_variant(int);
@@ -788,6 +797,113 @@ int pgb_linear_act(const void *x, const void *W, const void *bias, void *y, long
     return linear_gelu_launch(x, W, bias, y, M, N, K, act, (cudaStream_t)stream);
 }
 
+// ---- losses over the vocabulary, straight from the hidden states; the embedding
+namespace {
+constexpr int HEAD_MOST_K = 1024;
+constexpr long long HEAD_MOST_ROWS = 1LL << 30;
+int head_sizes(long long N, int V, int d, int dtype) {
+    if (dtype != PGB_F32 && dtype != PGB_BF16) return PGB_ERR_BAD_DTYPE;
+    if (N < 1 || V < 1 || d < 8 || (d % 8) != 0) return PGB_ERR_BAD_SHAPE;
+    if (N > HEAD_MOST_ROWS || V > HEAD_MOST_ROWS || d > 65536) return PGB_ERR_TOO_LARGE;
+    return PGB_OK;
+}
+int head_args(HeadLossArgs &x, const void *h, const void *W, int dtype, const long long *target, long long ignore, const int *ids, const float *p,
+              const float *ent, int k, float tau, int reduction, long long N, int V, int d) {
+    x = {h, W, dtype, target, ignore, ids, p, ent, k, tau, reduction, N, V, d};
+    if (!h || !W) return PGB_ERR_NULL_POINTER;
+    if (target == nullptr && (!ids || !p || !ent)) return PGB_ERR_NULL_POINTER;
+    int rc = head_sizes(N, V, d, dtype);
+    if (rc != PGB_OK) return rc;
+    if (reduction < 0 || reduction > 2 || !(tau > 0.f) || tau > 3e38f || (ids && k < 1)) return PGB_ERR_BAD_SHAPE;
+    if (ids && k > HEAD_MOST_K) return PGB_ERR_TOO_LARGE;
+    if (!aligned(h, 16) || !aligned(W, 16) || (target && !aligned(target, 8)) || (ids && (!aligned(ids, 4) || !aligned(p, 4) || !aligned(ent, 4))))
+        return PGB_ERR_MISALIGNED;
+    return PGB_OK;
+}
+int head_fwd(const HeadLossArgs &x, float *row_loss, float *loss, float *count, float *L, void *scratch, long long scratch_bytes, void *stream) {
+    if (!L || !scratch || (x.reduction == 0 ? !row_loss : !loss || !count)) return PGB_ERR_NULL_POINTER;
+    if (!aligned(L, 8) || !aligned(scratch, 256)) return PGB_ERR_MISALIGNED;
+    if (scratch_bytes < head_loss_fwd_bytes(x.N, x.V, x.d, x.dtype, x.ids ? x.k : 0)) return PGB_ERR_BAD_SHAPE;
+    return head_loss_fwd_launch(x, row_loss, loss, count, L, scratch, (cudaStream_t)stream);
+}
+int head_bwd(const HeadLossArgs &x, const float *L, const float *count, const float *grad, void *dh, void *dW, void *scratch, long long scratch_bytes,
+             void *stream) {
+    if (!L || !grad || !scratch || (x.reduction == 2 && !count) || (!dh && !dW)) return PGB_ERR_NULL_POINTER;
+    if (!aligned(L, 8) || !aligned(scratch, 256) || (dh && !aligned(dh, 16)) || (dW && !aligned(dW, 16))) return PGB_ERR_MISALIGNED;
+    if (scratch_bytes < head_loss_bwd_bytes(x.N, x.V, x.d, x.dtype, dh != nullptr, dW != nullptr)) return PGB_ERR_BAD_SHAPE;
+    return head_loss_bwd_launch(x, L, count, grad, dh, dW, scratch, (cudaStream_t)stream);
+}
+}  // namespace
+
+long long pgb_head_loss_fwd_scratch_bytes(long long N, int V, int d, int dtype, int k) {
+    return head_sizes(N, V, d, dtype) != PGB_OK || k < 0 || k > HEAD_MOST_K ? 0 : head_loss_fwd_bytes(N, V, d, dtype, k);
+}
+long long pgb_head_loss_bwd_scratch_bytes(long long N, int V, int d, int dtype, int want_dh, int want_dW) {
+    return head_sizes(N, V, d, dtype) != PGB_OK ? 0 : head_loss_bwd_bytes(N, V, d, dtype, want_dh, want_dW);
+}
+int pgb_linear_xent_fwd(const void *h, const void *W, int dtype, const long long *target, long long ignore_index, float *row_loss, float *loss, float *count,
+                        float *L, void *scratch, long long scratch_bytes, int reduction, long long N, int V, int d, void *stream) {
+    if (!target) return PGB_ERR_NULL_POINTER;
+    HeadLossArgs x;
+    const int rc = head_args(x, h, W, dtype, target, ignore_index, nullptr, nullptr, nullptr, 0, 1.f, reduction, N, V, d);
+    return rc != PGB_OK ? rc : head_fwd(x, row_loss, loss, count, L, scratch, scratch_bytes, stream);
+}
+int pgb_linear_xent_bwd(const void *h, const void *W, int dtype, const long long *target, long long ignore_index, const float *L, const float *count,
+                        const float *grad, void *dh, void *dW, void *scratch, long long scratch_bytes, int reduction, long long N, int V, int d, void *stream) {
+    if (!target) return PGB_ERR_NULL_POINTER;
+    HeadLossArgs x;
+    const int rc = head_args(x, h, W, dtype, target, ignore_index, nullptr, nullptr, nullptr, 0, 1.f, reduction, N, V, d);
+    return rc != PGB_OK ? rc : head_bwd(x, L, count, grad, dh, dW, scratch, scratch_bytes, stream);
+}
+int pgb_teacher_lists(const long long *teacher_ids, const float *teacher_logits, float temperature, int *ids, float *p, float *ent, long long N, int V, int k,
+                      void *stream) {
+    if (!teacher_ids || !teacher_logits || !ids || !p || !ent) return PGB_ERR_NULL_POINTER;
+    if (N < 1 || V < 1 || k < 1 || !(temperature > 0.f) || temperature > 3e38f) return PGB_ERR_BAD_SHAPE;
+    if (N > HEAD_MOST_ROWS || V > HEAD_MOST_ROWS || k > HEAD_MOST_K) return PGB_ERR_TOO_LARGE;
+    if (!aligned(teacher_ids, 8) || !aligned(teacher_logits, 4) || !aligned(ids, 4) || !aligned(p, 4) || !aligned(ent, 4)) return PGB_ERR_MISALIGNED;
+    return head_teacher_launch(teacher_ids, teacher_logits, ids, p, ent, N, V, k, temperature, (cudaStream_t)stream);
+}
+int pgb_linear_distill_fwd(const void *h, const void *W, int dtype, const int *ids, const float *p, const float *ent, int k, float temperature, float *row_loss,
+                           float *loss, float *count, float *L, void *scratch, long long scratch_bytes, int reduction, long long N, int V, int d, void *stream) {
+    HeadLossArgs x;
+    const int rc = head_args(x, h, W, dtype, nullptr, 0, ids, p, ent, k, temperature, reduction, N, V, d);
+    return rc != PGB_OK ? rc : head_fwd(x, row_loss, loss, count, L, scratch, scratch_bytes, stream);
+}
+int pgb_linear_distill_bwd(const void *h, const void *W, int dtype, const int *ids, const float *p, const float *ent, int k, float temperature, const float *L,
+                           const float *count, const float *grad, void *dh, void *dW, void *scratch, long long scratch_bytes, int reduction, long long N, int V,
+                           int d, void *stream) {
+    HeadLossArgs x;
+    const int rc = head_args(x, h, W, dtype, nullptr, 0, ids, p, ent, k, temperature, reduction, N, V, d);
+    return rc != PGB_OK ? rc : head_bwd(x, L, count, grad, dh, dW, scratch, scratch_bytes, stream);
+}
+
+static int embedding_sizes(long long N, int V, int d, int dtype) {
+    if (dtype != PGB_F32 && dtype != PGB_BF16) return PGB_ERR_BAD_DTYPE;
+    if (N < 1 || V < 1 || d < 1) return PGB_ERR_BAD_SHAPE;
+    return N > HEAD_MOST_ROWS || V > HEAD_MOST_ROWS || d > 65536 ? PGB_ERR_TOO_LARGE : PGB_OK;
+}
+int pgb_embedding_fwd(const long long *ids, const void *W, int dtype, float scale, void *y, long long N, int V, int d, void *stream) {
+    if (!ids || !W || !y) return PGB_ERR_NULL_POINTER;
+    const int rc = embedding_sizes(N, V, d, dtype);
+    if (rc != PGB_OK) return rc;
+    const size_t e = dtype == PGB_F32 ? 4 : 2;
+    if (!aligned(ids, 8) || !aligned(W, e) || !aligned(y, e)) return PGB_ERR_MISALIGNED;
+    return embedding_fwd_launch(ids, W, dtype, scale, y, N, V, d, (cudaStream_t)stream);
+}
+long long pgb_embedding_bwd_scratch_bytes(long long N, int V, int d) {
+    return embedding_sizes(N, V, d, PGB_F32) != PGB_OK ? 0 : embedding_bwd_bytes(N, V, d);
+}
+int pgb_embedding_bwd(const long long *ids, const void *grad, int dtype, float scale, long long padding_idx, void *dW, void *scratch, long long scratch_bytes,
+                      long long N, int V, int d, void *stream) {
+    if (!ids || !grad || !dW || !scratch) return PGB_ERR_NULL_POINTER;
+    const int rc = embedding_sizes(N, V, d, dtype);
+    if (rc != PGB_OK) return rc;
+    const size_t e = dtype == PGB_F32 ? 4 : 2;
+    if (!aligned(ids, 8) || !aligned(grad, e) || !aligned(dW, e) || !aligned(scratch, 16)) return PGB_ERR_MISALIGNED;
+    if (scratch_bytes < embedding_bwd_bytes(N, V, d)) return PGB_ERR_BAD_SHAPE;
+    return embedding_bwd_launch(ids, grad, dtype, scale, padding_idx, dW, scratch, N, V, d, (cudaStream_t)stream);
+}
+
 int pgb_linear_act_set_variant(int variant) { return linear_gelu_set_variant(variant); }
 
 int pgb_decode_set_variant(int variant) { return decode_set_variant(variant); }
@@ -883,6 +999,8 @@ int pgb_tc_error_flag(int *out_host) {
     if (rc == PGB_OK) rc = decode_linear_error_flag(&g);
     f = f > g ? f : g;
     if (rc == PGB_OK) rc = delta_segments_error_flag(&g);
+    f = f > g ? f : g;
+    if (rc == PGB_OK) rc = head_loss_error_flag(&g);
     f = f > g ? f : g;
     e = e > f ? e : f;
     b = b > c ? b : c;

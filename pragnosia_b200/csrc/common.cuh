@@ -122,6 +122,11 @@ struct TrainBwdArgs {
     void *dq, *dk, *dv; float *dla, *dbeta, *dS0; void *scratch;
     int B, H, T;
 };
+// a loss over the vocabulary (head_loss.cu): target, or ids (with p, ent, k); reduction 0 none, 1 sum, 2 mean
+struct HeadLossArgs {
+    const void *h, *W; int dtype; const long long *target; long long ignore; const int *ids; const float *p, *ent; int k;
+    float tau; int reduction; long long N; int V, d;
+};
 struct DecodeArgs {
     const void *qp, *kp, *vp; long long in_sb; int normalize;
     const void *gate; long long gate_sb; int gate_is_logit;

@@ -14,7 +14,7 @@
 //   per element decides the kernel's speed: see lg_gelu.
 //   One CTA per SM walks tiles blockIdx.x, blockIdx.x + gridDim.x, ... (column blocks fastest, so the CTAs running together
 //   share rows of x in L2). Every mbarrier wait is bounded; a wait that runs out sets the error flag and the CTA winds down.
-#include "tc_common.cuh"
+#include "tc_pair.cuh"
 
 namespace pgb {
 
@@ -59,12 +59,6 @@ __device__ __forceinline__ float lg_gelu(float x) {
     const float e = fast_exp2(x * p);                                 // exp(-2 x p(x^2))
     return __fdividef(x, 1.0f + e);
 }
-__device__ __forceinline__ bool elect_one() {
-    uint32_t e;
-    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(e));
-    return e != 0;
-}
-
 // columns of its block an epilogue warp stages at a time: half of a 64-column block, the whole of a 48-column one
 template <int CW> struct LgStage { static constexpr int cols = CW == 64 ? 32 : CW; };
 
@@ -249,50 +243,6 @@ struct LpCfg {
     static_assert(BN == 256 || BN == 192, "tile width");
     static_assert(STAGE % 1024 == 0 && SMEM <= 232448, "shared memory of the pair kernel");
 };
-
-__device__ __forceinline__ uint32_t cluster_rank() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-// the address, in the cluster's shared window, of this CTA's shared-memory address `addr` in the CTA of rank `rank`
-__device__ __forceinline__ uint32_t cluster_addr(uint32_t addr, uint32_t rank) {
-    uint32_t r;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-    return r;
-}
-__device__ __forceinline__ void cluster_sync_all() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void lp_arrive_cluster(uint32_t cluster_bar) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
-}
-// bounded wait on a barrier of this CTA whose arrivals come from both CTAs of the pair
-__device__ __forceinline__ bool lp_wait_cluster(uint32_t bar, uint32_t parity, int code) {
-    for (uint32_t n = WAIT_TRIES; n != 0; --n) {
-        uint32_t ok;
-        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\tselp.b32 %0, 1, 0, p;\n\t}"
-                     : "=r"(ok) : "r"(bar), "r"(parity), "r"(WAIT_HINT) : "memory");
-        if (ok) return true;
-    }
-    atomicExch(&g_tc_error, code);
-    return false;
-}
-// this CTA's half of a stage; the bytes are counted on `cluster_bar`, a barrier of the pair's first CTA
-__device__ __forceinline__ void lp_tma_load(uint32_t dst, const CUtensorMap *map, uint32_t cluster_bar, int c0, int c1) {
-    asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
-                 ::"r"(dst), "l"(map), "r"(cluster_bar), "r"(c0), "r"(c1), "r"(0) : "memory");
-}
-__device__ __forceinline__ void lp_mma_elect(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n\t.reg .pred p, e;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "@e tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5, %5, %5, %5, %5}, p;\n\t}"
-                 ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(0u) : "memory");
-}
-// one arrival on `cluster_bar` (any CTA of the pair) once every MMA this thread has issued so far is complete
-__device__ __forceinline__ void lp_commit_elect(uint32_t cluster_bar) {
-    asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
-                 "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(cluster_bar) : "memory");
-}
 
 template <int BN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LG_NT, 1)

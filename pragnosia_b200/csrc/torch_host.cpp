@@ -394,6 +394,216 @@ Three scan_diff(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor 
     variable_list r = Scan::apply(q, k, v, la, beta, S0);
     return std::make_tuple(r[0], r[1], r[2]);
 }
+
+// ------------------------------------------------------------------------------------------------ losses over the vocabulary
+enum { REDUCE_NONE = 0, REDUCE_SUM = 1, REDUCE_MEAN = 2 };
+void same_device(const char *what, const Tensor &a, const Tensor &b) {
+    TORCH_CHECK_VALUE(a.device() == b.device(), what, ": its tensors are on ", a.device(), " and ", b.device());
+}
+Tensor whole_numbers(const char *what, const Tensor &t) {
+    TORCH_CHECK_TYPE(t.scalar_type() == at::kLong || t.scalar_type() == at::kInt, what, ": ids are int64 or int32, got ", t.scalar_type());
+    return like(t, at::kLong);
+}
+// h as [N][d], W as it is: both contiguous, of one of the two types, 16-byte aligned (a view into a larger tensor need not be)
+struct HeadIn { Tensor h, w; int64_t N, V, d; };
+Tensor head_operand(const Tensor &t) {
+    const Tensor c = t.contiguous();
+    return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 == 0 ? c : c.clone();
+}
+HeadIn head_in(const char *what, const Tensor &h, const Tensor &w) {
+    need_cuda(h, w);
+    same_device(what, h, w);
+    TORCH_CHECK_VALUE(w.dim() == 2 && h.dim() >= 1 && h.size(-1) == w.size(1), what, ": h is (..., d) and the weight (V, d), got ", h.sizes(), " and ", w.sizes());
+    TORCH_CHECK_TYPE(h.scalar_type() == w.scalar_type() && io_type(h.scalar_type()), what, ": h and the weight are both float32 or both bfloat16, got ",
+                     h.scalar_type(), " and ", w.scalar_type());
+    const int64_t d = w.size(1);
+    TORCH_CHECK_VALUE(w.size(0) >= 1 && d >= 8 && d % 8 == 0, what, ": the weight is (V, d) with V at least 1 and d a multiple of 8, got ", w.sizes());
+    return {head_operand(h.reshape({-1, d})), head_operand(w), h.numel() / d, w.size(0), d};
+}
+// What a row is held to: a word each (target), or a teacher's lists (ids, p, ent).
+struct HeadWant { Tensor target; int64_t ignore; Tensor ids, p, ent; double tau; };
+struct HeadOut { Tensor loss, L, count; };                            // loss: [N] or 0-d
+HeadOut head_fwd(const char *what, const HeadIn &x, const HeadWant &t, int reduction) {
+    OnDevice dev(x.h);
+    HeadOut r{alloc(x.h, reduction == REDUCE_NONE ? at::IntArrayRef({x.N}) : at::IntArrayRef(), at::kFloat), alloc(x.h, {x.N, 2}, at::kFloat),
+              alloc(x.h, {}, at::kFloat)};
+    if (x.N == 0) {                                                    // nothing to add up: 0, and 0 / 0 as the mean
+        if (reduction == REDUCE_SUM) r.loss.zero_();
+        if (reduction == REDUCE_MEAN) r.loss.fill_(std::numeric_limits<float>::quiet_NaN());
+        r.count.zero_();
+        return r;
+    }
+    const bool list = t.ids.defined();
+    const int k = list ? t.ids.size(1) : 0;
+    const long long n = pgb_head_loss_fwd_scratch_bytes(x.N, x.V, x.d, code(x.h), k);
+    const Tensor scratch = bytes(x.h, n);
+    float *row = reduction == REDUCE_NONE ? fp(r.loss) : nullptr, *loss = reduction == REDUCE_NONE ? nullptr : fp(r.loss);
+    if (list)
+        check(pgb_linear_distill_fwd(vp(x.h), vp(x.w), code(x.h), static_cast<int *>(vp(t.ids)), fp(t.p), fp(t.ent), k, t.tau, row, loss, fp(r.count), fp(r.L),
+                                     vp(scratch), n, reduction, x.N, x.V, x.d, dev.stream), what);
+    else
+        check(pgb_linear_xent_fwd(vp(x.h), vp(x.w), code(x.h), static_cast<long long *>(vp(t.target)), t.ignore, row, loss, fp(r.count), fp(r.L), vp(scratch),
+                                  n, reduction, x.N, x.V, x.d, dev.stream), what);
+    return r;
+}
+std::tuple<Tensor, Tensor> head_bwd(const char *what, const HeadIn &x, const HeadWant &t, const Tensor &L, const Tensor &count, const Tensor &grad_, int reduction,
+                                    bool want_dh, bool want_dw) {
+    OnDevice dev(x.h);
+    Tensor dh, dw;
+    if (want_dh) dh = alloc(x.h, {x.N, x.d}, x.h.scalar_type());
+    if (want_dw) dw = alloc(x.h, {x.V, x.d}, x.h.scalar_type());
+    if (x.N == 0) {
+        if (want_dw) dw.zero_();
+        return {dh, dw};
+    }
+    const Tensor grad = f32c(grad_);
+    const long long n = pgb_head_loss_bwd_scratch_bytes(x.N, x.V, x.d, code(x.h), want_dh, want_dw);
+    const Tensor scratch = bytes(x.h, n);
+    if (t.ids.defined())
+        check(pgb_linear_distill_bwd(vp(x.h), vp(x.w), code(x.h), static_cast<int *>(vp(t.ids)), fp(t.p), fp(t.ent), t.ids.size(1), t.tau, fp(L), fp(count),
+                                     fp(grad), vp(dh), vp(dw), vp(scratch), n, reduction, x.N, x.V, x.d, dev.stream), what);
+    else
+        check(pgb_linear_xent_bwd(vp(x.h), vp(x.w), code(x.h), static_cast<long long *>(vp(t.target)), t.ignore, fp(L), fp(count), fp(grad), vp(dh), vp(dw),
+                                  vp(scratch), n, reduction, x.N, x.V, x.d, dev.stream), what);
+    return {dh, dw};
+}
+const char *const XENT = "linear_cross_entropy", *const DISTILL = "linear_distill", *const EMBED = "embedding";
+HeadWant xent_want(const HeadIn &x, const Tensor &h, const Tensor &target, int64_t ignore) {
+    need_cuda(target);
+    same_device(XENT, h, target);
+    TORCH_CHECK_VALUE(target.sizes() == h.sizes().slice(0, h.dim() - 1), XENT, ": a target per row of h, got ", target.sizes(), " for ", h.sizes());
+    return {whole_numbers(XENT, target).reshape({x.N}), ignore, Tensor(), Tensor(), Tensor(), 1.0};
+}
+std::tuple<Tensor, Tensor, Tensor> teacher_lists(const Tensor &ids_, const Tensor &logits_, double tau, int64_t V) {
+    need_cuda(ids_, logits_);
+    same_device(DISTILL, ids_, logits_);
+    TORCH_CHECK_VALUE(ids_.dim() >= 1 && ids_.sizes() == logits_.sizes(), DISTILL, ": a teacher's ids and logits share their shape, got ", ids_.sizes(), " and ",
+                      logits_.sizes());
+    TORCH_CHECK_VALUE(tau > 0.0 && tau < 3e38, DISTILL, ": the temperature is positive, got ", tau);
+    const int64_t k = ids_.size(-1);
+    TORCH_CHECK_VALUE(k >= 1 && k <= 1024, DISTILL, ": 1 to 1024 teacher entries a row, got ", k);
+    const int64_t N = ids_.numel() / k;
+    OnDevice dev(ids_);
+    const Tensor ids = whole_numbers(DISTILL, ids_).reshape({N, k}), logits = f32c(logits_).reshape({N, k});
+    Tensor out = alloc(ids, {N, k}, at::kInt), p = alloc(ids, {N, k}, at::kFloat), ent = alloc(ids, {N}, at::kFloat);
+    if (N > 0)
+        check(pgb_teacher_lists(static_cast<long long *>(vp(ids)), fp(logits), tau, static_cast<int *>(vp(out)), fp(p), fp(ent), N, V, k, dev.stream),
+              "pgb_teacher_lists");
+    return {out, p, ent};
+}
+HeadWant distill_want(const HeadIn &x, const Tensor &h, const Tensor &ids, const Tensor &logits, double tau) {
+    same_device(DISTILL, h, ids);
+    TORCH_CHECK_VALUE(ids.dim() == h.dim() && ids.sizes().slice(0, ids.dim() - 1) == h.sizes().slice(0, h.dim() - 1), DISTILL, ": k teacher entries per row of h, got ",
+                      ids.sizes(), " for ", h.sizes());
+    auto [i, p, ent] = teacher_lists(ids, logits, tau, x.V);
+    return {Tensor(), 0, i, p, ent, tau};
+}
+
+// Either loss with its gradients: what the backward pass reads is h, W, the targets and two numbers a row.
+struct HeadLoss : torch::autograd::Function<HeadLoss> {
+    static variable_list forward(AutogradContext *ctx, const Tensor &h_, const Tensor &w_, const OptTensor &target, int64_t ignore, const OptTensor &ids,
+                                 const OptTensor &logits, double tau, int64_t reduction) {
+        const char *what = target ? XENT : DISTILL;
+        const HeadIn x = head_in(what, h_, w_);
+        const HeadWant t = target ? xent_want(x, h_, *target, ignore) : distill_want(x, h_, *ids, *logits, tau);
+        HeadOut r = head_fwd(what, x, t, reduction);
+        ctx->save_for_backward({x.h, x.w, t.target, t.ids, t.p, t.ent, r.L, r.count});
+        auto &d = ctx->saved_data;
+        d["ignore"] = ignore; d["tau"] = tau; d["reduction"] = reduction; d["shape"] = h_.sizes().vec();
+        ctx->set_materialize_grads(false);
+        if (reduction != REDUCE_NONE) return {r.loss};
+        return {r.loss.view(h_.sizes().slice(0, h_.dim() - 1))};
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list g) {
+        variable_list none(8);
+        if (!g[0].defined()) return none;
+        const variable_list s = ctx->get_saved_variables();
+        auto &d = ctx->saved_data;
+        const HeadIn x{s[0], s[1], s[0].size(0), s[1].size(0), s[1].size(1)};
+        const HeadWant t{s[2], d["ignore"].toInt(), s[3], s[4], s[5], d["tau"].toDouble()};
+        const bool list = t.ids.defined();
+        auto [dh, dw] = head_bwd(list ? DISTILL : XENT, x, t, s[6], s[7], g[0].reshape({-1}), d["reduction"].toInt(), ctx->needs_input_grad(0), ctx->needs_input_grad(1));
+        none[0] = dh.defined() ? dh.view(d["shape"].toIntVector()) : dh;
+        none[1] = dw;
+        return once(list ? "pragnosia_b200 linear_distill" : "pragnosia_b200 linear_cross_entropy", s, none, g);
+    }
+};
+// nullopt: something wants to see the registered operators (see plain)
+OptTensor linear_xent(const Tensor &h, const Tensor &w, const Tensor &target, int64_t ignore, int64_t reduction) {
+    if (!plain(h, w, target)) return std::nullopt;
+    if (at::GradMode::is_enabled() && (wants_grad(h) || wants_grad(w)))
+        return HeadLoss::apply(h, w, OptTensor(target), ignore, OptTensor(), OptTensor(), 1.0, reduction)[0];
+    const HeadIn x = head_in(XENT, h, w);
+    const Tensor loss = head_fwd(XENT, x, xent_want(x, h, target, ignore), reduction).loss;
+    return reduction == REDUCE_NONE ? loss.view(target.sizes()) : loss;
+}
+OptTensor linear_distill(const Tensor &h, const Tensor &w, const Tensor &ids, const Tensor &logits, double tau, int64_t reduction) {
+    if (!plain(h, w, ids, logits)) return std::nullopt;
+    if (at::GradMode::is_enabled() && (wants_grad(h) || wants_grad(w)))
+        return HeadLoss::apply(h, w, OptTensor(), 0, OptTensor(ids), OptTensor(logits.detach()), tau, reduction)[0];
+    const HeadIn x = head_in(DISTILL, h, w);
+    const Tensor loss = head_fwd(DISTILL, x, distill_want(x, h, ids, logits, tau), reduction).loss;
+    return reduction == REDUCE_NONE ? loss.view(h.sizes().slice(0, h.dim() - 1)) : loss;
+}
+
+// ------------------------------------------------------------------------------------------------ embedding
+Tensor embed_weight(const Tensor &w) {
+    TORCH_CHECK_TYPE(io_type(w.scalar_type()), EMBED, ": the weight is float32 or bfloat16, got ", w.scalar_type());
+    TORCH_CHECK_VALUE(w.dim() == 2 && w.size(0) >= 1 && w.size(1) >= 1, EMBED, ": the weight is (V, d), got ", w.sizes());
+    return w.contiguous();
+}
+Tensor embed_fwd(const Tensor &ids_, const Tensor &w_, double scale) {
+    need_cuda(ids_, w_);
+    same_device(EMBED, ids_, w_);
+    OnDevice dev(w_);
+    const Tensor w = embed_weight(w_), ids = whole_numbers(EMBED, ids_);
+    std::vector<int64_t> shape = ids_.sizes().vec();
+    shape.push_back(w.size(1));
+    Tensor y = alloc(w, shape, w.scalar_type());
+    if (ids.numel() > 0)
+        check(pgb_embedding_fwd(static_cast<long long *>(vp(ids)), vp(w), code(w), scale, vp(y), ids.numel(), w.size(0), w.size(1), dev.stream),
+              "pgb_embedding_fwd");
+    return y;
+}
+Tensor embed_bwd(const Tensor &ids_, const Tensor &g_, double scale, int64_t padding, int64_t V) {
+    need_cuda(ids_, g_);
+    same_device(EMBED, ids_, g_);
+    OnDevice dev(g_);
+    TORCH_CHECK_TYPE(io_type(g_.scalar_type()), EMBED, ": the gradient is float32 or bfloat16, got ", g_.scalar_type());
+    const Tensor g = g_.contiguous(), ids = whole_numbers(EMBED, ids_);
+    const int64_t d = g.size(-1), N = ids.numel();
+    TORCH_CHECK_VALUE(g.numel() == N * d && V >= 1, EMBED, ": a row of gradient per id, got ", g.sizes(), " for ", ids.sizes());
+    Tensor dw = alloc(g, {V, d}, g.scalar_type());
+    if (N == 0) return dw.zero_();
+    const long long n = pgb_embedding_bwd_scratch_bytes(N, V, d);
+    const Tensor scratch = bytes(g, n);
+    check(pgb_embedding_bwd(static_cast<long long *>(vp(ids)), vp(g), code(g), scale, padding, vp(dw), vp(scratch), n, N, V, d, dev.stream), "pgb_embedding_bwd");
+    return dw;
+}
+struct Embed : torch::autograd::Function<Embed> {
+    static variable_list forward(AutogradContext *ctx, const Tensor &ids, const Tensor &w, double scale, int64_t padding) {
+        ctx->save_for_backward({ids});
+        auto &d = ctx->saved_data;
+        d["scale"] = scale; d["padding"] = padding; d["V"] = w.size(0);
+        ctx->set_materialize_grads(false);
+        return {embed_fwd(ids, w, scale)};
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list g) {
+        if (!g[0].defined()) return variable_list(4);
+        const variable_list s = ctx->get_saved_variables();
+        auto &d = ctx->saved_data;
+        return once("pragnosia_b200 embedding", s, {Tensor(), embed_bwd(s[0], g[0], d["scale"].toDouble(), d["padding"].toInt(), d["V"].toInt()), Tensor(), Tensor()}, g);
+    }
+};
+OptTensor embedding(const Tensor &ids, const Tensor &w, double scale, int64_t padding) {
+    if (!plain(ids, w)) return std::nullopt;
+    if (at::GradMode::is_enabled() && wants_grad(w)) {
+        need_cuda(ids, w);
+        embed_weight(w);
+        return Embed::apply(ids, w, scale, padding)[0];
+    }
+    return embed_fwd(ids, w, scale);
+}
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -423,4 +633,32 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         return std::make_tuple(r.dq, r.dk, r.dv, r.dla, some(r.dbe), some(r.dS0));
     }, nogil);
     m.def("scan_diff", &scan_diff, nogil);
+    m.def("linear_xent", &linear_xent, nogil);
+    m.def("linear_xent_fwd", [](const Tensor &h, const Tensor &w, const Tensor &target, int64_t ignore, int reduction) {
+        const HeadIn x = head_in(XENT, h, w);
+        HeadOut r = head_fwd(XENT, x, xent_want(x, h, target, ignore), reduction);
+        return std::make_tuple(r.loss, r.L, r.count);
+    }, nogil);
+    m.def("linear_xent_bwd", [](const Tensor &h, const Tensor &w, const Tensor &target, int64_t ignore, const Tensor &L, const Tensor &count, const Tensor &grad,
+                                int reduction, bool want_dh, bool want_dw) {
+        const HeadIn x = head_in(XENT, h, w);
+        auto [dh, dw] = head_bwd(XENT, x, xent_want(x, h, target, ignore), L, count, grad, reduction, want_dh, want_dw);
+        return std::make_tuple(some(dh), some(dw));
+    }, nogil);
+    m.def("teacher_lists", &teacher_lists, nogil);
+    m.def("linear_distill", &linear_distill, nogil);
+    m.def("linear_distill_fwd", [](const Tensor &h, const Tensor &w, const Tensor &ids, const Tensor &p, const Tensor &ent, double tau, int reduction) {
+        const HeadIn x = head_in(DISTILL, h, w);
+        HeadOut r = head_fwd(DISTILL, x, {Tensor(), 0, ids, p, ent, tau}, reduction);
+        return std::make_tuple(r.loss, r.L, r.count);
+    }, nogil);
+    m.def("linear_distill_bwd", [](const Tensor &h, const Tensor &w, const Tensor &ids, const Tensor &p, const Tensor &ent, double tau, const Tensor &L,
+                                   const Tensor &count, const Tensor &grad, int reduction, bool want_dh, bool want_dw) {
+        const HeadIn x = head_in(DISTILL, h, w);
+        auto [dh, dw] = head_bwd(DISTILL, x, {Tensor(), 0, ids, p, ent, tau}, L, count, grad, reduction, want_dh, want_dw);
+        return std::make_tuple(some(dh), some(dw));
+    }, nogil);
+    m.def("embedding", &embedding, nogil);
+    m.def("embedding_fwd", &embed_fwd, nogil);
+    m.def("embedding_bwd", &embed_bwd, nogil);
 }

@@ -21,6 +21,7 @@ import torch
 from torch import Tensor
 
 from . import ops
+from ._lib import host
 
 NS = "pragnosia_b200"
 _BF16, _F32 = torch.bfloat16, torch.float32
@@ -433,3 +434,139 @@ def linear_act(x: Tensor, W: Tensor, bias: Optional[Tensor], act: int) -> Tensor
 @linear_act.register_fake
 def _(x, W, bias, act):
     return _e(x, *x.shape[:-1], W.shape[0])
+
+
+# ------------------------------------------------------------------------------------------------ embedding, losses over the vocabulary
+def _rows(h):
+    n = 1
+    for s in h.shape[:-1]:
+        n = n * s
+    return n
+
+
+def _loss_like(h, reduction):
+    return _e(h, _rows(h), dtype=_F32) if reduction == 0 else _e(h, dtype=_F32)
+
+
+def _grads_like(h, W, want_dh, want_dW):
+    return (_e(h, *h.shape) if want_dh else _none(h)), (_e(W, *W.shape) if want_dW else _none(W))
+
+
+@torch.library.custom_op(f"{NS}::linear_xent", mutates_args=())
+def linear_xent(h: Tensor, W: Tensor, target: Tensor, ignore_index: int, reduction: int) -> Tuple[Tensor, Tensor, Tensor]:
+    """(loss, the rows' log2 sums of exponentials in two parts, rows that count); reduction 0 none, 1 sum, 2 mean."""
+    return host().linear_xent_fwd(h, W, target, ignore_index, reduction)
+
+
+@linear_xent.register_fake
+def _(h, W, target, ignore_index, reduction):
+    return _loss_like(h, reduction), _e(h, _rows(h), 2, dtype=_F32), _e(h, dtype=_F32)
+
+
+@torch.library.custom_op(f"{NS}::linear_xent_bwd", mutates_args=())
+def linear_xent_bwd(h: Tensor, W: Tensor, target: Tensor, ignore_index: int, L: Tensor, count: Tensor, grad: Tensor, reduction: int, want_dh: bool,
+                    want_dW: bool) -> Tuple[Tensor, Tensor]:
+    dh, dW = host().linear_xent_bwd(h, W, target, ignore_index, L, count, grad, reduction, want_dh, want_dW)
+    return (dh.view(h.shape) if want_dh else _none(h)), (dW if want_dW else _none(W))
+
+
+@linear_xent_bwd.register_fake
+def _(h, W, target, ignore_index, L, count, grad, reduction, want_dh, want_dW):
+    return _grads_like(h, W, want_dh, want_dW)
+
+
+def _xent_ctx(ctx, inputs, output):
+    h, W, target, ctx.ignore_index, ctx.reduction = inputs
+    ctx.save_for_backward(h, W, target, output[1], output[2])
+
+
+def _xent_grads(ctx, g, _L, _count):
+    h, W, target, L, count = ctx.saved_tensors
+    want = ctx.needs_input_grad[:2]
+    dh, dW = torch.ops.pragnosia_b200.linear_xent_bwd(h, W, target, ctx.ignore_index, L, count, g, ctx.reduction, *want)
+    return (dh if want[0] else None), (dW if want[1] else None), None, None, None
+
+
+linear_xent.register_autograd(_xent_grads, setup_context=_xent_ctx)
+
+
+@torch.library.custom_op(f"{NS}::teacher_lists", mutates_args=())
+def teacher_lists(ids: Tensor, logits: Tensor, temperature: float, V: int) -> Tuple[Tensor, Tensor, Tensor]:
+    """A teacher's entries as linear_distill takes them: ids ascending, their probabilities, the sum of p log p."""
+    return host().teacher_lists(ids, logits, temperature, V)
+
+
+@teacher_lists.register_fake
+def _(ids, logits, temperature, V):
+    n, k = _rows(ids), ids.shape[-1]
+    return _e(ids, n, k, dtype=torch.int32), _e(ids, n, k, dtype=_F32), _e(ids, n, dtype=_F32)
+
+
+@torch.library.custom_op(f"{NS}::linear_distill", mutates_args=())
+def linear_distill(h: Tensor, W: Tensor, ids: Tensor, p: Tensor, ent: Tensor, temperature: float, reduction: int) -> Tuple[Tensor, Tensor, Tensor]:
+    return host().linear_distill_fwd(h, W, ids, p, ent, temperature, reduction)
+
+
+@linear_distill.register_fake
+def _(h, W, ids, p, ent, temperature, reduction):
+    return _loss_like(h, reduction), _e(h, _rows(h), 2, dtype=_F32), _e(h, dtype=_F32)
+
+
+@torch.library.custom_op(f"{NS}::linear_distill_bwd", mutates_args=())
+def linear_distill_bwd(h: Tensor, W: Tensor, ids: Tensor, p: Tensor, ent: Tensor, temperature: float, L: Tensor, count: Tensor, grad: Tensor, reduction: int,
+                       want_dh: bool, want_dW: bool) -> Tuple[Tensor, Tensor]:
+    dh, dW = host().linear_distill_bwd(h, W, ids, p, ent, temperature, L, count, grad, reduction, want_dh, want_dW)
+    return (dh.view(h.shape) if want_dh else _none(h)), (dW if want_dW else _none(W))
+
+
+@linear_distill_bwd.register_fake
+def _(h, W, ids, p, ent, temperature, L, count, grad, reduction, want_dh, want_dW):
+    return _grads_like(h, W, want_dh, want_dW)
+
+
+def _distill_ctx(ctx, inputs, output):
+    h, W, ids, p, ent, ctx.temperature, ctx.reduction = inputs
+    ctx.save_for_backward(h, W, ids, p, ent, output[1], output[2])
+
+
+def _distill_grads(ctx, g, _L, _count):
+    h, W, ids, p, ent, L, count = ctx.saved_tensors
+    want = ctx.needs_input_grad[:2]
+    dh, dW = torch.ops.pragnosia_b200.linear_distill_bwd(h, W, ids, p, ent, ctx.temperature, L, count, g, ctx.reduction, *want)
+    return (dh if want[0] else None), (dW if want[1] else None), None, None, None, None, None
+
+
+linear_distill.register_autograd(_distill_grads, setup_context=_distill_ctx)
+
+
+@torch.library.custom_op(f"{NS}::embedding", mutates_args=())
+def embedding(ids: Tensor, W: Tensor, scale: float, padding_idx: int) -> Tensor:
+    return host().embedding_fwd(ids, W, scale)
+
+
+@embedding.register_fake
+def _(ids, W, scale, padding_idx):
+    return _e(W, *ids.shape, W.shape[1])
+
+
+@torch.library.custom_op(f"{NS}::embedding_bwd", mutates_args=())
+def embedding_bwd(ids: Tensor, g: Tensor, scale: float, padding_idx: int, V: int) -> Tensor:
+    return host().embedding_bwd(ids, g, scale, padding_idx, V)
+
+
+@embedding_bwd.register_fake
+def _(ids, g, scale, padding_idx, V):
+    return _e(g, V, g.shape[-1])
+
+
+def _embed_ctx(ctx, inputs, output):
+    ids, W, ctx.scale, ctx.padding_idx = inputs
+    ctx.V = W.shape[0]
+    ctx.save_for_backward(ids)
+
+
+def _embed_grads(ctx, g):
+    return None, torch.ops.pragnosia_b200.embedding_bwd(ctx.saved_tensors[0], g, ctx.scale, ctx.padding_idx, ctx.V), None, None
+
+
+embedding.register_autograd(_embed_grads, setup_context=_embed_ctx)
