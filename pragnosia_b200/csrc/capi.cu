@@ -804,7 +804,7 @@ constexpr long long HEAD_MOST_ROWS = 1LL << 30;
 int head_sizes(long long N, int V, int d, int dtype) {
     if (dtype != PGB_F32 && dtype != PGB_BF16) return PGB_ERR_BAD_DTYPE;
     if (N < 1 || V < 1 || d < 8 || (d % 8) != 0) return PGB_ERR_BAD_SHAPE;
-    if (N > HEAD_MOST_ROWS || V > HEAD_MOST_ROWS || d > 65536) return PGB_ERR_TOO_LARGE;
+    if (N > HEAD_MOST_ROWS || V > HEAD_MOST_ROWS || d > 65536 || ((N + 255) / 256) * ((V + 255) / 256) > 0x40000000LL) return PGB_ERR_TOO_LARGE;
     return PGB_OK;
 }
 int head_args(HeadLossArgs &x, const void *h, const void *W, int dtype, const long long *target, long long ignore, const int *ids, const float *p,

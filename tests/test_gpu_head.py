@@ -157,16 +157,20 @@ def test_forms_of_the_call():
     a = xent(h.view(12, 31, 64), w, t.view(12, 31).int(), c, "none")
     assert a[0].shape == (12, 31) and a[1].shape == (12, 31, 64)
     assert all(torch.equal(x.reshape(y.shape), y) for x, y in zip(a, want))
+    # rows in another order, and one gradient alone: the K axis of the gradients' products is cut at other places, so the bits may differ
+    p, live = one_hot(t, 333)
+    ref, off = dense(h, w, p, live, 1.0, c.view(-1), "none")
     a = xent(h.view(12, 31, 64).transpose(0, 1), w.t().contiguous().t(), t.view(12, 31).t(), c.t(), "none")
-    assert torch.equal(a[0].t().reshape(-1), want[0]) and torch.equal(a[1].transpose(0, 1).reshape(-1, 64), want[1])
+    assert torch.equal(a[0].t().reshape(-1), want[0])
+    within((want[0], a[1].transpose(0, 1).reshape(-1, 64), a[2]), ref, off)
     room = torch.empty(h.numel() + 1, device=DEV, dtype=BF)
-    off = room[1:].view_as(h).copy_(h)
-    assert all(torch.equal(x, y) for x, y in zip(xent(off, w, t, c.view(-1), "none"), want))
+    moved = room[1:].view_as(h).copy_(h)
+    assert all(torch.equal(x, y) for x, y in zip(xent(moved, w, t, c.view(-1), "none"), want))
     for wrt in (0, 1):
         x = [h.clone(), w.clone()]
         x[wrt].requires_grad_()
         (got,) = torch.autograd.grad(head.linear_cross_entropy(*x, t, reduction="none"), [x[wrt]], c.view(-1))
-        assert torch.equal(got, want[1 + wrt])
+        within((got,), ref[1 + wrt:2 + wrt], off[1 + wrt:2 + wrt])
     with torch.no_grad():
         assert torch.equal(head.linear_cross_entropy(h, w, t, reduction="none"), want[0])
     ig = int(t[5])
