@@ -31,14 +31,14 @@ constexpr long long HL_PIECE_BYTES = 96LL << 20;                      // of ds i
 static_assert(HL_STAGE % 1024 == 0 && HL_SMEM <= 232448, "shared memory");
 constexpr float LOG2E_F = 1.4426950408889634f;
 
-struct HlMaps { CUtensorMap a[2], b[2]; };
-// An epilogue warp's share of a tile: rows row0 .. +31 (a lane each), columns col0 .. +63; block: which of the tile's 32 it is. t, k0, k1, kt: the
-// tile and what of its K blocks the accumulator holds.
-struct HlTile { int lane, sub, part, block, n, row0, col0, g, t, k0, k1, kt; uint32_t ti; };
-// One product C[M][N] = A B^T over kb blocks of 64 (npairs times: the products of the operands' bf16 terms).
+struct HlMaps { CUtensorMap a[3], b[3], ds; };                        // of the products; ds: the piece of it that is written
+// An epilogue warp's share of a tile: rows row0 .. +31 (a lane each), columns col0 .. +63; block: which of the tile's 32 it is. g, t, sp: the
+// product, its tile, and the part of K that the accumulator holds.
+struct HlTile { int lane, sub, part, block, n, row0, col0, g, t, sp; uint32_t ti; };
+// One product C[M][N] = A B^T over kb blocks of 64 (npairs times: the products of the operands' bf16 terms), its K axis in `splits` parts.
 // a_mn / b_mn: the operand lies with its M / N axis contiguous instead of K.
 struct HlProduct {
-    int tiles_m = 0, tiles_n = 0, kb = 0, npairs = 1, a_mn = 0, b_mn = 0;
+    int tiles_m = 0, tiles_n = 0, kb = 0, npairs = 1, splits = 1, a_mn = 0, b_mn = 0;
     __host__ __device__ int tiles() const { return tiles_m * tiles_n; }
     __host__ __device__ int kt() const { return kb * npairs; }
     // row blocks fastest, HL_GROUP of them at a time: B is read once per group, whatever its size
@@ -49,48 +49,48 @@ struct HlProduct {
         m = g * HL_GROUP + in - n * gm;
     }
 };
-// What a pair of SMs does: whole tiles, dealt out in turn (CUT false), or an equal share of all K blocks of both products, so that the first
-// and the last tile of a share may be a part of one (CUT true).
-template <bool CUT>
-struct HlShare {
-    const HlProduct *pr;
-    int g = 0, t = 0, k0 = 0, k1 = 0, kt = 0;                         // the part at hand: product, tile, K blocks
-    long long left = 0;
-    static __host__ __device__ long long units(const HlProduct *pr) { return (long long)pr[0].tiles() * pr[0].kt() + (long long)pr[1].tiles() * pr[1].kt(); }
-    static __device__ long long bound(long long total, int pair, int pairs) { return total / pairs * pair + total % pairs * pair / pairs; }
-    // the pair whose share holds K block u
-    static __device__ int owner(long long total, long long u, int pairs) {
-        int q = (int)((double)u * pairs / (double)total);
-        while (q + 1 < pairs && bound(total, q + 1, pairs) <= u) ++q;
-        while (q > 0 && bound(total, q, pairs) > u) --q;
-        return q;
+// What a pair of SMs does, one part of a tile after the other. One product (forward): every pairs-th tile. Three (backward): every pairs-th of
+// [dh's parts][dW's], a product's by part of K, then by tile, and behind them its share of ds's tiles, which are short: the shares level out what
+// the long parts leave uneven.
+//   So the pairs that run side by side walk the same stretch of K together and what they read they share through the L2: with equal shares of
+// all K blocks instead (tiles cut where a share ends) each was somewhere else, 15 of 38 million sectors missed the near L2, and the
+// products took as long as with a quarter of the pairs idle in the last round.
+constexpr int HL_MOST_PAIRS = 127;
+struct HlTrio { HlProduct p[3]; int share[HL_MOST_PAIRS + 1]; };      // dh, dW, ds; pair q has ds's tiles share[q] .. share[q + 1] - 1
+struct HlOne {
+    const HlProduct &pr;
+    int pairs, t;
+    static constexpr int g = 0, sp = 0, k0 = 0;
+    int k1;
+    __device__ HlOne(const HlProduct &pr, int pair, int pairs) : pr(pr), pairs(pairs), t(pair), k1(pr.kt()) {}
+    __device__ __forceinline__ const HlProduct &product() const { return pr; }
+    __device__ __forceinline__ bool more() const { return t < pr.tiles(); }
+    __device__ __forceinline__ void next() { t += pairs; }
+};
+struct HlThree {
+    const HlTrio &w;
+    int pairs, i, end, g = 0, t = 0, sp = 0, k0 = 0, k1 = 0;
+    __device__ HlThree(const HlTrio &w, int pair, int pairs) : w(w), pairs(pairs), i(pair), end(w.share[pair + 1]) { place(w.share[pair]); }
+    __device__ __forceinline__ const HlProduct &product() const { return w.p[g]; }
+    __device__ __forceinline__ bool more() const { return g < 2 || t < end; }
+    __device__ __forceinline__ void next() {
+        if (g == 2) { ++t; return; }
+        i += pairs;
+        place(-1);
     }
-    __device__ HlShare(const HlProduct *pr, int pair, int pairs) : pr(pr) {
-        if constexpr (CUT) {
-            const long long total = units(pr), n0 = (long long)pr[0].tiles() * pr[0].kt(), from = bound(total, pair, pairs);
-            left = bound(total, pair + 1, pairs) - from;
-            g = from >= n0;
-            kt = pr[g].kt();
-            const long long in = g ? from - n0 : from;
-            t = kt > 0 ? (int)(in / kt) : 0;
-            k0 = kt > 0 ? (int)(in - (long long)t * kt) : 0;
-            k1 = (int)(kt - k0 < left ? kt : k0 + left);
-        } else {
-            t = pair; kt = k1 = pr[0].kt();
-            left = t < pr[0].tiles();
+    __device__ __forceinline__ void place(int first) {
+        const int n0 = w.p[0].tiles() * w.p[0].splits, n1 = w.p[1].tiles() * w.p[1].splits;
+        if (i >= n0 + n1) {
+            g = 2; sp = 0; k0 = 0; k1 = w.p[2].kt();
+            t = first >= 0 ? first : w.share[i % pairs];               // i % pairs: the pair
+            return;
         }
-    }
-    __device__ bool more() const { return left > 0; }
-    __device__ void next(int pairs) {
-        if constexpr (CUT) {
-            left -= k1 - k0;
-            if (++t == pr[g].tiles() && g == 0) { g = 1; t = 0; kt = pr[1].kt(); }
-            k0 = 0;
-            k1 = (int)(kt < left ? kt : left);
-        } else {
-            t += pairs;
-            left = t < pr[0].tiles();
-        }
+        g = i >= n0;
+        const int in = g ? i - n0 : i, tiles = w.p[g].tiles(), kt = w.p[g].kt();
+        sp = in / tiles;
+        t = in - sp * tiles;
+        k0 = (int)((long long)kt * sp / w.p[g].splits);
+        k1 = (int)((long long)kt * (sp + 1) / w.p[g].splits);
     }
 };
 // the terms of the two operands that product number pp of npairs multiplies (0: the head), small products first
@@ -102,8 +102,8 @@ __device__ __forceinline__ void hl_terms(int pp, int npairs, int &ta, int &tb) {
 
 // The roles of the kernel. An epilogue warp takes its 32 x 64 block of a complete accumulator into registers, hands the accumulator back at once, and
 // works on them while what the next tile needs of its rows (epi.fetch) is on its way.
-template <bool CUT, class Epi>
-__device__ __forceinline__ void hl_body(const HlMaps &maps, const HlProduct *pr, Epi &epi) {
+template <class Work, class What, class Epi>
+__device__ __forceinline__ void hl_body(const HlMaps &maps, const What &what, Epi &epi) {
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;      // the same offset in both CTAs: one descriptor serves both
     uint8_t *sm = smem_raw + (base - smem_u32(smem_raw));
@@ -133,15 +133,15 @@ __device__ __forceinline__ void hl_body(const HlMaps &maps, const HlProduct *pr,
     pdl_wait();
     pdl_launch_dependents();
 
-    HlShare<CUT> w(pr, pair, pairs);
+    Work w(what, pair, pairs);
     int m, n;
     if (warp == 0) {
         // ------------------------------------------------------------------------------------------ producer (both CTAs)
         const bool leader = elect_one();
         uint32_t it = 0;
         bool ok = true;
-        for (; w.more() && ok; w.next(pairs)) {
-            const HlProduct &p = pr[w.g];
+        for (; w.more() && ok; w.next()) {
+            const HlProduct &p = w.product();
             p.at(w.t, m, n);
             const int m0 = m * HL_B + (int)rank * (HL_B / 2), n0 = n * HL_B + (int)rank * (HL_B / 2);
             const CUtensorMap *ma = &maps.a[w.g], *mbm = &maps.b[w.g];
@@ -176,8 +176,8 @@ __device__ __forceinline__ void hl_body(const HlMaps &maps, const HlProduct *pr,
         if (rank == 0) {
             uint32_t it = 0, ti = 0;
             bool ok = true;
-            for (; w.more() && ok; w.next(pairs), ++ti) {
-                const int amn = pr[w.g].a_mn, bmn = pr[w.g].b_mn;
+            for (; w.more() && ok; w.next(), ++ti) {
+                const int amn = w.product().a_mn, bmn = w.product().b_mn;
                 const uint32_t idesc = idesc_bf16(HL_B, HL_B, amn, bmn), a = ti & 1;
                 const uint32_t stepa = amn ? 128 : 2, stepb = bmn ? 128 : 2;
                 if (ti >= 2) ok = __all_sync(0xffffffffu, lp_wait_cluster(bar_acc_empty(a), ((ti >> 1) + 1) & 1, 92));
@@ -211,13 +211,13 @@ __device__ __forceinline__ void hl_body(const HlMaps &maps, const HlProduct *pr,
         uint32_t ti = 0;
         bool ok = w.more();
         if (ok) {
-            pr[w.g].at(w.t, m, n);
-            epi.fetch(m * HL_B + row_in + lane, n * HL_B + col_in);
+            w.product().at(w.t, m, n);
+            epi.fetch(w.g, m * HL_B + row_in + lane);
         }
         for (; ok; ++ti) {
             const uint32_t a = ti & 1;
             x.n = n; x.row0 = m * HL_B + row_in; x.col0 = n * HL_B + col_in; x.ti = ti;
-            x.g = w.g; x.t = w.t; x.k0 = w.k0; x.k1 = w.k1; x.kt = w.kt;
+            x.g = w.g; x.t = w.t; x.sp = w.sp;
             epi.begin(x);
             ok = __all_sync(0xffffffffu, mbar_wait(bar_acc_full(a), (ti >> 1) & 1, 94));
             if (!ok) break;
@@ -229,17 +229,22 @@ __device__ __forceinline__ void hl_body(const HlMaps &maps, const HlProduct *pr,
             tmem_ld_wait();
 #pragma unroll
             for (int i = 0; i < 64; ++i) asm volatile("" : "+f"(v[i >> 5][i & 31]));      // nothing that uses them moves ahead of the wait
+            if (w.k0 == w.k1) {                          // a part of K with nothing in it (fewer blocks than parts)
+#pragma unroll
+                for (int i = 0; i < 64; ++i) v[i >> 5][i & 31] = 0.f;
+            }
             tc_fence_before();
             __syncwarp();
             if (lane == 0) lp_arrive_cluster(a ? acc_empty1 : acc_empty0);
-            w.next(pairs);
+            w.next();
             const bool more = w.more();
             if (more) {
-                pr[w.g].at(w.t, m, n);
-                epi.fetch(m * HL_B + row_in + lane, n * HL_B + col_in);
+                w.product().at(w.t, m, n);
+                epi.fetch(w.g, m * HL_B + row_in + lane);
             }
             ok = epi.tile(x, v, stage, shared, bar_quarters(sub, ti & 3)) && more;
         }
+        epi.end(lane);
     }
     tc_fence_before();
     __syncthreads();
@@ -305,7 +310,8 @@ struct HlFwdEpi {
     const HlFwd &f;
     HlWalk<LIST> w;
     long long row, word;                                               // of the tile fetched for
-    __device__ __forceinline__ void fetch(int r, int) {
+    __device__ __forceinline__ void end(int) {}
+    __device__ __forceinline__ void fetch(int, int r) {
         row = r < f.N ? r : -1;
         if (!LIST) word = row >= 0 ? f.t.target[row] : f.t.ignore;
     }
@@ -369,7 +375,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(HL_NT, 1)
 head_loss_fwd_kernel(const __grid_constant__ HlMaps maps, const __grid_constant__ HlProduct pr, const __grid_constant__ HlFwd f) {
     if (blockIdx.x == 0 && threadIdx.x == 0) { pdl_wait(); *f.ticket = 0u; }
     HlFwdEpi<LIST> epi{f, {}, 0, 0};
-    hl_body<false>(maps, &pr, epi);
+    hl_body<HlOne>(maps, pr, epi);
 }
 
 // Joins a row's tiles: 32 rows a block (a lane each), the tiles dealt out to its 8 warps, then the block's losses and live rows as one
@@ -509,17 +515,18 @@ __global__ void __launch_bounds__(128) head_teacher_kernel(const long long *__re
 // ------------------------------------------------------------------------------------------------ backward
 struct HlProb {
     HlTargets t; const float2 *L; const float *row_weight;            // row_weight NULL: 1
-    float a; __nv_bfloat16 *P; long long ldp, part_stride;            // P [terms][rows of the piece][ldp]
+    float a;
     long long row_from; int V, col_from, cols, rows;                  // the piece: rows and columns it begins at, how many
     unsigned *tickets; int n_tickets;                                 // set to zero for the products behind
 };
 template <bool LIST, int TERMS>
 struct HlProbEpi {
     const HlProb &f;
+    const CUtensorMap *map;
     HlWalk<LIST> w;
     long long row, word; float2 L; float weight, ent; int id0;         // of the tile fetched for
     float a_hi, a_lo, c; bool live;                                   // of the tile at hand
-    __device__ __forceinline__ void fetch(int r, int) {
+    __device__ __forceinline__ void fetch(int r) {
         row = r < f.rows ? f.row_from + r : -1;
         if (row < 0) return;
         L = f.L[row];
@@ -533,10 +540,11 @@ struct HlProbEpi {
         live = row >= 0 && (LIST ? bad || id0 != 0x7fffffff : word != f.t.ignore);
         c = bad ? NAN : weight;
     }
-    __device__ __forceinline__ bool tile(const HlTile &x, float (&vv)[2][32], uint8_t *stage, uint8_t *, uint32_t) {
+    // Rounded, the block goes out by two TMA stores a term, 32 columns each, from the warp's staging: 64-byte rows, their 16-byte chunks swapped
+    // as the store's 64-byte swizzle has them, so that the row-per-lane writes touch every bank once. What lies outside the piece is not written.
+    __device__ __forceinline__ void tile(const HlTile &x, float (&vv)[2][32], uint8_t *stage) {
         const int lane = x.lane;
-        // 64-byte rows, their 16-byte chunks rotated by the row: the row-per-lane writes and the chunk-per-lane reads both touch every bank once
-        auto chunk_at = [&](int r, int ch) { return stage + r * 64 + ((ch ^ ((r >> 1) & 3)) << 4); };
+        const bool plain = __all_sync(0xffffffffu, live && c == 1.f);  // no row to weigh or to leave out
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
             const int c0 = x.col0 + 32 * b, v0 = f.col_from + c0;
@@ -552,10 +560,14 @@ struct HlProbEpi {
                 for (int i = 0; i < 32; ++i) v[i] -= i == at ? less : 0.f;
                 if (hit) w.advance();
             }
+            if (!plain) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = live ? c * v[i] : 0.f;
+                for (int i = 0; i < 32; ++i) v[i] = live ? c * v[i] : 0.f;
+            }
 #pragma unroll
             for (int term = 0; term < TERMS; ++term) {
+                if (lane == 0) tma_store_source_free();
+                __syncwarp();
 #pragma unroll
                 for (int ch = 0; ch < 4; ++ch) {
                     __nv_bfloat162 o[4];
@@ -567,30 +579,15 @@ struct HlProbEpi {
                             v[8 * ch + 2 * i] -= h.x; v[8 * ch + 2 * i + 1] -= h.y;
                         }
                     }
-                    *reinterpret_cast<uint4 *>(chunk_at(lane, ch)) = *reinterpret_cast<uint4 *>(o);
+                    *reinterpret_cast<uint4 *>(stage + lane * 64 + ((ch ^ ((lane >> 1) & 3)) << 4)) = *reinterpret_cast<uint4 *>(o);
                 }
+                fence_proxy_async();
                 __syncwarp();
-                __nv_bfloat16 *P = f.P + term * f.part_stride;
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int r = (lane >> 2) + 8 * q, ch = lane & 3;
-                    const uint4 val = *reinterpret_cast<const uint4 *>(chunk_at(r, ch));
-                    if (x.row0 + r < f.rows && c0 + 8 * ch < f.ldp) *reinterpret_cast<uint4 *>(P + (long long)(x.row0 + r) * f.ldp + c0 + 8 * ch) = val;
-                }
-                __syncwarp();
+                if (lane == 0 && x.row0 < f.rows) tma_store_3d(map, smem_u32(stage), c0, x.row0, term);
             }
         }
-        return true;
     }
 };
-template <bool LIST, int TERMS>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(HL_NT, 1)
-head_loss_ds_kernel(const __grid_constant__ HlMaps maps, const __grid_constant__ HlProduct pr, const __grid_constant__ HlProb f) {
-    pdl_wait();
-    for (int i = blockIdx.x * HL_NT + threadIdx.x; i < f.n_tickets; i += gridDim.x * HL_NT) f.tickets[i] = 0u;
-    HlProbEpi<LIST, TERMS> epi{f};
-    hl_body<false>(maps, &pr, epi);
-}
 
 // The upstream scale that all rows share: g the gradient of the (summed or averaged) loss, count the rows averaged over.
 __device__ __forceinline__ float hl_alpha(const float *g, const float *count, float tau, int reduction) {
@@ -599,64 +596,40 @@ __device__ __forceinline__ float hl_alpha(const float *g, const float *count, fl
     const float n = *count;
     return n > 0.f ? tau * *g / n : 0.f;                              // no row counts: no gradient (the loss itself is 0 / 0)
 }
-// What becomes of a product's tiles: out = alpha * (acc +) C, or acc (+)= C where further pieces follow. acc [rows][d] fp32.
+// What becomes of a product's tiles: out = alpha * (acc +) C, or acc (+)= C where further pieces follow or the other parts of K are to
+// come. acc [splits][rows][d] fp32. A tile in parts is summed by whoever finishes it last (each of its 32 blocks by itself), in the order of
+// K and from memory all of it, so the sum does not depend on who that is.
 struct HlGrad { float *acc; void *out; long long rows; int adds, last; };
-struct HlGrads {
-    HlGrad g[2]; const float *up, *count; float tau; int reduction, d, out_f32;
-    float *parts; unsigned *tickets;                                  // parts [pairs][2][32][2048]: what pairs hold of cut tiles
-};
-// A tile that shares cut is summed by whoever finishes it last (each of its 32 blocks by itself): the others have left their parts in
-// memory, and all are added in the order of K, so the sum does not depend on who that is.
+struct HlGrads { HlGrad g[2]; const float *up, *count; float tau; int reduction, d, out_f32; unsigned *tickets; };
 struct HlGradEpi {
     const HlGrads &f;
     const HlProduct *pr;
     float alpha;
-    __device__ __forceinline__ void fetch(int, int) {}
-    __device__ __forceinline__ void begin(const HlTile &) {}
-    __device__ __forceinline__ float4 *part_of(int pair, bool head, int block, int lane) const {
-        return reinterpret_cast<float4 *>(f.parts) + (((long long)pair * 2 + head) * 32 + block) * 512 + lane;
-    }
-    __device__ __forceinline__ bool tile(const HlTile &x, float (&v)[2][32], uint8_t *stage, uint8_t *, uint32_t) {
-        const HlGrad &o = f.g[x.g];
-        const int lane = x.lane;
-        if (x.col0 >= f.d || x.row0 >= o.rows) return true;           // nothing of the matrix in this block; its ticket is not drawn by anyone
-        if (x.k1 - x.k0 < x.kt) {
-            const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
-            float4 *mine = part_of(pair, x.k0 == 0, x.block, lane);
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                const float *s = &v[j >> 3][4 * (j & 7)];
-                mine[32 * j] = make_float4(s[0], s[1], s[2], s[3]);
-            }
-            const long long total = HlShare<true>::units(pr), from = (x.g ? (long long)pr[0].tiles() * pr[0].kt() : 0) + (long long)x.t * x.kt;
-            const int q0 = HlShare<true>::owner(total, from, pairs), q1 = HlShare<true>::owner(total, from + x.kt - 1, pairs);
-            __threadfence();
-            __syncwarp();
-            unsigned before = 0;
-            if (lane == 0) before = atomicAdd(f.tickets + ((long long)(x.g ? pr[0].tiles() : 0) + x.t) * 32 + x.block, 1u);
-            before = __shfl_sync(0xffffffffu, before, 0);
-            if (before != (unsigned)(q1 - q0)) return true;
-            __threadfence();
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                const float4 a = __ldcg(part_of(q0, true, x.block, lane) + 32 * j);
-                float *s = &v[j >> 3][4 * (j & 7)];
-                s[0] = a.x; s[1] = a.y; s[2] = a.z; s[3] = a.w;
-            }
-            for (int q = q0 + 1; q <= q1; ++q) {
-#pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    const float4 a = __ldcg(part_of(q, false, x.block, lane) + 32 * j);
-                    float *s = &v[j >> 3][4 * (j & 7)];
-                    s[0] += a.x; s[1] += a.y; s[2] += a.z; s[3] += a.w;
-                }
-            }
+    __device__ __forceinline__ void put(const HlGrad &o, long long at, float4 val) const {
+        val.x *= alpha; val.y *= alpha; val.z *= alpha; val.w *= alpha;
+        if (f.out_f32) {
+            *reinterpret_cast<float4 *>(static_cast<float *>(o.out) + at) = val;
+        } else {
+            __nv_bfloat162 h[2] = {__floats2bfloat162_rn(val.x, val.y), __floats2bfloat162_rn(val.z, val.w)};
+            *reinterpret_cast<uint2 *>(static_cast<__nv_bfloat16 *>(o.out) + at) = *reinterpret_cast<uint2 *>(h);
         }
+    }
+    __device__ __forceinline__ void tile(const HlTile &x, float (&v)[2][32], uint8_t *stage) {
+        const HlGrad &o = f.g[x.g];
+        const int lane = x.lane, splits = pr[x.g].splits, rl = lane >> 2, cl = 4 * (lane & 3);
+        if (x.col0 >= f.d || x.row0 >= o.rows) return;           // nothing of the matrix in this block; nobody draws its ticket
+        const long long plane = o.rows * f.d, base = (long long)(x.row0 + rl) * f.d + x.col0 + cl;
+        float *acc = o.acc ? o.acc + x.sp * plane + base : nullptr;
         auto chunk_at = [&](int r, int ch) { return stage + r * 64 + ((ch ^ ((r >> 1) & 3)) << 4); };
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-            const int c0 = x.col0 + 16 * b;
-            if (c0 >= f.d) break;
+        for (int b = 0; b < 4; ++b) {                                  // 16 columns: through shared memory, so that rows leave in 64-byte pieces
+            const bool in_cols = x.col0 + 16 * b + cl < f.d;
+            float4 old[4];
+            if (o.adds) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    old[q] = in_cols && x.row0 + rl + 8 * q < o.rows ? *reinterpret_cast<const float4 *>(acc + 8LL * q * f.d + 16 * b) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
 #pragma unroll
             for (int ch = 0; ch < 4; ++ch) {
                 const float *s = &v[b >> 1][16 * (b & 1) + 4 * ch];
@@ -665,39 +638,70 @@ struct HlGradEpi {
             __syncwarp();
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                const int r = (lane >> 2) + 8 * q, ch = lane & 3, col = c0 + 4 * ch;
-                float4 val = *reinterpret_cast<const float4 *>(chunk_at(r, ch));
-                if (x.row0 + r < o.rows && col < f.d) {
-                    const long long at = (long long)(x.row0 + r) * f.d + col;
-                    if (o.adds) {
-                        const float4 old = *reinterpret_cast<const float4 *>(o.acc + at);
-                        val.x += old.x; val.y += old.y; val.z += old.z; val.w += old.w;
-                    }
-                    if (!o.last) {
-                        *reinterpret_cast<float4 *>(o.acc + at) = val;
-                    } else {
-                        val.x *= alpha; val.y *= alpha; val.z *= alpha; val.w *= alpha;
-                        if (f.out_f32) {
-                            *reinterpret_cast<float4 *>(static_cast<float *>(o.out) + at) = val;
-                        } else {
-                            __nv_bfloat162 h[2] = {__floats2bfloat162_rn(val.x, val.y), __floats2bfloat162_rn(val.z, val.w)};
-                            *reinterpret_cast<uint2 *>(static_cast<__nv_bfloat16 *>(o.out) + at) = *reinterpret_cast<uint2 *>(h);
-                        }
-                    }
+                float4 val = *reinterpret_cast<const float4 *>(chunk_at(rl + 8 * q, lane & 3));
+                if (in_cols && x.row0 + rl + 8 * q < o.rows) {
+                    if (o.adds) { val.x += old[q].x; val.y += old[q].y; val.z += old[q].z; val.w += old[q].w; }
+                    if (o.last && splits == 1) put(o, base + 8LL * q * f.d + 16 * b, val);
+                    else *reinterpret_cast<float4 *>(acc + 8LL * q * f.d + 16 * b) = val;
                 }
             }
             __syncwarp();
         }
-        return true;
+        if (!o.last || splits == 1) return;
+        __threadfence();
+        __syncwarp();
+        unsigned before = 0;
+        if (lane == 0) before = atomicAdd(f.tickets + ((x.g ? pr[0].tiles() : 0) + x.t) * 32 + x.block, 1u);
+        if (__shfl_sync(0xffffffffu, before, 0) != (unsigned)splits - 1) return;
+        __threadfence();
+#pragma unroll 1
+        for (int b = 0; b < 4; ++b) {
+            if (x.col0 + 16 * b + cl >= f.d) break;
+            float4 sum[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) sum[q] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
+            for (int sp = 0; sp < splits; ++sp)
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    if (x.row0 + rl + 8 * q < o.rows) {
+                        const float4 a = __ldcg(reinterpret_cast<const float4 *>(o.acc + sp * plane + base + 8LL * q * f.d + 16 * b));
+                        sum[q].x += a.x; sum[q].y += a.y; sum[q].z += a.z; sum[q].w += a.w;
+                    }
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (x.row0 + rl + 8 * q < o.rows) put(o, base + 8LL * q * f.d + 16 * b, sum[q]);
+        }
     }
 };
-struct HlPair { HlProduct p[2]; };
+// One launch of the backward pass: the gradients' products of one piece and ds of the next, which do not depend on one another.
+struct HlBwd { HlProb ds; HlGrads grads; };
+template <bool LIST, int TERMS>
+struct HlBwdEpi {
+    HlProbEpi<LIST, TERMS> ds;
+    HlGradEpi grad;
+    __device__ __forceinline__ void fetch(int g, int r) { if (g == 2) ds.fetch(r); }
+    __device__ __forceinline__ void begin(const HlTile &x) { if (x.g == 2) ds.begin(x); }
+    __device__ __forceinline__ bool tile(const HlTile &x, float (&v)[2][32], uint8_t *stage, uint8_t *, uint32_t) {
+        if (x.g == 2) {
+            ds.tile(x, v, stage);
+        } else {                                                       // all of them before a warp's first of ds: the staging is free
+            grad.tile(x, v, stage);
+            fence_proxy_async();
+        }
+        return true;
+    }
+    __device__ __forceinline__ void end(int lane) { if (lane == 0) tma_store_done(); }
+};
+template <bool LIST, int TERMS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(HL_NT, 1)
-head_loss_grad_kernel(const __grid_constant__ HlMaps maps, const __grid_constant__ HlPair pr, const __grid_constant__ HlGrads f) {
-    HlGradEpi epi{f, pr.p, 0.f};
-    if (threadIdx.x >= 64) { pdl_wait(); epi.alpha = hl_alpha(f.up, f.count, f.tau, f.reduction); }
-    hl_body<true>(maps, pr.p, epi);
+head_loss_bwd_kernel(const __grid_constant__ HlMaps maps, const __grid_constant__ HlTrio work, const __grid_constant__ HlBwd f) {
+    pdl_wait();
+    for (int i = blockIdx.x * HL_NT + threadIdx.x; i < f.ds.n_tickets; i += gridDim.x * HL_NT) f.ds.tickets[i] = 0u;
+    HlBwdEpi<LIST, TERMS> epi{{f.ds, &maps.ds}, {f.grads, work.p, hl_alpha(f.grads.up, f.grads.count, f.grads.tau, f.grads.reduction)}};
+    hl_body<HlThree>(maps, work, epi);
 }
+
 // x as three bf16 terms, [3][n]; eight values a thread (n a multiple of 8)
 __global__ void __launch_bounds__(256) head_split_kernel(const float *__restrict__ x, __nv_bfloat16 *__restrict__ out, long long n) {
     pdl_wait();
@@ -749,6 +753,13 @@ static int hl_launch(K kernel, int which, const char *name, const HlMaps &maps, 
 
 // an operand of the products: its first element, terms (1: the caller's bf16; 3: split), the elements between terms, rows' pitch
 struct HlOperand { const void *ptr; int terms; long long term_stride, ld; };
+// what warps store ds through: 32 x 32 blocks, 64-byte swizzle
+static bool hl_store_map(CUtensorMap *m, const HlOperand &o, long long rows, long long cols) {
+    const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)o.terms};
+    const cuuint64_t strides[2] = {(cuuint64_t)o.ld * 2, (cuuint64_t)(o.terms > 1 ? o.term_stride : rows * o.ld) * 2};
+    const cuuint32_t box[3] = {32, 32, 1};
+    return tc_encode_map(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, o.ptr, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE);
+}
 // rows x cols of it as K-major blocks of 128 x 64, or as 64 x 64 ones whose columns are M or N
 static bool hl_map(CUtensorMap *m, const HlOperand &o, long long row_from, long long col_from, long long rows, long long cols, bool mn) {
     const char *p = static_cast<const char *>(o.ptr) + 2 * (row_from * o.ld + col_from);
@@ -806,7 +817,6 @@ int head_loss_fwd_launch(const HeadLossArgs &x, float *row_loss, float *loss, fl
     if (rc != PGB_OK) return rc;
     HlMaps maps;
     if (!hl_map(&maps.a[0], h, 0, 0, x.N, x.d, false) || !hl_map(&maps.b[0], w, 0, 0, x.V, x.d, false)) return hl_no_map();
-    maps.a[1] = maps.a[0]; maps.b[1] = maps.b[0];
     HlProduct pr;
     pr.tiles_m = hl_tiles(x.N); pr.tiles_n = (int)pl.tiles; pr.kb = (x.d + HL_BK - 1) / HL_BK; pr.npairs = h.terms == 3 ? 6 : 1;
     const HlTargets t{x.target, x.ignore, x.ids, x.p, x.ent, x.k};
@@ -822,38 +832,121 @@ int head_loss_fwd_launch(const HeadLossArgs &x, float *row_loss, float *loss, fl
     return check_launch("head_loss_join_kernel");
 }
 
-// How the backward pass is cut: pieces of `step` rows (by_rows) or columns.
+// How the backward pass is cut: pieces of `step` rows (by_rows) or columns, and the parts of K of the two gradients' products.
 struct HlBwdPlan {
-    bool by_rows; long long step, pieces, ldp, rows, cols; int terms, pairs;   // pairs: that the products are shared out to at most
-    long long off_p, off_acc, off_parts, off_tickets, off_h, off_w, total;
+    bool by_rows; long long step, pieces, ldp, rows, cols; int terms, s_dh[2], s_dw[2];          // parts in all pieces but the last, in the last
+    long long off_p[2], off_dh, off_dw, off_tickets, n_tickets, off_h, off_w, total;
 };
-constexpr int HL_LEAST = 8;                                           // K blocks a pair takes at least: with fewer its parts cost more than its products
+// A launch's work in units of a K block's time: a part of a tile costs its K blocks and about four more (its epilogue's end and the next one's
+// beginning); one of several passes its fp32 sums through memory, once more where it is the last to finish.
+struct HlLoad {
+    long long n0, n, f0, r0, f, r; double c0, c1;                      // parts of the first product, of both; rounds and rest of either number over the pairs
+    HlLoad(long long t0, long long k0, int s0, long long t1, long long k1, int s1, int pairs) : n0(t0 * s0), n(t0 * s0 + t1 * s1), f0(n0 / pairs), r0(n0 % pairs),
+        f(n / pairs), r(n % pairs), c0((double)k0 / s0 + 4.0 + (s0 > 1 ? 2.0 + 0.5 * s0 : 0.0)), c1((double)k1 / s1 + 4.0 + (s1 > 1 ? 2.0 + 0.5 * s1 : 0.0)) {}
+    double of(long long p) const {                                     // pair p's long parts
+        const long long first = f0 + (p < r0), both = f + (p < r);
+        return first * c0 + (both - first) * c1;
+    }
+    double most() const {                                              // of the first pair, or of the first behind the last full round of either product
+        const double a = of(0), b = of(r0), c = of(r);
+        return a > b ? (a > c ? a : c) : (b > c ? b : c);
+    }
+    double all() const { return n0 * c0 + (n - n0) * c1; }
+};
+constexpr double HL_DS = 2.0;                                         // what a tile of ds costs beyond its K blocks
+struct HlSplits { int dh, dw; double cost; };
+// The parts of K with which the pairs finish earliest, `filler` units of short tiles dealt out behind them. fix0, fix1: parts that are given (0: to be chosen).
+static HlSplits hl_splits(long long t0, long long k0, long long t1, long long k1, double filler, int pairs, int fix0, int fix1) {
+    static const int choice[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 24, 32};
+    HlSplits best{1, 1, 1e300};
+    for (int a : choice) {
+        if (a > 1 && (fix0 || t0 == 0 || k0 / a < 4)) break;
+        for (int b : choice) {
+            if (b > 1 && (fix1 || t1 == 0 || k1 / b < 4)) break;
+            const int s0 = fix0 ? fix0 : a, s1 = fix1 ? fix1 : b;
+            const HlLoad load(t0, k0, s0, t1, k1, s1, pairs);
+            const double level = (load.all() + filler) / pairs, most = load.most(), cost = level > most ? level : most;
+            if (cost < best.cost) best = {s0, s1, cost};
+        }
+    }
+    return best;
+}
 static HlBwdPlan hl_bwd_plan(long long N, int V, int d, int dtype, bool dh, bool dw) {
     HlBwdPlan p;
     p.terms = dtype == PGB_F32 ? 3 : 1;
     p.by_rows = N >= V;
+    const int pairs = sm_count() / 2, np = p.terms == 3 ? 6 : 1;
     const long long most = HL_PIECE_BYTES / (2 * p.terms), across = hl_up(p.by_rows ? V : N, 64), along = p.by_rows ? N : V;
+    const long long td = hl_tiles(d), kd = (d + HL_BK - 1) / HL_BK * np, ta = hl_tiles(across), ka = (across + HL_BK - 1) / HL_BK * np;
+    const bool along_d = p.by_rows ? dh : dw, across_d = p.by_rows ? dw : dh;                    // the gradient that has a piece's rows, the one that gathers over pieces
+    // a launch with the products of n rows or columns and ds of the next m
+    auto of = [&](long long n, long long m, int gather) {
+        const long long t0 = along_d ? hl_tiles(n) * td : 0, t1 = across_d ? ta * td : 0, k1 = (n + HL_BK - 1) / HL_BK * np;
+        const double filler = (double)hl_tiles(m) * ta * (kd + HL_DS);
+        HlSplits s = p.by_rows ? hl_splits(t0, ka, t1, k1, filler, pairs, 0, gather) : hl_splits(t1, k1, t0, ka, filler, pairs, gather, 0);
+        s.cost += 20.0;                                                // a launch's beginning and end
+        return s;
+    };
     long long step = most / across / HL_B * HL_B;
     if (step < HL_B) step = HL_B;
-    p.pieces = (along + step - 1) / step;
-    p.step = hl_up((along + p.pieces - 1) / p.pieces, HL_B);
+    HlSplits best{1, 1, 1e300}, last{1, 1, 0.0};
+    if (step >= along) {
+        p.step = hl_up(along, HL_B);
+        best = last = of(along, 0, 0);
+    } else {
+        const long long stride = step / 32 / HL_B * HL_B + HL_B;       // sixteen steps or fewer are looked at
+        for (long long n = step; 2 * n > step; n -= stride) {          // the one whose launches take the least
+            const long long pieces = (along + n - 1) / n, rest = along - (pieces - 1) * n;
+            HlSplits s = of(n, n, 0);
+            const HlSplits r = of(rest, 0, p.by_rows ? s.dw : s.dh);   // the gathering gradient's sums go on in the same parts
+            s.cost = s.cost * (pieces - 1) + r.cost;
+            if (s.cost < best.cost) { best = s; last = r; p.step = n; }
+        }
+    }
     p.pieces = (along + p.step - 1) / p.step;
+    p.s_dh[0] = best.dh; p.s_dw[0] = best.dw; p.s_dh[1] = last.dh; p.s_dw[1] = last.dw;
     p.ldp = p.by_rows ? hl_up(V, 64) : p.step;
     p.rows = p.by_rows && p.step < N ? p.step : N;
     p.cols = !p.by_rows && p.step < V ? p.step : V;
-    const long long units = (long long)hl_tiles(d) * (p.terms == 3 ? 6 : 1) * (hl_tiles(p.rows) * hl_up(p.cols, HL_BK) + hl_tiles(p.cols) * hl_up(p.rows, HL_BK)) / HL_BK;
-    p.pairs = sm_count() / 2;
-    if (units / HL_LEAST < p.pairs) p.pairs = units / HL_LEAST < 1 ? 1 : (int)(units / HL_LEAST);
     long long at = 0;
     auto take = [&](long long bytes) { const long long o = at; at += hl_up(bytes, 256); return o; };
-    p.off_p = take(2 * p.terms * p.rows * p.ldp);
-    p.off_acc = p.pieces > 1 && (p.by_rows ? dw : dh) ? take(4 * (p.by_rows ? (long long)V : N) * d) : -1;   // of the gradient that gathers over pieces
-    p.off_parts = take((long long)p.pairs * 2 * 32 * 2048 * 4);
-    p.off_tickets = take(4LL * 32 * ((long long)hl_tiles(p.rows) + hl_tiles(p.cols)) * hl_tiles(d));
+    p.off_p[0] = take(2 * p.terms * p.rows * p.ldp);
+    p.off_p[1] = p.pieces > 1 ? take(2 * p.terms * p.rows * p.ldp) : p.off_p[0];
+    // fp32 sums: of the gradient that gathers over pieces, and of one whose K axis is in parts
+    const int sh = p.s_dh[0] > p.s_dh[1] ? p.s_dh[0] : p.s_dh[1], sw = p.s_dw[0] > p.s_dw[1] ? p.s_dw[0] : p.s_dw[1];
+    p.off_dh = dh && (sh > 1 || (!p.by_rows && p.pieces > 1)) ? take(4LL * sh * p.rows * d) : -1;
+    p.off_dw = dw && (sw > 1 || (p.by_rows && p.pieces > 1)) ? take(4LL * sw * p.cols * d) : -1;
+    p.n_tickets = 32 * ((long long)hl_tiles(p.rows) + hl_tiles(p.cols)) * hl_tiles(d);
+    p.off_tickets = take(2 * 4 * p.n_tickets);
     p.off_h = dtype == PGB_F32 ? take(6 * N * d) : 0;
     p.off_w = dtype == PGB_F32 ? take(6LL * V * d) : 0;
     p.total = at;
     return p;
+}
+// pair q's tiles of ds: as many as bring it to the level that all of them reach
+static void hl_share(HlTrio &w, int pairs) {
+    const HlProduct &a = w.p[0], &b = w.p[1];
+    const int tiles = w.p[2].tiles();
+    const HlLoad load(a.tiles(), a.kt(), a.splits, b.tiles(), b.kt(), b.splits, pairs);
+    const double c = w.p[2].kt() + HL_DS;
+    double level = (load.all() + tiles * c) / pairs;
+    for (int round = 0; round < 4 && load.n > 0 && tiles > 0; ++round) {                         // pairs above the level have none and raise it for the others
+        double over = 0.0;
+        int below = 0;
+        for (int q = 0; q < pairs; ++q) {
+            const double l = load.of(q);
+            if (l >= level) over += l; else ++below;
+        }
+        if (below == 0 || below == pairs) break;
+        level = (load.all() + tiles * c - over) / below;
+    }
+    double due = 0.0;
+    for (int q = 0; q < pairs; ++q) {
+        w.share[q] = (int)due < tiles ? (int)due : tiles;
+        const double l = load.of(q);
+        if (l < level) due += (level - l) / c;
+    }
+    w.share[pairs] = tiles;
 }
 long long head_loss_bwd_bytes(long long N, int V, int d, int dtype, int want_dh, int want_dw) {
     return hl_bwd_plan(N, V, d, dtype, want_dh != 0, want_dw != 0).total;
@@ -867,48 +960,61 @@ int head_loss_bwd_launch(const HeadLossArgs &x, const float *L, const float *cou
     if (rc == PGB_OK) rc = hl_operand(w, x.W, x.dtype, x.V, x.d, s + pl.off_w, stream);
     if (rc != PGB_OK) return rc;
     const int np = pl.terms == 3 ? 6 : 1, esize = x.dtype == PGB_F32 ? 4 : 2;
-    const HlOperand P{s + pl.off_p, pl.terms, pl.rows * pl.ldp, pl.ldp};
+    const int which = (pl.terms == 3) * 2 + list;
+    const int room = which == 0 ? hl_pairs(head_loss_bwd_kernel<false, 1>, 2) : which == 1 ? hl_pairs(head_loss_bwd_kernel<true, 1>, 3)
+                   : which == 2 ? hl_pairs(head_loss_bwd_kernel<false, 3>, 4) : hl_pairs(head_loss_bwd_kernel<true, 3>, 5);
+    if (room < 1) { set_cuda_error(cudaGetLastError(), "head_loss_bwd_kernel"); return PGB_ERR_CUDA; }
     unsigned *tickets = reinterpret_cast<unsigned *>(s + pl.off_tickets);
-    HlProb f{{x.target, x.ignore, x.ids, x.p, x.ent, x.k}, reinterpret_cast<const float2 *>(L), x.reduction == 0 ? up : nullptr, LOG2E_F / x.tau,
-             reinterpret_cast<__nv_bfloat16 *>(s + pl.off_p), pl.ldp, pl.rows * pl.ldp, 0, x.V, 0, 0, 0, tickets, 0};
-    HlGrads o{{}, up, count, x.tau, x.reduction, x.d, x.dtype == PGB_F32, reinterpret_cast<float *>(s + pl.off_parts), tickets};
-    float *acc = pl.off_acc >= 0 ? reinterpret_cast<float *>(s + pl.off_acc) : nullptr;
-    for (long long i = 0; i < pl.pieces; ++i) {
-        const long long from = i * pl.step, row_from = pl.by_rows ? from : 0, col_from = pl.by_rows ? 0 : from;
-        const long long rows = pl.by_rows ? (from + pl.step < x.N ? pl.step : x.N - from) : x.N;
-        const long long cols = pl.by_rows ? x.V : (from + pl.step < x.V ? pl.step : x.V - from);
-        const bool first = i == 0, last = i + 1 == pl.pieces;
+    auto at = [&](long long off) { return off >= 0 ? reinterpret_cast<float *>(s + off) : nullptr; };
+    auto piece = [&](int i) { return HlOperand{s + pl.off_p[i & 1], pl.terms, pl.rows * pl.ldp, pl.ldp}; };
+    HlBwd f{};
+    f.ds.t = {x.target, x.ignore, x.ids, x.p, x.ent, x.k};
+    f.ds.L = reinterpret_cast<const float2 *>(L); f.ds.row_weight = x.reduction == 0 ? up : nullptr; f.ds.a = LOG2E_F / x.tau; f.ds.V = x.V;
+    f.grads.up = up; f.grads.count = count; f.grads.tau = x.tau; f.grads.reduction = x.reduction; f.grads.d = x.d; f.grads.out_f32 = x.dtype == PGB_F32;
+    // launch i: the products of piece i - 1, ds of piece i
+    for (long long i = 0; i <= pl.pieces; ++i) {
         HlMaps maps;
-        if (!hl_map(&maps.a[0], h, row_from, 0, rows, x.d, false) || !hl_map(&maps.b[0], w, col_from, 0, cols, x.d, false)) return hl_no_map();
-        maps.a[1] = maps.a[0]; maps.b[1] = maps.b[0];
-        HlPair two;
-        if (dh) {                                                     // dh[rows] += P W[cols]
-            HlProduct &q = two.p[0];
-            q.tiles_m = hl_tiles(rows); q.tiles_n = hl_tiles(x.d); q.kb = (int)((cols + HL_BK - 1) / HL_BK); q.npairs = np; q.b_mn = 1;
-            const bool gathers = !pl.by_rows && pl.pieces > 1;
-            o.g[0] = {acc, static_cast<char *>(dh) + row_from * x.d * esize, rows, gathers && !first, !gathers || last};
+        HlTrio work{};
+        auto rows_of = [&](long long j) { return pl.by_rows && (j + 1) * pl.step > x.N ? x.N - j * pl.step : pl.rows; };
+        auto cols_of = [&](long long j) { return !pl.by_rows && (j + 1) * pl.step > x.V ? x.V - j * pl.step : pl.cols; };
+        bool mapped = true;
+        if (i < pl.pieces) {
+            const long long rows = rows_of(i), cols = cols_of(i), row_from = pl.by_rows ? i * pl.step : 0, col_from = pl.by_rows ? 0 : i * pl.step;
+            mapped = hl_map(&maps.a[2], h, row_from, 0, rows, x.d, false) && hl_map(&maps.b[2], w, col_from, 0, cols, x.d, false) && hl_store_map(&maps.ds, piece(i), rows, cols);
+            HlProduct &q = work.p[2];
+            q.tiles_m = hl_tiles(rows); q.tiles_n = hl_tiles(cols); q.kb = (x.d + HL_BK - 1) / HL_BK; q.npairs = np;
+            f.ds.row_from = row_from; f.ds.rows = (int)rows; f.ds.col_from = (int)col_from; f.ds.cols = (int)cols;
+            f.ds.tickets = tickets + (i & 1) * pl.n_tickets; f.ds.n_tickets = (int)pl.n_tickets;
+        } else {
+            f.ds.n_tickets = 0;
         }
-        if (dw) {                                                     // dW[cols] += P^T h[rows]
-            HlProduct &q = two.p[1];
-            q.tiles_m = hl_tiles(cols); q.tiles_n = hl_tiles(x.d); q.kb = (int)((rows + HL_BK - 1) / HL_BK); q.npairs = np; q.a_mn = 1; q.b_mn = 1;
-            const bool gathers = pl.by_rows && pl.pieces > 1;
-            o.g[1] = {acc, static_cast<char *>(dw) + col_from * x.d * esize, cols, gathers && !first, !gathers || last};
+        if (i > 0) {
+            const long long j = i - 1, rows = rows_of(j), cols = cols_of(j), row_from = pl.by_rows ? j * pl.step : 0, col_from = pl.by_rows ? 0 : j * pl.step;
+            const bool first = j == 0, last = i == pl.pieces;
+            f.grads.tickets = tickets + (j & 1) * pl.n_tickets;
+            if (dh) {                                                  // dh[rows] += ds W[cols]
+                mapped = mapped && hl_map(&maps.a[0], piece(j), 0, 0, rows, cols, false) && hl_map(&maps.b[0], w, col_from, 0, cols, x.d, true);
+                HlProduct &q = work.p[0];
+                q.tiles_m = hl_tiles(rows); q.tiles_n = hl_tiles(x.d); q.kb = (int)((cols + HL_BK - 1) / HL_BK); q.npairs = np; q.splits = pl.s_dh[last]; q.b_mn = 1;
+                const bool gathers = !pl.by_rows && pl.pieces > 1;
+                f.grads.g[0] = {at(pl.off_dh), static_cast<char *>(dh) + row_from * x.d * esize, rows, gathers && !first, !gathers || last};
+            }
+            if (dw) {                                                  // dW[cols] += ds^T h[rows]
+                mapped = mapped && hl_map(&maps.a[1], piece(j), 0, 0, rows, cols, true) && hl_map(&maps.b[1], h, row_from, 0, rows, x.d, true);
+                HlProduct &q = work.p[1];
+                q.tiles_m = hl_tiles(cols); q.tiles_n = hl_tiles(x.d); q.kb = (int)((rows + HL_BK - 1) / HL_BK); q.npairs = np; q.splits = pl.s_dw[last]; q.a_mn = 1; q.b_mn = 1;
+                const bool gathers = pl.by_rows && pl.pieces > 1;
+                f.grads.g[1] = {at(pl.off_dw), static_cast<char *>(dw) + col_from * x.d * esize, cols, gathers && !first, !gathers || last};
+            }
         }
-        HlProduct pr;
-        pr.tiles_m = hl_tiles(rows); pr.tiles_n = hl_tiles(cols); pr.kb = (x.d + HL_BK - 1) / HL_BK; pr.npairs = np;
-        f.row_from = row_from; f.rows = (int)rows; f.col_from = (int)col_from; f.cols = (int)cols; f.n_tickets = 32 * (two.p[0].tiles() + two.p[1].tiles());
-        if (pl.terms == 3)
-            rc = list ? hl_launch(head_loss_ds_kernel<true, 3>, 2, "head_loss_ds_kernel", maps, pr, pr.tiles(), f, stream)
-                      : hl_launch(head_loss_ds_kernel<false, 3>, 3, "head_loss_ds_kernel", maps, pr, pr.tiles(), f, stream);
-        else
-            rc = list ? hl_launch(head_loss_ds_kernel<true, 1>, 4, "head_loss_ds_kernel", maps, pr, pr.tiles(), f, stream)
-                      : hl_launch(head_loss_ds_kernel<false, 1>, 5, "head_loss_ds_kernel", maps, pr, pr.tiles(), f, stream);
-        if (rc != PGB_OK) return rc;
-        if (dh && (!hl_map(&maps.a[0], P, 0, 0, rows, cols, false) || !hl_map(&maps.b[0], w, col_from, 0, cols, x.d, true))) return hl_no_map();
-        if (dw && (!hl_map(&maps.a[1], P, 0, 0, rows, cols, true) || !hl_map(&maps.b[1], h, row_from, 0, rows, x.d, true))) return hl_no_map();
-        long long pairs = HlShare<true>::units(two.p) / HL_LEAST;
-        pairs = pairs < 1 ? 1 : pairs < pl.pairs ? pairs : pl.pairs;
-        rc = hl_launch(head_loss_grad_kernel, 6, "head_loss_grad_kernel", maps, two, pairs, o, stream);
+        if (!mapped) return hl_no_map();
+        const long long parts = (long long)work.p[0].tiles() * work.p[0].splits + (long long)work.p[1].tiles() * work.p[1].splits + work.p[2].tiles();
+        const int pairs = (int)(parts < room ? parts : room < HL_MOST_PAIRS ? room : HL_MOST_PAIRS);
+        hl_share(work, pairs);
+        rc = which == 0 ? hl_launch(head_loss_bwd_kernel<false, 1>, 2, "head_loss_bwd_kernel", maps, work, pairs, f, stream)
+           : which == 1 ? hl_launch(head_loss_bwd_kernel<true, 1>, 3, "head_loss_bwd_kernel", maps, work, pairs, f, stream)
+           : which == 2 ? hl_launch(head_loss_bwd_kernel<false, 3>, 4, "head_loss_bwd_kernel", maps, work, pairs, f, stream)
+                        : hl_launch(head_loss_bwd_kernel<true, 3>, 5, "head_loss_bwd_kernel", maps, work, pairs, f, stream);
         if (rc != PGB_OK) return rc;
     }
     return PGB_OK;
