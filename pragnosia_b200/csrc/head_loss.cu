@@ -27,7 +27,7 @@ constexpr int HL_CW = HL_B / (HL_EPI / 4);                            // columns
 constexpr int HL_OUT_BYTES = 32 * 64;                                 // staging of an epilogue warp: 32 rows of 64 bytes
 constexpr int HL_SMEM = HL_STAGES * HL_STAGE + 1024 + HL_EPI * HL_OUT_BYTES + 1024;
 constexpr int HL_GROUP = 16;                                          // row blocks that a sweep over the columns takes together
-constexpr long long HL_PIECE_BYTES = 96LL << 20;                      // of ds in the workspace at once: what stays in the 126 MB L2
+constexpr long long HL_PIECE_BYTES = 64LL << 20;                      // of ds, two such pieces in the workspace: one written, one read
 static_assert(HL_STAGE % 1024 == 0 && HL_SMEM <= 232448, "shared memory");
 constexpr float LOG2E_F = 1.4426950408889634f;
 
@@ -208,11 +208,12 @@ __device__ __forceinline__ void hl_body(const HlMaps &maps, const What &what, Ep
         const int row_in = (int)rank * (HL_B / 2) + 32 * sub, col_in = part * HL_CW;
         HlTile x;
         x.lane = lane; x.sub = sub; x.part = part; x.block = (int)rank * HL_EPI + (warp - 2);
+        epi.start(tid - 64);
         uint32_t ti = 0;
         bool ok = w.more();
         if (ok) {
             w.product().at(w.t, m, n);
-            epi.fetch(w.g, m * HL_B + row_in + lane);
+            epi.fetch(w.g, m * HL_B + row_in + lane, n * HL_B + col_in);
         }
         for (; ok; ++ti) {
             const uint32_t a = ti & 1;
@@ -240,7 +241,7 @@ __device__ __forceinline__ void hl_body(const HlMaps &maps, const What &what, Ep
             const bool more = w.more();
             if (more) {
                 w.product().at(w.t, m, n);
-                epi.fetch(w.g, m * HL_B + row_in + lane);
+                epi.fetch(w.g, m * HL_B + row_in + lane, n * HL_B + col_in);
             }
             ok = epi.tile(x, v, stage, shared, bar_quarters(sub, ti & 3)) && more;
         }
@@ -264,37 +265,40 @@ __device__ __forceinline__ float pick32(const float (&v)[32], int i) {
     return a[0];
 }
 
-// What a row's target distribution is read from: a word per row (target), or a list of k (ids ascending, INT_MAX behind the last entry;
-// p their probabilities; ent the sum of p log p, NaN where an id was out of range).
+// What a row's target distribution is read from: a word per row (target), or a teacher's entries: lists [N][k] of (id, probability's bits), ids
+// ascending, INT_MAX behind the last; starts [blocks of 64 words][N], the place of the first entry at or behind the block's first word times 256
+// plus its column, 255 where it is not in the block; ent, the sum of p log p, inf for a row without an entry, NaN for one with an id out of range.
 struct HlTargets {
-    const long long *target; long long ignore; const int *ids; const float *p, *ent; int k;
+    const long long *target; long long ignore; const int2 *lists; const unsigned *starts; const float *ent; int k; long long N;
 };
 
-// A lane's walk over its row's targets: nx is the column of the one to come (INT_MAX: none), in ascending order.
+// A lane's walk over its row's targets within its 64 columns: nx is the column of the one to come (INT_MAX: none), in ascending order, p what it
+// holds. The entry behind it is loaded ahead.
 template <bool LIST>
 struct HlWalk {
     int nx = 0x7fffffff, pos = 0, k = 0;
-    const int *ids = nullptr; const float *p = nullptr;
-    // the targets from column `from` (of the whole vocabulary) on; word: the row's target; row < 0: none
-    __device__ __forceinline__ void begin(const HlTargets &t, long long row, long long word, int from) {
+    float p = 1.f;
+    int2 ahead;
+    const int2 *list = nullptr;
+    // the targets from column `from` (of the whole vocabulary) on; where: the row's target, or its entry in starts; row < 0: none
+    __device__ __forceinline__ void begin(const HlTargets &t, long long row, long long where, int from) {
         nx = 0x7fffffff;
         if (row < 0) return;
         if constexpr (LIST) {
-            k = t.k; ids = t.ids + row * k; p = t.p + row * k;
-            int lo = 0, hi = k;
-            while (lo < hi) {
-                const int mid = (lo + hi) >> 1;
-                if (ids[mid] < from) lo = mid + 1; else hi = mid;
-            }
-            pos = lo;
-            if (pos < k) nx = ids[pos];
+            const unsigned col = (unsigned)where & 255u;
+            if (col == 255u) return;
+            k = t.k; list = t.lists + row * k; pos = (int)((unsigned)where >> 8);
+            nx = from + (int)col;
+            p = __int_as_float(list[pos].y);
+            look();
         } else {
-            if (word != t.ignore && word >= from && word < 0x7fffffff) nx = (int)word;
+            if (where != t.ignore && where >= from && where < 0x7fffffff) nx = (int)where;
         }
     }
-    __device__ __forceinline__ float weight() const { return LIST ? p[pos] : 1.0f; }
+    __device__ __forceinline__ void look() { ahead = pos + 1 < k ? list[pos + 1] : make_int2(0x7fffffff, 0); }
     __device__ __forceinline__ void advance() {
-        if constexpr (LIST) { ++pos; nx = pos < k ? ids[pos] : 0x7fffffff; } else nx = 0x7fffffff;
+        nx = 0x7fffffff;
+        if constexpr (LIST) { ++pos; nx = ahead.x; p = __int_as_float(ahead.y); if (nx != 0x7fffffff) look(); }
     }
 };
 
@@ -309,13 +313,14 @@ template <bool LIST>
 struct HlFwdEpi {
     const HlFwd &f;
     HlWalk<LIST> w;
-    long long row, word;                                               // of the tile fetched for
+    long long row, where;                                              // of the tile fetched for
+    __device__ __forceinline__ void start(int i) { if (i == 0 && blockIdx.x == 0) *f.ticket = 0u; }
     __device__ __forceinline__ void end(int) {}
-    __device__ __forceinline__ void fetch(int, int r) {
-        row = r < f.N ? r : -1;
-        if (!LIST) word = row >= 0 ? f.t.target[row] : f.t.ignore;
+    __device__ __forceinline__ void fetch(int, int r, int c) {
+        row = r < f.N && c < f.V ? r : -1;
+        if (row >= 0) where = LIST ? f.t.starts[(c >> 6) * f.t.N + row] : f.t.target[row];
     }
-    __device__ __forceinline__ void begin(const HlTile &x) { w.begin(f.t, row, word, x.col0); }
+    __device__ __forceinline__ void begin(const HlTile &x) { w.begin(f.t, row, where, x.col0); }
     __device__ __forceinline__ bool tile(const HlTile &x, float (&v)[2][32], uint8_t *, uint8_t *shared, uint32_t quarters) {
         float m = -INFINITY, l = 0.f, dot = 0.f;
         const int row = x.row0 + x.lane;
@@ -326,7 +331,7 @@ struct HlFwdEpi {
             while (__any_sync(0xffffffffu, w.nx < c0 + 32)) {          // this block holds a target of some row
                 const bool hit = w.nx < c0 + 32;
                 const float s = pick32(v[b], hit ? w.nx - c0 : 0);
-                if (hit) { dot = fmaf(w.weight(), s, dot); w.advance(); if (!LIST) f.dot[row] = s; }
+                if (hit) { dot = fmaf(w.p, s, dot); w.advance(); if (!LIST) f.dot[row] = s; }
             }
             if (c0 + 32 > f.V) {
 #pragma unroll
@@ -373,7 +378,6 @@ struct HlFwdEpi {
 template <bool LIST>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(HL_NT, 1)
 head_loss_fwd_kernel(const __grid_constant__ HlMaps maps, const __grid_constant__ HlProduct pr, const __grid_constant__ HlFwd f) {
-    if (blockIdx.x == 0 && threadIdx.x == 0) { pdl_wait(); *f.ticket = 0u; }
     HlFwdEpi<LIST> epi{f, {}, 0, 0};
     hl_body<HlOne>(maps, pr, epi);
 }
@@ -422,7 +426,7 @@ __global__ void __launch_bounds__(256) head_loss_join_kernel(const HlJoin j) {
         j.L[row] = make_float2(hi, (float)(L - hi));
         if (LIST) {
             const float ent = j.t.ent[row];
-            live = j.t.ids[row * j.t.k] != 0x7fffffff || ent != ent;
+            live = ent != INFINITY;
             loss = (double)j.tau * j.tau * (ent + L * 0.693147180559945309) - j.tau * d;
         } else {
             const long long w = j.t.target[row];
@@ -468,8 +472,8 @@ __global__ void __launch_bounds__(256) head_loss_join_kernel(const HlJoin j) {
 // ------------------------------------------------------------------------------------------------ a teacher's lists
 // A warp per row: probabilities of the entries that are there (id >= 0, logit not -inf) at the temperature, in ascending order of their
 // ids (a rank per entry: k comparisons each).
-__global__ void __launch_bounds__(128) head_teacher_kernel(const long long *__restrict__ in_ids, const float *__restrict__ in_logits, int *__restrict__ ids,
-                                                           float *__restrict__ p, float *__restrict__ ent, long long N, int V, int k, float inv_tau) {
+__global__ void __launch_bounds__(128) head_teacher_kernel(const long long *__restrict__ in_ids, const float *__restrict__ in_logits, int2 *__restrict__ lists,
+                                                           float *__restrict__ ent, long long N, int V, int k, float inv_tau) {
     extern __shared__ int teacher_smem[];
     pdl_wait();
     pdl_launch_dependents();
@@ -494,9 +498,11 @@ __global__ void __launch_bounds__(128) head_teacher_kernel(const long long *__re
     bad = __any_sync(0xffffffffu, bad);
     __syncwarp();
     float sum = 0.f;
+    bool any = false;
     for (int j = lane; j < k; j += 32)
-        if (id[j] != 0x7fffffff) sum += expf(z[j] - top);
+        if (id[j] != 0x7fffffff) { sum += expf(z[j] - top); any = true; }
     sum = warp_sum(sum);
+    any = __any_sync(0xffffffffu, any);
     float e = 0.f;
     for (int j = lane; j < k; j += 32) {
         const int me = id[j];
@@ -505,11 +511,30 @@ __global__ void __launch_bounds__(128) head_teacher_kernel(const long long *__re
         if (here && !(q <= 0.f)) e += q * ((z[j] - top) - logf(sum));  // NaN stays
         int rank = 0;
         for (int i = 0; i < k; ++i) rank += id[i] < me || (id[i] == me && i < j);
-        ids[row * k + rank] = me;
-        p[row * k + rank] = q;
+        lists[row * k + rank] = make_int2(me, __float_as_int(q));
     }
     e = warp_sum(e);
-    if (lane == 0) ent[row] = bad ? NAN : e;
+    if (lane == 0) ent[row] = bad ? NAN : any ? e : INFINITY;
+}
+// starts, a warp per 32 rows (a lane each) and HL_BLOCKS blocks of 64 words: where its first block begins by bisection, then along the list
+constexpr int HL_BLOCKS = 32;
+__global__ void __launch_bounds__(128) head_starts_kernel(const int2 *__restrict__ lists, unsigned *__restrict__ starts, long long N, int blocks, int k) {
+    pdl_wait();
+    pdl_launch_dependents();
+    const long long row = (long long)blockIdx.x * 128 + threadIdx.x;
+    if (row >= N) return;
+    const int2 *list = lists + row * k;
+    const int b0 = blockIdx.y * HL_BLOCKS, b1 = min(b0 + HL_BLOCKS, blocks);
+    int lo = 0, hi = k;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (list[mid].x < 64 * b0) lo = mid + 1; else hi = mid;
+    }
+    int id = lo < k ? list[lo].x : 0x7fffffff;
+    for (int b = b0; b < b1; ++b) {
+        while (id < 64 * b) { ++lo; id = lo < k ? list[lo].x : 0x7fffffff; }
+        starts[(long long)b * N + row] = ((unsigned)lo << 8) | (id < 64 * b + 64 ? (unsigned)(id - 64 * b) : 255u);
+    }
 }
 
 // ------------------------------------------------------------------------------------------------ backward
@@ -524,20 +549,20 @@ struct HlProbEpi {
     const HlProb &f;
     const CUtensorMap *map;
     HlWalk<LIST> w;
-    long long row, word; float2 L; float weight, ent; int id0;         // of the tile fetched for
+    long long row, where, word; float2 L; float weight, ent;           // of the tile fetched for
     float a_hi, a_lo, c; bool live;                                   // of the tile at hand
-    __device__ __forceinline__ void fetch(int r) {
-        row = r < f.rows ? f.row_from + r : -1;
+    __device__ __forceinline__ void fetch(int r, int c) {
+        row = r < f.rows && c < f.cols ? f.row_from + r : -1;
         if (row < 0) return;
         L = f.L[row];
         weight = f.row_weight ? f.row_weight[row] : 1.f;
-        if (LIST) { ent = f.t.ent[row]; id0 = f.t.ids[row * f.t.k]; } else word = f.t.target[row];
+        if (LIST) { ent = f.t.ent[row]; where = f.t.starts[((f.col_from + c) >> 6) * f.t.N + row]; } else word = where = f.t.target[row];
     }
     __device__ __forceinline__ void begin(const HlTile &x) {
-        w.begin(f.t, row, word, f.col_from + x.col0);
+        w.begin(f.t, row, where, f.col_from + x.col0);
         a_hi = -L.x; a_lo = -L.y;
         const bool bad = LIST ? ent != ent : word != f.t.ignore && (word < 0 || word >= f.V);
-        live = row >= 0 && (LIST ? bad || id0 != 0x7fffffff : word != f.t.ignore);
+        live = row >= 0 && (LIST ? ent != INFINITY : word != f.t.ignore);
         c = bad ? NAN : weight;
     }
     // Rounded, the block goes out by two TMA stores a term, 32 columns each, from the warp's staging: 64-byte rows, their 16-byte chunks swapped
@@ -555,7 +580,7 @@ struct HlProbEpi {
             while (__any_sync(0xffffffffu, w.nx < v0 + 32)) {
                 const bool hit = w.nx < v0 + 32;
                 const int at = hit ? w.nx - v0 : -1;
-                const float less = hit ? w.weight() : 0.f;
+                const float less = hit ? w.p : 0.f;
 #pragma unroll
                 for (int i = 0; i < 32; ++i) v[i] -= i == at ? less : 0.f;
                 if (hit) w.advance();
@@ -621,11 +646,12 @@ struct HlGradEpi {
         const long long plane = o.rows * f.d, base = (long long)(x.row0 + rl) * f.d + x.col0 + cl;
         float *acc = o.acc ? o.acc + x.sp * plane + base : nullptr;
         auto chunk_at = [&](int r, int ch) { return stage + r * 64 + ((ch ^ ((r >> 1) & 3)) << 4); };
+        const bool direct = o.last && splits == 1;
 #pragma unroll
         for (int b = 0; b < 4; ++b) {                                  // 16 columns: through shared memory, so that rows leave in 64-byte pieces
             const bool in_cols = x.col0 + 16 * b + cl < f.d;
             float4 old[4];
-            if (o.adds) {
+            if (direct && o.adds) {
 #pragma unroll
                 for (int q = 0; q < 4; ++q)
                     old[q] = in_cols && x.row0 + rl + 8 * q < o.rows ? *reinterpret_cast<const float4 *>(acc + 8LL * q * f.d + 16 * b) : make_float4(0.f, 0.f, 0.f, 0.f);
@@ -640,9 +666,15 @@ struct HlGradEpi {
             for (int q = 0; q < 4; ++q) {
                 float4 val = *reinterpret_cast<const float4 *>(chunk_at(rl + 8 * q, lane & 3));
                 if (in_cols && x.row0 + rl + 8 * q < o.rows) {
-                    if (o.adds) { val.x += old[q].x; val.y += old[q].y; val.z += old[q].z; val.w += old[q].w; }
-                    if (o.last && splits == 1) put(o, base + 8LL * q * f.d + 16 * b, val);
-                    else *reinterpret_cast<float4 *>(acc + 8LL * q * f.d + 16 * b) = val;
+                    float *to = acc + 8LL * q * f.d + 16 * b;
+                    if (direct) {
+                        if (o.adds) { val.x += old[q].x; val.y += old[q].y; val.z += old[q].z; val.w += old[q].w; }
+                        put(o, base + 8LL * q * f.d + 16 * b, val);
+                    } else if (o.adds) {                               // nobody else adds to it in this launch, so the order is that of the pieces
+                        asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(to), "f"(val.x), "f"(val.y), "f"(val.z), "f"(val.w) : "memory");
+                    } else {
+                        *reinterpret_cast<float4 *>(to) = val;
+                    }
                 }
             }
             __syncwarp();
@@ -660,14 +692,19 @@ struct HlGradEpi {
             float4 sum[4];
 #pragma unroll
             for (int q = 0; q < 4; ++q) sum[q] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 2
-            for (int sp = 0; sp < splits; ++sp)
+            for (int sp0 = 0; sp0 < splits; sp0 += 2) {
+                float4 a[2][4];                                        // eight loads on their way
 #pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    if (x.row0 + rl + 8 * q < o.rows) {
-                        const float4 a = __ldcg(reinterpret_cast<const float4 *>(o.acc + sp * plane + base + 8LL * q * f.d + 16 * b));
-                        sum[q].x += a.x; sum[q].y += a.y; sum[q].z += a.z; sum[q].w += a.w;
-                    }
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        a[j][q] = sp0 + j < splits && x.row0 + rl + 8 * q < o.rows
+                                      ? __ldcg(reinterpret_cast<const float4 *>(o.acc + (sp0 + j) * plane + base + 8LL * q * f.d + 16 * b)) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) { sum[q].x += a[j][q].x; sum[q].y += a[j][q].y; sum[q].z += a[j][q].z; sum[q].w += a[j][q].w; }
+            }
 #pragma unroll
             for (int q = 0; q < 4; ++q)
                 if (x.row0 + rl + 8 * q < o.rows) put(o, base + 8LL * q * f.d + 16 * b, sum[q]);
@@ -680,7 +717,11 @@ template <bool LIST, int TERMS>
 struct HlBwdEpi {
     HlProbEpi<LIST, TERMS> ds;
     HlGradEpi grad;
-    __device__ __forceinline__ void fetch(int g, int r) { if (g == 2) ds.fetch(r); }
+    __device__ __forceinline__ void start(int i) {
+        for (i += blockIdx.x * HL_EPI * 32; i < ds.f.n_tickets; i += gridDim.x * HL_EPI * 32) ds.f.tickets[i] = 0u;
+        grad.alpha = hl_alpha(grad.f.up, grad.f.count, grad.f.tau, grad.f.reduction);
+    }
+    __device__ __forceinline__ void fetch(int g, int r, int c) { if (g == 2) ds.fetch(r, c); }
     __device__ __forceinline__ void begin(const HlTile &x) { if (x.g == 2) ds.begin(x); }
     __device__ __forceinline__ bool tile(const HlTile &x, float (&v)[2][32], uint8_t *stage, uint8_t *, uint32_t) {
         if (x.g == 2) {
@@ -696,9 +737,7 @@ struct HlBwdEpi {
 template <bool LIST, int TERMS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(HL_NT, 1)
 head_loss_bwd_kernel(const __grid_constant__ HlMaps maps, const __grid_constant__ HlTrio work, const __grid_constant__ HlBwd f) {
-    pdl_wait();
-    for (int i = blockIdx.x * HL_NT + threadIdx.x; i < f.ds.n_tickets; i += gridDim.x * HL_NT) f.ds.tickets[i] = 0u;
-    HlBwdEpi<LIST, TERMS> epi{{f.ds, &maps.ds}, {f.grads, work.p, hl_alpha(f.grads.up, f.grads.count, f.grads.tau, f.grads.reduction)}};
+    HlBwdEpi<LIST, TERMS> epi{{f.ds, &maps.ds}, {f.grads, work.p, 0.f}};
     hl_body<HlThree>(maps, work, epi);
 }
 
@@ -799,16 +838,20 @@ static int hl_operand(HlOperand &o, const void *x, int dtype, long long rows, in
 }
 static int hl_no_map() { set_cuda_error(cudaErrorUnknown, "cuTensorMapEncodeTiled"); return PGB_ERR_CUDA; }
 
-int head_teacher_launch(const long long *in_ids, const float *in_logits, int *ids, float *p, float *ent, long long N, int V, int k, float tau,
+int head_teacher_launch(const long long *in_ids, const float *in_logits, int *lists, unsigned *starts, float *ent, long long N, int V, int k, float tau,
                         cudaStream_t stream) {
-    cudaError_t e = pdl_launch(head_teacher_kernel, dim3((unsigned)((N + 3) / 4)), dim3(128), (size_t)(4 * k * 8), stream, in_ids, in_logits, ids, p, ent, N, V,
-                               k, 1.0f / tau);
+    cudaError_t e = pdl_launch(head_teacher_kernel, dim3((unsigned)((N + 3) / 4)), dim3(128), (size_t)(4 * k * 8), stream, in_ids, in_logits,
+                               reinterpret_cast<int2 *>(lists), ent, N, V, k, 1.0f / tau);
+    const int blocks = (V + 63) / 64;
+    if (e == cudaSuccess)
+        e = pdl_launch(head_starts_kernel, dim3((unsigned)((N + 127) / 128), (unsigned)((blocks + HL_BLOCKS - 1) / HL_BLOCKS)), dim3(128), 0, stream,
+                       reinterpret_cast<const int2 *>(lists), starts, N, blocks, k);
     if (e != cudaSuccess) { set_cuda_error(e, "head_teacher launch"); return PGB_ERR_CUDA; }
     return check_launch("head_teacher_kernel");
 }
 
 int head_loss_fwd_launch(const HeadLossArgs &x, float *row_loss, float *loss, float *count, float *L, void *scratch, cudaStream_t stream) {
-    const bool list = x.ids != nullptr;
+    const bool list = x.lists != nullptr;
     const HlFwdPlan pl = hl_fwd_plan(x.N, x.V, x.d, x.dtype, list);
     char *s = static_cast<char *>(scratch);
     HlOperand h, w;
@@ -819,7 +862,7 @@ int head_loss_fwd_launch(const HeadLossArgs &x, float *row_loss, float *loss, fl
     if (!hl_map(&maps.a[0], h, 0, 0, x.N, x.d, false) || !hl_map(&maps.b[0], w, 0, 0, x.V, x.d, false)) return hl_no_map();
     HlProduct pr;
     pr.tiles_m = hl_tiles(x.N); pr.tiles_n = (int)pl.tiles; pr.kb = (x.d + HL_BK - 1) / HL_BK; pr.npairs = h.terms == 3 ? 6 : 1;
-    const HlTargets t{x.target, x.ignore, x.ids, x.p, x.ent, x.k};
+    const HlTargets t{x.target, x.ignore, reinterpret_cast<const int2 *>(x.lists), x.starts, x.ent, x.k, x.N};
     const HlFwd f{t, LOG2E_F / x.tau, reinterpret_cast<float2 *>(s + pl.off_ml), reinterpret_cast<float *>(s + pl.off_dot),
                   reinterpret_cast<unsigned *>(s + pl.off_ticket), x.N, pl.Np, x.V};
     rc = list ? hl_launch(head_loss_fwd_kernel<true>, 0, "head_loss_fwd_kernel", maps, pr, pr.tiles(), f, stream)
@@ -853,7 +896,7 @@ struct HlLoad {
     }
     double all() const { return n0 * c0 + (n - n0) * c1; }
 };
-constexpr double HL_DS = 2.0;                                         // what a tile of ds costs beyond its K blocks
+constexpr double HL_DS = 5.0;                                         // what a tile of ds costs beyond its K blocks
 struct HlSplits { int dh, dw; double cost; };
 // The parts of K with which the pairs finish earliest, `filler` units of short tiles dealt out behind them. fix0, fix1: parts that are given (0: to be chosen).
 static HlSplits hl_splits(long long t0, long long k0, long long t1, long long k1, double filler, int pairs, int fix0, int fix1) {
@@ -952,7 +995,7 @@ long long head_loss_bwd_bytes(long long N, int V, int d, int dtype, int want_dh,
     return hl_bwd_plan(N, V, d, dtype, want_dh != 0, want_dw != 0).total;
 }
 int head_loss_bwd_launch(const HeadLossArgs &x, const float *L, const float *count, const float *up, void *dh, void *dw, void *scratch, cudaStream_t stream) {
-    const bool list = x.ids != nullptr;
+    const bool list = x.lists != nullptr;
     const HlBwdPlan pl = hl_bwd_plan(x.N, x.V, x.d, x.dtype, dh != nullptr, dw != nullptr);
     char *s = static_cast<char *>(scratch);
     HlOperand h, w;
@@ -968,7 +1011,7 @@ int head_loss_bwd_launch(const HeadLossArgs &x, const float *L, const float *cou
     auto at = [&](long long off) { return off >= 0 ? reinterpret_cast<float *>(s + off) : nullptr; };
     auto piece = [&](int i) { return HlOperand{s + pl.off_p[i & 1], pl.terms, pl.rows * pl.ldp, pl.ldp}; };
     HlBwd f{};
-    f.ds.t = {x.target, x.ignore, x.ids, x.p, x.ent, x.k};
+    f.ds.t = {x.target, x.ignore, reinterpret_cast<const int2 *>(x.lists), x.starts, x.ent, x.k, x.N};
     f.ds.L = reinterpret_cast<const float2 *>(L); f.ds.row_weight = x.reduction == 0 ? up : nullptr; f.ds.a = LOG2E_F / x.tau; f.ds.V = x.V;
     f.grads.up = up; f.grads.count = count; f.grads.tau = x.tau; f.grads.reduction = x.reduction; f.grads.d = x.d; f.grads.out_f32 = x.dtype == PGB_F32;
     // launch i: the products of piece i - 1, ds of piece i
