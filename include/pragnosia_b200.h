@@ -542,7 +542,7 @@ int pgb_linear_act(const void *x, const void *W, const void *bias, void *y, long
  * Cross entropy: rows whose target is ignore_index lose 0 and have no gradient (h must be finite there all the same if dW is
  * wanted); any other target outside 0 .. V-1 gives NaN, as loss and as gradients of its row and of W.
  * Distillation: pgb_teacher_lists makes of a teacher's k entries per row (ids in any order; an entry with id < 0 or logit -inf is
- * absent) what the losses read: lists [N][k][2] (id, bits of its probability p at the temperature; by id), starts [ceil(V / 64)][N] (where the entries
+ * absent) what the losses read: lists [N][k][2] (id, bits of its probability p at the temperature; by id), starts [N][ceil(V / 64)] (where the entries
  * of every 64 words begin) and ent [N], the sum of p log p. lists 8-byte aligned. A row's loss is
  * temperature^2 KL(p || softmax(s / temperature)), 0 without gradient for rows without an entry; the same id twice counts twice; an id >= V gives NaN.
  * N, V up to 2^30, d up to 65536, k 1 .. 1024. Bounded waits as in the prefill kernels (pgb_tc_error_flag: 91-95). The same call gives

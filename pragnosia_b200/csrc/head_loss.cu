@@ -266,19 +266,19 @@ __device__ __forceinline__ float pick32(const float (&v)[32], int i) {
 }
 
 // What a row's target distribution is read from: a word per row (target), or a teacher's entries: lists [N][k] of (id, probability's bits), ids
-// ascending, INT_MAX behind the last; starts [blocks of 64 words][N], the place of the first entry at or behind the block's first word times 256
+// ascending, INT_MAX behind the last; starts [N][blocks of 64 words], the place of the first entry at or behind the block's first word times 256
 // plus its column, 255 where it is not in the block; ent, the sum of p log p, inf for a row without an entry, NaN for one with an id out of range.
 struct HlTargets {
-    const long long *target; long long ignore; const int2 *lists; const unsigned *starts; const float *ent; int k; long long N;
+    const long long *target; long long ignore; const int2 *lists; const unsigned *starts; const float *ent; int k, blocks;
 };
 
 // A lane's walk over its row's targets within its 64 columns: nx is the column of the one to come (INT_MAX: none), in ascending order, p what it
-// holds. The entry behind it is loaded ahead.
+// holds. The two entries behind it are loaded ahead.
 template <bool LIST>
 struct HlWalk {
     int nx = 0x7fffffff, pos = 0, k = 0;
     float p = 1.f;
-    int2 ahead;
+    int2 a1, a2;
     const int2 *list = nullptr;
     // the targets from column `from` (of the whole vocabulary) on; where: the row's target, or its entry in starts; row < 0: none
     __device__ __forceinline__ void begin(const HlTargets &t, long long row, long long where, int from) {
@@ -290,15 +290,16 @@ struct HlWalk {
             k = t.k; list = t.lists + row * k; pos = (int)((unsigned)where >> 8);
             nx = from + (int)col;
             p = __int_as_float(list[pos].y);
-            look();
+            a1 = entry(pos + 1);
+            a2 = entry(pos + 2);
         } else {
             if (where != t.ignore && where >= from && where < 0x7fffffff) nx = (int)where;
         }
     }
-    __device__ __forceinline__ void look() { ahead = pos + 1 < k ? list[pos + 1] : make_int2(0x7fffffff, 0); }
+    __device__ __forceinline__ int2 entry(int i) const { return i < k ? list[i] : make_int2(0x7fffffff, 0); }
     __device__ __forceinline__ void advance() {
         nx = 0x7fffffff;
-        if constexpr (LIST) { ++pos; nx = ahead.x; p = __int_as_float(ahead.y); if (nx != 0x7fffffff) look(); }
+        if constexpr (LIST) { nx = a1.x; p = __int_as_float(a1.y); a1 = a2; a2 = entry(++pos + 2); }
     }
 };
 
@@ -318,7 +319,7 @@ struct HlFwdEpi {
     __device__ __forceinline__ void end(int) {}
     __device__ __forceinline__ void fetch(int, int r, int c) {
         row = r < f.N && c < f.V ? r : -1;
-        if (row >= 0) where = LIST ? f.t.starts[(c >> 6) * f.t.N + row] : f.t.target[row];
+        if (row >= 0) where = LIST ? f.t.starts[row * f.t.blocks + (c >> 6)] : f.t.target[row];
     }
     __device__ __forceinline__ void begin(const HlTile &x) { w.begin(f.t, row, where, x.col0); }
     __device__ __forceinline__ bool tile(const HlTile &x, float (&v)[2][32], uint8_t *, uint8_t *shared, uint32_t quarters) {
@@ -413,17 +414,18 @@ __global__ void __launch_bounds__(256) head_loss_join_kernel(const HlJoin j) {
     double loss = 0.0;
     bool live = false;
     if (warp == 0 && row < j.N) {
-        double sum = l, d = dot;
+#pragma unroll
         for (int q = 1; q < 8; ++q) {
             const float3 o = part[q][lane];
             const float top = fmaxf(m, o.x), at = top == -INFINITY ? 0.f : top;
-            sum = sum * exp2((double)m - at) + o.y * exp2((double)o.x - at);
+            l = l * fast_exp2(m - at) + o.y * fast_exp2(o.x - at);
             m = top;
-            d += o.z;
+            dot += o.z;
         }
-        const double L = (double)m + log2(sum);
-        const float hi = (float)L;
-        j.L[row] = make_float2(hi, (float)(L - hi));
+        const float lg = log2f(l), hi = m + lg;                        // hi + lo = m + lg, exactly
+        const float back = hi - m, rest = (m - (hi - back)) + (lg - back), lo = rest == rest ? rest : 0.f;
+        const double L = (double)hi + lo, d = dot;
+        j.L[row] = make_float2(hi, lo);
         if (LIST) {
             const float ent = j.t.ent[row];
             live = ent != INFINITY;
@@ -471,69 +473,65 @@ __global__ void __launch_bounds__(256) head_loss_join_kernel(const HlJoin j) {
 
 // ------------------------------------------------------------------------------------------------ a teacher's lists
 // A warp per row: probabilities of the entries that are there (id >= 0, logit not -inf) at the temperature, in ascending order of their
-// ids (a rank per entry: k comparisons each).
+// ids (a rank per entry: k comparisons each), and where the entries of every 64 words begin (a bisection per block).
 __global__ void __launch_bounds__(128) head_teacher_kernel(const long long *__restrict__ in_ids, const float *__restrict__ in_logits, int2 *__restrict__ lists,
-                                                           float *__restrict__ ent, long long N, int V, int k, float inv_tau) {
-    extern __shared__ int teacher_smem[];
+                                                           unsigned *__restrict__ starts, float *__restrict__ ent, long long N, int V, int k, float inv_tau) {
+    extern __shared__ __align__(16) long long teacher_smem[];
     pdl_wait();
     pdl_launch_dependents();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, kk = (k + 1) & ~1;
     const long long row = (long long)blockIdx.x * 4 + warp;
     if (row >= N) return;
-    int *id = teacher_smem + 2 * k * warp;
-    float *z = reinterpret_cast<float *>(id + k);
+    long long *key = teacher_smem + kk * warp;                         // id times 1024 plus place: none twice; absent ones behind all others
+    int *sorted = reinterpret_cast<int *>(teacher_smem + 4 * kk) + kk * warp;
+    constexpr long long ABSENT = 0x7fffffffLL << 10;
     float top = -INFINITY;
     bool bad = false;
-    for (int j = lane; j < k; j += 32) {
-        const long long i = in_ids[row * k + j];
-        const float x = in_logits[row * k + j] * inv_tau;
-        const bool here = i >= 0 && x != -INFINITY;
-        bad |= here && i >= V;
-        id[j] = here ? (i >= V ? V : (int)i) : 0x7fffffff;
-        z[j] = here ? x : -INFINITY;
-        if (here) top = fmaxf(top, x);
+    int here = 0;
+    for (int j = lane; j < kk; j += 32) {
+        const long long i = j < k ? in_ids[row * k + j] : -1;
+        const float x = j < k ? in_logits[row * k + j] * inv_tau : -INFINITY;
+        const bool is = i >= 0 && x != -INFINITY;
+        bad |= is && i >= V;
+        key[j] = is ? (i >= V ? V : i) << 10 | j : ABSENT | j;
+        if (is) { top = fmaxf(top, x); ++here; }
     }
+    for (int j = lane; j < k; j += 32) sorted[j] = 0x7fffffff;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    for (int o = 16; o > 0; o >>= 1) { top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o)); here += __shfl_xor_sync(0xffffffffu, here, o); }
     bad = __any_sync(0xffffffffu, bad);
     __syncwarp();
     float sum = 0.f;
-    bool any = false;
     for (int j = lane; j < k; j += 32)
-        if (id[j] != 0x7fffffff) { sum += expf(z[j] - top); any = true; }
+        if (key[j] < ABSENT) sum += expf(in_logits[row * k + j] * inv_tau - top);
     sum = warp_sum(sum);
-    any = __any_sync(0xffffffffu, any);
     float e = 0.f;
     for (int j = lane; j < k; j += 32) {
-        const int me = id[j];
-        const bool here = me != 0x7fffffff;
-        const float q = here ? expf(z[j] - top) / sum : 0.f;
-        if (here && !(q <= 0.f)) e += q * ((z[j] - top) - logf(sum));  // NaN stays
+        const long long me = key[j];
+        if (me >= ABSENT) continue;
+        const float z = in_logits[row * k + j] * inv_tau - top, q = expf(z) / sum;
+        if (!(q <= 0.f)) e += q * (z - logf(sum));                     // NaN stays
         int rank = 0;
-        for (int i = 0; i < k; ++i) rank += id[i] < me || (id[i] == me && i < j);
-        lists[row * k + rank] = make_int2(me, __float_as_int(q));
+        for (int i = 0; i < kk; i += 2) {
+            const longlong2 o = *reinterpret_cast<const longlong2 *>(key + i);
+            rank += (o.x < me) + (o.y < me);
+        }
+        sorted[rank] = (int)(me >> 10);
+        lists[row * k + rank] = make_int2((int)(me >> 10), __float_as_int(q));
     }
+    for (int j = here + lane; j < k; j += 32) lists[row * k + j] = make_int2(0x7fffffff, 0);
     e = warp_sum(e);
-    if (lane == 0) ent[row] = bad ? NAN : any ? e : INFINITY;
-}
-// starts, a warp per 32 rows (a lane each) and HL_BLOCKS blocks of 64 words: where its first block begins by bisection, then along the list
-constexpr int HL_BLOCKS = 32;
-__global__ void __launch_bounds__(128) head_starts_kernel(const int2 *__restrict__ lists, unsigned *__restrict__ starts, long long N, int blocks, int k) {
-    pdl_wait();
-    pdl_launch_dependents();
-    const long long row = (long long)blockIdx.x * 128 + threadIdx.x;
-    if (row >= N) return;
-    const int2 *list = lists + row * k;
-    const int b0 = blockIdx.y * HL_BLOCKS, b1 = min(b0 + HL_BLOCKS, blocks);
-    int lo = 0, hi = k;
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (list[mid].x < 64 * b0) lo = mid + 1; else hi = mid;
-    }
-    int id = lo < k ? list[lo].x : 0x7fffffff;
-    for (int b = b0; b < b1; ++b) {
-        while (id < 64 * b) { ++lo; id = lo < k ? list[lo].x : 0x7fffffff; }
-        starts[(long long)b * N + row] = ((unsigned)lo << 8) | (id < 64 * b + 64 ? (unsigned)(id - 64 * b) : 255u);
+    if (lane == 0) ent[row] = bad ? NAN : here > 0 ? e : INFINITY;
+    __syncwarp();
+    const int blocks = (V + 63) / 64;
+    for (int b = lane; b < blocks; b += 32) {
+        int lo = 0, hi = here;
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (sorted[mid] < 64 * b) lo = mid + 1; else hi = mid;
+        }
+        const int id = lo < here ? sorted[lo] : 0x7fffffff;
+        starts[row * blocks + b] = ((unsigned)lo << 8) | (id - 64 * b < 64 ? (unsigned)(id - 64 * b) : 255u);
     }
 }
 
@@ -542,7 +540,6 @@ struct HlProb {
     HlTargets t; const float2 *L; const float *row_weight;            // row_weight NULL: 1
     float a;
     long long row_from; int V, col_from, cols, rows;                  // the piece: rows and columns it begins at, how many
-    unsigned *tickets; int n_tickets;                                 // set to zero for the products behind
 };
 template <bool LIST, int TERMS>
 struct HlProbEpi {
@@ -556,7 +553,7 @@ struct HlProbEpi {
         if (row < 0) return;
         L = f.L[row];
         weight = f.row_weight ? f.row_weight[row] : 1.f;
-        if (LIST) { ent = f.t.ent[row]; where = f.t.starts[((f.col_from + c) >> 6) * f.t.N + row]; } else word = where = f.t.target[row];
+        if (LIST) { ent = f.t.ent[row]; where = f.t.starts[row * f.t.blocks + ((f.col_from + c) >> 6)]; } else word = where = f.t.target[row];
     }
     __device__ __forceinline__ void begin(const HlTile &x) {
         w.begin(f.t, row, where, f.col_from + x.col0);
@@ -577,13 +574,15 @@ struct HlProbEpi {
             float (&v)[32] = vv[b];
 #pragma unroll
             for (int i = 0; i < 32; ++i) v[i] = TERMS == 3 ? fast_exp2(fmaf(v[i], f.a, a_hi) + a_lo) : fast_exp2(fmaf(v[i], f.a, a_hi));
-            while (__any_sync(0xffffffffu, w.nx < v0 + 32)) {
-                const bool hit = w.nx < v0 + 32;
-                const int at = hit ? w.nx - v0 : -1;
-                const float less = hit ? w.p : 0.f;
+            if constexpr (TERMS == 3) {                                // before the values are taken apart
+                while (__any_sync(0xffffffffu, w.nx < v0 + 32)) {
+                    const bool hit = w.nx < v0 + 32;
+                    const int at = hit ? w.nx - v0 : -1;
+                    const float less = hit ? w.p : 0.f;
 #pragma unroll
-                for (int i = 0; i < 32; ++i) v[i] -= i == at ? less : 0.f;
-                if (hit) w.advance();
+                    for (int i = 0; i < 32; ++i) v[i] -= i == at ? less : 0.f;
+                    if (hit) w.advance();
+                }
             }
             if (!plain) {
 #pragma unroll
@@ -606,6 +605,18 @@ struct HlProbEpi {
                     }
                     *reinterpret_cast<uint4 *>(stage + lane * 64 + ((ch ^ ((lane >> 1) & 3)) << 4)) = *reinterpret_cast<uint4 *>(o);
                 }
+                if constexpr (TERMS == 1) {                            // the few columns that hold a target, over what was staged for them
+                    while (__any_sync(0xffffffffu, w.nx < v0 + 32)) {
+                        const int at = w.nx - v0;
+                        const float q = pick32(v, at & 31);
+                        if (at < 32) {
+                            float less = w.p;
+                            for (w.advance(); LIST && w.nx - v0 == at; w.advance()) less += w.p;
+                            const __nv_bfloat16 x = __float2bfloat16_rn(live ? fmaf(-c, less, q) : 0.f);
+                            *reinterpret_cast<__nv_bfloat16 *>(stage + lane * 64 + (((at >> 3) ^ ((lane >> 1) & 3)) << 4) + 2 * (at & 7)) = x;
+                        }
+                    }
+                }
                 fence_proxy_async();
                 __syncwarp();
                 if (lane == 0 && x.row0 < f.rows) tma_store_3d(map, smem_u32(stage), c0, x.row0, term);
@@ -621,11 +632,10 @@ __device__ __forceinline__ float hl_alpha(const float *g, const float *count, fl
     const float n = *count;
     return n > 0.f ? tau * *g / n : 0.f;                              // no row counts: no gradient (the loss itself is 0 / 0)
 }
-// What becomes of a product's tiles: out = alpha * (acc +) C, or acc (+)= C where further pieces follow or the other parts of K are to
-// come. acc [splits][rows][d] fp32. A tile in parts is summed by whoever finishes it last (each of its 32 blocks by itself), in the order of
-// K and from memory all of it, so the sum does not depend on who that is.
+// What becomes of a product's tiles: out = alpha * (acc +) C, or acc (+)= C where further pieces follow or the other parts of K have sums of
+// their own, which a kernel behind this one adds up. acc [splits][rows][d] fp32.
 struct HlGrad { float *acc; void *out; long long rows; int adds, last; };
-struct HlGrads { HlGrad g[2]; const float *up, *count; float tau; int reduction, d, out_f32; unsigned *tickets; };
+struct HlGrads { HlGrad g[2]; const float *up, *count; float tau; int reduction, d, out_f32; };
 struct HlGradEpi {
     const HlGrads &f;
     const HlProduct *pr;
@@ -642,7 +652,7 @@ struct HlGradEpi {
     __device__ __forceinline__ void tile(const HlTile &x, float (&v)[2][32], uint8_t *stage) {
         const HlGrad &o = f.g[x.g];
         const int lane = x.lane, splits = pr[x.g].splits, rl = lane >> 2, cl = 4 * (lane & 3);
-        if (x.col0 >= f.d || x.row0 >= o.rows) return;           // nothing of the matrix in this block; nobody draws its ticket
+        if (x.col0 >= f.d || x.row0 >= o.rows) return;
         const long long plane = o.rows * f.d, base = (long long)(x.row0 + rl) * f.d + x.col0 + cl;
         float *acc = o.acc ? o.acc + x.sp * plane + base : nullptr;
         auto chunk_at = [&](int r, int ch) { return stage + r * 64 + ((ch ^ ((r >> 1) & 3)) << 4); };
@@ -679,46 +689,37 @@ struct HlGradEpi {
             }
             __syncwarp();
         }
-        if (!o.last || splits == 1) return;
-        __threadfence();
-        __syncwarp();
-        unsigned before = 0;
-        if (lane == 0) before = atomicAdd(f.tickets + ((x.g ? pr[0].tiles() : 0) + x.t) * 32 + x.block, 1u);
-        if (__shfl_sync(0xffffffffu, before, 0) != (unsigned)splits - 1) return;
-        __threadfence();
-#pragma unroll 1
-        for (int b = 0; b < 4; ++b) {
-            if (x.col0 + 16 * b + cl >= f.d) break;
-            float4 sum[4];
-#pragma unroll
-            for (int q = 0; q < 4; ++q) sum[q] = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int sp0 = 0; sp0 < splits; sp0 += 2) {
-                float4 a[2][4];                                        // eight loads on their way
-#pragma unroll
-                for (int j = 0; j < 2; ++j)
-#pragma unroll
-                    for (int q = 0; q < 4; ++q)
-                        a[j][q] = sp0 + j < splits && x.row0 + rl + 8 * q < o.rows
-                                      ? __ldcg(reinterpret_cast<const float4 *>(o.acc + (sp0 + j) * plane + base + 8LL * q * f.d + 16 * b)) : make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-                for (int j = 0; j < 2; ++j)
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) { sum[q].x += a[j][q].x; sum[q].y += a[j][q].y; sum[q].z += a[j][q].z; sum[q].w += a[j][q].w; }
-            }
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-                if (x.row0 + rl + 8 * q < o.rows) put(o, base + 8LL * q * f.d + 16 * b, sum[q]);
-        }
     }
 };
+// out = alpha * the sum over the parts of K, in their order; four columns a thread
+__global__ void __launch_bounds__(256) head_loss_sum_kernel(const float *__restrict__ acc, void *__restrict__ out, long long n, int splits, const float *up,
+                                                            const float *count, float tau, int reduction, int out_f32) {
+    pdl_wait();
+    pdl_launch_dependents();
+    const float alpha = hl_alpha(up, count, tau, reduction);
+    for (long long i = 4 * ((long long)blockIdx.x * 256 + threadIdx.x); i < n; i += 1024LL * gridDim.x) {
+        float4 s = *reinterpret_cast<const float4 *>(acc + i);
+#pragma unroll 8
+        for (int q = 1; q < splits; ++q) {
+            const float4 o = *reinterpret_cast<const float4 *>(acc + q * n + i);
+            s.x += o.x; s.y += o.y; s.z += o.z; s.w += o.w;
+        }
+        s.x *= alpha; s.y *= alpha; s.z *= alpha; s.w *= alpha;
+        if (out_f32) {
+            *reinterpret_cast<float4 *>(static_cast<float *>(out) + i) = s;
+        } else {
+            __nv_bfloat162 h[2] = {__floats2bfloat162_rn(s.x, s.y), __floats2bfloat162_rn(s.z, s.w)};
+            *reinterpret_cast<uint2 *>(static_cast<__nv_bfloat16 *>(out) + i) = *reinterpret_cast<uint2 *>(h);
+        }
+    }
+}
 // One launch of the backward pass: the gradients' products of one piece and ds of the next, which do not depend on one another.
 struct HlBwd { HlProb ds; HlGrads grads; };
 template <bool LIST, int TERMS>
 struct HlBwdEpi {
     HlProbEpi<LIST, TERMS> ds;
     HlGradEpi grad;
-    __device__ __forceinline__ void start(int i) {
-        for (i += blockIdx.x * HL_EPI * 32; i < ds.f.n_tickets; i += gridDim.x * HL_EPI * 32) ds.f.tickets[i] = 0u;
+    __device__ __forceinline__ void start(int) {
         grad.alpha = hl_alpha(grad.f.up, grad.f.count, grad.f.tau, grad.f.reduction);
     }
     __device__ __forceinline__ void fetch(int g, int r, int c) { if (g == 2) ds.fetch(r, c); }
@@ -840,12 +841,8 @@ static int hl_no_map() { set_cuda_error(cudaErrorUnknown, "cuTensorMapEncodeTile
 
 int head_teacher_launch(const long long *in_ids, const float *in_logits, int *lists, unsigned *starts, float *ent, long long N, int V, int k, float tau,
                         cudaStream_t stream) {
-    cudaError_t e = pdl_launch(head_teacher_kernel, dim3((unsigned)((N + 3) / 4)), dim3(128), (size_t)(4 * k * 8), stream, in_ids, in_logits,
-                               reinterpret_cast<int2 *>(lists), ent, N, V, k, 1.0f / tau);
-    const int blocks = (V + 63) / 64;
-    if (e == cudaSuccess)
-        e = pdl_launch(head_starts_kernel, dim3((unsigned)((N + 127) / 128), (unsigned)((blocks + HL_BLOCKS - 1) / HL_BLOCKS)), dim3(128), 0, stream,
-                       reinterpret_cast<const int2 *>(lists), starts, N, blocks, k);
+    cudaError_t e = pdl_launch(head_teacher_kernel, dim3((unsigned)((N + 3) / 4)), dim3(128), (size_t)(4 * ((k + 1) & ~1) * 12), stream, in_ids, in_logits,
+                               reinterpret_cast<int2 *>(lists), starts, ent, N, V, k, 1.0f / tau);
     if (e != cudaSuccess) { set_cuda_error(e, "head_teacher launch"); return PGB_ERR_CUDA; }
     return check_launch("head_teacher_kernel");
 }
@@ -862,7 +859,7 @@ int head_loss_fwd_launch(const HeadLossArgs &x, float *row_loss, float *loss, fl
     if (!hl_map(&maps.a[0], h, 0, 0, x.N, x.d, false) || !hl_map(&maps.b[0], w, 0, 0, x.V, x.d, false)) return hl_no_map();
     HlProduct pr;
     pr.tiles_m = hl_tiles(x.N); pr.tiles_n = (int)pl.tiles; pr.kb = (x.d + HL_BK - 1) / HL_BK; pr.npairs = h.terms == 3 ? 6 : 1;
-    const HlTargets t{x.target, x.ignore, reinterpret_cast<const int2 *>(x.lists), x.starts, x.ent, x.k, x.N};
+    const HlTargets t{x.target, x.ignore, reinterpret_cast<const int2 *>(x.lists), x.starts, x.ent, x.k, (x.V + 63) / 64};
     const HlFwd f{t, LOG2E_F / x.tau, reinterpret_cast<float2 *>(s + pl.off_ml), reinterpret_cast<float *>(s + pl.off_dot),
                   reinterpret_cast<unsigned *>(s + pl.off_ticket), x.N, pl.Np, x.V};
     rc = list ? hl_launch(head_loss_fwd_kernel<true>, 0, "head_loss_fwd_kernel", maps, pr, pr.tiles(), f, stream)
@@ -878,14 +875,14 @@ int head_loss_fwd_launch(const HeadLossArgs &x, float *row_loss, float *loss, fl
 // How the backward pass is cut: pieces of `step` rows (by_rows) or columns, and the parts of K of the two gradients' products.
 struct HlBwdPlan {
     bool by_rows; long long step, pieces, ldp, rows, cols; int terms, s_dh[2], s_dw[2];          // parts in all pieces but the last, in the last
-    long long off_p[2], off_dh, off_dw, off_tickets, n_tickets, off_h, off_w, total;
+    long long off_p[2], off_dh, off_dw, off_h, off_w, total;
 };
-// A launch's work in units of a K block's time: a part of a tile costs its K blocks and about four more (its epilogue's end and the next one's
-// beginning); one of several passes its fp32 sums through memory, once more where it is the last to finish.
+// A launch's work in units of a K block's time (0.33 us): a part of a tile costs its K blocks and about four more (its epilogue's end and the
+// next one's beginning).
 struct HlLoad {
     long long n0, n, f0, r0, f, r; double c0, c1;                      // parts of the first product, of both; rounds and rest of either number over the pairs
     HlLoad(long long t0, long long k0, int s0, long long t1, long long k1, int s1, int pairs) : n0(t0 * s0), n(t0 * s0 + t1 * s1), f0(n0 / pairs), r0(n0 % pairs),
-        f(n / pairs), r(n % pairs), c0((double)k0 / s0 + 4.0 + (s0 > 1 ? 2.0 + 0.5 * s0 : 0.0)), c1((double)k1 / s1 + 4.0 + (s1 > 1 ? 2.0 + 0.5 * s1 : 0.0)) {}
+        f(n / pairs), r(n % pairs), c0((double)k0 / s0 + 4.0), c1((double)k1 / s1 + 4.0) {}
     double of(long long p) const {                                     // pair p's long parts
         const long long first = f0 + (p < r0), both = f + (p < r);
         return first * c0 + (both - first) * c1;
@@ -908,7 +905,9 @@ static HlSplits hl_splits(long long t0, long long k0, long long t1, long long k1
             if (b > 1 && (fix1 || t1 == 0 || k1 / b < 4)) break;
             const int s0 = fix0 ? fix0 : a, s1 = fix1 ? fix1 : b;
             const HlLoad load(t0, k0, s0, t1, k1, s1, pairs);
-            const double level = (load.all() + filler) / pairs, most = load.most(), cost = level > most ? level : most;
+            const double level = (load.all() + filler) / pairs, most = load.most();
+            // the kernel that adds up the parts' sums: 10 and what it reads, 256 KiB a tile and part
+            const double cost = (level > most ? level : most) + (s0 > 1 ? 10.0 + 0.15 * t0 * s0 : 0.0) + (s1 > 1 ? 10.0 + 0.15 * t1 * s1 : 0.0);
             if (cost < best.cost) best = {s0, s1, cost};
         }
     }
@@ -959,8 +958,6 @@ static HlBwdPlan hl_bwd_plan(long long N, int V, int d, int dtype, bool dh, bool
     const int sh = p.s_dh[0] > p.s_dh[1] ? p.s_dh[0] : p.s_dh[1], sw = p.s_dw[0] > p.s_dw[1] ? p.s_dw[0] : p.s_dw[1];
     p.off_dh = dh && (sh > 1 || (!p.by_rows && p.pieces > 1)) ? take(4LL * sh * p.rows * d) : -1;
     p.off_dw = dw && (sw > 1 || (p.by_rows && p.pieces > 1)) ? take(4LL * sw * p.cols * d) : -1;
-    p.n_tickets = 32 * ((long long)hl_tiles(p.rows) + hl_tiles(p.cols)) * hl_tiles(d);
-    p.off_tickets = take(2 * 4 * p.n_tickets);
     p.off_h = dtype == PGB_F32 ? take(6 * N * d) : 0;
     p.off_w = dtype == PGB_F32 ? take(6LL * V * d) : 0;
     p.total = at;
@@ -994,6 +991,13 @@ static void hl_share(HlTrio &w, int pairs) {
 long long head_loss_bwd_bytes(long long N, int V, int d, int dtype, int want_dh, int want_dw) {
     return hl_bwd_plan(N, V, d, dtype, want_dh != 0, want_dw != 0).total;
 }
+static int hl_sum(const float *acc, void *out, long long n, int splits, const HlGrads &f, cudaStream_t stream) {
+    const long long blocks = (n / 4 + 255) / 256;
+    cudaError_t e = pdl_launch(head_loss_sum_kernel, dim3((unsigned)(blocks < 2368 ? blocks : 2368)), dim3(256), 0, stream, acc, out, n, splits, f.up, f.count, f.tau,
+                               f.reduction, f.out_f32);
+    if (e != cudaSuccess) { set_cuda_error(e, "head_loss_sum launch"); return PGB_ERR_CUDA; }
+    return check_launch("head_loss_sum_kernel");
+}
 int head_loss_bwd_launch(const HeadLossArgs &x, const float *L, const float *count, const float *up, void *dh, void *dw, void *scratch, cudaStream_t stream) {
     const bool list = x.lists != nullptr;
     const HlBwdPlan pl = hl_bwd_plan(x.N, x.V, x.d, x.dtype, dh != nullptr, dw != nullptr);
@@ -1007,11 +1011,10 @@ int head_loss_bwd_launch(const HeadLossArgs &x, const float *L, const float *cou
     const int room = which == 0 ? hl_pairs(head_loss_bwd_kernel<false, 1>, 2) : which == 1 ? hl_pairs(head_loss_bwd_kernel<true, 1>, 3)
                    : which == 2 ? hl_pairs(head_loss_bwd_kernel<false, 3>, 4) : hl_pairs(head_loss_bwd_kernel<true, 3>, 5);
     if (room < 1) { set_cuda_error(cudaGetLastError(), "head_loss_bwd_kernel"); return PGB_ERR_CUDA; }
-    unsigned *tickets = reinterpret_cast<unsigned *>(s + pl.off_tickets);
     auto at = [&](long long off) { return off >= 0 ? reinterpret_cast<float *>(s + off) : nullptr; };
     auto piece = [&](int i) { return HlOperand{s + pl.off_p[i & 1], pl.terms, pl.rows * pl.ldp, pl.ldp}; };
     HlBwd f{};
-    f.ds.t = {x.target, x.ignore, reinterpret_cast<const int2 *>(x.lists), x.starts, x.ent, x.k, x.N};
+    f.ds.t = {x.target, x.ignore, reinterpret_cast<const int2 *>(x.lists), x.starts, x.ent, x.k, (x.V + 63) / 64};
     f.ds.L = reinterpret_cast<const float2 *>(L); f.ds.row_weight = x.reduction == 0 ? up : nullptr; f.ds.a = LOG2E_F / x.tau; f.ds.V = x.V;
     f.grads.up = up; f.grads.count = count; f.grads.tau = x.tau; f.grads.reduction = x.reduction; f.grads.d = x.d; f.grads.out_f32 = x.dtype == PGB_F32;
     // launch i: the products of piece i - 1, ds of piece i
@@ -1027,14 +1030,10 @@ int head_loss_bwd_launch(const HeadLossArgs &x, const float *L, const float *cou
             HlProduct &q = work.p[2];
             q.tiles_m = hl_tiles(rows); q.tiles_n = hl_tiles(cols); q.kb = (x.d + HL_BK - 1) / HL_BK; q.npairs = np;
             f.ds.row_from = row_from; f.ds.rows = (int)rows; f.ds.col_from = (int)col_from; f.ds.cols = (int)cols;
-            f.ds.tickets = tickets + (i & 1) * pl.n_tickets; f.ds.n_tickets = (int)pl.n_tickets;
-        } else {
-            f.ds.n_tickets = 0;
         }
         if (i > 0) {
             const long long j = i - 1, rows = rows_of(j), cols = cols_of(j), row_from = pl.by_rows ? j * pl.step : 0, col_from = pl.by_rows ? 0 : j * pl.step;
             const bool first = j == 0, last = i == pl.pieces;
-            f.grads.tickets = tickets + (j & 1) * pl.n_tickets;
             if (dh) {                                                  // dh[rows] += ds W[cols]
                 mapped = mapped && hl_map(&maps.a[0], piece(j), 0, 0, rows, cols, false) && hl_map(&maps.b[0], w, col_from, 0, cols, x.d, true);
                 HlProduct &q = work.p[0];
@@ -1058,6 +1057,10 @@ int head_loss_bwd_launch(const HeadLossArgs &x, const float *L, const float *cou
            : which == 1 ? hl_launch(head_loss_bwd_kernel<true, 1>, 3, "head_loss_bwd_kernel", maps, work, pairs, f, stream)
            : which == 2 ? hl_launch(head_loss_bwd_kernel<false, 3>, 4, "head_loss_bwd_kernel", maps, work, pairs, f, stream)
                         : hl_launch(head_loss_bwd_kernel<true, 3>, 5, "head_loss_bwd_kernel", maps, work, pairs, f, stream);
+        for (int g = 0; g < 2 && rc == PGB_OK && i > 0; ++g) {
+            const HlGrad &o = f.grads.g[g];
+            if (work.p[g].tiles() > 0 && work.p[g].splits > 1 && o.last) rc = hl_sum(o.acc, o.out, o.rows * x.d, work.p[g].splits, f.grads, stream);
+        }
         if (rc != PGB_OK) return rc;
     }
     return PGB_OK;

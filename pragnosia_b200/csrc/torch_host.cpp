@@ -485,7 +485,7 @@ std::tuple<Tensor, Tensor, Tensor> teacher_lists(const Tensor &ids_, const Tenso
     const int64_t N = ids_.numel() / k;
     OnDevice dev(ids_);
     const Tensor ids = whole_numbers(DISTILL, ids_).reshape({N, k}), logits = f32c(logits_).reshape({N, k});
-    Tensor lists = alloc(ids, {N, k, 2}, at::kInt), starts = alloc(ids, {(V + 63) / 64, N}, at::kInt), ent = alloc(ids, {N}, at::kFloat);
+    Tensor lists = alloc(ids, {N, k, 2}, at::kInt), starts = alloc(ids, {N, (V + 63) / 64}, at::kInt), ent = alloc(ids, {N}, at::kFloat);
     if (N > 0)
         check(pgb_teacher_lists(static_cast<long long *>(vp(ids)), fp(logits), tau, static_cast<int *>(vp(lists)), static_cast<unsigned *>(vp(starts)), fp(ent), N, V,
                                 k, dev.stream), "pgb_teacher_lists");

@@ -499,7 +499,7 @@ def teacher_lists(ids: Tensor, logits: Tensor, temperature: float, V: int) -> Tu
 @teacher_lists.register_fake
 def _(ids, logits, temperature, V):
     n, k = _rows(ids), ids.shape[-1]
-    return _e(ids, n, k, 2, dtype=torch.int32), _e(ids, (V + 63) // 64, n, dtype=torch.int32), _e(ids, n, dtype=_F32)
+    return _e(ids, n, k, 2, dtype=torch.int32), _e(ids, n, (V + 63) // 64, dtype=torch.int32), _e(ids, n, dtype=_F32)
 
 
 @torch.library.custom_op(f"{NS}::linear_distill", mutates_args=())
