@@ -84,7 +84,7 @@ int decode_linear_launch(const void *, const void *, const void *, const float *
 int decode_linear_error_flag(int *);
 int decode_sample_launch(const void *, int, float, float, unsigned long long, long long *, long long *, int, long long *, long long *, float *,
                          unsigned int *, int, int, int, cudaStream_t);
-long long head_loss_fwd_bytes(long long, int, int, int, int);
+long long head_loss_fwd_bytes(long long, int, int, int);
 long long head_loss_bwd_bytes(long long, int, int, int, int, int);
 int head_teacher_launch(const long long *, const float *, int *, unsigned *, float *, long long, int, int, float, cudaStream_t);
 int head_loss_fwd_launch(const HeadLossArgs &, float *, float *, float *, float *, void *, cudaStream_t);
@@ -807,23 +807,23 @@ int head_sizes(long long N, int V, int d, int dtype) {
     if (N > HEAD_MOST_ROWS || V > HEAD_MOST_ROWS || d > 65536 || ((N + 255) / 256) * ((V + 255) / 256) > 0x40000000LL) return PGB_ERR_TOO_LARGE;
     return PGB_OK;
 }
-int head_args(HeadLossArgs &x, const void *h, const void *W, int dtype, const long long *target, long long ignore, const int *lists, const unsigned *starts,
-              const float *ent, int k, float tau, int reduction, long long N, int V, int d) {
-    x = {h, W, dtype, target, ignore, lists, starts, ent, k, tau, reduction, N, V, d};
+int head_args(HeadLossArgs &x, const void *h, const void *W, int dtype, const long long *target, long long ignore, const int *lists, const unsigned *marks,
+              const float *ent, float *kept, int k, float tau, int reduction, long long N, int V, int d) {
+    x = {h, W, dtype, target, ignore, lists, marks, ent, kept, k, tau, reduction, N, V, d};
     if (!h || !W) return PGB_ERR_NULL_POINTER;
-    if (target == nullptr && (!lists || !starts || !ent)) return PGB_ERR_NULL_POINTER;
+    if (target == nullptr && (!lists || !marks || !ent || !kept)) return PGB_ERR_NULL_POINTER;
     int rc = head_sizes(N, V, d, dtype);
     if (rc != PGB_OK) return rc;
     if (reduction < 0 || reduction > 2 || !(tau > 0.f) || tau > 3e38f || (lists && k < 1)) return PGB_ERR_BAD_SHAPE;
     if (lists && k > HEAD_MOST_K) return PGB_ERR_TOO_LARGE;
-    if (!aligned(h, 16) || !aligned(W, 16) || (target && !aligned(target, 8)) || (lists && (!aligned(lists, 8) || !aligned(starts, 4) || !aligned(ent, 4))))
+    if (!aligned(h, 16) || !aligned(W, 16) || (target && !aligned(target, 8)) || (lists && (!aligned(lists, 8) || !aligned(marks, 16) || !aligned(ent, 4) || !aligned(kept, 4))))
         return PGB_ERR_MISALIGNED;
     return PGB_OK;
 }
 int head_fwd(const HeadLossArgs &x, float *row_loss, float *loss, float *count, float *L, void *scratch, long long scratch_bytes, void *stream) {
     if (!L || !scratch || (x.reduction == 0 ? !row_loss : !loss || !count)) return PGB_ERR_NULL_POINTER;
     if (!aligned(L, 8) || !aligned(scratch, 256)) return PGB_ERR_MISALIGNED;
-    if (scratch_bytes < head_loss_fwd_bytes(x.N, x.V, x.d, x.dtype, x.lists ? x.k : 0)) return PGB_ERR_BAD_SHAPE;
+    if (scratch_bytes < head_loss_fwd_bytes(x.N, x.V, x.d, x.dtype)) return PGB_ERR_BAD_SHAPE;
     return head_loss_fwd_launch(x, row_loss, loss, count, L, scratch, (cudaStream_t)stream);
 }
 int head_bwd(const HeadLossArgs &x, const float *L, const float *count, const float *grad, void *dh, void *dW, void *scratch, long long scratch_bytes,
@@ -835,8 +835,8 @@ int head_bwd(const HeadLossArgs &x, const float *L, const float *count, const fl
 }
 }  // namespace
 
-long long pgb_head_loss_fwd_scratch_bytes(long long N, int V, int d, int dtype, int k) {
-    return head_sizes(N, V, d, dtype) != PGB_OK || k < 0 || k > HEAD_MOST_K ? 0 : head_loss_fwd_bytes(N, V, d, dtype, k);
+long long pgb_head_loss_fwd_scratch_bytes(long long N, int V, int d, int dtype) {
+    return head_sizes(N, V, d, dtype) != PGB_OK ? 0 : head_loss_fwd_bytes(N, V, d, dtype);
 }
 long long pgb_head_loss_bwd_scratch_bytes(long long N, int V, int d, int dtype, int want_dh, int want_dW) {
     return head_sizes(N, V, d, dtype) != PGB_OK ? 0 : head_loss_bwd_bytes(N, V, d, dtype, want_dh, want_dW);
@@ -845,35 +845,35 @@ int pgb_linear_xent_fwd(const void *h, const void *W, int dtype, const long long
                         float *L, void *scratch, long long scratch_bytes, int reduction, long long N, int V, int d, void *stream) {
     if (!target) return PGB_ERR_NULL_POINTER;
     HeadLossArgs x;
-    const int rc = head_args(x, h, W, dtype, target, ignore_index, nullptr, nullptr, nullptr, 0, 1.f, reduction, N, V, d);
+    const int rc = head_args(x, h, W, dtype, target, ignore_index, nullptr, nullptr, nullptr, nullptr, 0, 1.f, reduction, N, V, d);
     return rc != PGB_OK ? rc : head_fwd(x, row_loss, loss, count, L, scratch, scratch_bytes, stream);
 }
 int pgb_linear_xent_bwd(const void *h, const void *W, int dtype, const long long *target, long long ignore_index, const float *L, const float *count,
                         const float *grad, void *dh, void *dW, void *scratch, long long scratch_bytes, int reduction, long long N, int V, int d, void *stream) {
     if (!target) return PGB_ERR_NULL_POINTER;
     HeadLossArgs x;
-    const int rc = head_args(x, h, W, dtype, target, ignore_index, nullptr, nullptr, nullptr, 0, 1.f, reduction, N, V, d);
+    const int rc = head_args(x, h, W, dtype, target, ignore_index, nullptr, nullptr, nullptr, nullptr, 0, 1.f, reduction, N, V, d);
     return rc != PGB_OK ? rc : head_bwd(x, L, count, grad, dh, dW, scratch, scratch_bytes, stream);
 }
-int pgb_teacher_lists(const long long *teacher_ids, const float *teacher_logits, float temperature, int *lists, unsigned *starts, float *ent, long long N, int V, int k,
+int pgb_teacher_lists(const long long *teacher_ids, const float *teacher_logits, float temperature, int *lists, unsigned *marks, float *ent, long long N, int V, int k,
                       void *stream) {
-    if (!teacher_ids || !teacher_logits || !lists || !starts || !ent) return PGB_ERR_NULL_POINTER;
+    if (!teacher_ids || !teacher_logits || !lists || !marks || !ent) return PGB_ERR_NULL_POINTER;
     if (N < 1 || V < 1 || k < 1 || !(temperature > 0.f) || temperature > 3e38f) return PGB_ERR_BAD_SHAPE;
     if (N > HEAD_MOST_ROWS || V > HEAD_MOST_ROWS || k > HEAD_MOST_K) return PGB_ERR_TOO_LARGE;
-    if (!aligned(teacher_ids, 8) || !aligned(teacher_logits, 4) || !aligned(lists, 8) || !aligned(starts, 4) || !aligned(ent, 4)) return PGB_ERR_MISALIGNED;
-    return head_teacher_launch(teacher_ids, teacher_logits, lists, starts, ent, N, V, k, temperature, (cudaStream_t)stream);
+    if (!aligned(teacher_ids, 8) || !aligned(teacher_logits, 4) || !aligned(lists, 8) || !aligned(marks, 16) || !aligned(ent, 4)) return PGB_ERR_MISALIGNED;
+    return head_teacher_launch(teacher_ids, teacher_logits, lists, marks, ent, N, V, k, temperature, (cudaStream_t)stream);
 }
-int pgb_linear_distill_fwd(const void *h, const void *W, int dtype, const int *lists, const unsigned *starts, const float *ent, int k, float temperature, float *row_loss,
+int pgb_linear_distill_fwd(const void *h, const void *W, int dtype, const int *lists, const unsigned *marks, const float *ent, float *kept, int k, float temperature, float *row_loss,
                            float *loss, float *count, float *L, void *scratch, long long scratch_bytes, int reduction, long long N, int V, int d, void *stream) {
     HeadLossArgs x;
-    const int rc = head_args(x, h, W, dtype, nullptr, 0, lists, starts, ent, k, temperature, reduction, N, V, d);
+    const int rc = head_args(x, h, W, dtype, nullptr, 0, lists, marks, ent, kept, k, temperature, reduction, N, V, d);
     return rc != PGB_OK ? rc : head_fwd(x, row_loss, loss, count, L, scratch, scratch_bytes, stream);
 }
-int pgb_linear_distill_bwd(const void *h, const void *W, int dtype, const int *lists, const unsigned *starts, const float *ent, int k, float temperature, const float *L,
+int pgb_linear_distill_bwd(const void *h, const void *W, int dtype, const int *lists, const unsigned *marks, const float *ent, const float *kept, int k, float temperature, const float *L,
                            const float *count, const float *grad, void *dh, void *dW, void *scratch, long long scratch_bytes, int reduction, long long N, int V,
                            int d, void *stream) {
     HeadLossArgs x;
-    const int rc = head_args(x, h, W, dtype, nullptr, 0, lists, starts, ent, k, temperature, reduction, N, V, d);
+    const int rc = head_args(x, h, W, dtype, nullptr, 0, lists, marks, ent, const_cast<float *>(kept), k, temperature, reduction, N, V, d);
     return rc != PGB_OK ? rc : head_bwd(x, L, count, grad, dh, dW, scratch, scratch_bytes, stream);
 }
 

@@ -122,9 +122,9 @@ struct TrainBwdArgs {
     void *dq, *dk, *dv; float *dla, *dbeta, *dS0; void *scratch;
     int B, H, T;
 };
-// a loss over the vocabulary (head_loss.cu): target, or a teacher's lists (with starts, ent, k); reduction 0 none, 1 sum, 2 mean
+// a loss over the vocabulary (head_loss.cu): target, or a teacher's lists (with marks, ent, k; kept [N][k]: their logits, from the forward pass to the backward pass); reduction 0 none, 1 sum, 2 mean
 struct HeadLossArgs {
-    const void *h, *W; int dtype; const long long *target; long long ignore; const int *lists; const unsigned *starts; const float *ent; int k;
+    const void *h, *W; int dtype; const long long *target; long long ignore; const int *lists; const unsigned *marks; const float *ent; float *kept; int k;
     float tau; int reduction; long long N; int V, d;
 };
 struct DecodeArgs {

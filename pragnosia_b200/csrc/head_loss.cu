@@ -265,74 +265,55 @@ __device__ __forceinline__ float pick32(const float (&v)[32], int i) {
     return a[0];
 }
 
-// What a row's target distribution is read from: a word per row (target), or a teacher's entries: lists [N][k] of (id, probability's bits), ids
-// ascending, INT_MAX behind the last; starts [N][blocks of 64 words], the place of the first entry at or behind the block's first word times 256
-// plus its column, 255 where it is not in the block; ent, the sum of p log p, inf for a row without an entry, NaN for one with an id out of range.
+// What a row's target distribution is read from: a word per row (target), or a teacher's entries, no id twice: lists [N][k] of (id, probability's
+// bits), ids ascending, INT_MAX behind the last; marks [N][blocks of 64 words], which of a block's words they are (64 bits) and the place of the
+// first of them; ent, the sum of p log p, inf for a row without an entry, NaN for one with an id out of range.
 struct HlTargets {
-    const long long *target; long long ignore; const int2 *lists; const unsigned *starts; const float *ent; int k, blocks;
-};
-
-// A lane's walk over its row's targets within its 64 columns: nx is the column of the one to come (INT_MAX: none), in ascending order, p what it
-// holds. The two entries behind it are loaded ahead.
-template <bool LIST>
-struct HlWalk {
-    int nx = 0x7fffffff, pos = 0, k = 0;
-    float p = 1.f;
-    int2 a1, a2;
-    const int2 *list = nullptr;
-    // the targets from column `from` (of the whole vocabulary) on; where: the row's target, or its entry in starts; row < 0: none
-    __device__ __forceinline__ void begin(const HlTargets &t, long long row, long long where, int from) {
-        nx = 0x7fffffff;
-        if (row < 0) return;
-        if constexpr (LIST) {
-            const unsigned col = (unsigned)where & 255u;
-            if (col == 255u) return;
-            k = t.k; list = t.lists + row * k; pos = (int)((unsigned)where >> 8);
-            nx = from + (int)col;
-            p = __int_as_float(list[pos].y);
-            a1 = entry(pos + 1);
-            a2 = entry(pos + 2);
-        } else {
-            if (where != t.ignore && where >= from && where < 0x7fffffff) nx = (int)where;
-        }
-    }
-    __device__ __forceinline__ int2 entry(int i) const { return i < k ? list[i] : make_int2(0x7fffffff, 0); }
-    __device__ __forceinline__ void advance() {
-        nx = 0x7fffffff;
-        if constexpr (LIST) { nx = a1.x; p = __int_as_float(a1.y); a1 = a2; a2 = entry(++pos + 2); }
-    }
+    const long long *target; long long ignore; const int2 *lists; const uint4 *marks; const float *ent; int k, blocks;
 };
 
 // ------------------------------------------------------------------------------------------------ forward
 struct HlFwd {
     HlTargets t; float a;
     float2 *ml;                                                       // [tiles_n][Np]: maximum (times a) and sum of a tile's row
-    float *dot;                                                       // list: [tiles_n][Np], sum of p s over the tile; else [N], the target's s
+    float *dot;                                                       // the targets' s: [N], or [N][k] where there are lists
     unsigned *ticket; long long N, Np; int V;
 };
 template <bool LIST>
 struct HlFwdEpi {
     const HlFwd &f;
-    HlWalk<LIST> w;
-    long long row, where;                                              // of the tile fetched for
+    uint4 marks; int target;                                           // of the tile fetched for
+    uint64_t bits; int place, nx;                                      // of the tile at hand: targets by column, and the first one's place; or the target
     __device__ __forceinline__ void start(int i) { if (i == 0 && blockIdx.x == 0) *f.ticket = 0u; }
     __device__ __forceinline__ void end(int) {}
     __device__ __forceinline__ void fetch(int, int r, int c) {
-        row = r < f.N && c < f.V ? r : -1;
-        if (row >= 0) where = LIST ? f.t.starts[row * f.t.blocks + (c >> 6)] : f.t.target[row];
+        const bool in = r < f.N && c < f.V;
+        if constexpr (LIST) {
+            marks = in ? f.t.marks[(long long)r * f.t.blocks + (c >> 6)] : make_uint4(0u, 0u, 0u, 0u);
+        } else {
+            const long long w = in ? f.t.target[r] : -1;
+            target = w >= 0 && w < f.V && w != f.t.ignore ? (int)w : -1;
+        }
     }
-    __device__ __forceinline__ void begin(const HlTile &x) { w.begin(f.t, row, where, x.col0); }
+    __device__ __forceinline__ void begin(const HlTile &) {
+        if constexpr (LIST) { bits = (uint64_t)marks.y << 32 | marks.x; place = (int)marks.z; } else nx = target;
+    }
     __device__ __forceinline__ bool tile(const HlTile &x, float (&v)[2][32], uint8_t *, uint8_t *shared, uint32_t quarters) {
-        float m = -INFINITY, l = 0.f, dot = 0.f;
+        float m = -INFINITY, l = 0.f;
         const int row = x.row0 + x.lane;
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
             const int c0 = x.col0 + 32 * b;
             if (c0 >= f.V) break;
-            while (__any_sync(0xffffffffu, w.nx < c0 + 32)) {          // this block holds a target of some row
-                const bool hit = w.nx < c0 + 32;
-                const float s = pick32(v[b], hit ? w.nx - c0 : 0);
-                if (hit) { dot = fmaf(w.p, s, dot); w.advance(); if (!LIST) f.dot[row] = s; }
+            if constexpr (LIST) {
+                uint32_t todo = (uint32_t)(bits >> (32 * b));
+                while (__any_sync(0xffffffffu, todo != 0u)) {
+                    const float s = pick32(v[b], __ffs(todo) - 1);
+                    if (todo != 0u) { f.dot[(long long)row * f.t.k + place] = s; ++place; todo &= todo - 1u; }
+                }
+            } else if (__any_sync(0xffffffffu, (unsigned)(nx - c0) < 32u)) {
+                const float s = pick32(v[b], nx - c0);
+                if ((unsigned)(nx - c0) < 32u) f.dot[row] = s;
             }
             if (c0 + 32 > f.V) {
 #pragma unroll
@@ -351,9 +332,9 @@ struct HlFwdEpi {
         }
         // The four column quarters of a row, by the first one's warp. Four sets in turn, each with a barrier: a warp has tile t + 3 in hand only
         // once every warp has taken tile t + 1 out of tensor memory, which is behind its work on tile t.
-        float3 *mine = reinterpret_cast<float3 *>(shared) + ((x.ti & 3) * 128 + 32 * x.sub + x.lane) * 4;
+        float2 *mine = reinterpret_cast<float2 *>(shared) + ((x.ti & 3) * 128 + 32 * x.sub + x.lane) * 4;
         if (x.part != 0) {
-            mine[x.part] = make_float3(m, l, dot);
+            mine[x.part] = make_float2(m, l);
             __syncwarp();
             if (x.lane == 0) mbar_arrive(quarters);
             return true;
@@ -362,16 +343,12 @@ struct HlFwdEpi {
         if (ok) {
 #pragma unroll
             for (int q = 1; q < 4; ++q) {
-                const float3 o = mine[q];
+                const float2 o = mine[q];
                 const float top = fmaxf(m, o.x), at = top == -INFINITY ? 0.f : top;
                 l = l * fast_exp2(m - at) + o.y * fast_exp2(o.x - at);
                 m = top;
-                dot += o.z;
             }
-            if (row < f.N) {
-                f.ml[(long long)x.n * f.Np + row] = make_float2(m, l);
-                if (LIST) f.dot[(long long)x.n * f.Np + row] = dot;
-            }
+            if (row < f.N) f.ml[(long long)x.n * f.Np + row] = make_float2(m, l);
         }
         return ok;
     }
@@ -379,7 +356,7 @@ struct HlFwdEpi {
 template <bool LIST>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(HL_NT, 1)
 head_loss_fwd_kernel(const __grid_constant__ HlMaps maps, const __grid_constant__ HlProduct pr, const __grid_constant__ HlFwd f) {
-    HlFwdEpi<LIST> epi{f, {}, 0, 0};
+    HlFwdEpi<LIST> epi{f};
     hl_body<HlOne>(maps, pr, epi);
 }
 
@@ -406,7 +383,15 @@ __global__ void __launch_bounds__(256) head_loss_join_kernel(const HlJoin j) {
             const float top = fmaxf(m, o.x), at = top == -INFINITY ? 0.f : top;
             l = l * fast_exp2(m - at) + o.y * fast_exp2(o.x - at);
             m = top;
-            if (LIST) dot += j.dot[(long long)n * j.Np + row];
+        }
+        if constexpr (LIST) {
+            const int2 *list = j.t.lists + row * j.t.k;
+#pragma unroll 4
+            for (int i = warp; i < j.t.k; i += 8) {
+                const int2 e = list[i];
+                const float s = j.dot[row * j.t.k + i];
+                if (e.x < j.V) dot = fmaf(__int_as_float(e.y), s, dot);
+            }
         }
     }
     part[warp][lane] = make_float3(m, l, dot);
@@ -473,9 +458,9 @@ __global__ void __launch_bounds__(256) head_loss_join_kernel(const HlJoin j) {
 
 // ------------------------------------------------------------------------------------------------ a teacher's lists
 // A warp per row: probabilities of the entries that are there (id >= 0, logit not -inf) at the temperature, in ascending order of their
-// ids (a rank per entry: k comparisons each), and where the entries of every 64 words begin (a bisection per block).
+// ids (a rank per entry: k comparisons each), an id that comes again added to the first, and the marks (a bisection per block of 64 words).
 __global__ void __launch_bounds__(128) head_teacher_kernel(const long long *__restrict__ in_ids, const float *__restrict__ in_logits, int2 *__restrict__ lists,
-                                                           unsigned *__restrict__ starts, float *__restrict__ ent, long long N, int V, int k, float inv_tau) {
+                                                           uint4 *__restrict__ marks, float *__restrict__ ent, long long N, int V, int k, float inv_tau) {
     extern __shared__ __align__(16) long long teacher_smem[];
     pdl_wait();
     pdl_launch_dependents();
@@ -483,7 +468,7 @@ __global__ void __launch_bounds__(128) head_teacher_kernel(const long long *__re
     const long long row = (long long)blockIdx.x * 4 + warp;
     if (row >= N) return;
     long long *key = teacher_smem + kk * warp;                         // id times 1024 plus place: none twice; absent ones behind all others
-    int *sorted = reinterpret_cast<int *>(teacher_smem + 4 * kk) + kk * warp;
+    int2 *sorted = reinterpret_cast<int2 *>(teacher_smem + 4 * kk) + kk * warp;
     constexpr long long ABSENT = 0x7fffffffLL << 10;
     float top = -INFINITY;
     bool bad = false;
@@ -496,7 +481,6 @@ __global__ void __launch_bounds__(128) head_teacher_kernel(const long long *__re
         key[j] = is ? (i >= V ? V : i) << 10 | j : ABSENT | j;
         if (is) { top = fmaxf(top, x); ++here; }
     }
-    for (int j = lane; j < k; j += 32) sorted[j] = 0x7fffffff;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) { top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o)); here += __shfl_xor_sync(0xffffffffu, here, o); }
     bad = __any_sync(0xffffffffu, bad);
@@ -516,22 +500,35 @@ __global__ void __launch_bounds__(128) head_teacher_kernel(const long long *__re
             const longlong2 o = *reinterpret_cast<const longlong2 *>(key + i);
             rank += (o.x < me) + (o.y < me);
         }
-        sorted[rank] = (int)(me >> 10);
-        lists[row * k + rank] = make_int2((int)(me >> 10), __float_as_int(q));
+        sorted[rank] = make_int2((int)(me >> 10), __float_as_int(q));
     }
-    for (int j = here + lane; j < k; j += 32) lists[row * k + j] = make_int2(0x7fffffff, 0);
+    __syncwarp();
+    // ids that come again: the first has their probabilities, they leave the list
+    bool again = false;
+    for (int j = lane; j < here; j += 32) again |= j > 0 && sorted[j].x == sorted[j - 1].x;
+    if (__any_sync(0xffffffffu, again)) {
+        int n = 0;
+        if (lane == 0)
+            for (int j = 0; j < here; ++j) {
+                if (n > 0 && sorted[j].x == sorted[n - 1].x) sorted[n - 1].y = __float_as_int(__int_as_float(sorted[n - 1].y) + __int_as_float(sorted[j].y));
+                else sorted[n++] = sorted[j];
+            }
+        here = __shfl_sync(0xffffffffu, n, 0);
+        __syncwarp();
+    }
+    for (int j = lane; j < k; j += 32) lists[row * k + j] = j < here ? sorted[j] : make_int2(0x7fffffff, 0);
     e = warp_sum(e);
     if (lane == 0) ent[row] = bad ? NAN : here > 0 ? e : INFINITY;
-    __syncwarp();
     const int blocks = (V + 63) / 64;
     for (int b = lane; b < blocks; b += 32) {
         int lo = 0, hi = here;
         while (lo < hi) {
             const int mid = (lo + hi) >> 1;
-            if (sorted[mid] < 64 * b) lo = mid + 1; else hi = mid;
+            if (sorted[mid].x < 64 * b) lo = mid + 1; else hi = mid;
         }
-        const int id = lo < here ? sorted[lo] : 0x7fffffff;
-        starts[row * blocks + b] = ((unsigned)lo << 8) | (id - 64 * b < 64 ? (unsigned)(id - 64 * b) : 255u);
+        uint64_t bits = 0;
+        for (int j = lo; j < here && sorted[j].x < V && sorted[j].x - 64 * b < 64; ++j) bits |= 1ull << (sorted[j].x - 64 * b);
+        marks[row * blocks + b] = make_uint4((unsigned)bits, (unsigned)(bits >> 32), (unsigned)lo, 0u);
     }
 }
 
@@ -539,28 +536,27 @@ __global__ void __launch_bounds__(128) head_teacher_kernel(const long long *__re
 struct HlProb {
     HlTargets t; const float2 *L; const float *row_weight;            // row_weight NULL: 1
     float a;
-    long long row_from; int V, col_from, cols, rows;                  // the piece: rows and columns it begins at, how many
+    int row_from, V, col_from, cols, rows;                            // the piece: rows and columns it begins at, how many
 };
 template <bool LIST, int TERMS>
 struct HlProbEpi {
     const HlProb &f;
     const CUtensorMap *map;
-    HlWalk<LIST> w;
-    long long row, where, word; float2 L; float weight, ent;           // of the tile fetched for
-    float a_hi, a_lo, c; bool live;                                   // of the tile at hand
+    int row; long long word; float2 L; float weight, ent;              // of the tile fetched for
+    float a_hi, a_lo, c; bool live; int nx;                           // of the tile at hand; nx: the target's column
     __device__ __forceinline__ void fetch(int r, int c) {
         row = r < f.rows && c < f.cols ? f.row_from + r : -1;
         if (row < 0) return;
         L = f.L[row];
         weight = f.row_weight ? f.row_weight[row] : 1.f;
-        if (LIST) { ent = f.t.ent[row]; where = f.t.starts[row * f.t.blocks + ((f.col_from + c) >> 6)]; } else word = where = f.t.target[row];
+        if (LIST) ent = f.t.ent[row]; else word = f.t.target[row];
     }
-    __device__ __forceinline__ void begin(const HlTile &x) {
-        w.begin(f.t, row, where, f.col_from + x.col0);
+    __device__ __forceinline__ void begin(const HlTile &) {
         a_hi = -L.x; a_lo = -L.y;
         const bool bad = LIST ? ent != ent : word != f.t.ignore && (word < 0 || word >= f.V);
         live = row >= 0 && (LIST ? ent != INFINITY : word != f.t.ignore);
         c = bad ? NAN : weight;
+        if (!LIST) nx = live && !bad ? (int)word : -1;
     }
     // Rounded, the block goes out by two TMA stores a term, 32 columns each, from the warp's staging: 64-byte rows, their 16-byte chunks swapped
     // as the store's 64-byte swizzle has them, so that the row-per-lane writes touch every bank once. What lies outside the piece is not written.
@@ -574,15 +570,10 @@ struct HlProbEpi {
             float (&v)[32] = vv[b];
 #pragma unroll
             for (int i = 0; i < 32; ++i) v[i] = TERMS == 3 ? fast_exp2(fmaf(v[i], f.a, a_hi) + a_lo) : fast_exp2(fmaf(v[i], f.a, a_hi));
-            if constexpr (TERMS == 3) {                                // before the values are taken apart
-                while (__any_sync(0xffffffffu, w.nx < v0 + 32)) {
-                    const bool hit = w.nx < v0 + 32;
-                    const int at = hit ? w.nx - v0 : -1;
-                    const float less = hit ? w.p : 0.f;
+            const bool target = !LIST && __any_sync(0xffffffffu, (unsigned)(nx - v0) < 32u);     // of some row; a teacher's are put in behind this launch
+            if (TERMS == 3 && target) {                                // before the values are taken apart
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) v[i] -= i == at ? less : 0.f;
-                    if (hit) w.advance();
-                }
+                for (int i = 0; i < 32; ++i) v[i] -= i == nx - v0 ? 1.f : 0.f;
             }
             if (!plain) {
 #pragma unroll
@@ -605,17 +596,11 @@ struct HlProbEpi {
                     }
                     *reinterpret_cast<uint4 *>(stage + lane * 64 + ((ch ^ ((lane >> 1) & 3)) << 4)) = *reinterpret_cast<uint4 *>(o);
                 }
-                if constexpr (TERMS == 1) {                            // the few columns that hold a target, over what was staged for them
-                    while (__any_sync(0xffffffffu, w.nx < v0 + 32)) {
-                        const int at = w.nx - v0;
-                        const float q = pick32(v, at & 31);
-                        if (at < 32) {
-                            float less = w.p;
-                            for (w.advance(); LIST && w.nx - v0 == at; w.advance()) less += w.p;
-                            const __nv_bfloat16 x = __float2bfloat16_rn(live ? fmaf(-c, less, q) : 0.f);
-                            *reinterpret_cast<__nv_bfloat16 *>(stage + lane * 64 + (((at >> 3) ^ ((lane >> 1) & 3)) << 4) + 2 * (at & 7)) = x;
-                        }
-                    }
+                if (TERMS == 1 && target) {                            // over what was staged for the column
+                    const int at = nx - v0;
+                    const float q = pick32(v, at & 31);
+                    if ((unsigned)at < 32u)
+                        *reinterpret_cast<__nv_bfloat16 *>(stage + lane * 64 + (((at >> 3) ^ ((lane >> 1) & 3)) << 4) + 2 * (at & 7)) = __float2bfloat16_rn(q - c);
                 }
                 fence_proxy_async();
                 __syncwarp();
@@ -624,6 +609,31 @@ struct HlProbEpi {
         }
     }
 };
+
+// A teacher's columns of a piece of ds, exactly: c (q - p) from the logits that the forward pass kept, over the q that the product's epilogue wrote.
+// An entry per thread. (Looked for in that epilogue, the entries of 32 rows were as long as the rest of it: 64 a row in 8192 words, 87 us
+// against 43 for 4096 rows.)
+template <int TERMS>
+__global__ void __launch_bounds__(256) head_teacher_ds_kernel(const HlProb f, const float *__restrict__ kept, __nv_bfloat16 *__restrict__ P, long long ldp,
+                                                              long long term_stride) {
+    pdl_wait();
+    pdl_launch_dependents();
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x, all = (long long)f.rows * f.t.k;
+    if (i >= all) return;
+    const int row = (int)(i / f.t.k), full = f.row_from + row;
+    const int2 e = f.t.lists[(long long)f.row_from * f.t.k + i];
+    const int col = e.x - f.col_from;
+    if (col < 0 || col >= f.cols) return;
+    const float2 L = f.L[full];
+    const float ent = f.t.ent[full], c = ent != ent ? NAN : f.row_weight ? f.row_weight[full] : 1.f;
+    float x = c * (fast_exp2(fmaf(kept[(long long)f.row_from * f.t.k + i], f.a, -L.x) - L.y) - __int_as_float(e.y));
+#pragma unroll
+    for (int term = 0; term < TERMS; ++term) {
+        const __nv_bfloat16 h = __float2bfloat16_rn(x);
+        P[term * term_stride + row * ldp + col] = h;
+        x -= __bfloat162float(h);
+    }
+}
 
 // The upstream scale that all rows share: g the gradient of the (summed or averaged) loss, count the rows averaged over.
 __device__ __forceinline__ float hl_alpha(const float *g, const float *count, float tau, int reduction) {
@@ -807,13 +817,13 @@ static bool hl_map(CUtensorMap *m, const HlOperand &o, long long row_from, long 
 }
 
 struct HlFwdPlan { long long Np, tiles, off_ml, off_dot, off_partial, off_ticket, off_h, off_w, total; };
-static HlFwdPlan hl_fwd_plan(long long N, int V, int d, int dtype, bool list) {
+static HlFwdPlan hl_fwd_plan(long long N, int V, int d, int dtype) {
     HlFwdPlan p;
     p.Np = hl_up(N, 32); p.tiles = hl_tiles(V);
     long long at = 0;
     auto take = [&](long long bytes) { const long long o = at; at += hl_up(bytes, 256); return o; };
     p.off_ml = take(p.tiles * p.Np * 8);
-    p.off_dot = take((list ? p.tiles : 1) * p.Np * 4);
+    p.off_dot = take(p.Np * 4);
     p.off_partial = take(p.Np / 32 * 16);
     p.off_ticket = take(4);
     p.off_h = dtype == PGB_F32 ? take(6 * N * d) : 0;
@@ -821,7 +831,7 @@ static HlFwdPlan hl_fwd_plan(long long N, int V, int d, int dtype, bool list) {
     p.total = at;
     return p;
 }
-long long head_loss_fwd_bytes(long long N, int V, int d, int dtype, int k) { return hl_fwd_plan(N, V, d, dtype, k > 0).total; }
+long long head_loss_fwd_bytes(long long N, int V, int d, int dtype) { return hl_fwd_plan(N, V, d, dtype).total; }
 
 static int hl_split(const void *x, void *out, long long n, cudaStream_t stream) {
     const long long blocks = (n / 8 + 255) / 256;
@@ -839,17 +849,20 @@ static int hl_operand(HlOperand &o, const void *x, int dtype, long long rows, in
 }
 static int hl_no_map() { set_cuda_error(cudaErrorUnknown, "cuTensorMapEncodeTiled"); return PGB_ERR_CUDA; }
 
-int head_teacher_launch(const long long *in_ids, const float *in_logits, int *lists, unsigned *starts, float *ent, long long N, int V, int k, float tau,
+static_assert(4 * 1024 * 16 <= 65536, "a teacher's entries in shared memory");
+int head_teacher_launch(const long long *in_ids, const float *in_logits, int *lists, unsigned *marks, float *ent, long long N, int V, int k, float tau,
                         cudaStream_t stream) {
-    cudaError_t e = pdl_launch(head_teacher_kernel, dim3((unsigned)((N + 3) / 4)), dim3(128), (size_t)(4 * ((k + 1) & ~1) * 12), stream, in_ids, in_logits,
-                               reinterpret_cast<int2 *>(lists), starts, ent, N, V, k, 1.0f / tau);
+    cudaError_t e = cudaFuncSetAttribute(head_teacher_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 65536);
+    if (e == cudaSuccess)
+        e = pdl_launch(head_teacher_kernel, dim3((unsigned)((N + 3) / 4)), dim3(128), (size_t)(4 * ((k + 1) & ~1) * 16), stream, in_ids, in_logits,
+                               reinterpret_cast<int2 *>(lists), reinterpret_cast<uint4 *>(marks), ent, N, V, k, 1.0f / tau);
     if (e != cudaSuccess) { set_cuda_error(e, "head_teacher launch"); return PGB_ERR_CUDA; }
     return check_launch("head_teacher_kernel");
 }
 
 int head_loss_fwd_launch(const HeadLossArgs &x, float *row_loss, float *loss, float *count, float *L, void *scratch, cudaStream_t stream) {
     const bool list = x.lists != nullptr;
-    const HlFwdPlan pl = hl_fwd_plan(x.N, x.V, x.d, x.dtype, list);
+    const HlFwdPlan pl = hl_fwd_plan(x.N, x.V, x.d, x.dtype);
     char *s = static_cast<char *>(scratch);
     HlOperand h, w;
     int rc = hl_operand(h, x.h, x.dtype, x.N, x.d, s + pl.off_h, stream);
@@ -859,8 +872,8 @@ int head_loss_fwd_launch(const HeadLossArgs &x, float *row_loss, float *loss, fl
     if (!hl_map(&maps.a[0], h, 0, 0, x.N, x.d, false) || !hl_map(&maps.b[0], w, 0, 0, x.V, x.d, false)) return hl_no_map();
     HlProduct pr;
     pr.tiles_m = hl_tiles(x.N); pr.tiles_n = (int)pl.tiles; pr.kb = (x.d + HL_BK - 1) / HL_BK; pr.npairs = h.terms == 3 ? 6 : 1;
-    const HlTargets t{x.target, x.ignore, reinterpret_cast<const int2 *>(x.lists), x.starts, x.ent, x.k, (x.V + 63) / 64};
-    const HlFwd f{t, LOG2E_F / x.tau, reinterpret_cast<float2 *>(s + pl.off_ml), reinterpret_cast<float *>(s + pl.off_dot),
+    const HlTargets t{x.target, x.ignore, reinterpret_cast<const int2 *>(x.lists), reinterpret_cast<const uint4 *>(x.marks), x.ent, x.k, (x.V + 63) / 64};
+    const HlFwd f{t, LOG2E_F / x.tau, reinterpret_cast<float2 *>(s + pl.off_ml), list ? x.kept : reinterpret_cast<float *>(s + pl.off_dot),
                   reinterpret_cast<unsigned *>(s + pl.off_ticket), x.N, pl.Np, x.V};
     rc = list ? hl_launch(head_loss_fwd_kernel<true>, 0, "head_loss_fwd_kernel", maps, pr, pr.tiles(), f, stream)
               : hl_launch(head_loss_fwd_kernel<false>, 1, "head_loss_fwd_kernel", maps, pr, pr.tiles(), f, stream);
@@ -1014,7 +1027,7 @@ int head_loss_bwd_launch(const HeadLossArgs &x, const float *L, const float *cou
     auto at = [&](long long off) { return off >= 0 ? reinterpret_cast<float *>(s + off) : nullptr; };
     auto piece = [&](int i) { return HlOperand{s + pl.off_p[i & 1], pl.terms, pl.rows * pl.ldp, pl.ldp}; };
     HlBwd f{};
-    f.ds.t = {x.target, x.ignore, reinterpret_cast<const int2 *>(x.lists), x.starts, x.ent, x.k, (x.V + 63) / 64};
+    f.ds.t = {x.target, x.ignore, reinterpret_cast<const int2 *>(x.lists), reinterpret_cast<const uint4 *>(x.marks), x.ent, x.k, (x.V + 63) / 64};
     f.ds.L = reinterpret_cast<const float2 *>(L); f.ds.row_weight = x.reduction == 0 ? up : nullptr; f.ds.a = LOG2E_F / x.tau; f.ds.V = x.V;
     f.grads.up = up; f.grads.count = count; f.grads.tau = x.tau; f.grads.reduction = x.reduction; f.grads.d = x.d; f.grads.out_f32 = x.dtype == PGB_F32;
     // launch i: the products of piece i - 1, ds of piece i
@@ -1029,7 +1042,7 @@ int head_loss_bwd_launch(const HeadLossArgs &x, const float *L, const float *cou
             mapped = hl_map(&maps.a[2], h, row_from, 0, rows, x.d, false) && hl_map(&maps.b[2], w, col_from, 0, cols, x.d, false) && hl_store_map(&maps.ds, piece(i), rows, cols);
             HlProduct &q = work.p[2];
             q.tiles_m = hl_tiles(rows); q.tiles_n = hl_tiles(cols); q.kb = (x.d + HL_BK - 1) / HL_BK; q.npairs = np;
-            f.ds.row_from = row_from; f.ds.rows = (int)rows; f.ds.col_from = (int)col_from; f.ds.cols = (int)cols;
+            f.ds.row_from = (int)row_from; f.ds.rows = (int)rows; f.ds.col_from = (int)col_from; f.ds.cols = (int)cols;
         }
         if (i > 0) {
             const long long j = i - 1, rows = rows_of(j), cols = cols_of(j), row_from = pl.by_rows ? j * pl.step : 0, col_from = pl.by_rows ? 0 : j * pl.step;
@@ -1057,6 +1070,14 @@ int head_loss_bwd_launch(const HeadLossArgs &x, const float *L, const float *cou
            : which == 1 ? hl_launch(head_loss_bwd_kernel<true, 1>, 3, "head_loss_bwd_kernel", maps, work, pairs, f, stream)
            : which == 2 ? hl_launch(head_loss_bwd_kernel<false, 3>, 4, "head_loss_bwd_kernel", maps, work, pairs, f, stream)
                         : hl_launch(head_loss_bwd_kernel<true, 3>, 5, "head_loss_bwd_kernel", maps, work, pairs, f, stream);
+        if (rc == PGB_OK && list && i < pl.pieces) {
+            const HlOperand P = piece(i);
+            __nv_bfloat16 *to = static_cast<__nv_bfloat16 *>(const_cast<void *>(P.ptr));
+            const dim3 grid((unsigned)(((long long)f.ds.rows * x.k + 255) / 256));
+            const cudaError_t e = pl.terms == 3 ? pdl_launch(head_teacher_ds_kernel<3>, grid, dim3(256), 0, stream, f.ds, (const float *)x.kept, to, P.ld, P.term_stride)
+                                                : pdl_launch(head_teacher_ds_kernel<1>, grid, dim3(256), 0, stream, f.ds, (const float *)x.kept, to, P.ld, P.term_stride);
+            if (e != cudaSuccess) { set_cuda_error(e, "head_teacher_ds launch"); return PGB_ERR_CUDA; }
+        }
         for (int g = 0; g < 2 && rc == PGB_OK && i > 0; ++g) {
             const HlGrad &o = f.grads.g[g];
             if (work.p[g].tiles() > 0 && work.p[g].splits > 1 && o.last) rc = hl_sum(o.acc, o.out, o.rows * x.d, work.p[g].splits, f.grads, stream);

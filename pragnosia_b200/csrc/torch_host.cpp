@@ -420,8 +420,8 @@ HeadIn head_in(const char *what, const Tensor &h, const Tensor &w) {
     TORCH_CHECK_VALUE(w.size(0) >= 1 && d >= 8 && d % 8 == 0, what, ": the weight is (V, d) with V at least 1 and d a multiple of 8, got ", w.sizes());
     return {head_operand(h.reshape({-1, d})), head_operand(w), h.numel() / d, w.size(0), d};
 }
-// What a row is held to: a word each (target), or a teacher's entries (lists, starts, ent).
-struct HeadWant { Tensor target; int64_t ignore; Tensor lists, starts, ent; double tau; };
+// What a row is held to: a word each (target), or a teacher's entries (lists, marks, ent; kept: their logits).
+struct HeadWant { Tensor target; int64_t ignore; Tensor lists, marks, ent, kept; double tau; };
 struct HeadOut { Tensor loss, L, count; };                            // loss: [N] or 0-d
 HeadOut head_fwd(const char *what, const HeadIn &x, const HeadWant &t, int reduction) {
     OnDevice dev(x.h);
@@ -435,11 +435,11 @@ HeadOut head_fwd(const char *what, const HeadIn &x, const HeadWant &t, int reduc
     }
     const bool list = t.lists.defined();
     const int k = list ? t.lists.size(1) : 0;
-    const long long n = pgb_head_loss_fwd_scratch_bytes(x.N, x.V, x.d, code(x.h), k);
+    const long long n = pgb_head_loss_fwd_scratch_bytes(x.N, x.V, x.d, code(x.h));
     const Tensor scratch = bytes(x.h, n);
     float *row = reduction == REDUCE_NONE ? fp(r.loss) : nullptr, *loss = reduction == REDUCE_NONE ? nullptr : fp(r.loss);
     if (list)
-        check(pgb_linear_distill_fwd(vp(x.h), vp(x.w), code(x.h), static_cast<int *>(vp(t.lists)), static_cast<unsigned *>(vp(t.starts)), fp(t.ent), k, t.tau, row, loss, fp(r.count), fp(r.L),
+        check(pgb_linear_distill_fwd(vp(x.h), vp(x.w), code(x.h), static_cast<int *>(vp(t.lists)), static_cast<unsigned *>(vp(t.marks)), fp(t.ent), fp(t.kept), k, t.tau, row, loss, fp(r.count), fp(r.L),
                                      vp(scratch), n, reduction, x.N, x.V, x.d, dev.stream), what);
     else
         check(pgb_linear_xent_fwd(vp(x.h), vp(x.w), code(x.h), static_cast<long long *>(vp(t.target)), t.ignore, row, loss, fp(r.count), fp(r.L), vp(scratch),
@@ -460,7 +460,7 @@ std::tuple<Tensor, Tensor> head_bwd(const char *what, const HeadIn &x, const Hea
     const long long n = pgb_head_loss_bwd_scratch_bytes(x.N, x.V, x.d, code(x.h), want_dh, want_dw);
     const Tensor scratch = bytes(x.h, n);
     if (t.lists.defined())
-        check(pgb_linear_distill_bwd(vp(x.h), vp(x.w), code(x.h), static_cast<int *>(vp(t.lists)), static_cast<unsigned *>(vp(t.starts)), fp(t.ent), t.lists.size(1), t.tau, fp(L), fp(count),
+        check(pgb_linear_distill_bwd(vp(x.h), vp(x.w), code(x.h), static_cast<int *>(vp(t.lists)), static_cast<unsigned *>(vp(t.marks)), fp(t.ent), fp(t.kept), t.lists.size(1), t.tau, fp(L), fp(count),
                                      fp(grad), vp(dh), vp(dw), vp(scratch), n, reduction, x.N, x.V, x.d, dev.stream), what);
     else
         check(pgb_linear_xent_bwd(vp(x.h), vp(x.w), code(x.h), static_cast<long long *>(vp(t.target)), t.ignore, fp(L), fp(count), fp(grad), vp(dh), vp(dw),
@@ -472,7 +472,7 @@ HeadWant xent_want(const HeadIn &x, const Tensor &h, const Tensor &target, int64
     need_cuda(target);
     same_device(XENT, h, target);
     TORCH_CHECK_VALUE(target.sizes() == h.sizes().slice(0, h.dim() - 1), XENT, ": a target per row of h, got ", target.sizes(), " for ", h.sizes());
-    return {whole_numbers(XENT, target).reshape({x.N}), ignore, Tensor(), Tensor(), Tensor(), 1.0};
+    return {whole_numbers(XENT, target).reshape({x.N}), ignore, Tensor(), Tensor(), Tensor(), Tensor(), 1.0};
 }
 std::tuple<Tensor, Tensor, Tensor> teacher_lists(const Tensor &ids_, const Tensor &logits_, double tau, int64_t V) {
     need_cuda(ids_, logits_);
@@ -485,18 +485,18 @@ std::tuple<Tensor, Tensor, Tensor> teacher_lists(const Tensor &ids_, const Tenso
     const int64_t N = ids_.numel() / k;
     OnDevice dev(ids_);
     const Tensor ids = whole_numbers(DISTILL, ids_).reshape({N, k}), logits = f32c(logits_).reshape({N, k});
-    Tensor lists = alloc(ids, {N, k, 2}, at::kInt), starts = alloc(ids, {N, (V + 63) / 64}, at::kInt), ent = alloc(ids, {N}, at::kFloat);
+    Tensor lists = alloc(ids, {N, k, 2}, at::kInt), marks = alloc(ids, {N, (V + 63) / 64, 4}, at::kInt), ent = alloc(ids, {N}, at::kFloat);
     if (N > 0)
-        check(pgb_teacher_lists(static_cast<long long *>(vp(ids)), fp(logits), tau, static_cast<int *>(vp(lists)), static_cast<unsigned *>(vp(starts)), fp(ent), N, V,
+        check(pgb_teacher_lists(static_cast<long long *>(vp(ids)), fp(logits), tau, static_cast<int *>(vp(lists)), static_cast<unsigned *>(vp(marks)), fp(ent), N, V,
                                 k, dev.stream), "pgb_teacher_lists");
-    return {lists, starts, ent};
+    return {lists, marks, ent};
 }
 HeadWant distill_want(const HeadIn &x, const Tensor &h, const Tensor &ids, const Tensor &logits, double tau) {
     same_device(DISTILL, h, ids);
     TORCH_CHECK_VALUE(ids.dim() == h.dim() && ids.sizes().slice(0, ids.dim() - 1) == h.sizes().slice(0, h.dim() - 1), DISTILL, ": k teacher entries per row of h, got ",
                       ids.sizes(), " for ", h.sizes());
-    auto [lists, starts, ent] = teacher_lists(ids, logits, tau, x.V);
-    return {Tensor(), 0, lists, starts, ent, tau};
+    auto [lists, marks, ent] = teacher_lists(ids, logits, tau, x.V);
+    return {Tensor(), 0, lists, marks, ent, alloc(x.h, {x.N, lists.size(1)}, at::kFloat), tau};
 }
 
 // Either loss with its gradients: what the backward pass reads is h, W, the targets and two numbers a row.
@@ -507,7 +507,7 @@ struct HeadLoss : torch::autograd::Function<HeadLoss> {
         const HeadIn x = head_in(what, h_, w_);
         const HeadWant t = target ? xent_want(x, h_, *target, ignore) : distill_want(x, h_, *ids, *logits, tau);
         HeadOut r = head_fwd(what, x, t, reduction);
-        ctx->save_for_backward({x.h, x.w, t.target, t.lists, t.starts, t.ent, r.L, r.count});
+        ctx->save_for_backward({x.h, x.w, t.target, t.lists, t.marks, t.ent, t.kept, r.L, r.count});
         auto &d = ctx->saved_data;
         d["ignore"] = ignore; d["tau"] = tau; d["reduction"] = reduction; d["shape"] = h_.sizes().vec();
         ctx->set_materialize_grads(false);
@@ -520,9 +520,9 @@ struct HeadLoss : torch::autograd::Function<HeadLoss> {
         const variable_list s = ctx->get_saved_variables();
         auto &d = ctx->saved_data;
         const HeadIn x{s[0], s[1], s[0].size(0), s[1].size(0), s[1].size(1)};
-        const HeadWant t{s[2], d["ignore"].toInt(), s[3], s[4], s[5], d["tau"].toDouble()};
+        const HeadWant t{s[2], d["ignore"].toInt(), s[3], s[4], s[5], s[6], d["tau"].toDouble()};
         const bool list = t.lists.defined();
-        auto [dh, dw] = head_bwd(list ? DISTILL : XENT, x, t, s[6], s[7], g[0].reshape({-1}), d["reduction"].toInt(), ctx->needs_input_grad(0), ctx->needs_input_grad(1));
+        auto [dh, dw] = head_bwd(list ? DISTILL : XENT, x, t, s[7], s[8], g[0].reshape({-1}), d["reduction"].toInt(), ctx->needs_input_grad(0), ctx->needs_input_grad(1));
         none[0] = dh.defined() ? dh.view(d["shape"].toIntVector()) : dh;
         none[1] = dw;
         return once(list ? "pragnosia_b200 linear_distill" : "pragnosia_b200 linear_cross_entropy", s, none, g);
@@ -647,15 +647,16 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     }, nogil);
     m.def("teacher_lists", &teacher_lists, nogil);
     m.def("linear_distill", &linear_distill, nogil);
-    m.def("linear_distill_fwd", [](const Tensor &h, const Tensor &w, const Tensor &lists, const Tensor &starts, const Tensor &ent, double tau, int reduction) {
+    m.def("linear_distill_fwd", [](const Tensor &h, const Tensor &w, const Tensor &lists, const Tensor &marks, const Tensor &ent, double tau, int reduction) {
         const HeadIn x = head_in(DISTILL, h, w);
-        HeadOut r = head_fwd(DISTILL, x, {Tensor(), 0, lists, starts, ent, tau}, reduction);
-        return std::make_tuple(r.loss, r.L, r.count);
+        const Tensor kept = alloc(x.h, {x.N, lists.size(1)}, at::kFloat);
+        HeadOut r = head_fwd(DISTILL, x, {Tensor(), 0, lists, marks, ent, kept, tau}, reduction);
+        return std::make_tuple(r.loss, r.L, r.count, kept);
     }, nogil);
-    m.def("linear_distill_bwd", [](const Tensor &h, const Tensor &w, const Tensor &lists, const Tensor &starts, const Tensor &ent, double tau, const Tensor &L,
-                                   const Tensor &count, const Tensor &grad, int reduction, bool want_dh, bool want_dw) {
+    m.def("linear_distill_bwd", [](const Tensor &h, const Tensor &w, const Tensor &lists, const Tensor &marks, const Tensor &ent, const Tensor &kept, double tau,
+                                   const Tensor &L, const Tensor &count, const Tensor &grad, int reduction, bool want_dh, bool want_dw) {
         const HeadIn x = head_in(DISTILL, h, w);
-        auto [dh, dw] = head_bwd(DISTILL, x, {Tensor(), 0, lists, starts, ent, tau}, L, count, grad, reduction, want_dh, want_dw);
+        auto [dh, dw] = head_bwd(DISTILL, x, {Tensor(), 0, lists, marks, ent, kept, tau}, L, count, grad, reduction, want_dh, want_dw);
         return std::make_tuple(some(dh), some(dw));
     }, nogil);
     m.def("embedding", &embedding, nogil);

@@ -492,47 +492,49 @@ linear_xent.register_autograd(_xent_grads, setup_context=_xent_ctx)
 
 @torch.library.custom_op(f"{NS}::teacher_lists", mutates_args=())
 def teacher_lists(ids: Tensor, logits: Tensor, temperature: float, V: int) -> Tuple[Tensor, Tensor, Tensor]:
-    """A teacher's entries as linear_distill takes them: (id, bits of its probability) by id, where the entries of every 64 words begin, the sum of p log p."""
+    """A teacher's entries as linear_distill takes them: (id, bits of its probability) by id, which of every 64 words they are, the sum of p log p."""
     return host().teacher_lists(ids, logits, temperature, V)
 
 
 @teacher_lists.register_fake
 def _(ids, logits, temperature, V):
     n, k = _rows(ids), ids.shape[-1]
-    return _e(ids, n, k, 2, dtype=torch.int32), _e(ids, n, (V + 63) // 64, dtype=torch.int32), _e(ids, n, dtype=_F32)
+    return _e(ids, n, k, 2, dtype=torch.int32), _e(ids, n, (V + 63) // 64, 4, dtype=torch.int32), _e(ids, n, dtype=_F32)
 
 
 @torch.library.custom_op(f"{NS}::linear_distill", mutates_args=())
-def linear_distill(h: Tensor, W: Tensor, lists: Tensor, starts: Tensor, ent: Tensor, temperature: float, reduction: int) -> Tuple[Tensor, Tensor, Tensor]:
-    return host().linear_distill_fwd(h, W, lists, starts, ent, temperature, reduction)
+def linear_distill(h: Tensor, W: Tensor, lists: Tensor, marks: Tensor, ent: Tensor, temperature: float,
+                   reduction: int) -> Tuple[Tensor, Tensor, Tensor, Tensor]:
+    """As linear_xent, and the entries' logits for the backward pass."""
+    return host().linear_distill_fwd(h, W, lists, marks, ent, temperature, reduction)
 
 
 @linear_distill.register_fake
-def _(h, W, lists, starts, ent, temperature, reduction):
-    return _loss_like(h, reduction), _e(h, _rows(h), 2, dtype=_F32), _e(h, dtype=_F32)
+def _(h, W, lists, marks, ent, temperature, reduction):
+    return _loss_like(h, reduction), _e(h, _rows(h), 2, dtype=_F32), _e(h, dtype=_F32), _e(h, _rows(h), lists.shape[1], dtype=_F32)
 
 
 @torch.library.custom_op(f"{NS}::linear_distill_bwd", mutates_args=())
-def linear_distill_bwd(h: Tensor, W: Tensor, lists: Tensor, starts: Tensor, ent: Tensor, temperature: float, L: Tensor, count: Tensor, grad: Tensor, reduction: int,
-                       want_dh: bool, want_dW: bool) -> Tuple[Tensor, Tensor]:
-    dh, dW = host().linear_distill_bwd(h, W, lists, starts, ent, temperature, L, count, grad, reduction, want_dh, want_dW)
+def linear_distill_bwd(h: Tensor, W: Tensor, lists: Tensor, marks: Tensor, ent: Tensor, kept: Tensor, temperature: float, L: Tensor, count: Tensor, grad: Tensor,
+                       reduction: int, want_dh: bool, want_dW: bool) -> Tuple[Tensor, Tensor]:
+    dh, dW = host().linear_distill_bwd(h, W, lists, marks, ent, kept, temperature, L, count, grad, reduction, want_dh, want_dW)
     return (dh.view(h.shape) if want_dh else _none(h)), (dW if want_dW else _none(W))
 
 
 @linear_distill_bwd.register_fake
-def _(h, W, lists, starts, ent, temperature, L, count, grad, reduction, want_dh, want_dW):
+def _(h, W, lists, marks, ent, kept, temperature, L, count, grad, reduction, want_dh, want_dW):
     return _grads_like(h, W, want_dh, want_dW)
 
 
 def _distill_ctx(ctx, inputs, output):
-    h, W, lists, starts, ent, ctx.temperature, ctx.reduction = inputs
-    ctx.save_for_backward(h, W, lists, starts, ent, output[1], output[2])
+    h, W, lists, marks, ent, ctx.temperature, ctx.reduction = inputs
+    ctx.save_for_backward(h, W, lists, marks, ent, output[3], output[1], output[2])
 
 
-def _distill_grads(ctx, g, _L, _count):
-    h, W, lists, starts, ent, L, count = ctx.saved_tensors
+def _distill_grads(ctx, g, _L, _count, _kept):
+    h, W, lists, marks, ent, kept, L, count = ctx.saved_tensors
     want = ctx.needs_input_grad[:2]
-    dh, dW = torch.ops.pragnosia_b200.linear_distill_bwd(h, W, lists, starts, ent, ctx.temperature, L, count, g, ctx.reduction, *want)
+    dh, dW = torch.ops.pragnosia_b200.linear_distill_bwd(h, W, lists, marks, ent, kept, ctx.temperature, L, count, g, ctx.reduction, *want)
     return (dh if want[0] else None), (dW if want[1] else None), None, None, None, None, None
 
 

@@ -58,8 +58,8 @@ def linear_distill(h, weight, teacher_ids, teacher_logits, *, temperature: float
         if out is not None:
             return out
     ops = _operators()
-    lists, starts, ent = ops.teacher_lists(teacher_ids, teacher_logits.detach(), float(temperature), weight.shape[0])
-    loss = ops.linear_distill(h, weight, lists, starts, ent, float(temperature), r)[0]
+    lists, marks, ent = ops.teacher_lists(teacher_ids, teacher_logits.detach(), float(temperature), weight.shape[0])
+    loss = ops.linear_distill(h, weight, lists, marks, ent, float(temperature), r)[0]
     return loss.view(h.shape[:-1]) if r == 0 else loss
 
 
