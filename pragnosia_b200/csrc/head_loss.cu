@@ -11,8 +11,10 @@
 //   Pieces: along the longer of N and V, so that the gradient that gathers over pieces (fp32, added to in place) is the smaller one.
 //   ds holds no upstream scale where that is the same for every row (mean, sum): the scale is applied to the fp32 accumulators.
 //   Rounded to bf16, ds is off by 2^-9 of itself, as the gradients themselves are when they are bf16.
-//   fp32 operands: three bf16 terms each (24 bits), six of the nine products (what is left out is below 2^-23 of the sum's terms), small
-//   ones first, all into one accumulator; ds as three terms as well.
+//   fp32 operands: three bf16 terms each (24 bits), six of the nine products (what is left out is below 2^-23 of the sum's terms); ds as
+//   three terms as well. The tensor cores cut off what a partial sum has beyond fp32 instead of rounding it, so sums over a long K axis
+//   drift (gradients were off by 5e-6 to 8e-6): there a block of 64 has an accumulator of its own, small products first, and the
+//   blocks are added in registers.
 // The product: pairs of SMs, 256 x 256 tiles, tcgen05.mma.cta_group::2, six 32 KiB stages a CTA fed by TMA, two accumulators in tensor
 // memory so that a tile's epilogue runs under the next one's products; 16 epilogue warps, a row and a column quarter each.
 #include <math.h>
@@ -35,12 +37,11 @@ struct HlMaps { CUtensorMap a[3], b[3], ds; };                        // of the 
 // An epilogue warp's share of a tile: rows row0 .. +31 (a lane each), columns col0 .. +63; block: which of the tile's 32 it is. g, t, sp: the
 // product, its tile, and the part of K that the accumulator holds.
 struct HlTile { int lane, sub, part, block, n, row0, col0, g, t, sp; uint32_t ti; };
-// One product C[M][N] = A B^T over kb blocks of 64 (npairs times: the products of the operands' bf16 terms), its K axis in `splits` parts.
+// One product C[M][N] = A B^T over kb blocks of 64, its K axis in `splits` parts.
 // a_mn / b_mn: the operand lies with its M / N axis contiguous instead of K.
 struct HlProduct {
-    int tiles_m = 0, tiles_n = 0, kb = 0, npairs = 1, splits = 1, a_mn = 0, b_mn = 0;
+    int tiles_m = 0, tiles_n = 0, kb = 0, splits = 1, a_mn = 0, b_mn = 0;
     __host__ __device__ int tiles() const { return tiles_m * tiles_n; }
-    __host__ __device__ int kt() const { return kb * npairs; }
     // row blocks fastest, HL_GROUP of them at a time: B is read once per group, whatever its size
     __device__ void at(int t, int &m, int &n) const {
         const unsigned group = (unsigned)HL_GROUP * tiles_n, g = (unsigned)t / group, in = (unsigned)t - g * group;
@@ -62,7 +63,7 @@ struct HlOne {
     int pairs, t;
     static constexpr int g = 0, sp = 0, k0 = 0;
     int k1;
-    __device__ HlOne(const HlProduct &pr, int pair, int pairs) : pr(pr), pairs(pairs), t(pair), k1(pr.kt()) {}
+    __device__ HlOne(const HlProduct &pr, int pair, int pairs) : pr(pr), pairs(pairs), t(pair), k1(pr.kb) {}
     __device__ __forceinline__ const HlProduct &product() const { return pr; }
     __device__ __forceinline__ bool more() const { return t < pr.tiles(); }
     __device__ __forceinline__ void next() { t += pairs; }
@@ -81,29 +82,24 @@ struct HlThree {
     __device__ __forceinline__ void place(int first) {
         const int n0 = w.p[0].tiles() * w.p[0].splits, n1 = w.p[1].tiles() * w.p[1].splits;
         if (i >= n0 + n1) {
-            g = 2; sp = 0; k0 = 0; k1 = w.p[2].kt();
+            g = 2; sp = 0; k0 = 0; k1 = w.p[2].kb;
             t = first >= 0 ? first : w.share[i % pairs];               // i % pairs: the pair
             return;
         }
         g = i >= n0;
-        const int in = g ? i - n0 : i, tiles = w.p[g].tiles(), kt = w.p[g].kt();
+        const int in = g ? i - n0 : i, tiles = w.p[g].tiles(), kt = w.p[g].kb;
         sp = in / tiles;
         t = in - sp * tiles;
         k0 = (int)((long long)kt * sp / w.p[g].splits);
         k1 = (int)((long long)kt * (sp + 1) / w.p[g].splits);
     }
 };
-// the terms of the two operands that product number pp of npairs multiplies (0: the head), small products first
-__device__ __forceinline__ void hl_terms(int pp, int npairs, int &ta, int &tb) {
-    const int q = npairs == 1 ? 5 : pp;                               // (2,0) (0,2) (1,1) (1,0) (0,1) (0,0)
-    ta = (0x001102 >> (4 * q)) & 15;
-    tb = (0x010120 >> (4 * q)) & 15;
-}
-
 // The roles of the kernel. An epilogue warp takes its 32 x 64 block of a complete accumulator into registers, hands the accumulator back at once, and
 // works on them while what the next tile needs of its rows (epi.fetch) is on its way.
-template <class Work, class What, class Epi>
+// FINE: operands of three terms, a stage holds a block of all of them, and an accumulator a block's products.
+template <bool FINE, class Work, class What, class Epi>
 __device__ __forceinline__ void hl_body(const HlMaps &maps, const What &what, Epi &epi) {
+    constexpr int TERMS = FINE ? 3 : 1, STAGE = TERMS * HL_STAGE, STAGES = HL_STAGES / TERMS, OPERAND = TERMS * HL_HALF;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;      // the same offset in both CTAs: one descriptor serves both
     uint8_t *sm = smem_raw + (base - smem_u32(smem_raw));
@@ -145,59 +141,72 @@ __device__ __forceinline__ void hl_body(const HlMaps &maps, const What &what, Ep
             p.at(w.t, m, n);
             const int m0 = m * HL_B + (int)rank * (HL_B / 2), n0 = n * HL_B + (int)rank * (HL_B / 2);
             const CUtensorMap *ma = &maps.a[w.g], *mbm = &maps.b[w.g];
-            int pp = w.k0 / p.kb, kc = w.k0 - pp * p.kb, ta, tb;
-            hl_terms(pp, p.npairs, ta, tb);
             for (int k = w.k0; k < w.k1 && ok; ++k, ++it) {
-                const int s = it % HL_STAGES;
-                if (it >= HL_STAGES) ok = __all_sync(0xffffffffu, mbar_wait(bar_empty(s), ((it / HL_STAGES) + 1) & 1, 91));
+                const int s = it % STAGES;
+                if (it >= STAGES) ok = __all_sync(0xffffffffu, mbar_wait(bar_empty(s), ((it / STAGES) + 1) & 1, 91));
                 if (ok && leader) {
-                    const int c = kc * HL_BK;
-                    const uint32_t sa = base + s * HL_STAGE, sb = sa + HL_HALF, full0 = cluster_addr(bar_full(s), 0);
-                    if (rank == 0) mbar_expect_tx(bar_full(s), 2 * HL_STAGE);      // both CTAs' bytes
-                    if (p.a_mn) {                                      // 64 rows of K, 64 contiguous rows of M at a time
-                        lp_tma_load(sa, ma, full0, m0, c, ta);
-                        lp_tma_load(sa + HL_HALF / 2, ma, full0, m0 + 64, c, ta);
-                    } else {
-                        lp_tma_load(sa, ma, full0, c, m0, ta);
-                    }
-                    if (p.b_mn) {
-                        lp_tma_load(sb, mbm, full0, n0, c, tb);
-                        lp_tma_load(sb + HL_HALF / 2, mbm, full0, n0 + 64, c, tb);
-                    } else {
-                        lp_tma_load(sb, mbm, full0, c, n0, tb);
+                    const int c = k * HL_BK;
+                    const uint32_t full0 = cluster_addr(bar_full(s), 0);
+                    if (rank == 0) mbar_expect_tx(bar_full(s), 2 * STAGE);         // both CTAs' bytes
+#pragma unroll
+                    for (int t = 0; t < TERMS; ++t) {
+                        const uint32_t sa = base + s * STAGE + t * HL_HALF, sb = sa + OPERAND;
+                        if (p.a_mn) {                                  // 64 rows of K, 64 contiguous rows of M at a time
+                            lp_tma_load(sa, ma, full0, m0, c, t);
+                            lp_tma_load(sa + HL_HALF / 2, ma, full0, m0 + 64, c, t);
+                        } else {
+                            lp_tma_load(sa, ma, full0, c, m0, t);
+                        }
+                        if (p.b_mn) {
+                            lp_tma_load(sb, mbm, full0, n0, c, t);
+                            lp_tma_load(sb + HL_HALF / 2, mbm, full0, n0 + 64, c, t);
+                        } else {
+                            lp_tma_load(sb, mbm, full0, c, n0, t);
+                        }
                     }
                 }
-                if (++kc == p.kb) { kc = 0; hl_terms(++pp, p.npairs, ta, tb); }
                 __syncwarp();
             }
         }
     } else if (warp == 1) {
         // ------------------------------------------------------------------------------------------ MMA issuer (first CTA)
         if (rank == 0) {
-            uint32_t it = 0, ti = 0;
+            uint32_t it = 0, ai = 0;                                   // blocks, accumulators so far
             bool ok = true;
-            for (; w.more() && ok; w.next(), ++ti) {
-                const int amn = w.product().a_mn, bmn = w.product().b_mn;
-                const uint32_t idesc = idesc_bf16(HL_B, HL_B, amn, bmn), a = ti & 1;
-                const uint32_t stepa = amn ? 128 : 2, stepb = bmn ? 128 : 2;
-                if (ti >= 2) ok = __all_sync(0xffffffffu, lp_wait_cluster(bar_acc_empty(a), ((ti >> 1) + 1) & 1, 92));
+            auto fresh = [&]() {                                       // the next accumulator, once it has been read
+                if (ai >= 2) ok = __all_sync(0xffffffffu, lp_wait_cluster(bar_acc_empty(ai & 1), ((ai >> 1) + 1) & 1, 92));
                 tc_fence_after();
+                return ok;
+            };
+            auto done = [&]() {
+                lp_commit_elect(bar_acc_full(ai & 1));
+                lp_commit_elect(cluster_addr(bar_acc_full(ai & 1), 1));
+                ++ai;
+            };
+            for (; w.more() && ok; w.next()) {
+                const int amn = w.product().a_mn, bmn = w.product().b_mn;
+                const uint32_t idesc = idesc_bf16(HL_B, HL_B, amn, bmn), stepa = amn ? 128 : 2, stepb = bmn ? 128 : 2;
+                if (!FINE && !fresh()) break;
                 for (int k = w.k0; k < w.k1 && ok; ++k, ++it) {
-                    const int s = it % HL_STAGES;
-                    ok = __all_sync(0xffffffffu, lp_wait_cluster(bar_full(s), (it / HL_STAGES) & 1, 93));
+                    if (FINE && !fresh()) break;
+                    const int s = it % STAGES;
+                    ok = __all_sync(0xffffffffu, lp_wait_cluster(bar_full(s), (it / STAGES) & 1, 93));
                     if (!ok) break;
                     tc_fence_after();
-                    const uint32_t sa = base + s * HL_STAGE;
-                    const uint64_t da = smem_desc(sa, amn ? HL_HALF / 2 : 16, 1024), db = smem_desc(sa + HL_HALF, bmn ? HL_HALF / 2 : 16, 1024);
+                    const uint32_t sa = base + s * STAGE, acc = tmem + (ai & 1) * HL_B;
+                    const uint64_t da = smem_desc(sa, amn ? HL_HALF / 2 : 16, 1024), db = smem_desc(sa + OPERAND, bmn ? HL_HALF / 2 : 16, 1024);
 #pragma unroll
-                    for (int q = 0; q < HL_BK / 16; ++q) lp_mma_elect(tmem + a * HL_B, da + q * stepa, db + q * stepb, idesc, (k > w.k0) | (q > 0));
+                    for (int pp = FINE ? 0 : 5; pp < 6; ++pp) {        // the operands' terms: (2,0) (0,2) (1,1) (1,0) (0,1) (0,0)
+                        const uint32_t ta = (0x001102 >> (4 * pp)) & 15, tb = (0x010120 >> (4 * pp)) & 15;
+#pragma unroll
+                        for (int q = 0; q < HL_BK / 16; ++q)
+                            lp_mma_elect(acc, da + ta * (HL_HALF >> 4) + q * stepa, db + tb * (HL_HALF >> 4) + q * stepb, idesc, FINE ? pp > 0 || q > 0 : (k > w.k0) | (q > 0));
+                    }
                     lp_commit_elect(bar_empty(s));                     // the stage is free in both CTAs once these MMAs have read it
                     lp_commit_elect(cluster_addr(bar_empty(s), 1));
+                    if (FINE) done();
                 }
-                if (ok) {
-                    lp_commit_elect(bar_acc_full(a));
-                    lp_commit_elect(cluster_addr(bar_acc_full(a), 1));
-                }
+                if (!FINE && ok) done();
             }
         }
     } else {
@@ -209,34 +218,60 @@ __device__ __forceinline__ void hl_body(const HlMaps &maps, const What &what, Ep
         HlTile x;
         x.lane = lane; x.sub = sub; x.part = part; x.block = (int)rank * HL_EPI + (warp - 2);
         epi.start(tid - 64);
-        uint32_t ti = 0;
+        uint32_t ti = 0, ai = 0;
         bool ok = w.more();
         if (ok) {
             w.product().at(w.t, m, n);
             epi.fetch(w.g, m * HL_B + row_in + lane, n * HL_B + col_in);
         }
         for (; ok; ++ti) {
-            const uint32_t a = ti & 1;
             x.n = n; x.row0 = m * HL_B + row_in; x.col0 = n * HL_B + col_in; x.ti = ti;
             x.g = w.g; x.t = w.t; x.sp = w.sp;
             epi.begin(x);
-            ok = __all_sync(0xffffffffu, mbar_wait(bar_acc_full(a), (ti >> 1) & 1, 94));
-            if (!ok) break;
-            tc_fence_after();
             float v[2][32];
-            const uint32_t tacc = tmem + lane_base + a * HL_B + part * HL_CW;
-            tmem_ld32_nowait(tacc, v[0]);
-            tmem_ld32_nowait(tacc + 32, v[1]);
-            tmem_ld_wait();
-#pragma unroll
-            for (int i = 0; i < 64; ++i) asm volatile("" : "+f"(v[i >> 5][i & 31]));      // nothing that uses them moves ahead of the wait
-            if (w.k0 == w.k1) {                          // a part of K with nothing in it (fewer blocks than parts)
+            const uint32_t tacc = tmem + lane_base + part * HL_CW;
+            auto full = [&]() {
+                ok = __all_sync(0xffffffffu, mbar_wait(bar_acc_full(ai & 1), (ai >> 1) & 1, 94));
+                tc_fence_after();
+                return ok;
+            };
+            auto hand_back = [&]() {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) lp_arrive_cluster(ai & 1 ? acc_empty1 : acc_empty0);
+                ++ai;
+            };
+            // a load's registers as the wait leaves them: nothing that uses them moves ahead of it
+            if constexpr (FINE) {
 #pragma unroll
                 for (int i = 0; i < 64; ++i) v[i >> 5][i & 31] = 0.f;
+                for (int k = w.k0; k < w.k1 && full(); ++k) {
+#pragma unroll
+                    for (int b = 0; b < 4; ++b) {
+                        float u[16];
+                        tmem_ld16_nowait(tacc + (ai & 1) * HL_B + 16 * b, u);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) asm volatile("" : "+f"(u[i]));
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) v[b >> 1][16 * (b & 1) + i] += u[i];
+                    }
+                    hand_back();
+                }
+                if (!ok) break;
+            } else {
+                if (!full()) break;
+                tmem_ld32_nowait(tacc + (ai & 1) * HL_B, v[0]);
+                tmem_ld32_nowait(tacc + (ai & 1) * HL_B + 32, v[1]);
+                tmem_ld_wait();
+#pragma unroll
+                for (int i = 0; i < 64; ++i) asm volatile("" : "+f"(v[i >> 5][i & 31]));
+                if (w.k0 == w.k1) {                                    // a part of K with nothing in it (fewer blocks than parts)
+#pragma unroll
+                    for (int i = 0; i < 64; ++i) v[i >> 5][i & 31] = 0.f;
+                }
+                hand_back();
             }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) lp_arrive_cluster(a ? acc_empty1 : acc_empty0);
             w.next();
             const bool more = w.more();
             if (more) {
@@ -353,11 +388,11 @@ struct HlFwdEpi {
         return ok;
     }
 };
-template <bool LIST>
+template <bool LIST, bool FINE>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(HL_NT, 1)
 head_loss_fwd_kernel(const __grid_constant__ HlMaps maps, const __grid_constant__ HlProduct pr, const __grid_constant__ HlFwd f) {
     HlFwdEpi<LIST> epi{f};
-    hl_body<HlOne>(maps, pr, epi);
+    hl_body<FINE, HlOne>(maps, pr, epi);
 }
 
 // Joins a row's tiles: 32 rows a block (a lane each), the tiles dealt out to its 8 warps, then the block's losses and live rows as one
@@ -749,7 +784,7 @@ template <bool LIST, int TERMS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(HL_NT, 1)
 head_loss_bwd_kernel(const __grid_constant__ HlMaps maps, const __grid_constant__ HlTrio work, const __grid_constant__ HlBwd f) {
     HlBwdEpi<LIST, TERMS> epi{{f.ds, &maps.ds}, {f.grads, work.p, 0.f}};
-    hl_body<HlThree>(maps, work, epi);
+    hl_body<TERMS == 3, HlThree>(maps, work, epi);
 }
 
 // x as three bf16 terms, [3][n]; eight values a thread (n a multiple of 8)
@@ -871,12 +906,16 @@ int head_loss_fwd_launch(const HeadLossArgs &x, float *row_loss, float *loss, fl
     HlMaps maps;
     if (!hl_map(&maps.a[0], h, 0, 0, x.N, x.d, false) || !hl_map(&maps.b[0], w, 0, 0, x.V, x.d, false)) return hl_no_map();
     HlProduct pr;
-    pr.tiles_m = hl_tiles(x.N); pr.tiles_n = (int)pl.tiles; pr.kb = (x.d + HL_BK - 1) / HL_BK; pr.npairs = h.terms == 3 ? 6 : 1;
+    pr.tiles_m = hl_tiles(x.N); pr.tiles_n = (int)pl.tiles; pr.kb = (x.d + HL_BK - 1) / HL_BK;
     const HlTargets t{x.target, x.ignore, reinterpret_cast<const int2 *>(x.lists), reinterpret_cast<const uint4 *>(x.marks), x.ent, x.k, (x.V + 63) / 64};
     const HlFwd f{t, LOG2E_F / x.tau, reinterpret_cast<float2 *>(s + pl.off_ml), list ? x.kept : reinterpret_cast<float *>(s + pl.off_dot),
                   reinterpret_cast<unsigned *>(s + pl.off_ticket), x.N, pl.Np, x.V};
-    rc = list ? hl_launch(head_loss_fwd_kernel<true>, 0, "head_loss_fwd_kernel", maps, pr, pr.tiles(), f, stream)
-              : hl_launch(head_loss_fwd_kernel<false>, 1, "head_loss_fwd_kernel", maps, pr, pr.tiles(), f, stream);
+    if (h.terms == 3)
+        rc = list ? hl_launch(head_loss_fwd_kernel<true, true>, 0, "head_loss_fwd_kernel", maps, pr, pr.tiles(), f, stream)
+                  : hl_launch(head_loss_fwd_kernel<false, true>, 1, "head_loss_fwd_kernel", maps, pr, pr.tiles(), f, stream);
+    else
+        rc = list ? hl_launch(head_loss_fwd_kernel<true, false>, 2, "head_loss_fwd_kernel", maps, pr, pr.tiles(), f, stream)
+                  : hl_launch(head_loss_fwd_kernel<false, false>, 3, "head_loss_fwd_kernel", maps, pr, pr.tiles(), f, stream);
     if (rc != PGB_OK) return rc;
     const HlJoin j{t, f.ml, f.dot, reinterpret_cast<float2 *>(L), row_loss, loss, count, reinterpret_cast<double2 *>(s + pl.off_partial), f.ticket,
                    x.N, pl.Np, x.V, (int)pl.tiles, x.tau, x.reduction};
@@ -890,8 +929,8 @@ struct HlBwdPlan {
     bool by_rows; long long step, pieces, ldp, rows, cols; int terms, s_dh[2], s_dw[2];          // parts in all pieces but the last, in the last
     long long off_p[2], off_dh, off_dw, off_h, off_w, total;
 };
-// A launch's work in units of a K block's time (0.33 us): a part of a tile costs its K blocks and about four more (its epilogue's end and the
-// next one's beginning).
+// A launch's work in units of the time of a K block's one product (0.33 us; np of them a block): a part of a tile costs its own and about four
+// more (its epilogue's end and the next one's beginning).
 struct HlLoad {
     long long n0, n, f0, r0, f, r; double c0, c1;                      // parts of the first product, of both; rounds and rest of either number over the pairs
     HlLoad(long long t0, long long k0, int s0, long long t1, long long k1, int s1, int pairs) : n0(t0 * s0), n(t0 * s0 + t1 * s1), f0(n0 / pairs), r0(n0 % pairs),
@@ -909,13 +948,13 @@ struct HlLoad {
 constexpr double HL_DS = 5.0;                                         // what a tile of ds costs beyond its K blocks
 struct HlSplits { int dh, dw; double cost; };
 // The parts of K with which the pairs finish earliest, `filler` units of short tiles dealt out behind them. fix0, fix1: parts that are given (0: to be chosen).
-static HlSplits hl_splits(long long t0, long long k0, long long t1, long long k1, double filler, int pairs, int fix0, int fix1) {
+static HlSplits hl_splits(long long t0, long long k0, long long t1, long long k1, double filler, int np, int pairs, int fix0, int fix1) {
     static const int choice[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 24, 32};
     HlSplits best{1, 1, 1e300};
     for (int a : choice) {
-        if (a > 1 && (fix0 || t0 == 0 || k0 / a < 4)) break;
+        if (a > 1 && (fix0 || t0 == 0 || k0 / a < 4 * np)) break;
         for (int b : choice) {
-            if (b > 1 && (fix1 || t1 == 0 || k1 / b < 4)) break;
+            if (b > 1 && (fix1 || t1 == 0 || k1 / b < 4 * np)) break;
             const int s0 = fix0 ? fix0 : a, s1 = fix1 ? fix1 : b;
             const HlLoad load(t0, k0, s0, t1, k1, s1, pairs);
             const double level = (load.all() + filler) / pairs, most = load.most();
@@ -938,7 +977,7 @@ static HlBwdPlan hl_bwd_plan(long long N, int V, int d, int dtype, bool dh, bool
     auto of = [&](long long n, long long m, int gather) {
         const long long t0 = along_d ? hl_tiles(n) * td : 0, t1 = across_d ? ta * td : 0, k1 = (n + HL_BK - 1) / HL_BK * np;
         const double filler = (double)hl_tiles(m) * ta * (kd + HL_DS);
-        HlSplits s = p.by_rows ? hl_splits(t0, ka, t1, k1, filler, pairs, 0, gather) : hl_splits(t1, k1, t0, ka, filler, pairs, gather, 0);
+        HlSplits s = p.by_rows ? hl_splits(t0, ka, t1, k1, filler, np, pairs, 0, gather) : hl_splits(t1, k1, t0, ka, filler, np, pairs, gather, 0);
         s.cost += 20.0;                                                // a launch's beginning and end
         return s;
     };
@@ -977,11 +1016,11 @@ static HlBwdPlan hl_bwd_plan(long long N, int V, int d, int dtype, bool dh, bool
     return p;
 }
 // pair q's tiles of ds: as many as bring it to the level that all of them reach
-static void hl_share(HlTrio &w, int pairs) {
+static void hl_share(HlTrio &w, int np, int pairs) {
     const HlProduct &a = w.p[0], &b = w.p[1];
     const int tiles = w.p[2].tiles();
-    const HlLoad load(a.tiles(), a.kt(), a.splits, b.tiles(), b.kt(), b.splits, pairs);
-    const double c = w.p[2].kt() + HL_DS;
+    const HlLoad load(a.tiles(), (long long)a.kb * np, a.splits, b.tiles(), (long long)b.kb * np, b.splits, pairs);
+    const double c = w.p[2].kb * np + HL_DS;
     double level = (load.all() + tiles * c) / pairs;
     for (int round = 0; round < 4 && load.n > 0 && tiles > 0; ++round) {                         // pairs above the level have none and raise it for the others
         double over = 0.0;
@@ -1021,8 +1060,8 @@ int head_loss_bwd_launch(const HeadLossArgs &x, const float *L, const float *cou
     if (rc != PGB_OK) return rc;
     const int np = pl.terms == 3 ? 6 : 1, esize = x.dtype == PGB_F32 ? 4 : 2;
     const int which = (pl.terms == 3) * 2 + list;
-    const int room = which == 0 ? hl_pairs(head_loss_bwd_kernel<false, 1>, 2) : which == 1 ? hl_pairs(head_loss_bwd_kernel<true, 1>, 3)
-                   : which == 2 ? hl_pairs(head_loss_bwd_kernel<false, 3>, 4) : hl_pairs(head_loss_bwd_kernel<true, 3>, 5);
+    const int room = which == 0 ? hl_pairs(head_loss_bwd_kernel<false, 1>, 4) : which == 1 ? hl_pairs(head_loss_bwd_kernel<true, 1>, 5)
+                   : which == 2 ? hl_pairs(head_loss_bwd_kernel<false, 3>, 6) : hl_pairs(head_loss_bwd_kernel<true, 3>, 7);
     if (room < 1) { set_cuda_error(cudaGetLastError(), "head_loss_bwd_kernel"); return PGB_ERR_CUDA; }
     auto at = [&](long long off) { return off >= 0 ? reinterpret_cast<float *>(s + off) : nullptr; };
     auto piece = [&](int i) { return HlOperand{s + pl.off_p[i & 1], pl.terms, pl.rows * pl.ldp, pl.ldp}; };
@@ -1041,7 +1080,7 @@ int head_loss_bwd_launch(const HeadLossArgs &x, const float *L, const float *cou
             const long long rows = rows_of(i), cols = cols_of(i), row_from = pl.by_rows ? i * pl.step : 0, col_from = pl.by_rows ? 0 : i * pl.step;
             mapped = hl_map(&maps.a[2], h, row_from, 0, rows, x.d, false) && hl_map(&maps.b[2], w, col_from, 0, cols, x.d, false) && hl_store_map(&maps.ds, piece(i), rows, cols);
             HlProduct &q = work.p[2];
-            q.tiles_m = hl_tiles(rows); q.tiles_n = hl_tiles(cols); q.kb = (x.d + HL_BK - 1) / HL_BK; q.npairs = np;
+            q.tiles_m = hl_tiles(rows); q.tiles_n = hl_tiles(cols); q.kb = (x.d + HL_BK - 1) / HL_BK;
             f.ds.row_from = (int)row_from; f.ds.rows = (int)rows; f.ds.col_from = (int)col_from; f.ds.cols = (int)cols;
         }
         if (i > 0) {
@@ -1050,14 +1089,14 @@ int head_loss_bwd_launch(const HeadLossArgs &x, const float *L, const float *cou
             if (dh) {                                                  // dh[rows] += ds W[cols]
                 mapped = mapped && hl_map(&maps.a[0], piece(j), 0, 0, rows, cols, false) && hl_map(&maps.b[0], w, col_from, 0, cols, x.d, true);
                 HlProduct &q = work.p[0];
-                q.tiles_m = hl_tiles(rows); q.tiles_n = hl_tiles(x.d); q.kb = (int)((cols + HL_BK - 1) / HL_BK); q.npairs = np; q.splits = pl.s_dh[last]; q.b_mn = 1;
+                q.tiles_m = hl_tiles(rows); q.tiles_n = hl_tiles(x.d); q.kb = (int)((cols + HL_BK - 1) / HL_BK); q.splits = pl.s_dh[last]; q.b_mn = 1;
                 const bool gathers = !pl.by_rows && pl.pieces > 1;
                 f.grads.g[0] = {at(pl.off_dh), static_cast<char *>(dh) + row_from * x.d * esize, rows, gathers && !first, !gathers || last};
             }
             if (dw) {                                                  // dW[cols] += ds^T h[rows]
                 mapped = mapped && hl_map(&maps.a[1], piece(j), 0, 0, rows, cols, true) && hl_map(&maps.b[1], h, row_from, 0, rows, x.d, true);
                 HlProduct &q = work.p[1];
-                q.tiles_m = hl_tiles(cols); q.tiles_n = hl_tiles(x.d); q.kb = (int)((rows + HL_BK - 1) / HL_BK); q.npairs = np; q.splits = pl.s_dw[last]; q.a_mn = 1; q.b_mn = 1;
+                q.tiles_m = hl_tiles(cols); q.tiles_n = hl_tiles(x.d); q.kb = (int)((rows + HL_BK - 1) / HL_BK); q.splits = pl.s_dw[last]; q.a_mn = 1; q.b_mn = 1;
                 const bool gathers = pl.by_rows && pl.pieces > 1;
                 f.grads.g[1] = {at(pl.off_dw), static_cast<char *>(dw) + col_from * x.d * esize, cols, gathers && !first, !gathers || last};
             }
@@ -1065,11 +1104,11 @@ int head_loss_bwd_launch(const HeadLossArgs &x, const float *L, const float *cou
         if (!mapped) return hl_no_map();
         const long long parts = (long long)work.p[0].tiles() * work.p[0].splits + (long long)work.p[1].tiles() * work.p[1].splits + work.p[2].tiles();
         const int pairs = (int)(parts < room ? parts : room < HL_MOST_PAIRS ? room : HL_MOST_PAIRS);
-        hl_share(work, pairs);
-        rc = which == 0 ? hl_launch(head_loss_bwd_kernel<false, 1>, 2, "head_loss_bwd_kernel", maps, work, pairs, f, stream)
-           : which == 1 ? hl_launch(head_loss_bwd_kernel<true, 1>, 3, "head_loss_bwd_kernel", maps, work, pairs, f, stream)
-           : which == 2 ? hl_launch(head_loss_bwd_kernel<false, 3>, 4, "head_loss_bwd_kernel", maps, work, pairs, f, stream)
-                        : hl_launch(head_loss_bwd_kernel<true, 3>, 5, "head_loss_bwd_kernel", maps, work, pairs, f, stream);
+        hl_share(work, np, pairs);
+        rc = which == 0 ? hl_launch(head_loss_bwd_kernel<false, 1>, 4, "head_loss_bwd_kernel", maps, work, pairs, f, stream)
+           : which == 1 ? hl_launch(head_loss_bwd_kernel<true, 1>, 5, "head_loss_bwd_kernel", maps, work, pairs, f, stream)
+           : which == 2 ? hl_launch(head_loss_bwd_kernel<false, 3>, 6, "head_loss_bwd_kernel", maps, work, pairs, f, stream)
+                        : hl_launch(head_loss_bwd_kernel<true, 3>, 7, "head_loss_bwd_kernel", maps, work, pairs, f, stream);
         if (rc == PGB_OK && list && i < pl.pieces) {
             const HlOperand P = piece(i);
             __nv_bfloat16 *to = static_cast<__nv_bfloat16 *>(const_cast<void *>(P.ptr));
