@@ -436,6 +436,23 @@ def _(x, W, bias, act):
     return _e(x, *x.shape[:-1], W.shape[0])
 
 
+def _linear_act_ctx(ctx, inputs, output):
+    x, W, bias, ctx.act = inputs
+    ctx.save_for_backward(x, W, bias)
+
+
+def _linear_act_grads(ctx, g):
+    """Through the pre-activation, computed again: it is as large as the result, which the layer behind keeps."""
+    x, W, bias = ctx.saved_tensors
+    if ctx.act == 1:
+        g = torch.ops.aten.gelu_backward(g, torch.nn.functional.linear(x, W, bias))
+    want = ctx.needs_input_grad
+    return (g @ W if want[0] else None, g.t() @ x if want[1] else None, g.sum(0, dtype=_F32).to(g.dtype) if bias is not None and want[2] else None, None)
+
+
+linear_act.register_autograd(_linear_act_grads, setup_context=_linear_act_ctx)
+
+
 # ------------------------------------------------------------------------------------------------ embedding, losses over the vocabulary
 def _rows(h):
     n = 1

@@ -621,7 +621,7 @@ def decode_sample(logits, temp, seed, tok, count, ticket, hist=None, pos=None, s
 
 @on_device_of
 def linear_act(x, W, bias=None, act: Optional[str] = "gelu"):
-    """act(x W^T + bias) as one tensor-core GEMM with the bias and the (erf) GELU in its epilogue; x (..., K) bf16, W (N, K)."""
+    """act(x W^T + bias) as one tensor-core GEMM with the bias and the (erf) GELU in its epilogue; x (..., K) bf16, W (N, K). Differentiable."""
     need_cuda(x, W)
     if x.dtype != torch.bfloat16 or W.dtype != torch.bfloat16:
         raise ValueError("linear_act: bf16 only")
@@ -629,8 +629,8 @@ def linear_act(x, W, bias=None, act: Optional[str] = "gelu"):
     x2 = x.reshape(-1, K).contiguous()
     W = W.contiguous()
     b = None if bias is None else bias.to(x.dtype).contiguous()
-    if _compiling():
-        return _cops().linear_act(x2, W, b, 1 if act == "gelu" else 0).view(*x.shape[:-1], N)
+    if _compiling() or _needs_grad(x2, W, b):
+        return _cops().linear_act(x2, W, b, 1 if act == "gelu" else 0).view(*x.shape[:-1], N)      # the operator carries the backward
     y = torch.empty(x2.shape[0], N, device=x.device, dtype=x.dtype)
     check(lib().pgb_linear_act(ptr(x2), ptr(W), ptr(b), ptr(y), x2.shape[0], N, K, 1 if act == "gelu" else 0,
                                stream_of(x)), "pgb_linear_act")
