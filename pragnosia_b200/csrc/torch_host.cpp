@@ -528,19 +528,36 @@ struct HeadLoss : torch::autograd::Function<HeadLoss> {
         return once(list ? "pragnosia_b200 linear_distill" : "pragnosia_b200 linear_cross_entropy", s, none, g);
     }
 };
+// A backward pass captured into a graph hands its gradient to the leaf's accumulation node on the stream that node was made on. One that
+// lives on from an eager pass of another stream is outside of the capture, and torch ends the process: refused here, before anything is launched.
+void capture_alone(const char *what, const Tensor &leaf) {
+    if (!wants_grad(leaf) || !leaf.is_leaf() || !leaf.is_cuda()) return;
+    const c10::cuda::CUDAStream here = c10::cuda::getCurrentCUDAStream(leaf.device().index());
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(here.stream(), &status) != cudaSuccess || status == cudaStreamCaptureStatusNone) return;
+    const std::shared_ptr<torch::autograd::Node> node = torch::autograd::impl::try_get_grad_accumulator(leaf);
+    const std::optional<c10::Stream> made = node ? node->stream() : std::nullopt;
+    if (made && *made != here.unwrap())
+        throw std::runtime_error(std::string(what) + ": a backward pass of this weight or input from another stream is still alive (its loss is referenced), which a "
+                                 "capture cannot take in: drop it before capturing, or capture on the stream it ran on");
+}
 // nullopt: something wants to see the registered operators (see plain)
 OptTensor linear_xent(const Tensor &h, const Tensor &w, const Tensor &target, int64_t ignore, int64_t reduction) {
     if (!plain(h, w, target)) return std::nullopt;
-    if (at::GradMode::is_enabled() && (wants_grad(h) || wants_grad(w)))
+    if (at::GradMode::is_enabled() && (wants_grad(h) || wants_grad(w))) {
+        capture_alone(XENT, h); capture_alone(XENT, w);
         return HeadLoss::apply(h, w, OptTensor(target), ignore, OptTensor(), OptTensor(), 1.0, reduction)[0];
+    }
     const HeadIn x = head_in(XENT, h, w);
     const Tensor loss = head_fwd(XENT, x, xent_want(x, h, target, ignore), reduction).loss;
     return reduction == REDUCE_NONE ? loss.view(target.sizes()) : loss;
 }
 OptTensor linear_distill(const Tensor &h, const Tensor &w, const Tensor &ids, const Tensor &logits, double tau, int64_t reduction) {
     if (!plain(h, w, ids, logits)) return std::nullopt;
-    if (at::GradMode::is_enabled() && (wants_grad(h) || wants_grad(w)))
+    if (at::GradMode::is_enabled() && (wants_grad(h) || wants_grad(w))) {
+        capture_alone(DISTILL, h); capture_alone(DISTILL, w);
         return HeadLoss::apply(h, w, OptTensor(), 0, OptTensor(ids), OptTensor(logits.detach()), tau, reduction)[0];
+    }
     const HeadIn x = head_in(DISTILL, h, w);
     const Tensor loss = head_fwd(DISTILL, x, distill_want(x, h, ids, logits, tau), reduction).loss;
     return reduction == REDUCE_NONE ? loss.view(h.sizes().slice(0, h.dim() - 1)) : loss;
@@ -600,6 +617,7 @@ OptTensor embedding(const Tensor &ids, const Tensor &w, double scale, int64_t pa
     if (at::GradMode::is_enabled() && wants_grad(w)) {
         need_cuda(ids, w);
         embed_weight(w);
+        capture_alone(EMBED, w);
         return Embed::apply(ids, w, scale, padding)[0];
     }
     return embed_fwd(ids, w, scale);

@@ -10,7 +10,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from . import ops
+from . import head, ops
 from ._lib import Cached, graph_capture, lib, mark_constants, sm_count, warm_up
 from .assoc import AssocCarrier
 from .spin import SpinCarrier
@@ -216,6 +216,29 @@ class LM(nn.Module):
         h = self.trunk(x)
         logits = F.linear(h, self.e.weight)
         return (logits, h) if return_hidden else logits
+
+    def loss(self, x, targets=None, *, ignore_index=-100, reduction="mean", teacher=None, temperature=1.0, alpha=0.5):
+        """Cross entropy of the ids x (B,T) against `targets` (B,T) -- by default the next token of every token but a sequence's last --
+        without the logits in memory (the reference takes torch's of forward()'s logits, src/train.py:49). float32, differentiable; with
+        reduction "none" and no gradient, the scores of a text's tokens.
+
+        teacher: (ids (B,T,k), logits (B,T,k)), a teacher's top logits for the same targets; the loss is then (1 - alpha) cross entropy
+        + alpha distillation at `temperature` (head.linear_distill)."""
+        B, T = x.shape
+        if T < 2 and torch.is_grad_enabled():
+            raise ValueError("loss: a sequence of one token has no differentiable pass through the carrier layers (no_grad scores it)")
+        if targets is None:
+            targets = torch.cat([x[:, 1:], x.new_full((B, 1), ignore_index)], 1)
+        plain = type(self.e) is nn.Embedding and self.e.padding_idx is None and self.e.max_norm is None and not self.e.scale_grad_by_freq
+        e = head.embedding(x, self.e.weight) if plain and self.e.weight.dtype in (torch.bfloat16, torch.float32) else self.e(x)
+        e = e + self.p(torch.arange(T, device=x.device) % self.p.num_embeddings)
+        h = self._add_norm(*self._layers(e, [None] * self.layers), self.n)[1]
+        if teacher is None:
+            return head.linear_cross_entropy(h, self.e.weight, targets, ignore_index=ignore_index, reduction=reduction)
+        soft = head.linear_distill(h, self.e.weight, *teacher, temperature=temperature, reduction=reduction)
+        if alpha == 1.0:
+            return soft
+        return (1.0 - alpha) * head.linear_cross_entropy(h, self.e.weight, targets, ignore_index=ignore_index, reduction=reduction) + alpha * soft
 
     @torch.no_grad()
     def forward_carried(self, x, window=None, return_states=False):

@@ -10,7 +10,8 @@ import pytest
 import torch
 
 from pragnosia_b200 import head
-from pragnosia_b200._lib import check, lib
+from pragnosia_b200._lib import check, host, lib
+from pragnosia_b200.model import LM
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -388,3 +389,112 @@ def test_embedding_in_a_graph():
         torch.cuda.synchronize()
         a, b = embed(ids, w.detach(), gy)
         assert torch.equal(y, a) and torch.equal(dw, b)
+
+
+# ------------------------------------------------------------------------------------------------ the three together
+def lm(mixer, dtype, vocab=333, d=128):
+    torch.manual_seed(5)
+    return LM(vocab=vocab, d=d, layers=2, mlp_mult=2, ctx=64, mixer=mixer, norm="rms").to(DEV).to(dtype)
+
+
+@pytest.mark.parametrize("mixer,dtype,d", [("aspin", BF, 128), ("dspin", BF, 128), ("aspin", F32, 128), ("fspin", BF, 72), ("fspin", F32, 72)])
+def test_language_model_loss(mixer, dtype, d):
+    """LM.loss is the trunk with the three operators at its ends: loss, the trunk's gradients and the tied table's two shares of its own are
+    what those operators give, to the bit; the operators are held to their definitions above."""
+    m = lm(mixer, dtype, d=d)
+    g = torch.Generator(device=DEV).manual_seed(1)
+    x = torch.randint(0, 333, (3, 70), device=DEV, generator=g)
+    ids, logits = torch.randint(0, 333, (3, 70, 5), device=DEV, generator=g), torch.randn(3, 70, 5, device=DEV, generator=g)
+    target = torch.cat([x[:, 1:], torch.full_like(x[:, :1], -100)], 1)
+    for kw in ({}, dict(reduction="sum"), dict(teacher=(ids, logits), temperature=2.0, alpha=1.0)):
+        m.zero_grad()
+        loss = m.loss(x, **kw)
+        loss.backward()
+        e = m.e.weight.detach()[x].requires_grad_()
+        h = m._add_norm(*m._layers(e + m.p(torch.arange(70, device=DEV) % 64), [None] * 2), m.n)[1]
+        hd, wd = h.detach().requires_grad_(), m.e.weight.detach().requires_grad_()
+        want = head.linear_distill(hd, wd, ids, logits, temperature=2.0) if "teacher" in kw else head.linear_cross_entropy(hd, wd, target, **kw)
+        dh, dw = torch.autograd.grad(want, [hd, wd])
+        others = [(n, p) for n, p in m.named_parameters() if n != "e.weight" and p.grad is not None]
+        grads = torch.autograd.grad(h, [e] + [p for _, p in others], dh)
+        assert torch.equal(loss.detach(), want.detach())
+        assert all(".wi." in n and mixer == "dspin" for n, p in m.named_parameters() if p.grad is None)      # the delta rule has no write gate
+        for (n, p), b in zip(others, grads[1:]):
+            assert torch.equal(p.grad, b), n
+        assert torch.equal(m.e.weight.grad, dw + host().embedding_bwd(x, grads[0], 1.0, -1, 333))
+    with torch.no_grad():
+        rows = m.loss(x, reduction="none")
+        ref = torch.nn.functional.cross_entropy(torch.nn.functional.linear(m.trunk(x).double(), m.e.weight.double()).flatten(0, 1), target.flatten(), reduction="none")
+        assert rows.shape == (3, 70) and ((rows.flatten().double() - ref).abs() < 1e-4).all()
+        both = m.loss(x, teacher=(ids, logits), temperature=2.0, alpha=0.25)
+        assert abs(float(both) - 0.75 * float(m.loss(x)) - 0.25 * float(m.loss(x, teacher=(ids, logits), temperature=2.0, alpha=1.0))) < 1e-5
+        assert m.loss(x[:, :1], target[:, :1], reduction="none").shape == (3, 1)
+    with pytest.raises(ValueError):
+        m.loss(x[:, :1])
+
+
+def test_compiled_callers_take_the_operators():
+    """Under torch.compile and under a dispatch mode the same calls are the registered operators, with the same results."""
+    h, w, g = operands(100, 300, 64, F32, 1)
+    t = torch.randint(0, 300, (100,), device=DEV, generator=g)
+    ids, logits = lists(100, 300, 6, g, True)
+
+    def f(h, w):
+        z = head.embedding(t, w, scale=2.0)
+        return head.linear_cross_entropy(h + z, w, t) + head.linear_distill(h + z, w, ids, logits, temperature=2.0, reduction="none").sum()
+
+    want = torch.autograd.grad(f(*(a := [h.clone().requires_grad_(), w.clone().requires_grad_()])), a)
+    got = torch.autograd.grad(torch.compile(f, backend="aot_eager", fullgraph=True)(*(a := [h.clone().requires_grad_(), w.clone().requires_grad_()])), a)
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Seen(TorchDispatchMode):
+        names = set()
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            Seen.names.add(func.name())
+            return func(*args, **(kwargs or {}))
+    with Seen():
+        got = torch.autograd.grad(f(*(a := [h.clone().requires_grad_(), w.clone().requires_grad_()])), a)
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
+    assert {f"pragnosia_b200::{n}" for n in ("linear_xent", "linear_xent_bwd", "linear_distill", "linear_distill_bwd", "teacher_lists", "embedding", "embedding_bwd")} <= Seen.names
+
+
+def test_streams():
+    """Two streams at once, and tensors made on another stream than the one that uses them."""
+    h, w, g = operands(600, 2000, 128, BF, 3)
+    t = torch.randint(0, 2000, (600,), device=DEV, generator=g)
+    want = xent(h, w, t, None, "mean")
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    got = []
+    for _ in range(4):
+        for s in streams:
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                got.append(xent(h, w, t, None, "mean"))
+    for s in streams:
+        torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for o in got for a, b in zip(o, want))
+
+
+def test_a_capture_beside_an_eager_pass_of_the_same_leaves_is_refused():
+    h, w, g = operands(50, 60, 64, BF, 3)
+    w = w.requires_grad_()
+    t = torch.randint(0, 60, (50,), device=DEV, generator=g)
+    alive = head.linear_cross_entropy(h, w, t), head.embedding(t, w)
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    side.wait_stream(torch.cuda.current_stream())
+    errors = []
+    with torch.cuda.graph(graph, stream=side):
+        for call in (lambda: head.linear_cross_entropy(h, w, t), lambda: head.embedding(t, w), lambda: head.linear_distill(h, w, t[:, None], h[:, :1].float())):
+            try:
+                call()
+            except RuntimeError as e:
+                errors.append(str(e))
+        with torch.no_grad():
+            loss = head.linear_cross_entropy(h, w, t)
+    assert len(errors) == 3 and all("still alive" in e for e in errors)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(loss, alive[0].detach())
