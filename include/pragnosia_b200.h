@@ -534,13 +534,12 @@ int pgb_linear_act(const void *x, const void *W, const void *bias, void *y, long
  * N x V logits in memory: softmax cross entropy against a word per row, and distillation from a teacher's top logits at a
  * temperature. The reference's loss is torch's cross entropy on the logits (src/train.py:49, src/model.py:837).
  *   h [N][d], W [V][d]: dtype (fp32 or bf16), contiguous, 16-byte aligned, d a multiple of 8. Sums in fp32, losses fp32.
- *   reduction 0: a loss per row (row_loss [N]); 1: their sum; 2: their mean over the rows that count (loss, count: one fp32 each;
- *   row_loss may be NULL; 0 / 0 where no row counts). L [N][2] fp32: log2 of a row's sum of exponentials in two parts, which the
- *   backward pass reads.
+ *   reduction 0: a loss per row (row_loss [N]); 1: their sum; 2: their mean over the rows that count (loss, one fp32;
+ *   row_loss may be NULL; 0 / 0 where no row counts). For the backward pass: L [N][2] fp32, log2 of a row's sum of exponentials in two parts, and
+ *   stats [2] fp32, the rows that count (reductions 1 and 2) and whether one that does not holds what is no number.
  *   grad: the gradient of row_loss [N] (reduction 0) or of loss (one fp32). dh [N][d], dW [V][d]: dtype; either may be NULL.
  *   scratch: 256-byte aligned, at least what the _scratch_bytes call of the same sizes says (0: bad sizes; k 0: cross entropy).
- * Cross entropy: rows whose target is ignore_index lose 0 and have no gradient (h must be finite there all the same if dW is
- * wanted); any other target outside 0 .. V-1 gives NaN, as loss and as gradients of its row and of W.
+ * Cross entropy: rows whose target is ignore_index lose 0 and have no gradient, whatever h holds there; any other target outside 0 .. V-1 gives NaN, as loss and as gradients of its row and of W.
  * Distillation: pgb_teacher_lists makes of a teacher's k entries per row (ids in any order; an entry with id < 0 or logit -inf is
  * absent) what the losses read: lists [N][k][2] (id, bits of its probability p at the temperature; by id), marks [N][ceil(V / 64)][4] (which of every
  * 64 words they are, and the place of the first) and ent [N], the sum of p log p. lists 8-byte, marks 16-byte aligned. kept [N][k]: the entries' logits, which the forward pass
@@ -552,18 +551,18 @@ int pgb_linear_act(const void *x, const void *W, const void *bias, void *y, long
 long long pgb_head_loss_fwd_scratch_bytes(long long N, int V, int d, int dtype);
 long long pgb_head_loss_bwd_scratch_bytes(long long N, int V, int d, int dtype, int want_dh, int want_dW);
 int pgb_linear_xent_fwd(const void *h, const void *W, int dtype, const long long *target, long long ignore_index, float *row_loss,
-                        float *loss, float *count, float *L, void *scratch, long long scratch_bytes, int reduction, long long N,
+                        float *loss, float *stats, float *L, void *scratch, long long scratch_bytes, int reduction, long long N,
                         int V, int d, void *stream);
 int pgb_linear_xent_bwd(const void *h, const void *W, int dtype, const long long *target, long long ignore_index, const float *L,
-                        const float *count, const float *grad, void *dh, void *dW, void *scratch, long long scratch_bytes,
+                        const float *stats, const float *grad, void *dh, void *dW, void *scratch, long long scratch_bytes,
                         int reduction, long long N, int V, int d, void *stream);
 int pgb_teacher_lists(const long long *teacher_ids, const float *teacher_logits, float temperature, int *lists, unsigned *marks, float *ent,
                       long long N, int V, int k, void *stream);
 int pgb_linear_distill_fwd(const void *h, const void *W, int dtype, const int *lists, const unsigned *marks, const float *ent, float *kept, int k,
-                           float temperature, float *row_loss, float *loss, float *count, float *L, void *scratch,
+                           float temperature, float *row_loss, float *loss, float *stats, float *L, void *scratch,
                            long long scratch_bytes, int reduction, long long N, int V, int d, void *stream);
 int pgb_linear_distill_bwd(const void *h, const void *W, int dtype, const int *lists, const unsigned *marks, const float *ent, const float *kept, int k,
-                           float temperature, const float *L, const float *count, const float *grad, void *dh, void *dW,
+                           float temperature, const float *L, const float *stats, const float *grad, void *dh, void *dW,
                            void *scratch, long long scratch_bytes, int reduction, long long N, int V, int d, void *stream);
 
 /* ---------------------------------------------------------------------------------------------------------

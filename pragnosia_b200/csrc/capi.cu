@@ -820,18 +820,18 @@ int head_args(HeadLossArgs &x, const void *h, const void *W, int dtype, const lo
         return PGB_ERR_MISALIGNED;
     return PGB_OK;
 }
-int head_fwd(const HeadLossArgs &x, float *row_loss, float *loss, float *count, float *L, void *scratch, long long scratch_bytes, void *stream) {
-    if (!L || !scratch || (x.reduction == 0 ? !row_loss : !loss || !count)) return PGB_ERR_NULL_POINTER;
+int head_fwd(const HeadLossArgs &x, float *row_loss, float *loss, float *stats, float *L, void *scratch, long long scratch_bytes, void *stream) {
+    if (!L || !scratch || !stats || (x.reduction == 0 ? !row_loss : !loss)) return PGB_ERR_NULL_POINTER;
     if (!aligned(L, 8) || !aligned(scratch, 256)) return PGB_ERR_MISALIGNED;
     if (scratch_bytes < head_loss_fwd_bytes(x.N, x.V, x.d, x.dtype)) return PGB_ERR_BAD_SHAPE;
-    return head_loss_fwd_launch(x, row_loss, loss, count, L, scratch, (cudaStream_t)stream);
+    return head_loss_fwd_launch(x, row_loss, loss, stats, L, scratch, (cudaStream_t)stream);
 }
-int head_bwd(const HeadLossArgs &x, const float *L, const float *count, const float *grad, void *dh, void *dW, void *scratch, long long scratch_bytes,
+int head_bwd(const HeadLossArgs &x, const float *L, const float *stats, const float *grad, void *dh, void *dW, void *scratch, long long scratch_bytes,
              void *stream) {
-    if (!L || !grad || !scratch || (x.reduction == 2 && !count) || (!dh && !dW)) return PGB_ERR_NULL_POINTER;
+    if (!L || !grad || !scratch || !stats || (!dh && !dW)) return PGB_ERR_NULL_POINTER;
     if (!aligned(L, 8) || !aligned(scratch, 256) || (dh && !aligned(dh, 16)) || (dW && !aligned(dW, 16))) return PGB_ERR_MISALIGNED;
     if (scratch_bytes < head_loss_bwd_bytes(x.N, x.V, x.d, x.dtype, dh != nullptr, dW != nullptr)) return PGB_ERR_BAD_SHAPE;
-    return head_loss_bwd_launch(x, L, count, grad, dh, dW, scratch, (cudaStream_t)stream);
+    return head_loss_bwd_launch(x, L, stats, grad, dh, dW, scratch, (cudaStream_t)stream);
 }
 }  // namespace
 
@@ -841,19 +841,19 @@ long long pgb_head_loss_fwd_scratch_bytes(long long N, int V, int d, int dtype) 
 long long pgb_head_loss_bwd_scratch_bytes(long long N, int V, int d, int dtype, int want_dh, int want_dW) {
     return head_sizes(N, V, d, dtype) != PGB_OK ? 0 : head_loss_bwd_bytes(N, V, d, dtype, want_dh, want_dW);
 }
-int pgb_linear_xent_fwd(const void *h, const void *W, int dtype, const long long *target, long long ignore_index, float *row_loss, float *loss, float *count,
+int pgb_linear_xent_fwd(const void *h, const void *W, int dtype, const long long *target, long long ignore_index, float *row_loss, float *loss, float *stats,
                         float *L, void *scratch, long long scratch_bytes, int reduction, long long N, int V, int d, void *stream) {
     if (!target) return PGB_ERR_NULL_POINTER;
     HeadLossArgs x;
     const int rc = head_args(x, h, W, dtype, target, ignore_index, nullptr, nullptr, nullptr, nullptr, 0, 1.f, reduction, N, V, d);
-    return rc != PGB_OK ? rc : head_fwd(x, row_loss, loss, count, L, scratch, scratch_bytes, stream);
+    return rc != PGB_OK ? rc : head_fwd(x, row_loss, loss, stats, L, scratch, scratch_bytes, stream);
 }
-int pgb_linear_xent_bwd(const void *h, const void *W, int dtype, const long long *target, long long ignore_index, const float *L, const float *count,
+int pgb_linear_xent_bwd(const void *h, const void *W, int dtype, const long long *target, long long ignore_index, const float *L, const float *stats,
                         const float *grad, void *dh, void *dW, void *scratch, long long scratch_bytes, int reduction, long long N, int V, int d, void *stream) {
     if (!target) return PGB_ERR_NULL_POINTER;
     HeadLossArgs x;
     const int rc = head_args(x, h, W, dtype, target, ignore_index, nullptr, nullptr, nullptr, nullptr, 0, 1.f, reduction, N, V, d);
-    return rc != PGB_OK ? rc : head_bwd(x, L, count, grad, dh, dW, scratch, scratch_bytes, stream);
+    return rc != PGB_OK ? rc : head_bwd(x, L, stats, grad, dh, dW, scratch, scratch_bytes, stream);
 }
 int pgb_teacher_lists(const long long *teacher_ids, const float *teacher_logits, float temperature, int *lists, unsigned *marks, float *ent, long long N, int V, int k,
                       void *stream) {
@@ -864,17 +864,17 @@ int pgb_teacher_lists(const long long *teacher_ids, const float *teacher_logits,
     return head_teacher_launch(teacher_ids, teacher_logits, lists, marks, ent, N, V, k, temperature, (cudaStream_t)stream);
 }
 int pgb_linear_distill_fwd(const void *h, const void *W, int dtype, const int *lists, const unsigned *marks, const float *ent, float *kept, int k, float temperature, float *row_loss,
-                           float *loss, float *count, float *L, void *scratch, long long scratch_bytes, int reduction, long long N, int V, int d, void *stream) {
+                           float *loss, float *stats, float *L, void *scratch, long long scratch_bytes, int reduction, long long N, int V, int d, void *stream) {
     HeadLossArgs x;
     const int rc = head_args(x, h, W, dtype, nullptr, 0, lists, marks, ent, kept, k, temperature, reduction, N, V, d);
-    return rc != PGB_OK ? rc : head_fwd(x, row_loss, loss, count, L, scratch, scratch_bytes, stream);
+    return rc != PGB_OK ? rc : head_fwd(x, row_loss, loss, stats, L, scratch, scratch_bytes, stream);
 }
 int pgb_linear_distill_bwd(const void *h, const void *W, int dtype, const int *lists, const unsigned *marks, const float *ent, const float *kept, int k, float temperature, const float *L,
-                           const float *count, const float *grad, void *dh, void *dW, void *scratch, long long scratch_bytes, int reduction, long long N, int V,
+                           const float *stats, const float *grad, void *dh, void *dW, void *scratch, long long scratch_bytes, int reduction, long long N, int V,
                            int d, void *stream) {
     HeadLossArgs x;
     const int rc = head_args(x, h, W, dtype, nullptr, 0, lists, marks, ent, const_cast<float *>(kept), k, temperature, reduction, N, V, d);
-    return rc != PGB_OK ? rc : head_bwd(x, L, count, grad, dh, dW, scratch, scratch_bytes, stream);
+    return rc != PGB_OK ? rc : head_bwd(x, L, stats, grad, dh, dW, scratch, scratch_bytes, stream);
 }
 
 static int embedding_sizes(long long N, int V, int d, int dtype) {

@@ -9,6 +9,8 @@
 // workspace that holds a piece of the (N, V) matrix; behind it one launch multiplies the piece with W and with h. Arithmetic: 2 N V d
 // forward, 6 N V d backward (a third of it the logits again, the price of not keeping them).
 //   Pieces: along the longer of N and V, so that the gradient that gathers over pieces (fp32, added to in place) is the smaller one.
+//   A row that does not count has zeros in ds, but its h may hold what is no number, and zero times that is none either. The forward pass tells
+// (such a row's sum of exponentials is no number), and the backward pass then multiplies a copy of h with zeros in those rows.
 //   ds holds no upstream scale where that is the same for every row (mean, sum): the scale is applied to the fp32 accumulators.
 //   Rounded to bf16, ds is off by 2^-9 of itself, as the gradients themselves are when they are bf16.
 //   fp32 operands: three bf16 terms each (24 bits), six of the nine products (what is left out is below 2^-23 of the sum's terms); ds as
@@ -33,7 +35,7 @@ constexpr long long HL_PIECE_BYTES = 64LL << 20;                      // of ds, 
 static_assert(HL_STAGE % 1024 == 0 && HL_SMEM <= 232448, "shared memory");
 constexpr float LOG2E_F = 1.4426950408889634f;
 
-struct HlMaps { CUtensorMap a[3], b[3], ds; };                        // of the products; ds: the piece of it that is written
+struct HlMaps { CUtensorMap a[3], b[3], ds, clean; };                 // of the products; ds: the piece of it that is written; clean: b[1] where *dirty is set
 // An epilogue warp's share of a tile: rows row0 .. +31 (a lane each), columns col0 .. +63; block: which of the tile's 32 it is. g, t, sp: the
 // product, its tile, and the part of K that the accumulator holds.
 struct HlTile { int lane, sub, part, block, n, row0, col0, g, t, sp; uint32_t ti; };
@@ -145,7 +147,7 @@ __device__ __forceinline__ void hl_body(const HlMaps &maps, const What &what, Ep
     };
     if (warp == 0) {
         // ------------------------------------------------------------------------------------------ producer (both CTAs)
-        const bool leader = elect_one();
+        const bool leader = elect_one(), dirty = epi.dirty();
         uint32_t it = 0;
         bool ok = true;
         for (; w.more() && ok; w.next()) {
@@ -153,7 +155,7 @@ __device__ __forceinline__ void hl_body(const HlMaps &maps, const What &what, Ep
             if (w.g != 2) wait_for_launch();
             p.at(w.t, m, n);
             const int m0 = m * HL_B + (int)rank * (HL_B / 2), n0 = n * HL_B + (int)rank * (HL_B / 2);
-            const CUtensorMap *ma = &maps.a[w.g], *mbm = &maps.b[w.g];
+            const CUtensorMap *ma = &maps.a[w.g], *mbm = w.g == 1 && dirty ? &maps.clean : &maps.b[w.g];
             for (int k = w.k0; k < w.k1 && ok; ++k, ++it) {
                 const int s = it % STAGES;
                 if (it >= STAGES) ok = __all_sync(0xffffffffu, mbar_wait(bar_empty(s), ((it / STAGES) + 1) & 1, 91));
@@ -327,14 +329,15 @@ struct HlFwd {
     HlTargets t; float a;
     float2 *ml;                                                       // [tiles_n][Np]: maximum (times a) and sum of a tile's row
     float *dot;                                                       // the targets' s: [N], or [N][k] where there are lists
-    unsigned *ticket; long long N, Np; int V;
+    unsigned *ticket; float *stats; long long N, Np; int V;
 };
 template <bool LIST>
 struct HlFwdEpi {
     const HlFwd &f;
     uint4 marks; int target;                                           // of the tile fetched for
     uint64_t bits; int place, nx;                                      // of the tile at hand: targets by column, and the first one's place; or the target
-    __device__ __forceinline__ void start(int i) { if (i == 0 && blockIdx.x == 0) *f.ticket = 0u; }
+    __device__ __forceinline__ void start(int i) { if (i == 0 && blockIdx.x == 0) { *f.ticket = 0u; f.stats[0] = 0.f; f.stats[1] = 0.f; } }
+    __device__ __forceinline__ bool dirty() const { return false; }
     __device__ __forceinline__ void end(int) {}
     __device__ __forceinline__ void fetch(int, int r, int c) {
         const bool in = r < f.N && c < f.V;
@@ -413,7 +416,7 @@ head_loss_fwd_kernel(const __grid_constant__ HlMaps maps, const __grid_constant_
 // Joins a row's tiles: 32 rows a block (a lane each), the tiles dealt out to its 8 warps, then the block's losses and live rows as one
 // partial sum; the last block to finish adds the partials up in order, so the sum does not depend on who that is.
 struct HlJoin {
-    HlTargets t; const float2 *ml; const float *dot; float2 *L; float *row_loss, *loss, *count; double2 *partial; unsigned *ticket;
+    HlTargets t; const float2 *ml; const float *dot; float2 *L; float *row_loss, *loss, *stats; double2 *partial; unsigned *ticket;
     long long N, Np; int V, tiles; float tau; int reduction;
 };
 template <bool LIST>
@@ -470,7 +473,10 @@ __global__ void __launch_bounds__(256) head_loss_join_kernel(const HlJoin j) {
             live = w != j.t.ignore;
             loss = live && w >= 0 && w < j.V ? L * 0.693147180559945309 - j.dot[row] : NAN;
         }
-        if (!live) loss = 0.0;
+        if (!live) {
+            loss = 0.0;
+            if (!(l > 0.f && l < INFINITY)) j.stats[1] = 1.f;          // of whichever row: the same value
+        }
         if (j.row_loss) j.row_loss[row] = (float)loss;
     }
     if (j.reduction == 0) return;
@@ -502,7 +508,7 @@ __global__ void __launch_bounds__(256) head_loss_join_kernel(const HlJoin j) {
     if (threadIdx.x == 0) {
         for (int q = 1; q < 8; ++q) { s.x += sums[q].x; s.y += sums[q].y; }
         *j.loss = (float)(j.reduction == 2 ? s.x / s.y : s.x);
-        *j.count = (float)s.y;
+        j.stats[0] = (float)s.y;
     }
 }
 
@@ -776,12 +782,26 @@ __global__ void __launch_bounds__(256) head_loss_sum_kernel(const float *__restr
     }
 }
 // One launch of the backward pass: the gradients' products of one piece and ds of the next, which do not depend on one another.
-struct HlBwd { HlProb ds; HlGrads grads; };
+// dirty: not 0 where h of a row that does not count holds what is no number; the first launch then writes the clean copy (bf16; NULL: h is a copy already).
+struct HlBwd { HlProb ds; HlGrads grads; const float *dirty; const __nv_bfloat16 *h; __nv_bfloat16 *clean; long long N; };
+// whether a row counts
+__device__ __forceinline__ bool hl_counts(const HlTargets &t, long long row) { return t.lists ? t.ent[row] != INFINITY : t.target[row] != t.ignore; }
+// by the epilogue warps of the whole grid, a warp a row (i: the thread's number among its CTA's)
+__device__ __noinline__ void hl_clean(const HlBwd &f, int i) {
+    const int d = f.grads.d;
+    for (long long row = (i >> 5) + (long long)blockIdx.x * HL_EPI; row < f.N; row += (long long)gridDim.x * HL_EPI) {
+        const bool counts = hl_counts(f.ds.t, row);
+        for (int c = 8 * (i & 31); c < d; c += 256)
+            *reinterpret_cast<uint4 *>(f.clean + row * d + c) = counts ? *reinterpret_cast<const uint4 *>(f.h + row * d + c) : make_uint4(0u, 0u, 0u, 0u);
+    }
+}
 template <bool LIST, int TERMS>
 struct HlBwdEpi {
     HlProbEpi<LIST, TERMS> ds;
     HlGradEpi grad;
-    __device__ __forceinline__ void start(int) {
+    const HlBwd &f;
+    __device__ __forceinline__ void start(int i) {
+        if (TERMS == 1 && f.clean != nullptr && *f.dirty != 0.f) hl_clean(f, i);
         grad.alpha = hl_alpha(grad.f.up, grad.f.count, grad.f.tau, grad.f.reduction);
     }
     __device__ __forceinline__ void fetch(int g, int r, int c) { if (g == 2) ds.fetch(r, c); }
@@ -790,23 +810,29 @@ struct HlBwdEpi {
         if (x.g == 2) ds.tile(x, v, stage); else grad.tile(x, v, stage);
         return true;
     }
+    __device__ __forceinline__ bool dirty() const { return TERMS == 1 && *f.dirty != 0.f; }
     __device__ __forceinline__ void end(int lane) { if (lane == 0) tma_store_done(); }
 };
 template <bool LIST, int TERMS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(HL_NT, 1)
 head_loss_bwd_kernel(const __grid_constant__ HlMaps maps, const __grid_constant__ HlTrio work, const __grid_constant__ HlBwd f) {
-    HlBwdEpi<LIST, TERMS> epi{{f.ds, &maps.ds}, {f.grads, work.p, 0.f}};
+    HlBwdEpi<LIST, TERMS> epi{{f.ds, &maps.ds}, {f.grads, work.p, 0.f}, f};
     hl_body<TERMS == 3, HlThree>(maps, work, epi);
 }
 
-// x as three bf16 terms, [3][n]; eight values a thread (n a multiple of 8)
-__global__ void __launch_bounds__(256) head_split_kernel(const float *__restrict__ x, __nv_bfloat16 *__restrict__ out, long long n) {
+// x as three bf16 terms, [3][n]; eight values a thread (d, the values of a row, a multiple of 8). t not NULL: zeros in the rows that do not count
+template <bool ROWS>
+__global__ void __launch_bounds__(256) head_split_kernel(const float *__restrict__ x, __nv_bfloat16 *__restrict__ out, long long n, int d, const HlTargets t) {
     pdl_wait();
     pdl_launch_dependents();
     for (long long i = 8 * ((long long)blockIdx.x * 256 + threadIdx.x); i < n; i += 2048LL * gridDim.x) {
         float v[8];
         *reinterpret_cast<float4 *>(v) = *reinterpret_cast<const float4 *>(x + i);
         *reinterpret_cast<float4 *>(v + 4) = *reinterpret_cast<const float4 *>(x + i + 4);
+        if (ROWS && !hl_counts(t, i / d)) {
+#pragma unroll
+            for (int q = 0; q < 8; ++q) v[q] = 0.f;
+        }
         uint4 hi, lo, rest;
         split8(v, hi, lo, rest);
         *reinterpret_cast<uint4 *>(out + i) = hi;
@@ -880,19 +906,17 @@ static HlFwdPlan hl_fwd_plan(long long N, int V, int d, int dtype) {
 }
 long long head_loss_fwd_bytes(long long N, int V, int d, int dtype) { return hl_fwd_plan(N, V, d, dtype).total; }
 
-static int hl_split(const void *x, void *out, long long n, cudaStream_t stream) {
-    const long long blocks = (n / 8 + 255) / 256;
-    cudaError_t e = pdl_launch(head_split_kernel, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, stream, static_cast<const float *>(x),
-                               static_cast<__nv_bfloat16 *>(out), n);
-    if (e != cudaSuccess) { set_cuda_error(e, "head_split launch"); return PGB_ERR_CUDA; }
-    return check_launch("head_split_kernel");
-}
-// the operand as the products take it; fp32: split into `room` first
-static int hl_operand(HlOperand &o, const void *x, int dtype, long long rows, int d, void *room, cudaStream_t stream) {
+// the operand as the products take it; fp32: split into `room` first (t: without the rows that do not count)
+static int hl_operand(HlOperand &o, const void *x, int dtype, long long rows, int d, void *room, cudaStream_t stream, const HlTargets *t = nullptr) {
     o = {x, 1, 0, d};
     if (dtype != PGB_F32) return PGB_OK;
-    o = {room, 3, rows * d, d};
-    return hl_split(x, room, rows * d, stream);
+    const long long n = rows * d, blocks = (n / 8 + 255) / 256;
+    o = {room, 3, n, d};
+    const dim3 grid((unsigned)(blocks < 4096 ? blocks : 4096));
+    const cudaError_t e = t ? pdl_launch(head_split_kernel<true>, grid, dim3(256), 0, stream, static_cast<const float *>(x), static_cast<__nv_bfloat16 *>(room), n, d, *t)
+                            : pdl_launch(head_split_kernel<false>, grid, dim3(256), 0, stream, static_cast<const float *>(x), static_cast<__nv_bfloat16 *>(room), n, d, HlTargets{});
+    if (e != cudaSuccess) { set_cuda_error(e, "head_split launch"); return PGB_ERR_CUDA; }
+    return check_launch("head_split_kernel");
 }
 static int hl_no_map() { set_cuda_error(cudaErrorUnknown, "cuTensorMapEncodeTiled"); return PGB_ERR_CUDA; }
 
@@ -907,7 +931,7 @@ int head_teacher_launch(const long long *in_ids, const float *in_logits, int *li
     return check_launch("head_teacher_kernel");
 }
 
-int head_loss_fwd_launch(const HeadLossArgs &x, float *row_loss, float *loss, float *count, float *L, void *scratch, cudaStream_t stream) {
+int head_loss_fwd_launch(const HeadLossArgs &x, float *row_loss, float *loss, float *stats, float *L, void *scratch, cudaStream_t stream) {
     const bool list = x.lists != nullptr;
     const HlFwdPlan pl = hl_fwd_plan(x.N, x.V, x.d, x.dtype);
     char *s = static_cast<char *>(scratch);
@@ -921,7 +945,7 @@ int head_loss_fwd_launch(const HeadLossArgs &x, float *row_loss, float *loss, fl
     pr.tiles_m = hl_tiles(x.N); pr.tiles_n = (int)pl.tiles; pr.kb = (x.d + HL_BK - 1) / HL_BK;
     const HlTargets t{x.target, x.ignore, reinterpret_cast<const int2 *>(x.lists), reinterpret_cast<const uint4 *>(x.marks), x.ent, x.k, (x.V + 63) / 64};
     const HlFwd f{t, LOG2E_F / x.tau, reinterpret_cast<float2 *>(s + pl.off_ml), list ? x.kept : reinterpret_cast<float *>(s + pl.off_dot),
-                  reinterpret_cast<unsigned *>(s + pl.off_ticket), x.N, pl.Np, x.V};
+                  reinterpret_cast<unsigned *>(s + pl.off_ticket), stats, x.N, pl.Np, x.V};
     if (h.terms == 3)
         rc = list ? hl_launch(head_loss_fwd_kernel<true, true>, 0, "head_loss_fwd_kernel", maps, pr, pr.tiles(), f, stream)
                   : hl_launch(head_loss_fwd_kernel<false, true>, 1, "head_loss_fwd_kernel", maps, pr, pr.tiles(), f, stream);
@@ -929,7 +953,7 @@ int head_loss_fwd_launch(const HeadLossArgs &x, float *row_loss, float *loss, fl
         rc = list ? hl_launch(head_loss_fwd_kernel<true, false>, 2, "head_loss_fwd_kernel", maps, pr, pr.tiles(), f, stream)
                   : hl_launch(head_loss_fwd_kernel<false, false>, 3, "head_loss_fwd_kernel", maps, pr, pr.tiles(), f, stream);
     if (rc != PGB_OK) return rc;
-    const HlJoin j{t, f.ml, f.dot, reinterpret_cast<float2 *>(L), row_loss, loss, count, reinterpret_cast<double2 *>(s + pl.off_partial), f.ticket,
+    const HlJoin j{t, f.ml, f.dot, reinterpret_cast<float2 *>(L), row_loss, loss, stats, reinterpret_cast<double2 *>(s + pl.off_partial), f.ticket,
                    x.N, pl.Np, x.V, (int)pl.tiles, x.tau, x.reduction};
     cudaError_t e = pdl_launch(list ? head_loss_join_kernel<true> : head_loss_join_kernel<false>, dim3((unsigned)(pl.Np / 32)), dim3(256), 0, stream, j);
     if (e != cudaSuccess) { set_cuda_error(e, "head_loss_join launch"); return PGB_ERR_CUDA; }
@@ -1022,7 +1046,7 @@ static HlBwdPlan hl_bwd_plan(long long N, int V, int d, int dtype, bool dh, bool
     const int sh = p.s_dh[0] > p.s_dh[1] ? p.s_dh[0] : p.s_dh[1], sw = p.s_dw[0] > p.s_dw[1] ? p.s_dw[0] : p.s_dw[1];
     p.off_dh = dh && (sh > 1 || (!p.by_rows && p.pieces > 1)) ? take(4LL * sh * p.rows * d) : -1;
     p.off_dw = dw && (sw > 1 || (p.by_rows && p.pieces > 1)) ? take(4LL * sw * p.cols * d) : -1;
-    p.off_h = dtype == PGB_F32 ? take(6 * N * d) : 0;
+    p.off_h = dtype == PGB_F32 ? take(6 * N * d) : dw ? take(2 * N * d) : 0;                    // its terms, or room for a clean copy
     p.off_w = dtype == PGB_F32 ? take(6LL * V * d) : 0;
     p.total = at;
     return p;
@@ -1062,12 +1086,13 @@ static int hl_sum(const float *acc, void *out, long long n, int splits, const Hl
     if (e != cudaSuccess) { set_cuda_error(e, "head_loss_sum launch"); return PGB_ERR_CUDA; }
     return check_launch("head_loss_sum_kernel");
 }
-int head_loss_bwd_launch(const HeadLossArgs &x, const float *L, const float *count, const float *up, void *dh, void *dw, void *scratch, cudaStream_t stream) {
+int head_loss_bwd_launch(const HeadLossArgs &x, const float *L, const float *stats, const float *up, void *dh, void *dw, void *scratch, cudaStream_t stream) {
     const bool list = x.lists != nullptr;
     const HlBwdPlan pl = hl_bwd_plan(x.N, x.V, x.d, x.dtype, dh != nullptr, dw != nullptr);
     char *s = static_cast<char *>(scratch);
     HlOperand h, w;
-    int rc = hl_operand(h, x.h, x.dtype, x.N, x.d, s + pl.off_h, stream);
+    const HlTargets targets{x.target, x.ignore, reinterpret_cast<const int2 *>(x.lists), reinterpret_cast<const uint4 *>(x.marks), x.ent, x.k, (x.V + 63) / 64};
+    int rc = hl_operand(h, x.h, x.dtype, x.N, x.d, s + pl.off_h, stream, &targets);
     if (rc == PGB_OK) rc = hl_operand(w, x.W, x.dtype, x.V, x.d, s + pl.off_w, stream);
     if (rc != PGB_OK) return rc;
     const int np = pl.terms == 3 ? 6 : 1, esize = x.dtype == PGB_F32 ? 4 : 2;
@@ -1078,14 +1103,17 @@ int head_loss_bwd_launch(const HeadLossArgs &x, const float *L, const float *cou
     auto at = [&](long long off) { return off >= 0 ? reinterpret_cast<float *>(s + off) : nullptr; };
     auto piece = [&](long long i) { return HlOperand{s + pl.off_p[i % 3], pl.terms, pl.rows * pl.ldp, pl.ldp}; };
     HlBwd f{};
-    f.ds.t = {x.target, x.ignore, reinterpret_cast<const int2 *>(x.lists), reinterpret_cast<const uint4 *>(x.marks), x.ent, x.k, (x.V + 63) / 64};
+    f.ds.t = targets;
     f.ds.L = reinterpret_cast<const float2 *>(L); f.ds.row_weight = x.reduction == 0 ? up : nullptr; f.ds.a = LOG2E_F / x.tau; f.ds.V = x.V;
-    f.grads.up = up; f.grads.count = count; f.grads.tau = x.tau; f.grads.reduction = x.reduction; f.grads.d = x.d; f.grads.out_f32 = x.dtype == PGB_F32;
+    f.grads.up = up; f.grads.count = stats; f.grads.tau = x.tau; f.grads.reduction = x.reduction; f.grads.d = x.d; f.grads.out_f32 = x.dtype == PGB_F32;
+    const HlOperand clean{s + pl.off_h, 1, 0, x.d};                    // bf16: filled by the first launch where it is needed
+    f.dirty = stats + 1; f.h = static_cast<const __nv_bfloat16 *>(x.h); f.N = x.N;
     // launch i: the products of piece i - 1, ds of piece i
     for (long long i = 0; i <= pl.pieces; ++i) {
         HlMaps maps;
         HlTrio work{};
         work.first = i == 0;
+        f.clean = i == 0 && dw && pl.terms == 1 ? static_cast<__nv_bfloat16 *>(const_cast<void *>(clean.ptr)) : nullptr;
         auto rows_of = [&](long long j) { return pl.by_rows && (j + 1) * pl.step > x.N ? x.N - j * pl.step : pl.rows; };
         auto cols_of = [&](long long j) { return !pl.by_rows && (j + 1) * pl.step > x.V ? x.V - j * pl.step : pl.cols; };
         bool mapped = true;
@@ -1107,7 +1135,8 @@ int head_loss_bwd_launch(const HeadLossArgs &x, const float *L, const float *cou
                 f.grads.g[0] = {at(pl.off_dh), static_cast<char *>(dh) + row_from * x.d * esize, rows, gathers && !first, !gathers || last};
             }
             if (dw) {                                                  // dW[cols] += ds^T h[rows]
-                mapped = mapped && hl_map(&maps.a[1], piece(j), 0, 0, rows, cols, true) && hl_map(&maps.b[1], h, row_from, 0, rows, x.d, true);
+                mapped = mapped && hl_map(&maps.a[1], piece(j), 0, 0, rows, cols, true) && hl_map(&maps.b[1], h, row_from, 0, rows, x.d, true) &&
+                         (pl.terms == 3 || hl_map(&maps.clean, clean, row_from, 0, rows, x.d, true));
                 HlProduct &q = work.p[1];
                 q.tiles_m = hl_tiles(cols); q.tiles_n = hl_tiles(x.d); q.kb = (int)((rows + HL_BK - 1) / HL_BK); q.splits = pl.s_dw[last]; q.a_mn = 1; q.b_mn = 1;
                 const bool gathers = pl.by_rows && pl.pieces > 1;

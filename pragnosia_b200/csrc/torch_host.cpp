@@ -422,15 +422,15 @@ HeadIn head_in(const char *what, const Tensor &h, const Tensor &w) {
 }
 // What a row is held to: a word each (target), or a teacher's entries (lists, marks, ent; kept: their logits).
 struct HeadWant { Tensor target; int64_t ignore; Tensor lists, marks, ent, kept; double tau; };
-struct HeadOut { Tensor loss, L, count; };                            // loss: [N] or 0-d
+struct HeadOut { Tensor loss, L, stats; };                            // loss: [N] or 0-d; stats: rows that count, whether one that does not is no number
 HeadOut head_fwd(const char *what, const HeadIn &x, const HeadWant &t, int reduction) {
     OnDevice dev(x.h);
     HeadOut r{alloc(x.h, reduction == REDUCE_NONE ? at::IntArrayRef({x.N}) : at::IntArrayRef(), at::kFloat), alloc(x.h, {x.N, 2}, at::kFloat),
-              alloc(x.h, {}, at::kFloat)};
+              alloc(x.h, {2}, at::kFloat)};
     if (x.N == 0) {                                                    // nothing to add up: 0, and 0 / 0 as the mean
         if (reduction == REDUCE_SUM) r.loss.zero_();
         if (reduction == REDUCE_MEAN) r.loss.fill_(std::numeric_limits<float>::quiet_NaN());
-        r.count.zero_();
+        r.stats.zero_();
         return r;
     }
     const bool list = t.lists.defined();
@@ -439,14 +439,14 @@ HeadOut head_fwd(const char *what, const HeadIn &x, const HeadWant &t, int reduc
     const Tensor scratch = bytes(x.h, n);
     float *row = reduction == REDUCE_NONE ? fp(r.loss) : nullptr, *loss = reduction == REDUCE_NONE ? nullptr : fp(r.loss);
     if (list)
-        check(pgb_linear_distill_fwd(vp(x.h), vp(x.w), code(x.h), static_cast<int *>(vp(t.lists)), static_cast<unsigned *>(vp(t.marks)), fp(t.ent), fp(t.kept), k, t.tau, row, loss, fp(r.count), fp(r.L),
+        check(pgb_linear_distill_fwd(vp(x.h), vp(x.w), code(x.h), static_cast<int *>(vp(t.lists)), static_cast<unsigned *>(vp(t.marks)), fp(t.ent), fp(t.kept), k, t.tau, row, loss, fp(r.stats), fp(r.L),
                                      vp(scratch), n, reduction, x.N, x.V, x.d, dev.stream), what);
     else
-        check(pgb_linear_xent_fwd(vp(x.h), vp(x.w), code(x.h), static_cast<long long *>(vp(t.target)), t.ignore, row, loss, fp(r.count), fp(r.L), vp(scratch),
+        check(pgb_linear_xent_fwd(vp(x.h), vp(x.w), code(x.h), static_cast<long long *>(vp(t.target)), t.ignore, row, loss, fp(r.stats), fp(r.L), vp(scratch),
                                   n, reduction, x.N, x.V, x.d, dev.stream), what);
     return r;
 }
-std::tuple<Tensor, Tensor> head_bwd(const char *what, const HeadIn &x, const HeadWant &t, const Tensor &L, const Tensor &count, const Tensor &grad_, int reduction,
+std::tuple<Tensor, Tensor> head_bwd(const char *what, const HeadIn &x, const HeadWant &t, const Tensor &L, const Tensor &stats, const Tensor &grad_, int reduction,
                                     bool want_dh, bool want_dw) {
     OnDevice dev(x.h);
     Tensor dh, dw;
@@ -460,10 +460,10 @@ std::tuple<Tensor, Tensor> head_bwd(const char *what, const HeadIn &x, const Hea
     const long long n = pgb_head_loss_bwd_scratch_bytes(x.N, x.V, x.d, code(x.h), want_dh, want_dw);
     const Tensor scratch = bytes(x.h, n);
     if (t.lists.defined())
-        check(pgb_linear_distill_bwd(vp(x.h), vp(x.w), code(x.h), static_cast<int *>(vp(t.lists)), static_cast<unsigned *>(vp(t.marks)), fp(t.ent), fp(t.kept), t.lists.size(1), t.tau, fp(L), fp(count),
+        check(pgb_linear_distill_bwd(vp(x.h), vp(x.w), code(x.h), static_cast<int *>(vp(t.lists)), static_cast<unsigned *>(vp(t.marks)), fp(t.ent), fp(t.kept), t.lists.size(1), t.tau, fp(L), fp(stats),
                                      fp(grad), vp(dh), vp(dw), vp(scratch), n, reduction, x.N, x.V, x.d, dev.stream), what);
     else
-        check(pgb_linear_xent_bwd(vp(x.h), vp(x.w), code(x.h), static_cast<long long *>(vp(t.target)), t.ignore, fp(L), fp(count), fp(grad), vp(dh), vp(dw),
+        check(pgb_linear_xent_bwd(vp(x.h), vp(x.w), code(x.h), static_cast<long long *>(vp(t.target)), t.ignore, fp(L), fp(stats), fp(grad), vp(dh), vp(dw),
                                   vp(scratch), n, reduction, x.N, x.V, x.d, dev.stream), what);
     return {dh, dw};
 }
@@ -507,7 +507,7 @@ struct HeadLoss : torch::autograd::Function<HeadLoss> {
         const HeadIn x = head_in(what, h_, w_);
         const HeadWant t = target ? xent_want(x, h_, *target, ignore) : distill_want(x, h_, *ids, *logits, tau);
         HeadOut r = head_fwd(what, x, t, reduction);
-        ctx->save_for_backward({x.h, x.w, t.target, t.lists, t.marks, t.ent, t.kept, r.L, r.count});
+        ctx->save_for_backward({x.h, x.w, t.target, t.lists, t.marks, t.ent, t.kept, r.L, r.stats});
         auto &d = ctx->saved_data;
         d["ignore"] = ignore; d["tau"] = tau; d["reduction"] = reduction; d["shape"] = h_.sizes().vec();
         ctx->set_materialize_grads(false);
@@ -655,12 +655,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("linear_xent_fwd", [](const Tensor &h, const Tensor &w, const Tensor &target, int64_t ignore, int reduction) {
         const HeadIn x = head_in(XENT, h, w);
         HeadOut r = head_fwd(XENT, x, xent_want(x, h, target, ignore), reduction);
-        return std::make_tuple(r.loss, r.L, r.count);
+        return std::make_tuple(r.loss, r.L, r.stats);
     }, nogil);
-    m.def("linear_xent_bwd", [](const Tensor &h, const Tensor &w, const Tensor &target, int64_t ignore, const Tensor &L, const Tensor &count, const Tensor &grad,
+    m.def("linear_xent_bwd", [](const Tensor &h, const Tensor &w, const Tensor &target, int64_t ignore, const Tensor &L, const Tensor &stats, const Tensor &grad,
                                 int reduction, bool want_dh, bool want_dw) {
         const HeadIn x = head_in(XENT, h, w);
-        auto [dh, dw] = head_bwd(XENT, x, xent_want(x, h, target, ignore), L, count, grad, reduction, want_dh, want_dw);
+        auto [dh, dw] = head_bwd(XENT, x, xent_want(x, h, target, ignore), L, stats, grad, reduction, want_dh, want_dw);
         return std::make_tuple(some(dh), some(dw));
     }, nogil);
     m.def("teacher_lists", &teacher_lists, nogil);
@@ -669,12 +669,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         const HeadIn x = head_in(DISTILL, h, w);
         const Tensor kept = alloc(x.h, {x.N, lists.size(1)}, at::kFloat);
         HeadOut r = head_fwd(DISTILL, x, {Tensor(), 0, lists, marks, ent, kept, tau}, reduction);
-        return std::make_tuple(r.loss, r.L, r.count, kept);
+        return std::make_tuple(r.loss, r.L, r.stats, kept);
     }, nogil);
     m.def("linear_distill_bwd", [](const Tensor &h, const Tensor &w, const Tensor &lists, const Tensor &marks, const Tensor &ent, const Tensor &kept, double tau,
-                                   const Tensor &L, const Tensor &count, const Tensor &grad, int reduction, bool want_dh, bool want_dw) {
+                                   const Tensor &L, const Tensor &stats, const Tensor &grad, int reduction, bool want_dh, bool want_dw) {
         const HeadIn x = head_in(DISTILL, h, w);
-        auto [dh, dw] = head_bwd(DISTILL, x, {Tensor(), 0, lists, marks, ent, kept, tau}, L, count, grad, reduction, want_dh, want_dw);
+        auto [dh, dw] = head_bwd(DISTILL, x, {Tensor(), 0, lists, marks, ent, kept, tau}, L, stats, grad, reduction, want_dh, want_dw);
         return std::make_tuple(some(dh), some(dw));
     }, nogil);
     m.def("embedding", &embedding, nogil);

@@ -471,24 +471,24 @@ def _grads_like(h, W, want_dh, want_dW):
 
 @torch.library.custom_op(f"{NS}::linear_xent", mutates_args=())
 def linear_xent(h: Tensor, W: Tensor, target: Tensor, ignore_index: int, reduction: int) -> Tuple[Tensor, Tensor, Tensor]:
-    """(loss, the rows' log2 sums of exponentials in two parts, rows that count); reduction 0 none, 1 sum, 2 mean."""
+    """(loss, the rows' log2 sums of exponentials in two parts, [rows that count, whether one that does not is no number]); reduction 0 none, 1 sum, 2 mean."""
     return host().linear_xent_fwd(h, W, target, ignore_index, reduction)
 
 
 @linear_xent.register_fake
 def _(h, W, target, ignore_index, reduction):
-    return _loss_like(h, reduction), _e(h, _rows(h), 2, dtype=_F32), _e(h, dtype=_F32)
+    return _loss_like(h, reduction), _e(h, _rows(h), 2, dtype=_F32), _e(h, 2, dtype=_F32)
 
 
 @torch.library.custom_op(f"{NS}::linear_xent_bwd", mutates_args=())
-def linear_xent_bwd(h: Tensor, W: Tensor, target: Tensor, ignore_index: int, L: Tensor, count: Tensor, grad: Tensor, reduction: int, want_dh: bool,
+def linear_xent_bwd(h: Tensor, W: Tensor, target: Tensor, ignore_index: int, L: Tensor, stats: Tensor, grad: Tensor, reduction: int, want_dh: bool,
                     want_dW: bool) -> Tuple[Tensor, Tensor]:
-    dh, dW = host().linear_xent_bwd(h, W, target, ignore_index, L, count, grad, reduction, want_dh, want_dW)
+    dh, dW = host().linear_xent_bwd(h, W, target, ignore_index, L, stats, grad, reduction, want_dh, want_dW)
     return (dh.view(h.shape) if want_dh else _none(h)), (dW if want_dW else _none(W))
 
 
 @linear_xent_bwd.register_fake
-def _(h, W, target, ignore_index, L, count, grad, reduction, want_dh, want_dW):
+def _(h, W, target, ignore_index, L, stats, grad, reduction, want_dh, want_dW):
     return _grads_like(h, W, want_dh, want_dW)
 
 
@@ -497,10 +497,10 @@ def _xent_ctx(ctx, inputs, output):
     ctx.save_for_backward(h, W, target, output[1], output[2])
 
 
-def _xent_grads(ctx, g, _L, _count):
-    h, W, target, L, count = ctx.saved_tensors
+def _xent_grads(ctx, g, _L, _stats):
+    h, W, target, L, stats = ctx.saved_tensors
     want = ctx.needs_input_grad[:2]
-    dh, dW = torch.ops.pragnosia_b200.linear_xent_bwd(h, W, target, ctx.ignore_index, L, count, g, ctx.reduction, *want)
+    dh, dW = torch.ops.pragnosia_b200.linear_xent_bwd(h, W, target, ctx.ignore_index, L, stats, g, ctx.reduction, *want)
     return (dh if want[0] else None), (dW if want[1] else None), None, None, None
 
 
@@ -528,18 +528,18 @@ def linear_distill(h: Tensor, W: Tensor, lists: Tensor, marks: Tensor, ent: Tens
 
 @linear_distill.register_fake
 def _(h, W, lists, marks, ent, temperature, reduction):
-    return _loss_like(h, reduction), _e(h, _rows(h), 2, dtype=_F32), _e(h, dtype=_F32), _e(h, _rows(h), lists.shape[1], dtype=_F32)
+    return _loss_like(h, reduction), _e(h, _rows(h), 2, dtype=_F32), _e(h, 2, dtype=_F32), _e(h, _rows(h), lists.shape[1], dtype=_F32)
 
 
 @torch.library.custom_op(f"{NS}::linear_distill_bwd", mutates_args=())
-def linear_distill_bwd(h: Tensor, W: Tensor, lists: Tensor, marks: Tensor, ent: Tensor, kept: Tensor, temperature: float, L: Tensor, count: Tensor, grad: Tensor,
+def linear_distill_bwd(h: Tensor, W: Tensor, lists: Tensor, marks: Tensor, ent: Tensor, kept: Tensor, temperature: float, L: Tensor, stats: Tensor, grad: Tensor,
                        reduction: int, want_dh: bool, want_dW: bool) -> Tuple[Tensor, Tensor]:
-    dh, dW = host().linear_distill_bwd(h, W, lists, marks, ent, kept, temperature, L, count, grad, reduction, want_dh, want_dW)
+    dh, dW = host().linear_distill_bwd(h, W, lists, marks, ent, kept, temperature, L, stats, grad, reduction, want_dh, want_dW)
     return (dh.view(h.shape) if want_dh else _none(h)), (dW if want_dW else _none(W))
 
 
 @linear_distill_bwd.register_fake
-def _(h, W, lists, marks, ent, kept, temperature, L, count, grad, reduction, want_dh, want_dW):
+def _(h, W, lists, marks, ent, kept, temperature, L, stats, grad, reduction, want_dh, want_dW):
     return _grads_like(h, W, want_dh, want_dW)
 
 
@@ -548,10 +548,10 @@ def _distill_ctx(ctx, inputs, output):
     ctx.save_for_backward(h, W, lists, marks, ent, output[3], output[1], output[2])
 
 
-def _distill_grads(ctx, g, _L, _count, _kept):
-    h, W, lists, marks, ent, kept, L, count = ctx.saved_tensors
+def _distill_grads(ctx, g, _L, _stats, _kept):
+    h, W, lists, marks, ent, kept, L, stats = ctx.saved_tensors
     want = ctx.needs_input_grad[:2]
-    dh, dW = torch.ops.pragnosia_b200.linear_distill_bwd(h, W, lists, marks, ent, kept, ctx.temperature, L, count, g, ctx.reduction, *want)
+    dh, dW = torch.ops.pragnosia_b200.linear_distill_bwd(h, W, lists, marks, ent, kept, ctx.temperature, L, stats, g, ctx.reduction, *want)
     return (dh if want[0] else None), (dW if want[1] else None), None, None, None, None, None
 
 

@@ -31,8 +31,7 @@ def linear_cross_entropy(h, weight, target, *, ignore_index: int = -100, reducti
 
     h (..., d); weight (V, d) of h's type, d a multiple of 8; target (...) int64 or int32. Returns float32: a loss per row (reduction
     "none", target's shape), their sum, or their mean over the rows whose target is not ignore_index (nan where there is none, as torch has it).
-    Ignored rows lose 0 and have no gradient; with a gradient wanted for the weight, h has to be finite in them all the same. Any other
-    target outside 0 .. V-1 gives nan, in the loss and in the gradients of its row and of the weight.
+    Ignored rows lose 0 and have no gradient, whatever h holds there. Any other target outside 0 .. V-1 gives nan, in the loss and in the gradients of its row and of the weight.
 
     Without a gradient wanted (no_grad, or neither tensor requires one) this is the scoring of given tokens, one to many. bf16: products
     in bf16 with fp32 sums; the gradient of the logits is rounded to bf16 on its way into the two products behind it. float32: float32's own precision."""

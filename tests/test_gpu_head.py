@@ -149,6 +149,48 @@ def test_targets_outside_the_vocabulary_give_nan():
         assert torch.isnan(dh[17]).all() and torch.isfinite(dh[:17]).all() and torch.isfinite(dh[18:]).all() and torch.isnan(dw).all()
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("N,V", [(700, 300), (3000, 17000), (9000, 6200)])
+def test_rows_that_do_not_count_may_hold_anything(N, V, dtype):
+    """Infinities and NaN in ignored rows of h (padding that a kernel never wrote): the results are those with zeros there, to the bit."""
+    h, w, g = operands(N, V, 72, dtype, 11)
+    t = torch.randint(0, V, (N,), device=DEV, generator=g)
+    dead = torch.rand(N, device=DEV, generator=g) < 0.2
+    dead[-1] = True
+    t[dead] = -100
+    filled = h.clone()
+    filled[dead] = torch.tensor([math.nan, math.inf, -math.inf, 3e38], device=DEV)[torch.randint(0, 4, (int(dead.sum()), 72), device=DEV, generator=g)].to(dtype)
+    h[dead] = 0
+    ids, logits = lists(N, V, 3, g, False)
+    ids[dead] = -1
+    c = torch.rand(N, device=DEV, generator=g)
+    for call in (lambda x: xent(x, w, t, c, "mean"), lambda x: xent(x, w, t, c, "none"), lambda x: distill(x, w, ids, logits, 2.0, c, "mean")):
+        want, got = call(h), call(filled)
+        assert all(torch.isfinite(a).all() and torch.equal(a, b) for a, b in zip(want, got))
+
+
+def test_rows_past_32_bits():
+    """h of more than 2^31 elements: its last rows are as they are by themselves."""
+    N, V, d, n = 2_900_000, 70, 768, 300
+    g = torch.Generator(device=DEV).manual_seed(3)
+    h = torch.empty(N, d, device=DEV, dtype=BF).normal_(generator=g)
+    w = (0.05 * torch.randn(V, d, device=DEV, generator=g)).to(BF)
+    t = torch.randint(0, V, (N,), device=DEV, generator=g)
+    c = torch.rand(N, device=DEV, generator=g)
+    loss, dh, dw = xent(h, w, t, c, "none")
+    p, live = one_hot(t[-n:], V)
+    want, off = dense(h[-n:], w, p, live, 1.0, c[-n:], "none")
+    within((loss[-n:], dh[-n:]), want[:2], off[:2])
+    del loss, dh
+    y, de = embed(t, w, h)
+    assert torch.equal(y[-n:], w[t[-n:]])
+    ref = torch.zeros(V, d, device=DEV, dtype=torch.float64)
+    for a in range(0, N, 100_000):
+        ref.index_add_(0, t[a:a + 100_000], h[a:a + 100_000].double())
+    # chunks of 32 added one by one (32 roundings), their 1300 sums by eight threads: 163 + 8 roundings of sums of about 41400 normal numbers
+    assert ((de.double() - ref).abs() <= 2.0 ** -8 * ref.abs() + 210 * 2.0 ** -24 * 41400 * 0.9).all()
+
+
 def test_forms_of_the_call():
     """Leading axes, other strides and types of ids, a view off the 16-byte grid, one gradient alone, an ignore_index inside the vocabulary."""
     h, w, g = operands(12 * 31, 333, 64, BF, 4)

@@ -15,12 +15,12 @@ one, odd = ctypes.c_void_p(0x1000), ctypes.c_void_p(0x1004)           # never de
 BIG = 1 << 40
 
 
-def xent_fwd(h=one, W=one, dtype=1, target=one, ignore=-100, rows=None, loss=one, count=one, L=one, scratch=one, n=BIG, red=2, N=4, V=10, d=64):
-    return lib().pgb_linear_xent_fwd(h, W, dtype, target, ignore, rows, loss, count, L, scratch, n, red, N, V, d, None)
+def xent_fwd(h=one, W=one, dtype=1, target=one, ignore=-100, rows=None, loss=one, stats=one, L=one, scratch=one, n=BIG, red=2, N=4, V=10, d=64):
+    return lib().pgb_linear_xent_fwd(h, W, dtype, target, ignore, rows, loss, stats, L, scratch, n, red, N, V, d, None)
 
 
-def xent_bwd(h=one, W=one, dtype=1, target=one, L=one, count=one, grad=one, dh=one, dW=one, scratch=one, n=BIG, red=2, N=4, V=10, d=64):
-    return lib().pgb_linear_xent_bwd(h, W, dtype, target, -100, L, count, grad, dh, dW, scratch, n, red, N, V, d, None)
+def xent_bwd(h=one, W=one, dtype=1, target=one, L=one, stats=one, grad=one, dh=one, dW=one, scratch=one, n=BIG, red=2, N=4, V=10, d=64):
+    return lib().pgb_linear_xent_bwd(h, W, dtype, target, -100, L, stats, grad, dh, dW, scratch, n, red, N, V, d, None)
 
 
 def distill_fwd(lists=one, marks=one, ent=one, kept=one, k=4, tau=1.0):
@@ -31,12 +31,12 @@ NULL, SHAPE, ALIGN, DTYPE, LARGE = 1, 2, 4, 5, 7
 
 
 @pytest.mark.parametrize("call,kw,code", [
-    *[(xent_fwd, {n: None}, NULL) for n in ("h", "W", "target", "loss", "count", "L", "scratch")], (xent_fwd, dict(red=0), NULL),
+    *[(xent_fwd, {n: None}, NULL) for n in ("h", "W", "target", "loss", "stats", "L", "scratch")], (xent_fwd, dict(red=0), NULL),
     (xent_fwd, dict(dtype=2), DTYPE), (xent_fwd, dict(N=0), SHAPE), (xent_fwd, dict(V=0), SHAPE), (xent_fwd, dict(d=0), SHAPE), (xent_fwd, dict(d=60), SHAPE),
     (xent_fwd, dict(red=3), SHAPE), (xent_fwd, dict(red=-1), SHAPE), (xent_fwd, dict(n=100), SHAPE), (xent_fwd, dict(h=odd), ALIGN), (xent_fwd, dict(W=odd), ALIGN),
     (xent_fwd, dict(target=odd), ALIGN), (xent_fwd, dict(L=odd), ALIGN), (xent_fwd, dict(scratch=odd), ALIGN),
     (xent_fwd, dict(N=(1 << 30) + 1), LARGE), (xent_fwd, dict(V=(1 << 30) + 1), LARGE), (xent_fwd, dict(d=65544), LARGE), (xent_fwd, dict(N=1 << 30, V=1 << 24), LARGE),
-    *[(xent_bwd, {n: None}, NULL) for n in ("h", "W", "target", "L", "count", "grad", "scratch")], (xent_bwd, dict(dh=None, dW=None), NULL),
+    *[(xent_bwd, {n: None}, NULL) for n in ("h", "W", "target", "L", "stats", "grad", "scratch")], (xent_bwd, dict(dh=None, dW=None), NULL),
     (xent_bwd, dict(dh=odd), ALIGN), (xent_bwd, dict(dW=odd), ALIGN), (xent_bwd, dict(n=100), SHAPE), (xent_bwd, dict(d=12), SHAPE),
     *[(distill_fwd, {n: None}, NULL) for n in ("lists", "marks", "ent", "kept")], (distill_fwd, dict(k=0), SHAPE), (distill_fwd, dict(k=1025), LARGE),
     (distill_fwd, dict(tau=0.0), SHAPE), (distill_fwd, dict(tau=-1.0), SHAPE), (distill_fwd, dict(tau=float("inf")), SHAPE), (distill_fwd, dict(tau=float("nan")), SHAPE),
@@ -62,7 +62,7 @@ def test_bad_calls_of_teacher_lists_and_embedding():
                                          (7, 262144, 4096, 1), (1 << 20, 1 << 17, 4096, 1), (3, 1 << 24, 64, 0)])
 def test_scratch_stays_far_below_the_logits(N, V, d, dtype):
     """The workspace of the backward pass: three pieces of 64 MiB (a block of 256 rows or columns where that is more), fp32 sums of the smaller
-    gradient, split operands. Asked twice, the same."""
+    gradient, split operands or a clean copy of h. Asked twice, the same."""
     L = lib()
     for want in ((1, 1), (1, 0), (0, 1)):
         n = L.pgb_head_loss_bwd_scratch_bytes(N, V, d, dtype, *want)
@@ -70,7 +70,8 @@ def test_scratch_stays_far_below_the_logits(N, V, d, dtype):
         terms = 3 if dtype == 0 else 1
         pieces = 3 * max(64 << 20, 2 * terms * 256 * (min(N, V) + 512)) + (1 << 20)
         sums = 4 * 32 * d * 2 * (min(N, V) + 8192 + 512) if N * V < (1 << 27) else 4 * d * (min(N, V) + max(N, V)) * 4
-        assert n <= pieces + sums + (6 * d * (N + V) + 1024 if dtype == 0 else 0)
+        copies = 6 * d * (N + V) if dtype == 0 else 2 * d * N if want[1] else 0
+        assert n <= pieces + sums + copies + 1024
 
 
 def test_python_refusals():
@@ -96,17 +97,17 @@ def test_shape_functions():
         e = lambda *s, dtype=BF: torch.empty(*s, dtype=dtype, device="cuda")
         h, w, t = e(2, 5, 64), e(33, 64), e(2, 5, dtype=torch.long)
         for red, shape in ((0, (10,)), (1, ()), (2, ())):
-            loss, L, count = OPS.linear_xent(h, w, t, -100, red)
-            assert sig(loss) == (shape, F32) and sig(L) == ((10, 2), F32) and sig(count) == ((), F32)
-        dh, dw = OPS.linear_xent_bwd(h, w, t, -100, L, count, loss, 2, True, True)
+            loss, L, stats = OPS.linear_xent(h, w, t, -100, red)
+            assert sig(loss) == (shape, F32) and sig(L) == ((10, 2), F32) and sig(stats) == ((2,), F32)
+        dh, dw = OPS.linear_xent_bwd(h, w, t, -100, L, stats, loss, 2, True, True)
         assert sig(dh) == ((2, 5, 64), BF) and sig(dw) == ((33, 64), BF)
-        dh, dw = OPS.linear_xent_bwd(h, w, t, -100, L, count, loss, 2, True, False)
+        dh, dw = OPS.linear_xent_bwd(h, w, t, -100, L, stats, loss, 2, True, False)
         assert sig(dh) == ((2, 5, 64), BF) and dw.numel() == 0
         lists, marks, ent = OPS.teacher_lists(e(2, 5, 7, dtype=torch.long), e(2, 5, 7, dtype=F32), 2.0, 130)
         assert sig(lists) == ((10, 7, 2), torch.int32) and sig(marks) == ((10, 3, 4), torch.int32) and sig(ent) == ((10,), F32)
-        loss, L, count, kept = OPS.linear_distill(h, w, lists, marks, ent, 2.0, 0)
+        loss, L, stats, kept = OPS.linear_distill(h, w, lists, marks, ent, 2.0, 0)
         assert sig(loss) == ((10,), F32) and sig(kept) == ((10, 7), F32)
-        dh, dw = OPS.linear_distill_bwd(h, w, lists, marks, ent, kept, 2.0, L, count, loss, 0, True, True)
+        dh, dw = OPS.linear_distill_bwd(h, w, lists, marks, ent, kept, 2.0, L, stats, loss, 0, True, True)
         assert sig(dh) == ((2, 5, 64), BF) and sig(dw) == ((33, 64), BF)
         assert sig(OPS.embedding(t, w, 1.0, -1)) == ((2, 5, 64), BF) and sig(OPS.embedding_bwd(t, h, 1.0, -1, 33)) == ((33, 64), BF)
         with torch.enable_grad():
