@@ -31,7 +31,7 @@ constexpr int HL_CW = HL_B / (HL_EPI / 4);                            // columns
 constexpr int HL_OUT_BYTES = 32 * 64;                                 // staging of an epilogue warp: 32 rows of 64 bytes
 constexpr int HL_SMEM = HL_STAGES * HL_STAGE + 1024 + HL_EPI * HL_OUT_BYTES + 1024;
 constexpr int HL_GROUP = 16;                                          // row blocks that a sweep over the columns takes together
-constexpr long long HL_PIECE_BYTES = 64LL << 20;                      // of ds, three such pieces in the workspace: written, read, and about to be written by the next launch
+constexpr long long HL_PIECE_BYTES = 64LL << 20;                      // of ds, two such pieces in the workspace: one written, one read
 static_assert(HL_STAGE % 1024 == 0 && HL_SMEM <= 232448, "shared memory");
 constexpr float LOG2E_F = 1.4426950408889634f;
 
@@ -52,47 +52,43 @@ struct HlProduct {
         m = g * HL_GROUP + in - n * gm;
     }
 };
-// What a pair of SMs does, one part of a tile after the other. One product (forward): every pairs-th tile. Three (backward): its share of ds's
-// tiles, which are short, and then every pairs-th of [dh's parts][dW's], a product's by part of K, then by tile; the shares level out what the
-// long parts leave uneven. ds of a piece needs nothing of the launch before, whose products are those of the piece before (a third piece of
-// the workspace is what that launch reads): a pair whose SMs are free begins with it while others still work on that launch, and waits for it only then.
+// What a pair of SMs does, one part of a tile after the other. One product (forward): every pairs-th tile. Three (backward): every pairs-th of
+// [dh's parts][dW's], a product's by part of K, then by tile, and behind them its share of ds's tiles, which are short: the shares level out what
+// the long parts leave uneven.
 //   So the pairs that run side by side walk the same stretch of K together and what they read they share through the L2: with equal shares of
 // all K blocks instead (tiles cut where a share ends) each was somewhere else, 15 of 38 million sectors missed the near L2, and the
 // products took as long as with a quarter of the pairs idle in the last round.
 constexpr int HL_MOST_PAIRS = 127;
-struct HlTrio { HlProduct p[3]; int share[HL_MOST_PAIRS + 1], first; };   // dh, dW, ds; pair q has ds's tiles share[q] .. share[q + 1] - 1; first: the first launch
+struct HlTrio { HlProduct p[3]; int share[HL_MOST_PAIRS + 1]; };      // dh, dW, ds; pair q has ds's tiles share[q] .. share[q + 1] - 1
 struct HlOne {
     const HlProduct &pr;
     int pairs, t;
     static constexpr int g = 0, sp = 0, k0 = 0;
     int k1;
     __device__ HlOne(const HlProduct &pr, int pair, int pairs) : pr(pr), pairs(pairs), t(pair), k1(pr.kb) {}
-    static __device__ __forceinline__ bool early(const HlProduct &) { return false; }
     __device__ __forceinline__ const HlProduct &product() const { return pr; }
     __device__ __forceinline__ bool more() const { return t < pr.tiles(); }
     __device__ __forceinline__ void next() { t += pairs; }
 };
 struct HlThree {
     const HlTrio &w;
-    int pairs, i, end, g = 2, t, sp = 0, k0 = 0, k1;
-    __device__ HlThree(const HlTrio &w, int pair, int pairs) : w(w), pairs(pairs), i(pair), end(w.share[pair + 1]), t(w.share[pair]), k1(w.p[2].kb) {
-        if (t >= end) place();
-    }
-    static __device__ __forceinline__ bool early(const HlTrio &w) { return !w.first; }
+    int pairs, i, end, g = 0, t = 0, sp = 0, k0 = 0, k1 = 0;
+    __device__ HlThree(const HlTrio &w, int pair, int pairs) : w(w), pairs(pairs), i(pair), end(w.share[pair + 1]) { place(w.share[pair]); }
     __device__ __forceinline__ const HlProduct &product() const { return w.p[g]; }
-    __device__ __forceinline__ bool more() const { return t >= 0; }
+    __device__ __forceinline__ bool more() const { return g < 2 || t < end; }
     __device__ __forceinline__ void next() {
-        if (g == 2) {
-            if (++t >= end) place();
-        } else {
-            i += pairs;
-            place();
-        }
+        if (g == 2) { ++t; return; }
+        i += pairs;
+        place(-1);
     }
-    __device__ __forceinline__ void place() {                         // the long part number i
+    __device__ __forceinline__ void place(int first) {
         const int n0 = w.p[0].tiles() * w.p[0].splits, n1 = w.p[1].tiles() * w.p[1].splits;
+        if (i >= n0 + n1) {
+            g = 2; sp = 0; k0 = 0; k1 = w.p[2].kb;
+            t = first >= 0 ? first : w.share[i % pairs];               // i % pairs: the pair
+            return;
+        }
         g = i >= n0;
-        if (i >= n0 + n1) { t = -1; return; }
         const int in = g ? i - n0 : i, tiles = w.p[g].tiles(), kt = w.p[g].kb;
         sp = in / tiles;
         t = in - sp * tiles;
@@ -103,7 +99,6 @@ struct HlThree {
 // The roles of the kernel. An epilogue warp takes its 32 x 64 block of a complete accumulator into registers, hands the accumulator back at once, and
 // works on them while what the next tile needs of its rows (epi.fetch) is on its way.
 // FINE: operands of three terms, a stage holds a block of all of them, and an accumulator a block's products.
-// x.g is 2 for a tile of ds only.
 template <bool FINE, class Work, class What, class Epi>
 __device__ __forceinline__ void hl_body(const HlMaps &maps, const What &what, Epi &epi) {
     constexpr int TERMS = FINE ? 3 : 1, STAGE = TERMS * HL_STAGE, STAGES = HL_STAGES / TERMS, OPERAND = TERMS * HL_HALF;
@@ -133,18 +128,11 @@ __device__ __forceinline__ void hl_body(const HlMaps &maps, const What &what, Ep
     cluster_sync_all();                                                // the partner's barriers and tensor memory exist from here on
     tc_fence_after();
     const uint32_t tmem = warp_uniform(*tmem_slot);
-    const bool early = Work::early(what);                              // ds first, and then the wait for the launch before
-    if (!early) { pdl_wait(); pdl_launch_dependents(); }
+    pdl_wait();
+    pdl_launch_dependents();
 
     Work w(what, pair, pairs);
     int m, n;
-    bool waited = !early;
-    auto wait_for_launch = [&]() {
-        if (waited) return;
-        pdl_wait();
-        pdl_launch_dependents();                                       // not sooner: the launch behind begins with a piece that the one before this reads
-        waited = true;
-    };
     if (warp == 0) {
         // ------------------------------------------------------------------------------------------ producer (both CTAs)
         const bool leader = elect_one(), dirty = epi.dirty();
@@ -152,7 +140,6 @@ __device__ __forceinline__ void hl_body(const HlMaps &maps, const What &what, Ep
         bool ok = true;
         for (; w.more() && ok; w.next()) {
             const HlProduct &p = w.product();
-            if (w.g != 2) wait_for_launch();
             p.at(w.t, m, n);
             const int m0 = m * HL_B + (int)rank * (HL_B / 2), n0 = n * HL_B + (int)rank * (HL_B / 2);
             const CUtensorMap *ma = &maps.a[w.g], *mbm = w.g == 1 && dirty ? &maps.clean : &maps.b[w.g];
@@ -183,7 +170,6 @@ __device__ __forceinline__ void hl_body(const HlMaps &maps, const What &what, Ep
                 __syncwarp();
             }
         }
-        wait_for_launch();                                             // the launch is over only when the one before is
     } else if (warp == 1) {
         // ------------------------------------------------------------------------------------------ MMA issuer (first CTA)
         if (rank == 0) {
@@ -243,7 +229,6 @@ __device__ __forceinline__ void hl_body(const HlMaps &maps, const What &what, Ep
         for (; ok; ++ti) {
             x.n = n; x.row0 = m * HL_B + row_in; x.col0 = n * HL_B + col_in; x.ti = ti;
             x.g = w.g; x.t = w.t; x.sp = w.sp;
-            if (w.g != 2) wait_for_launch();
             epi.begin(x);
             float v[2][32];
             const uint32_t tacc = tmem + lane_base + part * HL_CW;
@@ -719,8 +704,6 @@ struct HlGradEpi {
         const HlGrad &o = f.g[x.g];
         const int lane = x.lane, splits = pr[x.g].splits, rl = lane >> 2, cl = 4 * (lane & 3);
         if (x.col0 >= f.d || x.row0 >= o.rows) return;
-        if (lane == 0) tma_store_source_free();                       // ds's last store has left the staging
-        __syncwarp();
         const long long plane = o.rows * f.d, base = (long long)(x.row0 + rl) * f.d + x.col0 + cl;
         float *acc = o.acc ? o.acc + x.sp * plane + base : nullptr;
         auto chunk_at = [&](int r, int ch) { return stage + r * 64 + ((ch ^ ((r >> 1) & 3)) << 4); };
@@ -807,7 +790,12 @@ struct HlBwdEpi {
     __device__ __forceinline__ void fetch(int g, int r, int c) { if (g == 2) ds.fetch(r, c); }
     __device__ __forceinline__ void begin(const HlTile &x) { if (x.g == 2) ds.begin(x); }
     __device__ __forceinline__ bool tile(const HlTile &x, float (&v)[2][32], uint8_t *stage, uint8_t *, uint32_t) {
-        if (x.g == 2) ds.tile(x, v, stage); else grad.tile(x, v, stage);
+        if (x.g == 2) {
+            ds.tile(x, v, stage);
+        } else {                                                       // all of them before a warp's first of ds: the staging is free
+            grad.tile(x, v, stage);
+            fence_proxy_async();
+        }
         return true;
     }
     __device__ __forceinline__ bool dirty() const { return TERMS == 1 && *f.dirty != 0.f; }
@@ -963,7 +951,7 @@ int head_loss_fwd_launch(const HeadLossArgs &x, float *row_loss, float *loss, fl
 // How the backward pass is cut: pieces of `step` rows (by_rows) or columns, and the parts of K of the two gradients' products.
 struct HlBwdPlan {
     bool by_rows; long long step, pieces, ldp, rows, cols; int terms, s_dh[2], s_dw[2];          // parts in all pieces but the last, in the last
-    long long off_p[3], off_dh, off_dw, off_h, off_w, total;
+    long long off_p[2], off_dh, off_dw, off_h, off_w, total;
 };
 // A launch's work in units of the time of a K block's one product (0.33 us; np of them a block): a part of a tile costs its own and about four
 // more (its epilogue's end and the next one's beginning).
@@ -1041,7 +1029,7 @@ static HlBwdPlan hl_bwd_plan(long long N, int V, int d, int dtype, bool dh, bool
     long long at = 0;
     auto take = [&](long long bytes) { const long long o = at; at += hl_up(bytes, 256); return o; };
     p.off_p[0] = take(2 * p.terms * p.rows * p.ldp);
-    for (int i = 1; i < 3; ++i) p.off_p[i] = p.pieces > i ? take(2 * p.terms * p.rows * p.ldp) : p.off_p[0];
+    p.off_p[1] = p.pieces > 1 ? take(2 * p.terms * p.rows * p.ldp) : p.off_p[0];
     // fp32 sums: of the gradient that gathers over pieces, and of one whose K axis is in parts
     const int sh = p.s_dh[0] > p.s_dh[1] ? p.s_dh[0] : p.s_dh[1], sw = p.s_dw[0] > p.s_dw[1] ? p.s_dw[0] : p.s_dw[1];
     p.off_dh = dh && (sh > 1 || (!p.by_rows && p.pieces > 1)) ? take(4LL * sh * p.rows * d) : -1;
@@ -1101,7 +1089,7 @@ int head_loss_bwd_launch(const HeadLossArgs &x, const float *L, const float *sta
                    : which == 2 ? hl_pairs(head_loss_bwd_kernel<false, 3>, 6) : hl_pairs(head_loss_bwd_kernel<true, 3>, 7);
     if (room < 1) { set_cuda_error(cudaGetLastError(), "head_loss_bwd_kernel"); return PGB_ERR_CUDA; }
     auto at = [&](long long off) { return off >= 0 ? reinterpret_cast<float *>(s + off) : nullptr; };
-    auto piece = [&](long long i) { return HlOperand{s + pl.off_p[i % 3], pl.terms, pl.rows * pl.ldp, pl.ldp}; };
+    auto piece = [&](int i) { return HlOperand{s + pl.off_p[i & 1], pl.terms, pl.rows * pl.ldp, pl.ldp}; };
     HlBwd f{};
     f.ds.t = targets;
     f.ds.L = reinterpret_cast<const float2 *>(L); f.ds.row_weight = x.reduction == 0 ? up : nullptr; f.ds.a = LOG2E_F / x.tau; f.ds.V = x.V;
@@ -1112,7 +1100,6 @@ int head_loss_bwd_launch(const HeadLossArgs &x, const float *L, const float *sta
     for (long long i = 0; i <= pl.pieces; ++i) {
         HlMaps maps;
         HlTrio work{};
-        work.first = i == 0;
         f.clean = i == 0 && dw && pl.terms == 1 ? static_cast<__nv_bfloat16 *>(const_cast<void *>(clean.ptr)) : nullptr;
         auto rows_of = [&](long long j) { return pl.by_rows && (j + 1) * pl.step > x.N ? x.N - j * pl.step : pl.rows; };
         auto cols_of = [&](long long j) { return !pl.by_rows && (j + 1) * pl.step > x.V ? x.V - j * pl.step : pl.cols; };

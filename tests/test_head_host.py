@@ -61,14 +61,14 @@ def test_bad_calls_of_teacher_lists_and_embedding():
 @pytest.mark.parametrize("N,V,d,dtype", [(1, 1, 8, 1), (511, 8192, 768, 1), (32768, 8192, 768, 1), (8192, 50257, 768, 1), (2000, 8192, 704, 0), (100000, 300, 4096, 1),
                                          (7, 262144, 4096, 1), (1 << 20, 1 << 17, 4096, 1), (3, 1 << 24, 64, 0)])
 def test_scratch_stays_far_below_the_logits(N, V, d, dtype):
-    """The workspace of the backward pass: three pieces of 64 MiB (a block of 256 rows or columns where that is more), fp32 sums of the smaller
+    """The workspace of the backward pass: two pieces of 64 MiB (a block of 256 rows or columns where that is more), fp32 sums of the smaller
     gradient, split operands or a clean copy of h. Asked twice, the same."""
     L = lib()
     for want in ((1, 1), (1, 0), (0, 1)):
         n = L.pgb_head_loss_bwd_scratch_bytes(N, V, d, dtype, *want)
         assert n == L.pgb_head_loss_bwd_scratch_bytes(N, V, d, dtype, *want) > 0
         terms = 3 if dtype == 0 else 1
-        pieces = 3 * max(64 << 20, 2 * terms * 256 * (min(N, V) + 512)) + (1 << 20)
+        pieces = 2 * max(64 << 20, 2 * terms * 256 * (min(N, V) + 512)) + (1 << 20)
         sums = 4 * 32 * d * 2 * (min(N, V) + 8192 + 512) if N * V < (1 << 27) else 4 * d * (min(N, V) + max(N, V)) * 4
         copies = 6 * d * (N + V) if dtype == 0 else 2 * d * N if want[1] else 0
         assert n <= pieces + sums + copies + 1024
