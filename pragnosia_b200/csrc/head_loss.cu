@@ -410,14 +410,15 @@ struct HlJoin {
 };
 template <bool LIST>
 __global__ void __launch_bounds__(256) head_loss_join_kernel(const HlJoin j) {
-    __shared__ float3 part[8][32];
+    __shared__ float2 part[8][32];
+    __shared__ float dots[32];
     __shared__ double2 sums[8];
     __shared__ bool last;
     pdl_wait();
     pdl_launch_dependents();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const long long row = (long long)blockIdx.x * 32 + lane;
-    float m = -INFINITY, l = 0.f, dot = 0.f;
+    float m = -INFINITY, l = 0.f;
     if (row < j.N) {
 #pragma unroll 4
         for (int n = warp; n < j.tiles; n += 8) {
@@ -426,37 +427,48 @@ __global__ void __launch_bounds__(256) head_loss_join_kernel(const HlJoin j) {
             l = l * fast_exp2(m - at) + o.y * fast_exp2(o.x - at);
             m = top;
         }
-        if constexpr (LIST) {
-            const int2 *list = j.t.lists + row * j.t.k;
-#pragma unroll 4
-            for (int i = warp; i < j.t.k; i += 8) {
-                const int2 e = list[i];
-                const float s = j.dot[row * j.t.k + i];
-                if (e.x < j.V) dot = fmaf(__int_as_float(e.y), s, dot);
+    }
+    if constexpr (LIST) {                                              // four rows a warp, the entries over its lanes
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int i = lane; i < j.t.k; i += 32) {
+            int2 e[4];
+            float s[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {                              // rows behind the last: the last again, all loads before the first use
+                const long long at = min((long long)blockIdx.x * 32 + 4 * warp + q, j.N - 1) * j.t.k + i;
+                e[q] = j.t.lists[at];
+                s[q] = j.dot[at];
             }
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (e[q].x < j.V) sum[q] = fmaf(__int_as_float(e[q].y), s[q], sum[q]);
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            sum[q] = warp_sum(sum[q]);
+            if (lane == 0) dots[4 * warp + q] = sum[q];
         }
     }
-    part[warp][lane] = make_float3(m, l, dot);
+    part[warp][lane] = make_float2(m, l);
     __syncthreads();
     double loss = 0.0;
     bool live = false;
     if (warp == 0 && row < j.N) {
 #pragma unroll
         for (int q = 1; q < 8; ++q) {
-            const float3 o = part[q][lane];
+            const float2 o = part[q][lane];
             const float top = fmaxf(m, o.x), at = top == -INFINITY ? 0.f : top;
             l = l * fast_exp2(m - at) + o.y * fast_exp2(o.x - at);
             m = top;
-            dot += o.z;
         }
         const float lg = log2f(l), hi = m + lg;                        // hi + lo = m + lg, exactly
         const float back = hi - m, rest = (m - (hi - back)) + (lg - back), lo = rest == rest ? rest : 0.f;
-        const double L = (double)hi + lo, d = dot;
+        const double L = (double)hi + lo;
         j.L[row] = make_float2(hi, lo);
         if (LIST) {
             const float ent = j.t.ent[row];
             live = ent != INFINITY;
-            loss = (double)j.tau * j.tau * (ent + L * 0.693147180559945309) - j.tau * d;
+            loss = (double)j.tau * j.tau * (ent + L * 0.693147180559945309) - j.tau * (double)dots[lane];
         } else {
             const long long w = j.t.target[row];
             live = w != j.t.ignore;
@@ -503,18 +515,18 @@ __global__ void __launch_bounds__(256) head_loss_join_kernel(const HlJoin j) {
 
 // ------------------------------------------------------------------------------------------------ a teacher's lists
 // A warp per row: probabilities of the entries that are there (id >= 0, logit not -inf) at the temperature, in ascending order of their
-// ids (a rank per entry: k comparisons each), an id that comes again added to the first, and the marks (a bisection per block of 64 words).
+// ids (a rank per entry: k comparisons each), an id that comes again added to the first, and the marks.
 __global__ void __launch_bounds__(128) head_teacher_kernel(const long long *__restrict__ in_ids, const float *__restrict__ in_logits, int2 *__restrict__ lists,
                                                            uint4 *__restrict__ marks, float *__restrict__ ent, long long N, int V, int k, float inv_tau) {
-    extern __shared__ __align__(16) long long teacher_smem[];
+    extern __shared__ __align__(16) int teacher_smem[];
     pdl_wait();
     pdl_launch_dependents();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, kk = (k + 1) & ~1;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, kk = (k + 3) & ~3;
     const long long row = (long long)blockIdx.x * 4 + warp;
     if (row >= N) return;
-    long long *key = teacher_smem + kk * warp;                         // id times 1024 plus place: none twice; absent ones behind all others
+    int *id = teacher_smem + kk * warp;                                // absent ones behind all others
     int2 *sorted = reinterpret_cast<int2 *>(teacher_smem + 4 * kk) + kk * warp;
-    constexpr long long ABSENT = 0x7fffffffLL << 10;
+    constexpr int ABSENT = 0x7fffffff;
     float top = -INFINITY;
     bool bad = false;
     int here = 0;
@@ -523,7 +535,7 @@ __global__ void __launch_bounds__(128) head_teacher_kernel(const long long *__re
         const float x = j < k ? in_logits[row * k + j] * inv_tau : -INFINITY;
         const bool is = i >= 0 && x != -INFINITY;
         bad |= is && i >= V;
-        key[j] = is ? (i >= V ? V : i) << 10 | j : ABSENT | j;
+        id[j] = is ? (int)(i >= V ? V : i) : ABSENT;
         if (is) { top = fmaxf(top, x); ++here; }
     }
 #pragma unroll
@@ -532,20 +544,24 @@ __global__ void __launch_bounds__(128) head_teacher_kernel(const long long *__re
     __syncwarp();
     float sum = 0.f;
     for (int j = lane; j < k; j += 32)
-        if (key[j] < ABSENT) sum += expf(in_logits[row * k + j] * inv_tau - top);
+        if (id[j] != ABSENT) sum += expf(in_logits[row * k + j] * inv_tau - top);
     sum = warp_sum(sum);
+    const float lse = logf(sum);
     float e = 0.f;
     for (int j = lane; j < k; j += 32) {
-        const long long me = key[j];
-        if (me >= ABSENT) continue;
+        const int me = id[j];
+        if (me == ABSENT) continue;
         const float z = in_logits[row * k + j] * inv_tau - top, q = expf(z) / sum;
-        if (!(q <= 0.f)) e += q * (z - logf(sum));                     // NaN stays
-        int rank = 0;
-        for (int i = 0; i < kk; i += 2) {
-            const longlong2 o = *reinterpret_cast<const longlong2 *>(key + i);
-            rank += (o.x < me) + (o.y < me);
+        if (!(q <= 0.f)) e += q * (z - lse);                     // NaN stays
+        int rank = 0;                                                  // entries of a smaller id, or of the same one and an earlier place
+        for (int i = 0; i < kk; i += 4) {
+            const int4 o = *reinterpret_cast<const int4 *>(id + i);
+            const int below = me + (i < (j & ~3));
+            rank += (o.x < below) + (o.y < below) + (o.z < below) + (o.w < below);
         }
-        sorted[rank] = make_int2((int)(me >> 10), __float_as_int(q));
+        const int4 own = *reinterpret_cast<const int4 *>(id + (j & ~3));
+        rank += (own.x == me && (j & 3) > 0) + (own.y == me && (j & 3) > 1) + (own.z == me && (j & 3) > 2);
+        sorted[rank] = make_int2(me, __float_as_int(q));
     }
     __syncwarp();
     // ids that come again: the first has their probabilities, they leave the list
@@ -564,16 +580,17 @@ __global__ void __launch_bounds__(128) head_teacher_kernel(const long long *__re
     for (int j = lane; j < k; j += 32) lists[row * k + j] = j < here ? sorted[j] : make_int2(0x7fffffff, 0);
     e = warp_sum(e);
     if (lane == 0) ent[row] = bad ? NAN : here > 0 ? e : INFINITY;
+    // blocks without an entry, which are nearly all, then the others, each by its first entry
     const int blocks = (V + 63) / 64;
-    for (int b = lane; b < blocks; b += 32) {
-        int lo = 0, hi = here;
-        while (lo < hi) {
-            const int mid = (lo + hi) >> 1;
-            if (sorted[mid].x < 64 * b) lo = mid + 1; else hi = mid;
-        }
+    uint4 *mine = marks + row * blocks;
+    for (int b = lane; b < blocks; b += 32) mine[b] = make_uint4(0u, 0u, 0u, 0u);
+    __syncwarp();
+    for (int j = lane; j < here; j += 32) {
+        const int v = sorted[j].x, b = v >> 6;
+        if (v >= V || (j > 0 && sorted[j - 1].x >> 6 == b)) continue;
         uint64_t bits = 0;
-        for (int j = lo; j < here && sorted[j].x < V && sorted[j].x - 64 * b < 64; ++j) bits |= 1ull << (sorted[j].x - 64 * b);
-        marks[row * blocks + b] = make_uint4((unsigned)bits, (unsigned)(bits >> 32), (unsigned)lo, 0u);
+        for (int i = j; i < here && sorted[i].x < V && sorted[i].x >> 6 == b; ++i) bits |= 1ull << (sorted[i].x & 63);
+        mine[b] = make_uint4((unsigned)bits, (unsigned)(bits >> 32), (unsigned)j, 0u);
     }
 }
 
@@ -912,13 +929,11 @@ static int hl_operand(HlOperand &o, const void *x, int dtype, long long rows, in
 }
 static int hl_no_map() { set_cuda_error(cudaErrorUnknown, "cuTensorMapEncodeTiled"); return PGB_ERR_CUDA; }
 
-static_assert(4 * 1024 * 16 <= 65536, "a teacher's entries in shared memory");
+static_assert(4 * 1024 * 12 <= 49152, "a teacher's entries in shared memory");
 int head_teacher_launch(const long long *in_ids, const float *in_logits, int *lists, unsigned *marks, float *ent, long long N, int V, int k, float tau,
                         cudaStream_t stream) {
-    cudaError_t e = cudaFuncSetAttribute(head_teacher_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 65536);
-    if (e == cudaSuccess)
-        e = pdl_launch(head_teacher_kernel, dim3((unsigned)((N + 3) / 4)), dim3(128), (size_t)(4 * ((k + 1) & ~1) * 16), stream, in_ids, in_logits,
-                               reinterpret_cast<int2 *>(lists), reinterpret_cast<uint4 *>(marks), ent, N, V, k, 1.0f / tau);
+    const cudaError_t e = pdl_launch(head_teacher_kernel, dim3((unsigned)((N + 3) / 4)), dim3(128), (size_t)(4 * ((k + 3) & ~3) * 12), stream, in_ids, in_logits,
+                                     reinterpret_cast<int2 *>(lists), reinterpret_cast<uint4 *>(marks), ent, N, V, k, 1.0f / tau);
     if (e != cudaSuccess) { set_cuda_error(e, "head_teacher launch"); return PGB_ERR_CUDA; }
     return check_launch("head_teacher_kernel");
 }
