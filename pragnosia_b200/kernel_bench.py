@@ -94,6 +94,34 @@ def _add_norm(rows, d):
     return (lambda: ops.add_norm(x, dl, n)), rows * d * 2 * 4
 
 
+def _head(N, V, d, backward=False, k=0):
+    """A loss over the vocabulary from the hidden states: its forward pass, or (backward) both of its gradients."""
+    dev = "cuda"
+    h, W = torch.randn(N, d, device=dev).to(torch.bfloat16), (2 * d ** -0.5 * torch.randn(V, d, device=dev)).to(torch.bfloat16)
+    one, host = torch.ones((), device=dev), _lib.host()
+    if k:
+        ids = torch.randint(0, V, (N, k), device=dev)
+        lists = host.teacher_lists(ids, torch.randn(N, k, device=dev), 2.0, V)
+        fwd = lambda: host.linear_distill_fwd(h, W, *lists, 2.0, 2)
+        _, L, stats, kept = fwd()
+        bwd = lambda: host.linear_distill_bwd(h, W, *lists, kept, 2.0, L, stats, one, 2, True, True)
+    else:
+        target = torch.randint(0, V, (N,), device=dev)
+        fwd = lambda: host.linear_xent_fwd(h, W, target, -100, 2)
+        _, L, stats = fwd()
+        bwd = lambda: host.linear_xent_bwd(h, W, target, -100, L, stats, one, 2, True, True)
+    return (bwd if backward else fwd), 2 * (N + V) * d * (2 if backward else 1) + N * (12 * k if k else 8)
+
+
+def _embed(N, V, d, backward=False):
+    dev = "cuda"
+    ids = (V * torch.rand(N, device=dev, dtype=torch.float64) ** 3).long().clamp_max(V - 1)
+    W, g = torch.randn(V, d, device=dev).to(torch.bfloat16), torch.randn(N, d, device=dev).to(torch.bfloat16)
+    if backward:
+        return (lambda: _lib.host().embedding_bwd(ids, g, 1.0, -1, V)), 2 * (N + V) * d + 8 * N
+    return (lambda: _lib.host().embedding_fwd(ids, W, 1.0)), 2 * (N + min(N, V)) * d + 8 * N
+
+
 CASES = {
     # name: (builder, what it is)
     "prefill": (lambda: _prefill(64, 12, 1024, 64), "aspin chunked prefill, plain rule, tensor cores: B64 H12 T1024 D64 bf16"),
@@ -113,6 +141,12 @@ CASES = {
     "add_norm": (lambda: _add_norm(8192, 768), "residual add + RMS norm: 8192 rows of 768 bf16"),
     "mlp_up": (lambda: _linear_act(8192, 768, 3072), "MLP up-projection + bias + erf-GELU as one tensor-core GEMM: M8192 K768 N3072 bf16"),
     "mlp_up_pair": (lambda: _linear_act(8192, 768, 3072, variant=1), "the same GEMM with a 256 x 256 tile per pair of SMs (two-CTA cluster, cta_group::2)"),
+    "xent": (lambda: _head(32768, 8192, 768), "cross entropy over the vocabulary without the logits: 32768 rows of 768, 8192 words"),
+    "xent_bwd": (lambda: _head(32768, 8192, 768, True), "both of its gradients, the logits again among them"),
+    "distill": (lambda: _head(8192, 8192, 768, k=64), "distillation from 64 top logits a row: 8192 rows of 768, 8192 words"),
+    "distill_bwd": (lambda: _head(8192, 8192, 768, True, k=64), "both of its gradients"),
+    "embed": (lambda: _embed(32768, 8192, 768), "embedding lookup: 32768 ids, 8192 words of 768 bf16"),
+    "embed_bwd": (lambda: _embed(32768, 8192, 768, True), "its gradient by sorted tokens"),
     "skinny": (lambda: _skinny(1, 768, 3072), "decode-step linear (add + RMS norm + linear + GELU) at batch 1: K768 N3072 bf16"),
     "batch_linear": (lambda: _batch_linear(64, 768, 2328), "decode-step linear for 64 rows on the tensor cores (bias): K768 N2328 bf16"),
     "decode_token": (lambda: _decode_token(1), "the whole decode step of the configuration-2 model as one launch, batch 1 (12 layers, d768, vocabulary 8192)"),
