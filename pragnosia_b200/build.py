@@ -40,9 +40,11 @@ def build_host(force: bool = False) -> None:
         return
     from torch.utils import cpp_extension as ext
     inc = [*ext.include_paths(), str(Path(NVCC).parents[1] / "include"), sysconfig.get_paths()["include"]]
+    # libstdc++ by its file's name: the one torch has loaded. A compiler that finds only the static one would put a second into the module, whose
+    # streams crash the process where a check writes its message.
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", f"-DTORCH_EXTENSION_NAME={HOST.stem}",
            "-DTORCH_API_INCLUDE_EXTENSION_H", *(f"-I{d}" for d in inc), str(HOST_SRC), "-o", str(HOST), *(f"-L{d}" for d in ext.library_paths()),
-           "-lc10", "-lc10_cuda", "-ltorch_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python", f"-L{LIBDIR}", f"-l:{LIB.name}", "-Wl,-rpath,$ORIGIN"]
+           "-lc10", "-lc10_cuda", "-ltorch_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python", f"-L{LIBDIR}", f"-l:{LIB.name}", "-l:libstdc++.so.6", "-Wl,-rpath,$ORIGIN"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"{cmd[0]} failed for {HOST_SRC.name}:\n{r.stdout}\n{r.stderr}")

@@ -7,7 +7,7 @@ import torch
 from torch._subclasses.fake_tensor import FakeTensorMode
 
 from pragnosia_b200 import custom_ops, head  # noqa: F401
-from pragnosia_b200._lib import lib
+from pragnosia_b200._lib import HOST_PATH, lib
 
 OPS = torch.ops.pragnosia_b200
 BF, F32 = torch.bfloat16, torch.float32
@@ -118,3 +118,9 @@ def test_shape_functions():
     for name in ("linear_xent", "linear_xent_bwd", "teacher_lists", "linear_distill", "linear_distill_bwd", "embedding", "embedding_bwd"):
         schema = getattr(OPS, name).default._schema
         assert not any(a.alias_info is not None and a.alias_info.is_write for a in schema.arguments), name
+
+
+def test_the_module_shares_torch_s_cxx_library():
+    """With a libstdc++ of its own in it, the check that refuses a call on a GPU crashes the process where it writes its message."""
+    with open(HOST_PATH, "rb") as f:
+        assert b"libstdc++.so.6\0" in f.read()
