@@ -542,7 +542,7 @@ int pgb_linear_act(const void *x, const void *W, const void *bias, void *y, long
  * Cross entropy: rows whose target is ignore_index lose 0 and have no gradient, whatever h holds there; any other target outside 0 .. V-1 gives NaN, as loss and as gradients of its row and of W.
  * Distillation: pgb_teacher_lists makes of a teacher's k entries per row (ids in any order; an entry with id < 0 or logit -inf is
  * absent) what the losses read: lists [N][k][2] (id, bits of its probability p at the temperature; by id), marks [N][ceil(V / 64)][4] (which of every
- * 64 words they are, and the place of the first) and ent [N], the sum of p log p. lists 8-byte, marks 16-byte aligned. kept [N][k]: the entries' logits, which the forward pass
+ * 64 words they are, and the place of the first; the forward pass alone reads it) and ent [N], the sum of p log p. lists 8-byte, marks 16-byte aligned. kept [N][k]: the entries' logits, which the forward pass
  * leaves to the backward pass. A row's loss is
  * temperature^2 KL(p || softmax(s / temperature)), 0 without gradient for rows without an entry; the same id twice counts twice; an id >= V gives NaN.
  * N, V up to 2^30, d up to 65536, k 1 .. 1024. Bounded waits as in the prefill kernels (pgb_tc_error_flag: 91-95). The same call gives
@@ -561,7 +561,7 @@ int pgb_teacher_lists(const long long *teacher_ids, const float *teacher_logits,
 int pgb_linear_distill_fwd(const void *h, const void *W, int dtype, const int *lists, const unsigned *marks, const float *ent, float *kept, int k,
                            float temperature, float *row_loss, float *loss, float *stats, float *L, void *scratch,
                            long long scratch_bytes, int reduction, long long N, int V, int d, void *stream);
-int pgb_linear_distill_bwd(const void *h, const void *W, int dtype, const int *lists, const unsigned *marks, const float *ent, const float *kept, int k,
+int pgb_linear_distill_bwd(const void *h, const void *W, int dtype, const int *lists, const float *ent, const float *kept, int k,
                            float temperature, const float *L, const float *stats, const float *grad, void *dh, void *dW,
                            void *scratch, long long scratch_bytes, int reduction, long long N, int V, int d, void *stream);
 

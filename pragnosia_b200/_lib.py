@@ -89,7 +89,7 @@ SIGNATURES = {
     "pgb_linear_xent_bwd": [_vp, _vp, _i, _vp, _ll, _vp, _vp, _vp, _vp, _vp, _vp, _ll, _i, _ll, _i, _i, _vp],
     "pgb_teacher_lists": [_vp, _vp, _f, _vp, _vp, _vp, _ll, _i, _i, _vp],
     "pgb_linear_distill_fwd": [_vp, _vp, _i, _vp, _vp, _vp, _vp, _i, _f, _vp, _vp, _vp, _vp, _vp, _ll, _i, _ll, _i, _i, _vp],
-    "pgb_linear_distill_bwd": [_vp, _vp, _i, _vp, _vp, _vp, _vp, _i, _f, _vp, _vp, _vp, _vp, _vp, _vp, _ll, _i, _ll, _i, _i, _vp],
+    "pgb_linear_distill_bwd": [_vp, _vp, _i, _vp, _vp, _vp, _i, _f, _vp, _vp, _vp, _vp, _vp, _vp, _ll, _i, _ll, _i, _i, _vp],
     "pgb_embedding_fwd": [_vp, _vp, _i, _f, _vp, _ll, _i, _i, _vp],
     "pgb_embedding_bwd_scratch_bytes": [_ll, _i, _i],
     "pgb_embedding_bwd": [_vp, _vp, _i, _f, _ll, _vp, _vp, _ll, _ll, _i, _i, _vp],

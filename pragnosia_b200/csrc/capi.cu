@@ -811,7 +811,7 @@ int head_args(HeadLossArgs &x, const void *h, const void *W, int dtype, const lo
               const float *ent, float *kept, int k, float tau, int reduction, long long N, int V, int d) {
     x = {h, W, dtype, target, ignore, lists, marks, ent, kept, k, tau, reduction, N, V, d};
     if (!h || !W) return PGB_ERR_NULL_POINTER;
-    if (target == nullptr && (!lists || !marks || !ent || !kept)) return PGB_ERR_NULL_POINTER;
+    if (target == nullptr && (!lists || !ent || !kept)) return PGB_ERR_NULL_POINTER;
     int rc = head_sizes(N, V, d, dtype);
     if (rc != PGB_OK) return rc;
     if (reduction < 0 || reduction > 2 || !(tau > 0.f) || tau > 3e38f || (lists && k < 1)) return PGB_ERR_BAD_SHAPE;
@@ -821,7 +821,7 @@ int head_args(HeadLossArgs &x, const void *h, const void *W, int dtype, const lo
     return PGB_OK;
 }
 int head_fwd(const HeadLossArgs &x, float *row_loss, float *loss, float *stats, float *L, void *scratch, long long scratch_bytes, void *stream) {
-    if (!L || !scratch || !stats || (x.reduction == 0 ? !row_loss : !loss)) return PGB_ERR_NULL_POINTER;
+    if ((x.lists && !x.marks) || !L || !scratch || !stats || (x.reduction == 0 ? !row_loss : !loss)) return PGB_ERR_NULL_POINTER;
     if (!aligned(L, 8) || !aligned(scratch, 256)) return PGB_ERR_MISALIGNED;
     if (scratch_bytes < head_loss_fwd_bytes(x.N, x.V, x.d, x.dtype)) return PGB_ERR_BAD_SHAPE;
     return head_loss_fwd_launch(x, row_loss, loss, stats, L, scratch, (cudaStream_t)stream);
@@ -869,11 +869,11 @@ int pgb_linear_distill_fwd(const void *h, const void *W, int dtype, const int *l
     const int rc = head_args(x, h, W, dtype, nullptr, 0, lists, marks, ent, kept, k, temperature, reduction, N, V, d);
     return rc != PGB_OK ? rc : head_fwd(x, row_loss, loss, stats, L, scratch, scratch_bytes, stream);
 }
-int pgb_linear_distill_bwd(const void *h, const void *W, int dtype, const int *lists, const unsigned *marks, const float *ent, const float *kept, int k, float temperature, const float *L,
+int pgb_linear_distill_bwd(const void *h, const void *W, int dtype, const int *lists, const float *ent, const float *kept, int k, float temperature, const float *L,
                            const float *stats, const float *grad, void *dh, void *dW, void *scratch, long long scratch_bytes, int reduction, long long N, int V,
                            int d, void *stream) {
     HeadLossArgs x;
-    const int rc = head_args(x, h, W, dtype, nullptr, 0, lists, marks, ent, const_cast<float *>(kept), k, temperature, reduction, N, V, d);
+    const int rc = head_args(x, h, W, dtype, nullptr, 0, lists, nullptr, ent, const_cast<float *>(kept), k, temperature, reduction, N, V, d);
     return rc != PGB_OK ? rc : head_bwd(x, L, stats, grad, dh, dW, scratch, scratch_bytes, stream);
 }
 

@@ -397,6 +397,8 @@ Three scan_diff(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor 
 
 // ------------------------------------------------------------------------------------------------ losses over the vocabulary
 enum { REDUCE_NONE = 0, REDUCE_SUM = 1, REDUCE_MEAN = 2 };
+constexpr int64_t MOST_WORDS = 1 << 30;                               // the entry points' V is an int
+const char *const XENT = "linear_cross_entropy", *const DISTILL = "linear_distill", *const EMBED = "embedding";
 void same_device(const char *what, const Tensor &a, const Tensor &b) {
     TORCH_CHECK_VALUE(a.device() == b.device(), what, ": its tensors are on ", a.device(), " and ", b.device());
 }
@@ -417,7 +419,8 @@ HeadIn head_in(const char *what, const Tensor &h, const Tensor &w) {
     TORCH_CHECK_TYPE(h.scalar_type() == w.scalar_type() && io_type(h.scalar_type()), what, ": h and the weight are both float32 or both bfloat16, got ",
                      h.scalar_type(), " and ", w.scalar_type());
     const int64_t d = w.size(1);
-    TORCH_CHECK_VALUE(w.size(0) >= 1 && d >= 8 && d % 8 == 0, what, ": the weight is (V, d) with V at least 1 and d a multiple of 8, got ", w.sizes());
+    TORCH_CHECK_VALUE(w.size(0) >= 1 && w.size(0) <= MOST_WORDS && d >= 8 && d <= 65536 && d % 8 == 0, what,
+                      ": the weight is (V, d) with V from 1 to 2^30 and d a multiple of 8 up to 65536, got ", w.sizes());
     return {head_operand(h.reshape({-1, d})), head_operand(w), h.numel() / d, w.size(0), d};
 }
 // What a row is held to: a word each (target), or a teacher's entries (lists, marks, ent; kept: their logits).
@@ -446,6 +449,21 @@ HeadOut head_fwd(const char *what, const HeadIn &x, const HeadWant &t, int reduc
                                   n, reduction, x.N, x.V, x.d, dev.stream), what);
     return r;
 }
+// what the forward pass left, as a registered operator's caller hands it over
+void head_state(const char *what, const HeadIn &x, const Tensor &t, at::IntArrayRef sizes, at::ScalarType type) {
+    TORCH_CHECK_VALUE(t.device() == x.h.device() && t.scalar_type() == type && t.sizes() == sizes && t.is_contiguous(), what, ": a tensor of the forward pass is ", type,
+                      sizes, ", contiguous, got ", t.scalar_type(), t.sizes(), " on ", t.device());
+}
+void head_state(const char *what, const HeadIn &x, const Tensor &L, const Tensor &stats, const Tensor &grad, int reduction) {
+    head_state(what, x, L, {x.N, 2}, at::kFloat);
+    head_state(what, x, stats, {2}, at::kFloat);
+    TORCH_CHECK_VALUE(grad.device() == x.h.device() && grad.numel() == (reduction == REDUCE_NONE ? x.N : 1), what, ": a gradient per loss, got ", grad.sizes());
+}
+void head_lists(const HeadIn &x, const Tensor &lists, const Tensor &ent) {
+    TORCH_CHECK_VALUE(lists.dim() == 3 && lists.size(1) >= 1, DISTILL, ": lists are (N, k, 2), got ", lists.sizes());
+    head_state(DISTILL, x, lists, {x.N, lists.size(1), 2}, at::kInt);
+    head_state(DISTILL, x, ent, {x.N}, at::kFloat);
+}
 std::tuple<Tensor, Tensor> head_bwd(const char *what, const HeadIn &x, const HeadWant &t, const Tensor &L, const Tensor &stats, const Tensor &grad_, int reduction,
                                     bool want_dh, bool want_dw) {
     OnDevice dev(x.h);
@@ -460,14 +478,13 @@ std::tuple<Tensor, Tensor> head_bwd(const char *what, const HeadIn &x, const Hea
     const long long n = pgb_head_loss_bwd_scratch_bytes(x.N, x.V, x.d, code(x.h), want_dh, want_dw);
     const Tensor scratch = bytes(x.h, n);
     if (t.lists.defined())
-        check(pgb_linear_distill_bwd(vp(x.h), vp(x.w), code(x.h), static_cast<int *>(vp(t.lists)), static_cast<unsigned *>(vp(t.marks)), fp(t.ent), fp(t.kept), t.lists.size(1), t.tau, fp(L), fp(stats),
+        check(pgb_linear_distill_bwd(vp(x.h), vp(x.w), code(x.h), static_cast<int *>(vp(t.lists)), fp(t.ent), fp(t.kept), t.lists.size(1), t.tau, fp(L), fp(stats),
                                      fp(grad), vp(dh), vp(dw), vp(scratch), n, reduction, x.N, x.V, x.d, dev.stream), what);
     else
         check(pgb_linear_xent_bwd(vp(x.h), vp(x.w), code(x.h), static_cast<long long *>(vp(t.target)), t.ignore, fp(L), fp(stats), fp(grad), vp(dh), vp(dw),
                                   vp(scratch), n, reduction, x.N, x.V, x.d, dev.stream), what);
     return {dh, dw};
 }
-const char *const XENT = "linear_cross_entropy", *const DISTILL = "linear_distill", *const EMBED = "embedding";
 HeadWant xent_want(const HeadIn &x, const Tensor &h, const Tensor &target, int64_t ignore) {
     need_cuda(target);
     same_device(XENT, h, target);
@@ -481,6 +498,7 @@ std::tuple<Tensor, Tensor, Tensor> teacher_lists(const Tensor &ids_, const Tenso
                       logits_.sizes());
     TORCH_CHECK_VALUE(tau > 0.0 && tau < 3e38, DISTILL, ": the temperature is positive, got ", tau);
     const int64_t k = ids_.size(-1);
+    TORCH_CHECK_VALUE(V >= 1 && V <= MOST_WORDS, DISTILL, ": 1 to 2^30 words, got ", V);
     TORCH_CHECK_VALUE(k >= 1 && k <= 1024, DISTILL, ": 1 to 1024 teacher entries a row, got ", k);
     const int64_t N = ids_.numel() / k;
     OnDevice dev(ids_);
@@ -507,7 +525,7 @@ struct HeadLoss : torch::autograd::Function<HeadLoss> {
         const HeadIn x = head_in(what, h_, w_);
         const HeadWant t = target ? xent_want(x, h_, *target, ignore) : distill_want(x, h_, *ids, *logits, tau);
         HeadOut r = head_fwd(what, x, t, reduction);
-        ctx->save_for_backward({x.h, x.w, t.target, t.lists, t.marks, t.ent, t.kept, r.L, r.stats});
+        ctx->save_for_backward({x.h, x.w, t.target, t.lists, t.ent, t.kept, r.L, r.stats});    // not marks: N V / 4 bytes that only the forward pass reads
         auto &d = ctx->saved_data;
         d["ignore"] = ignore; d["tau"] = tau; d["reduction"] = reduction; d["shape"] = h_.sizes().vec();
         ctx->set_materialize_grads(false);
@@ -520,9 +538,9 @@ struct HeadLoss : torch::autograd::Function<HeadLoss> {
         const variable_list s = ctx->get_saved_variables();
         auto &d = ctx->saved_data;
         const HeadIn x{s[0], s[1], s[0].size(0), s[1].size(0), s[1].size(1)};
-        const HeadWant t{s[2], d["ignore"].toInt(), s[3], s[4], s[5], s[6], d["tau"].toDouble()};
+        const HeadWant t{s[2], d["ignore"].toInt(), s[3], Tensor(), s[4], s[5], d["tau"].toDouble()};
         const bool list = t.lists.defined();
-        auto [dh, dw] = head_bwd(list ? DISTILL : XENT, x, t, s[7], s[8], g[0].reshape({-1}), d["reduction"].toInt(), ctx->needs_input_grad(0), ctx->needs_input_grad(1));
+        auto [dh, dw] = head_bwd(list ? DISTILL : XENT, x, t, s[6], s[7], g[0].reshape({-1}), d["reduction"].toInt(), ctx->needs_input_grad(0), ctx->needs_input_grad(1));
         none[0] = dh.defined() ? dh.view(d["shape"].toIntVector()) : dh;
         none[1] = dw;
         return once(list ? "pragnosia_b200 linear_distill" : "pragnosia_b200 linear_cross_entropy", s, none, g);
@@ -566,7 +584,8 @@ OptTensor linear_distill(const Tensor &h, const Tensor &w, const Tensor &ids, co
 // ------------------------------------------------------------------------------------------------ embedding
 Tensor embed_weight(const Tensor &w) {
     TORCH_CHECK_TYPE(io_type(w.scalar_type()), EMBED, ": the weight is float32 or bfloat16, got ", w.scalar_type());
-    TORCH_CHECK_VALUE(w.dim() == 2 && w.size(0) >= 1 && w.size(1) >= 1, EMBED, ": the weight is (V, d), got ", w.sizes());
+    TORCH_CHECK_VALUE(w.dim() == 2 && w.size(0) >= 1 && w.size(0) <= MOST_WORDS && w.size(1) >= 1 && w.size(1) <= 65536, EMBED,
+                      ": the weight is (V, d), V up to 2^30 and d up to 65536, got ", w.sizes());
     return w.contiguous();
 }
 Tensor embed_fwd(const Tensor &ids_, const Tensor &w_, double scale) {
@@ -589,7 +608,7 @@ Tensor embed_bwd(const Tensor &ids_, const Tensor &g_, double scale, int64_t pad
     TORCH_CHECK_TYPE(io_type(g_.scalar_type()), EMBED, ": the gradient is float32 or bfloat16, got ", g_.scalar_type());
     const Tensor g = g_.contiguous(), ids = whole_numbers(EMBED, ids_);
     const int64_t d = g.size(-1), N = ids.numel();
-    TORCH_CHECK_VALUE(g.numel() == N * d && V >= 1, EMBED, ": a row of gradient per id, got ", g.sizes(), " for ", ids.sizes());
+    TORCH_CHECK_VALUE(g.numel() == N * d && d >= 1 && d <= 65536 && V >= 1 && V <= MOST_WORDS, EMBED, ": a row of gradient per id, got ", g.sizes(), " for ", ids.sizes());
     Tensor dw = alloc(g, {V, d}, g.scalar_type());
     if (N == 0) return dw.zero_();
     const long long n = pgb_embedding_bwd_scratch_bytes(N, V, d);
@@ -660,6 +679,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("linear_xent_bwd", [](const Tensor &h, const Tensor &w, const Tensor &target, int64_t ignore, const Tensor &L, const Tensor &stats, const Tensor &grad,
                                 int reduction, bool want_dh, bool want_dw) {
         const HeadIn x = head_in(XENT, h, w);
+        head_state(XENT, x, L, stats, grad, reduction);
         auto [dh, dw] = head_bwd(XENT, x, xent_want(x, h, target, ignore), L, stats, grad, reduction, want_dh, want_dw);
         return std::make_tuple(some(dh), some(dw));
     }, nogil);
@@ -667,14 +687,19 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("linear_distill", &linear_distill, nogil);
     m.def("linear_distill_fwd", [](const Tensor &h, const Tensor &w, const Tensor &lists, const Tensor &marks, const Tensor &ent, double tau, int reduction) {
         const HeadIn x = head_in(DISTILL, h, w);
+        head_lists(x, lists, ent);
+        head_state(DISTILL, x, marks, {x.N, (x.V + 63) / 64, 4}, at::kInt);
         const Tensor kept = alloc(x.h, {x.N, lists.size(1)}, at::kFloat);
         HeadOut r = head_fwd(DISTILL, x, {Tensor(), 0, lists, marks, ent, kept, tau}, reduction);
         return std::make_tuple(r.loss, r.L, r.stats, kept);
     }, nogil);
-    m.def("linear_distill_bwd", [](const Tensor &h, const Tensor &w, const Tensor &lists, const Tensor &marks, const Tensor &ent, const Tensor &kept, double tau,
+    m.def("linear_distill_bwd", [](const Tensor &h, const Tensor &w, const Tensor &lists, const Tensor &ent, const Tensor &kept, double tau,
                                    const Tensor &L, const Tensor &stats, const Tensor &grad, int reduction, bool want_dh, bool want_dw) {
         const HeadIn x = head_in(DISTILL, h, w);
-        auto [dh, dw] = head_bwd(DISTILL, x, {Tensor(), 0, lists, marks, ent, kept, tau}, L, stats, grad, reduction, want_dh, want_dw);
+        head_lists(x, lists, ent);
+        head_state(DISTILL, x, kept, {x.N, lists.size(1)}, at::kFloat);
+        head_state(DISTILL, x, L, stats, grad, reduction);
+        auto [dh, dw] = head_bwd(DISTILL, x, {Tensor(), 0, lists, Tensor(), ent, kept, tau}, L, stats, grad, reduction, want_dh, want_dw);
         return std::make_tuple(some(dh), some(dw));
     }, nogil);
     m.def("embedding", &embedding, nogil);

@@ -532,26 +532,26 @@ def _(h, W, lists, marks, ent, temperature, reduction):
 
 
 @torch.library.custom_op(f"{NS}::linear_distill_bwd", mutates_args=())
-def linear_distill_bwd(h: Tensor, W: Tensor, lists: Tensor, marks: Tensor, ent: Tensor, kept: Tensor, temperature: float, L: Tensor, stats: Tensor, grad: Tensor,
+def linear_distill_bwd(h: Tensor, W: Tensor, lists: Tensor, ent: Tensor, kept: Tensor, temperature: float, L: Tensor, stats: Tensor, grad: Tensor,
                        reduction: int, want_dh: bool, want_dW: bool) -> Tuple[Tensor, Tensor]:
-    dh, dW = host().linear_distill_bwd(h, W, lists, marks, ent, kept, temperature, L, stats, grad, reduction, want_dh, want_dW)
+    dh, dW = host().linear_distill_bwd(h, W, lists, ent, kept, temperature, L, stats, grad, reduction, want_dh, want_dW)
     return (dh.view(h.shape) if want_dh else _none(h)), (dW if want_dW else _none(W))
 
 
 @linear_distill_bwd.register_fake
-def _(h, W, lists, marks, ent, kept, temperature, L, stats, grad, reduction, want_dh, want_dW):
+def _(h, W, lists, ent, kept, temperature, L, stats, grad, reduction, want_dh, want_dW):
     return _grads_like(h, W, want_dh, want_dW)
 
 
 def _distill_ctx(ctx, inputs, output):
-    h, W, lists, marks, ent, ctx.temperature, ctx.reduction = inputs
-    ctx.save_for_backward(h, W, lists, marks, ent, output[3], output[1], output[2])
+    h, W, lists, _marks, ent, ctx.temperature, ctx.reduction = inputs
+    ctx.save_for_backward(h, W, lists, ent, output[3], output[1], output[2])
 
 
 def _distill_grads(ctx, g, _L, _stats, _kept):
-    h, W, lists, marks, ent, kept, L, stats = ctx.saved_tensors
+    h, W, lists, ent, kept, L, stats = ctx.saved_tensors
     want = ctx.needs_input_grad[:2]
-    dh, dW = torch.ops.pragnosia_b200.linear_distill_bwd(h, W, lists, marks, ent, kept, ctx.temperature, L, stats, g, ctx.reduction, *want)
+    dh, dW = torch.ops.pragnosia_b200.linear_distill_bwd(h, W, lists, ent, kept, ctx.temperature, L, stats, g, ctx.reduction, *want)
     return (dh if want[0] else None), (dW if want[1] else None), None, None, None, None, None
 
 

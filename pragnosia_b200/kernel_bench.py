@@ -104,7 +104,7 @@ def _head(N, V, d, backward=False, k=0):
         lists = host.teacher_lists(ids, torch.randn(N, k, device=dev), 2.0, V)
         fwd = lambda: host.linear_distill_fwd(h, W, *lists, 2.0, 2)
         _, L, stats, kept = fwd()
-        bwd = lambda: host.linear_distill_bwd(h, W, *lists, kept, 2.0, L, stats, one, 2, True, True)
+        bwd = lambda: host.linear_distill_bwd(h, W, lists[0], lists[2], kept, 2.0, L, stats, one, 2, True, True)
     else:
         target = torch.randint(0, V, (N,), device=dev)
         fwd = lambda: host.linear_xent_fwd(h, W, target, -100, 2)

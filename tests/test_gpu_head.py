@@ -540,3 +540,112 @@ def test_a_capture_beside_an_eager_pass_of_the_same_leaves_is_refused():
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(loss, alive[0].detach())
+
+
+def test_what_the_forward_pass_leaves_is_checked():
+    """The registered operators' backward passes read what a caller hands them: other sizes, types or places are refused before a launch."""
+    ops = torch.ops.pragnosia_b200
+    h, w, g = operands(6, 70, 16, BF, 3)
+    t = torch.randint(0, 70, (6,), device=DEV, generator=g)
+    ids, logits = torch.randint(0, 70, (6, 3), device=DEV, generator=g), torch.randn(6, 3, device=DEV, generator=g)
+    loss, L, stats = ops.linear_xent(h, w, t, -100, 0)
+    one = torch.ones(6, device=DEV)
+    good = dict(L=L, stats=stats, grad=one)
+    for name, bad in (("L", L[:5]), ("L", L.double()), ("L", L.cpu()), ("L", torch.empty(2, 6, device=DEV).t()), ("stats", stats[:1]), ("grad", one[:5]), ("grad", one.cpu())):
+        with pytest.raises(ValueError):
+            ops.linear_xent_bwd(h, w, t, -100, *(good | {name: bad}).values(), 0, True, True)
+    lists, marks, ent = ops.teacher_lists(ids, logits, 1.0, 70)
+    loss, L, stats, kept = ops.linear_distill(h, w, lists, marks, ent, 1.0, 0)
+    for bad in ((lists[:5], marks, ent), (lists.long(), marks, ent), (lists, marks[:, :1], ent), (lists, marks, ent[:5]), (lists.view(6, 6), marks, ent)):
+        with pytest.raises(ValueError):
+            ops.linear_distill(h, w, *bad, 1.0, 0)
+    for bad in ((lists, ent, kept[:, :2]), (lists[:, :2], ent, kept), (lists, ent.double(), kept)):
+        with pytest.raises(ValueError):
+            ops.linear_distill_bwd(h, w, *bad, 1.0, L, stats, one, 0, True, True)
+
+
+def test_sizes_that_an_entry_point_cannot_hold_are_refused():
+    """2^32 + 8 words or columns would be 8 to a 32-bit size; nothing of that size is read or copied on the way."""
+    many = (1 << 32) + 8
+    row, t = torch.zeros(1, 8, device=DEV, dtype=BF), torch.zeros(1, device=DEV, dtype=torch.long)
+    tall, wide = row.expand(many, 8), row[:, :1].expand(1, many)
+    for call in (lambda: head.linear_cross_entropy(row, tall, t), lambda: head.linear_cross_entropy(wide, wide, t), lambda: head.embedding(t, tall), lambda: head.embedding(t, wide),
+                 lambda: head.linear_distill(row, tall, t[:, None], t[:, None].float()), lambda: torch.ops.pragnosia_b200.teacher_lists(t[:, None], t[:, None].float(), 1.0, many),
+                 lambda: torch.ops.pragnosia_b200.embedding_bwd(t, row, 1.0, -1, many)):
+        with pytest.raises(ValueError):
+            call()
+
+
+def test_distillation_keeps_little_for_its_gradient():
+    """From the forward pass to the backward pass: the lists and the entries' logits (12 k bytes a row), 16 bytes a row, and nothing that grows with the vocabulary."""
+    N, V, k = 2048, 8192, 16
+    h, w, g = operands(N, V, 64, BF, 3)
+    ids, logits = torch.randint(0, V, (N, k), device=DEV, generator=g), torch.randn(N, k, device=DEV, generator=g)
+    h.requires_grad_()
+    head.linear_distill(h, w, ids, logits).backward()
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    loss = head.linear_distill(h, w, ids, logits)
+    kept = torch.cuda.memory_allocated() - before
+    assert kept <= N * (12 * k + 16) + 8 * 512                        # blocks are handed out in multiples of 512 bytes
+    del loss
+
+
+def test_first_calls_inside_a_capture():
+    """A process whose first calls of all are captured: kernels are loaded, and their residency asked for, during the capture."""
+    import subprocess
+    import sys
+    code = """
+import torch
+from pragnosia_b200 import head
+g = torch.Generator(device="cuda").manual_seed(3)
+h, w = torch.randn(300, 64, device="cuda", generator=g).bfloat16(), torch.randn(500, 64, device="cuda", generator=g).bfloat16()
+t = torch.randint(0, 500, (300,), device="cuda", generator=g)
+x = torch.randn(300, 4, device="cuda", generator=g)
+ids = torch.randint(0, 500, (300, 4), device="cuda", generator=g)
+def step():
+    h.grad = w.grad = None
+    h.requires_grad_(); w.requires_grad_()
+    y = head.embedding(t, w) + h
+    loss = head.linear_cross_entropy(y, w, t) + head.linear_distill(y, w, ids, x)
+    loss.backward()
+    out = loss.detach(), h.grad, w.grad
+    return out
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = step()
+graph.replay()
+torch.cuda.synchronize()
+got = [a.clone() for a in got]
+want = step()
+assert all(torch.equal(a, b) for a, b in zip(got, want))
+print("same")
+"""
+    import os
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    out = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0 and "same" in out.stdout, out.stderr[-2000:]
+
+
+def test_refusals():
+    """Each with a message, before a launch: the process goes on."""
+    h, w, g = operands(6, 70, 16, BF, 3)
+    t = torch.randint(0, 70, (6,), device=DEV, generator=g)
+    x = torch.randn(6, 3, device=DEV, generator=g)
+    ids = torch.randint(0, 70, (6, 3), device=DEV, generator=g)
+    ce, kd, emb = head.linear_cross_entropy, head.linear_distill, head.embedding
+    bad = [(lambda: ce(h, w[:, :8], t), ValueError), (lambda: ce(h, w, t[:5]), ValueError), (lambda: ce(h, w.float(), t), TypeError), (lambda: ce(h.half(), w.half(), t), TypeError),
+           (lambda: ce(h, w, t.float()), TypeError), (lambda: ce(h[:, :12], w[:, :12], t), ValueError), (lambda: ce(h, w[:0], t), ValueError), (lambda: ce(h, w[0], t), ValueError),
+           (lambda: ce(h, w, t.cpu()), RuntimeError), (lambda: kd(h, w, ids, x[:5]), ValueError), (lambda: kd(h, w, ids[:5], x[:5]), ValueError),
+           (lambda: kd(h, w, ids, x, temperature=0.0), ValueError), (lambda: kd(h, w, ids, x, temperature=float("nan")), ValueError), (lambda: kd(h, w, ids[:, :0], x[:, :0]), ValueError),
+           (lambda: kd(h, w, ids[:, :1].expand(6, 1025), x[:, :1].expand(6, 1025)), ValueError), (lambda: kd(h, w, x, x), TypeError), (lambda: emb(x, w), TypeError),
+           (lambda: emb(t, w.half()), TypeError), (lambda: emb(t, w[0]), ValueError), (lambda: emb(t, w[:0]), ValueError), (lambda: emb(t, w.cpu()), RuntimeError)]
+    for grad in (False, True):
+        h.requires_grad_(grad)
+        w.requires_grad_(grad)
+        for i, (call, error) in enumerate(bad):
+            with pytest.raises(error):
+                call()
+                pytest.fail(f"call {i} was taken")
+    assert torch.isfinite(ce(h, w, t))

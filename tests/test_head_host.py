@@ -107,7 +107,7 @@ def test_shape_functions():
         assert sig(lists) == ((10, 7, 2), torch.int32) and sig(marks) == ((10, 3, 4), torch.int32) and sig(ent) == ((10,), F32)
         loss, L, stats, kept = OPS.linear_distill(h, w, lists, marks, ent, 2.0, 0)
         assert sig(loss) == ((10,), F32) and sig(kept) == ((10, 7), F32)
-        dh, dw = OPS.linear_distill_bwd(h, w, lists, marks, ent, kept, 2.0, L, stats, loss, 0, True, True)
+        dh, dw = OPS.linear_distill_bwd(h, w, lists, ent, kept, 2.0, L, stats, loss, 0, True, True)
         assert sig(dh) == ((2, 5, 64), BF) and sig(dw) == ((33, 64), BF)
         assert sig(OPS.embedding(t, w, 1.0, -1)) == ((2, 5, 64), BF) and sig(OPS.embedding_bwd(t, h, 1.0, -1, 33)) == ((33, 64), BF)
         with torch.enable_grad():
