@@ -570,7 +570,7 @@ int pgb_linear_distill_bwd(const void *h, const void *W, int dtype, const int *l
  *   y[n] = scale W[ids[n]];  dW[v] = scale * sum over ids[n] == v of grad[n], n ascending, added in fp32 and rounded once.
  *   ids [N] int64; W, dW [V][d], y, grad [N][d]: dtype, contiguous, aligned to their element (to 16 bytes, with d a multiple of
  *   16 bytes, rows move 16 bytes at a time). An id outside 0 .. V-1 gives a row of NaN and adds nothing to dW; nor does padding_idx (-1: none).
- *   scratch: 16-byte aligned, pgb_embedding_bwd_scratch_bytes. N, V up to 2^30. The same call gives the same bits.
+ *   scratch: 16-byte aligned, pgb_embedding_bwd_scratch_bytes (0 for up to 256 tokens: may be NULL). N, V up to 2^30. The same call gives the same bits.
  * ------------------------------------------------------------------------------------------------------- */
 int pgb_embedding_fwd(const long long *ids, const void *W, int dtype, float scale, void *y, long long N, int V, int d, void *stream);
 long long pgb_embedding_bwd_scratch_bytes(long long N, int V, int d);

@@ -895,12 +895,14 @@ long long pgb_embedding_bwd_scratch_bytes(long long N, int V, int d) {
 }
 int pgb_embedding_bwd(const long long *ids, const void *grad, int dtype, float scale, long long padding_idx, void *dW, void *scratch, long long scratch_bytes,
                       long long N, int V, int d, void *stream) {
-    if (!ids || !grad || !dW || !scratch) return PGB_ERR_NULL_POINTER;
+    if (!ids || !grad || !dW) return PGB_ERR_NULL_POINTER;
     const int rc = embedding_sizes(N, V, d, dtype);
     if (rc != PGB_OK) return rc;
     const size_t e = dtype == PGB_F32 ? 4 : 2;
+    const long long bytes = embedding_bwd_bytes(N, V, d);
+    if (bytes > 0 && !scratch) return PGB_ERR_NULL_POINTER;
     if (!aligned(ids, 8) || !aligned(grad, e) || !aligned(dW, e) || !aligned(scratch, 16)) return PGB_ERR_MISALIGNED;
-    if (scratch_bytes < embedding_bwd_bytes(N, V, d)) return PGB_ERR_BAD_SHAPE;
+    if (scratch_bytes < bytes) return PGB_ERR_BAD_SHAPE;
     return embedding_bwd_launch(ids, grad, dtype, scale, padding_idx, dW, scratch, N, V, d, (cudaStream_t)stream);
 }
 

@@ -1,7 +1,8 @@
 // Embedding lookup with scaling, y_n = scale w_{id_n}, and its gradient dw_v = scale sum_{n: id_n = v} g_n by sorted tokens: no atomics on
 // the sums, so the same call gives the same bits, and a word's gradients are added in fp32 and rounded once.
 //   Both directions move bytes and compute nothing to speak of: the lookup reads and writes N rows, the gradient reads N rows and writes V.
-//   The gradient is three launches, each a programmatic dependent of the one before:
+//   The gradient of more than EB_FEW tokens is three launches, each a programmatic dependent of the one before (32768 tokens of a text, 8192 words of
+//   768 bf16, alone with cold caches: 13 + 14 + 12 us, of which the bytes are 10; the lookup 12 for 10):
 //   embed_sort_kernel  a CTA owns a share of the vocabulary and reads all ids once (8 N bytes from the L2), which tells it its own tokens
 //                      in order and how many belong to the CTAs before it: a stable counting sort without a word exchanged between CTAs.
 //   embed_sum_kernel   the sorted tokens in chunks of EB_CHUNK, whatever words they hold, so a frequent word is spread over many CTAs: a run
@@ -280,6 +281,98 @@ __global__ void __launch_bounds__(EB_SLICES * EB_COLS) embed_join_kernel(const i
     }
 }
 
+// Up to EB_FEW tokens: one launch and no scratch. Against the three launches, 8192 words of 768 bf16: 64 tokens of a text 4.6 us for 17, 256 9.1 for 18,
+// 512 14 for 18; all tokens one word, whose sum is one thread's per column: 11 for 16, 37 for 17, 71 for 18. An eager training pass, bound by the
+// host at all of these, takes 51 us for 57. A CTA owns EB_FEW_WORDS words, its first warp finds their tokens and puts them in order of their words,
+// then a thread adds up its columns token by token, in parts of EB_CHUNK tokens like the others.
+constexpr int EB_FEW = 256, EB_FEW_WORDS = 32;
+template <typename T, int VEC>
+__global__ void __launch_bounds__(256) embed_few_kernel(const long long *__restrict__ ids, const T *__restrict__ g, float scale, T *__restrict__ dW, int N, int V,
+                                                        long long padding, int d) {
+    __shared__ int tok[EB_FEW], word_of[EB_FEW], first[EB_FEW_WORDS + 1], next[EB_FEW_WORDS];
+    pdl_wait();
+    pdl_launch_dependents();
+    const int lane = threadIdx.x & 31, v0 = blockIdx.x * EB_FEW_WORDS, words = min(EB_FEW_WORDS, V - v0);
+    if (threadIdx.x < 32) {
+        int word[EB_FEW / 32];
+        next[lane] = 0;
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < EB_FEW / 32; ++j) {
+            const long long id = 32 * j + lane < N ? ids[32 * j + lane] : -1;
+            const unsigned long long at = (unsigned long long)id - (unsigned)v0;
+            word[j] = at < (unsigned)words && id != padding ? (int)at : -1;
+        }
+#pragma unroll
+        for (int j = 0; j < EB_FEW / 32; ++j)
+            if (word[j] >= 0) atomicAdd(&next[word[j]], 1);            // whole numbers: the order does not matter
+        __syncwarp();
+        const int count = next[lane];
+        int inc = count;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) { const int up = __shfl_up_sync(0xffffffffu, inc, o); if (lane >= o) inc += up; }
+        first[lane + 1] = inc;
+        if (lane == 0) first[0] = 0;
+        next[lane] = inc - count;
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < EB_FEW / 32; ++j) {                        // the ones of a word ranked by the lanes before
+            const bool here = word[j] >= 0;
+            const unsigned who = __ballot_sync(0xffffffffu, here);
+            if (who == 0u) continue;
+            if (here) {
+                const unsigned same = __match_any_sync(who, word[j]), before = same & ((1u << lane) - 1u);
+                const int start = next[word[j]];
+                tok[start + __popc(before)] = 32 * j + lane;
+                word_of[start + __popc(before)] = word[j];
+                __syncwarp(who);
+                if (before == 0u) next[word[j]] = start + __popc(same);
+            }
+            __syncwarp();
+        }
+    }
+    __syncthreads();
+    const int c = (blockIdx.y * blockDim.x + threadIdx.x) * VEC;
+    if (c >= d) return;
+    for (int w = 0; w < words; ++w) {
+        float none[VEC];
+#pragma unroll
+        for (int q = 0; q < VEC; ++q) none[q] = 0.f;
+        if (first[w] == first[w + 1]) EbPack<T, VEC>::store(dW + (long long)(v0 + w) * d + c, none);
+    }
+    const int n = first[words];
+    float acc[VEC], sum[VEC];
+#pragma unroll
+    for (int q = 0; q < VEC; ++q) { acc[q] = 0.f; sum[q] = 0.f; }
+    constexpr int AHEAD = 16;
+    for (int i0 = 0; i0 < n; i0 += AHEAD) {
+        typename EbPack<T, VEC>::Raw buf[AHEAD];
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j)
+            if (i0 + j < n) buf[j] = EbPack<T, VEC>::load(g + (long long)tok[i0 + j] * d + c);
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
+            const int i = i0 + j;
+            if (i >= n) break;
+            float v[VEC];
+            EbPack<T, VEC>::floats(buf[j], v);
+#pragma unroll
+            for (int q = 0; q < VEC; ++q) acc[q] += v[q];
+            const int w = word_of[i];
+            const bool ends = i + 1 == first[w + 1];
+            if (!ends && ((i - first[w] + 1) % EB_CHUNK) != 0) continue;
+#pragma unroll
+            for (int q = 0; q < VEC; ++q) { sum[q] += acc[q]; acc[q] = 0.f; }
+            if (!ends) continue;
+#pragma unroll
+            for (int q = 0; q < VEC; ++q) sum[q] *= scale;
+            EbPack<T, VEC>::store(dW + (long long)(v0 + w) * d + c, sum);
+#pragma unroll
+            for (int q = 0; q < VEC; ++q) sum[q] = 0.f;
+        }
+    }
+}
+
 // ------------------------------------------------------------------------------------------------ host
 template <typename T, int VEC>
 static int embed_fwd(const long long *ids, const void *W, float scale, void *y, long long N, int V, int d, cudaStream_t stream) {
@@ -296,8 +389,17 @@ int embedding_fwd_launch(const long long *ids, const void *W, int dtype, float s
 
 static long long embed_chunks(long long N) { return (N + EB_CHUNK - 1) / EB_CHUNK; }
 long long embedding_bwd_bytes(long long N, int V, int d) {
+    if (N <= EB_FEW) return 0;
     auto up = [](long long x) { return (x + 255) / 256 * 256; };
     return up(8 * N) + up(8LL * (V + 1)) + up(embed_chunks(N) * 8 * d);
+}
+template <typename T, int VEC>
+static int embed_few(const long long *ids, const void *g, float scale, void *dW, int N, int V, long long padding, int d, cudaStream_t stream) {
+    const int cols = (d + VEC - 1) / VEC, nt = cols >= 256 ? 256 : (cols + 31) / 32 * 32;
+    const cudaError_t e = pdl_launch(embed_few_kernel<T, VEC>, dim3((unsigned)((V + EB_FEW_WORDS - 1) / EB_FEW_WORDS), (unsigned)((cols + nt - 1) / nt)), dim3((unsigned)nt), 0,
+                                     stream, ids, static_cast<const T *>(g), scale, static_cast<T *>(dW), N, V, padding, d);
+    if (e != cudaSuccess) { set_cuda_error(e, "embed_few launch"); return PGB_ERR_CUDA; }
+    return check_launch("embed_few_kernel");
 }
 template <typename T, int VEC>
 static int embed_bwd(const void *g, float scale, void *dW, const int2 *order, const int2 *run, float *part, long long N, int V, int d,
@@ -315,6 +417,13 @@ static int embed_bwd(const void *g, float scale, void *dW, const int2 *order, co
 }
 int embedding_bwd_launch(const long long *ids, const void *g, int dtype, float scale, long long padding, void *dW, void *scratch, long long N, int V, int d,
                          cudaStream_t stream) {
+    const bool wide = aligned(g, 16) && aligned(dW, 16) && d % (dtype == PGB_F32 ? 4 : 8) == 0;
+    if (N <= EB_FEW) {
+        if (dtype == PGB_F32)
+            return wide ? embed_few<float, 4>(ids, g, scale, dW, (int)N, V, padding, d, stream) : embed_few<float, 1>(ids, g, scale, dW, (int)N, V, padding, d, stream);
+        return wide ? embed_few<__nv_bfloat16, 8>(ids, g, scale, dW, (int)N, V, padding, d, stream)
+                    : embed_few<__nv_bfloat16, 1>(ids, g, scale, dW, (int)N, V, padding, d, stream);
+    }
     auto up = [](long long x) { return (x + 255) / 256 * 256; };
     char *s = static_cast<char *>(scratch);
     int2 *order = reinterpret_cast<int2 *>(s);
@@ -324,11 +433,11 @@ int embedding_bwd_launch(const long long *ids, const void *g, int dtype, float s
     while (((V - 1) >> log_ctas) + 1 > EB_ROWS) ++log_ctas;
     const int rows = (((V - 1) >> log_ctas) + 2) & ~1;                 // even: the list behind the histogram is 8-byte aligned
     const size_t smem = (size_t)EB_WARPS * rows * 4 + EB_WARPS * EB_LIST * 8;
-    cudaError_t e = cudaFuncSetAttribute(embed_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, EB_WARPS * EB_ROWS * 4 + EB_WARPS * EB_LIST * 8);
+    cudaError_t e = smem <= 49152 ? cudaSuccess
+                  : cudaFuncSetAttribute(embed_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, EB_WARPS * EB_ROWS * 4 + EB_WARPS * EB_LIST * 8);
     if (e == cudaSuccess)
         e = pdl_launch(embed_sort_kernel, dim3(1u << log_ctas), dim3(EB_NT), smem, stream, ids, order, run, (int)N, V, padding, rows, log_ctas);
     if (e != cudaSuccess) { set_cuda_error(e, "embed_sort launch"); return PGB_ERR_CUDA; }
-    const bool wide = aligned(g, 16) && aligned(dW, 16) && d % (dtype == PGB_F32 ? 4 : 8) == 0;
     if (dtype == PGB_F32)
         return wide ? embed_bwd<float, 4>(g, scale, dW, order, run, part, N, V, d, stream) : embed_bwd<float, 1>(g, scale, dW, order, run, part, N, V, d, stream);
     return wide ? embed_bwd<__nv_bfloat16, 8>(g, scale, dW, order, run, part, N, V, d, stream)

@@ -612,7 +612,7 @@ Tensor embed_bwd(const Tensor &ids_, const Tensor &g_, double scale, int64_t pad
     Tensor dw = alloc(g, {V, d}, g.scalar_type());
     if (N == 0) return dw.zero_();
     const long long n = pgb_embedding_bwd_scratch_bytes(N, V, d);
-    const Tensor scratch = bytes(g, n);
+    const Tensor scratch = n > 0 ? bytes(g, n) : Tensor();
     check(pgb_embedding_bwd(static_cast<long long *>(vp(ids)), vp(g), code(g), scale, padding, vp(dw), vp(scratch), n, N, V, d, dev.stream), "pgb_embedding_bwd");
     return dw;
 }

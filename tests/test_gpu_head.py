@@ -359,7 +359,8 @@ def embed(ids, w, gy, **kw):
 @pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("N,V,d,how", [(1, 1, 1, "one"), (1, 8192, 768, "uniform"), (31, 7, 33, "uniform"), (33, 1000, 64, "one"), (1000, 8192, 768, "text"),
                                        (5000, 100, 72, "uniform"), (20000, 50257, 128, "text"), (4096, 333, 1100, "one"), (4097, 100000, 40, "uniform"),
-                                       (777, 3, 2056, "uniform")])
+                                       (777, 3, 2056, "uniform"),
+                                       (256, 8192, 768, "text"), (257, 8192, 768, "text"), (255, 1, 2056, "one"), (100, 65, 31, "uniform"), (256, 33, 8, "one")])
 def test_embedding(N, V, d, how, dtype):
     """One word for all tokens, words in equal parts, words as in a text; rows of 16-byte pieces and others."""
     g = torch.Generator(device=DEV).manual_seed(N + V)

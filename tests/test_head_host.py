@@ -53,8 +53,10 @@ def test_bad_calls_of_teacher_lists_and_embedding():
     fwd = lambda i=one, w=one, dt=1, y=one, N=3, V=5, d=7: L.pgb_embedding_fwd(i, w, dt, 1.0, y, N, V, d, None)
     assert fwd(i=None) == fwd(w=None) == fwd(y=None) == NULL and fwd(dt=3) == DTYPE and fwd(N=0) == fwd(V=0) == fwd(d=0) == SHAPE
     assert fwd(i=odd) == fwd(w=ctypes.c_void_p(0x1001)) == ALIGN and fwd(N=(1 << 30) + 1) == LARGE
-    bwd = lambda i=one, g=one, dt=1, w=one, s=one, n=BIG, N=3, V=5, d=7: L.pgb_embedding_bwd(i, g, dt, 1.0, -1, w, s, n, N, V, d, None)
+    bwd = lambda i=one, g=one, dt=1, w=one, s=one, n=BIG, N=600, V=5, d=7: L.pgb_embedding_bwd(i, g, dt, 1.0, -1, w, s, n, N, V, d, None)
     assert bwd(i=None) == bwd(g=None) == bwd(w=None) == bwd(s=None) == NULL and bwd(n=10) == SHAPE and bwd(d=65537) == LARGE and bwd(s=odd) == ALIGN
+    assert bwd(N=3, s=None, n=0, g=None) == NULL and bwd(N=3, s=None, n=0, d=65537) == LARGE       # few tokens need no scratch
+    assert L.pgb_embedding_bwd_scratch_bytes(256, 9, 64) == 0 < L.pgb_embedding_bwd_scratch_bytes(257, 9, 64)
     assert L.pgb_head_loss_fwd_scratch_bytes(0, 5, 64, 1) == 0 and L.pgb_head_loss_bwd_scratch_bytes(5, 5, 63, 1, 1, 1) == 0 and L.pgb_embedding_bwd_scratch_bytes(1, 0, 4) == 0
 
 
