@@ -1,6 +1,6 @@
 """The language model around the carrier layers: same constructor arguments, parameter names and carried-state
 interface as the reference's src/model.py LM (:621-864), restricted to the pure-carrier mixers (aspin, dspin, hspin,
-hdspin, fspin). Attention controls, hybrids, growth and the training loss are other subsystems and are not here."""
+hdspin, fspin). Attention controls, hybrids and growth are other subsystems and are not here."""
 from __future__ import annotations
 
 import contextlib
