@@ -421,31 +421,34 @@ HeadIn head_in(const char *what, const Tensor &h, const Tensor &w) {
     const int64_t d = w.size(1);
     TORCH_CHECK_VALUE(w.size(0) >= 1 && w.size(0) <= MOST_WORDS && d >= 8 && d <= 65536 && d % 8 == 0, what,
                       ": the weight is (V, d) with V from 1 to 2^30 and d a multiple of 8 up to 65536, got ", w.sizes());
-    return {head_operand(h.reshape({-1, d})), head_operand(w), h.numel() / d, w.size(0), d};
+    return {head_operand(h.dim() == 2 ? h : h.reshape({-1, d})), head_operand(w), h.numel() / d, w.size(0), d};
 }
 // What a row is held to: a word each (target), or a teacher's entries (lists, marks, ent; kept: their logits).
 struct HeadWant { Tensor target; int64_t ignore; Tensor lists, marks, ent, kept; double tau; };
 struct HeadOut { Tensor loss, L, stats; };                            // loss: [N] or 0-d; stats: rows that count, whether one that does not is no number
-HeadOut head_fwd(const char *what, const HeadIn &x, const HeadWant &t, int reduction) {
+// keep: for a gradient. Without one, L and stats lie behind the scratch: few rows are scored in the time of this call (11.4 us with two allocations more, 8.9 now).
+HeadOut head_fwd(const char *what, const HeadIn &x, const HeadWant &t, int reduction, bool keep = true) {
     OnDevice dev(x.h);
-    HeadOut r{alloc(x.h, reduction == REDUCE_NONE ? at::IntArrayRef({x.N}) : at::IntArrayRef(), at::kFloat), alloc(x.h, {x.N, 2}, at::kFloat),
-              alloc(x.h, {2}, at::kFloat)};
+    HeadOut r{alloc(x.h, reduction == REDUCE_NONE ? at::IntArrayRef({x.N}) : at::IntArrayRef(), at::kFloat)};
+    if (keep) { r.L = alloc(x.h, {x.N, 2}, at::kFloat); r.stats = alloc(x.h, {2}, at::kFloat); }
     if (x.N == 0) {                                                    // nothing to add up: 0, and 0 / 0 as the mean
         if (reduction == REDUCE_SUM) r.loss.zero_();
         if (reduction == REDUCE_MEAN) r.loss.fill_(std::numeric_limits<float>::quiet_NaN());
-        r.stats.zero_();
+        if (keep) r.stats.zero_();
         return r;
     }
     const bool list = t.lists.defined();
     const int k = list ? t.lists.size(1) : 0;
     const long long n = pgb_head_loss_fwd_scratch_bytes(x.N, x.V, x.d, code(x.h));
-    const Tensor scratch = bytes(x.h, n);
+    const long long behind = (n + 255) / 256 * 256;
+    const Tensor scratch = bytes(x.h, keep ? n : behind + 8 * (x.N + 1));
+    float *const L = keep ? fp(r.L) : reinterpret_cast<float *>(static_cast<char *>(vp(scratch)) + behind), *const stats = keep ? fp(r.stats) : L + 2 * x.N;
     float *row = reduction == REDUCE_NONE ? fp(r.loss) : nullptr, *loss = reduction == REDUCE_NONE ? nullptr : fp(r.loss);
     if (list)
-        check(pgb_linear_distill_fwd(vp(x.h), vp(x.w), code(x.h), static_cast<int *>(vp(t.lists)), static_cast<unsigned *>(vp(t.marks)), fp(t.ent), fp(t.kept), k, t.tau, row, loss, fp(r.stats), fp(r.L),
+        check(pgb_linear_distill_fwd(vp(x.h), vp(x.w), code(x.h), static_cast<int *>(vp(t.lists)), static_cast<unsigned *>(vp(t.marks)), fp(t.ent), fp(t.kept), k, t.tau, row, loss, stats, L,
                                      vp(scratch), n, reduction, x.N, x.V, x.d, dev.stream), what);
     else
-        check(pgb_linear_xent_fwd(vp(x.h), vp(x.w), code(x.h), static_cast<long long *>(vp(t.target)), t.ignore, row, loss, fp(r.stats), fp(r.L), vp(scratch),
+        check(pgb_linear_xent_fwd(vp(x.h), vp(x.w), code(x.h), static_cast<long long *>(vp(t.target)), t.ignore, row, loss, stats, L, vp(scratch),
                                   n, reduction, x.N, x.V, x.d, dev.stream), what);
     return r;
 }
@@ -489,7 +492,8 @@ HeadWant xent_want(const HeadIn &x, const Tensor &h, const Tensor &target, int64
     need_cuda(target);
     same_device(XENT, h, target);
     TORCH_CHECK_VALUE(target.sizes() == h.sizes().slice(0, h.dim() - 1), XENT, ": a target per row of h, got ", target.sizes(), " for ", h.sizes());
-    return {whole_numbers(XENT, target).reshape({x.N}), ignore, Tensor(), Tensor(), Tensor(), Tensor(), 1.0};
+    const Tensor t = whole_numbers(XENT, target);
+    return {t.dim() == 1 ? t : t.reshape({x.N}), ignore, Tensor(), Tensor(), Tensor(), Tensor(), 1.0};
 }
 std::tuple<Tensor, Tensor, Tensor> teacher_lists(const Tensor &ids_, const Tensor &logits_, double tau, int64_t V) {
     need_cuda(ids_, logits_);
@@ -567,7 +571,7 @@ OptTensor linear_xent(const Tensor &h, const Tensor &w, const Tensor &target, in
         return HeadLoss::apply(h, w, OptTensor(target), ignore, OptTensor(), OptTensor(), 1.0, reduction)[0];
     }
     const HeadIn x = head_in(XENT, h, w);
-    const Tensor loss = head_fwd(XENT, x, xent_want(x, h, target, ignore), reduction).loss;
+    const Tensor loss = head_fwd(XENT, x, xent_want(x, h, target, ignore), reduction, false).loss;
     return reduction == REDUCE_NONE ? loss.view(target.sizes()) : loss;
 }
 OptTensor linear_distill(const Tensor &h, const Tensor &w, const Tensor &ids, const Tensor &logits, double tau, int64_t reduction) {
@@ -577,7 +581,7 @@ OptTensor linear_distill(const Tensor &h, const Tensor &w, const Tensor &ids, co
         return HeadLoss::apply(h, w, OptTensor(), 0, OptTensor(ids), OptTensor(logits.detach()), tau, reduction)[0];
     }
     const HeadIn x = head_in(DISTILL, h, w);
-    const Tensor loss = head_fwd(DISTILL, x, distill_want(x, h, ids, logits, tau), reduction).loss;
+    const Tensor loss = head_fwd(DISTILL, x, distill_want(x, h, ids, logits, tau), reduction, false).loss;
     return reduction == REDUCE_NONE ? loss.view(h.sizes().slice(0, h.dim() - 1)) : loss;
 }
 
