@@ -495,6 +495,7 @@ def _(h, W, target, ignore_index, L, stats, grad, reduction, want_dh, want_dW):
 def _xent_ctx(ctx, inputs, output):
     h, W, target, ctx.ignore_index, ctx.reduction = inputs
     ctx.save_for_backward(h, W, target, output[1], output[2])
+    ctx.mark_non_differentiable(output[1], output[2])
 
 
 def _xent_grads(ctx, g, _L, _stats):
@@ -546,6 +547,7 @@ def _(h, W, lists, ent, kept, temperature, L, stats, grad, reduction, want_dh, w
 def _distill_ctx(ctx, inputs, output):
     h, W, lists, _marks, ent, ctx.temperature, ctx.reduction = inputs
     ctx.save_for_backward(h, W, lists, ent, output[3], output[1], output[2])
+    ctx.mark_non_differentiable(*output[1:])
 
 
 def _distill_grads(ctx, g, _L, _stats, _kept):

@@ -549,7 +549,8 @@ def test_what_the_forward_pass_leaves_is_checked():
     h, w, g = operands(6, 70, 16, BF, 3)
     t = torch.randint(0, 70, (6,), device=DEV, generator=g)
     ids, logits = torch.randint(0, 70, (6, 3), device=DEV, generator=g), torch.randn(6, 3, device=DEV, generator=g)
-    loss, L, stats = ops.linear_xent(h, w, t, -100, 0)
+    loss, L, stats = ops.linear_xent(h, w.clone().requires_grad_(), t, -100, 0)
+    assert loss.requires_grad and not L.requires_grad and not stats.requires_grad       # no gradient passes through these
     one = torch.ones(6, device=DEV)
     good = dict(L=L, stats=stats, grad=one)
     for name, bad in (("L", L[:5]), ("L", L.double()), ("L", L.cpu()), ("L", torch.empty(2, 6, device=DEV).t()), ("stats", stats[:1]), ("grad", one[:5]), ("grad", one.cpu())):
