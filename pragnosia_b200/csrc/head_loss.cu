@@ -353,7 +353,10 @@ struct HlFwdEpi {
                 uint32_t todo = (uint32_t)(bits >> (32 * b));
                 while (__any_sync(0xffffffffu, todo != 0u)) {
                     const float s = pick32(v[b], __ffs(todo) - 1);
-                    if (todo != 0u) { f.dot[(long long)row * f.t.k + place] = s; ++place; todo &= todo - 1u; }
+                    if (todo != 0u) {
+                        if ((unsigned)place < (unsigned)f.t.k) f.dot[(long long)row * f.t.k + place] = s;     // marks are a caller's: never past its row
+                        ++place; todo &= todo - 1u;
+                    }
                 }
             } else if (__any_sync(0xffffffffu, (unsigned)(nx - c0) < 32u)) {
                 const float s = pick32(v[b], nx - c0);

@@ -1,0 +1,37 @@
+"""The head's losses where the other tests do not reach: what a caller hands to the registered operators and the C entry points, lists in several
+pieces, temperatures without an exact reciprocal, rows whose loss is next to nothing, teachers whose axes are not those of the hidden states,
+masked batches of the language model and its gradients against the formulas on its own logits, padding of a size that a launch takes long to copy."""
+import ctypes
+import math
+
+import pytest
+import torch
+import torch.nn.functional as F
+
+from pragnosia_b200 import head
+from pragnosia_b200._lib import check, host, lib
+from test_gpu_head import BF, DEV, F32, _grad_enabled_and_waits_fine, dense, distill, lm, operands, teacher, within, xent  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_marks_of_longer_lists_write_nothing_past_a_row(dtype):
+    """Marks say where in its list a word's logit goes. Those of lists of 40 beside lists of 3 point behind the end: what lies behind `kept` stays as it
+    was, and so does the result of entries that the lists have."""
+    N, V, d, k = 70, 300, 64, 3
+    h, w, g = operands(N, V, d, dtype, 1)
+    ids, logits = torch.rand(N, V, device=DEV, generator=g).argsort(1)[:, :40].contiguous(), torch.randn(N, 40, device=DEV, generator=g)
+    marks = host().teacher_lists(ids, logits, 1.0, V)[1]
+    first = host().teacher_lists(ids.sort(1).values[:, :k].contiguous(), logits[:, :k].contiguous(), 1.0, V)       # of the same rows, the first k words
+    room = torch.full((N * k + 4096,), 7.0, device=DEV)
+    loss, L, stats = torch.empty(N, device=DEV), torch.empty(N, 2, device=DEV), torch.empty(2, device=DEV)
+    n = lib().pgb_head_loss_fwd_scratch_bytes(N, V, d, int(dtype == BF))
+    scratch = torch.empty(n, device=DEV, dtype=torch.uint8)
+    at = lambda t: ctypes.c_void_p(t.data_ptr())
+    stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    check(lib().pgb_linear_distill_fwd(at(h), at(w), int(dtype == BF), at(first[0]), at(marks), at(first[2]), at(room), k, 1.0, at(loss), None, at(stats), at(L),
+                                       at(scratch), n, 0, N, V, d, stream), "pgb_linear_distill_fwd")
+    torch.cuda.synchronize()
+    assert (room[N * k:] == 7.0).all()
+    assert torch.equal(loss, host().linear_distill_fwd(h, w, *first, 1.0, 0)[0])
