@@ -288,7 +288,7 @@ __device__ __forceinline__ void hl_body(const HlMaps &maps, const What &what, Ep
             }
             ok = epi.tile(x, v, stage, shared, bar_quarters(sub, ti & 3)) && more;
         }
-        epi.end(lane);
+        epi.end(tid - 64, lane);
     }
     tc_fence_before();
     __syncthreads();
@@ -329,7 +329,7 @@ struct HlFwdEpi {
     uint64_t bits; int place, nx;                                      // of the tile at hand: targets by column, and the first one's place; or the target
     __device__ __forceinline__ void start(int i) { if (i == 0 && blockIdx.x == 0) { *f.ticket = 0u; f.stats[0] = 0.f; f.stats[1] = 0.f; } }
     __device__ __forceinline__ bool dirty() const { return false; }
-    __device__ __forceinline__ void end(int) {}
+    __device__ __forceinline__ void end(int, int) {}
     __device__ __forceinline__ void fetch(int, int r, int c) {
         const bool in = r < f.N && c < f.V;
         if constexpr (LIST) {
@@ -809,8 +809,7 @@ struct HlBwdEpi {
     HlProbEpi<LIST, TERMS> ds;
     HlGradEpi grad;
     const HlBwd &f;
-    __device__ __forceinline__ void start(int i) {
-        if (TERMS == 1 && f.clean != nullptr && *f.dirty != 0.f) hl_clean(f, i);
+    __device__ __forceinline__ void start(int) {
         grad.alpha = hl_alpha(grad.f.up, grad.f.count, grad.f.tau, grad.f.reduction);
     }
     __device__ __forceinline__ void fetch(int g, int r, int c) { if (g == 2) ds.fetch(r, c); }
@@ -825,7 +824,12 @@ struct HlBwdEpi {
         return true;
     }
     __device__ __forceinline__ bool dirty() const { return TERMS == 1 && *f.dirty != 0.f; }
-    __device__ __forceinline__ void end(int lane) { if (lane == 0) tma_store_done(); }
+    // The clean copy, which the next launch reads first, behind the tiles: its time grows with N d, and ahead of them the other roles would spend it in
+    // their bounded waits.
+    __device__ __forceinline__ void end(int i, int lane) {
+        if (lane == 0) tma_store_done();
+        if (TERMS == 1 && f.clean != nullptr && *f.dirty != 0.f) hl_clean(f, i);
+    }
 };
 template <bool LIST, int TERMS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(HL_NT, 1)
