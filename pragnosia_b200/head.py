@@ -56,6 +56,8 @@ def linear_distill(h, weight, teacher_ids, teacher_logits, *, temperature: float
         out = host().linear_distill(h, weight, teacher_ids, teacher_logits, float(temperature), r)
         if out is not None:
             return out
+    if teacher_ids.shape[:-1] != h.shape[:-1] or teacher_ids.dim() != h.dim() or teacher_logits.shape != teacher_ids.shape:     # the operators see rows only
+        raise ValueError(f"linear_distill: k teacher entries per row of h, got {tuple(teacher_ids.shape)} and {tuple(teacher_logits.shape)} for {tuple(h.shape)}")
     ops = _operators()
     lists, marks, ent = ops.teacher_lists(teacher_ids, teacher_logits.detach(), float(temperature), weight.shape[0])
     loss = ops.linear_distill(h, weight, lists, marks, ent, float(temperature), r)[0]

@@ -52,3 +52,27 @@ def test_long_padding_without_numbers():
     h[dead] = math.nan
     got = xent(h, w, t, None, "mean")
     assert all(torch.isfinite(a).all() and torch.equal(a, b) for a, b in zip(want, got))
+
+
+def test_a_teacher_of_other_axes_is_refused_everywhere():
+    """A teacher of (T, B) beside hidden states of (B, T) has as many rows: refused eagerly, under a dispatch mode and under a compiler alike."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Mode(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+    h, w, g = operands(6 * 5, 70, 16, BF, 3)
+    h = h.view(6, 5, 16)
+    ids, logits = torch.randint(0, 70, (6, 5, 3), device=DEV, generator=g), torch.randn(6, 5, 3, device=DEV, generator=g)
+    turned = ids.transpose(0, 1).contiguous(), logits.transpose(0, 1).contiguous()
+    for bad in (turned, (ids.flatten(0, 1), logits.flatten(0, 1)), (ids, logits[..., :2]), (ids[..., 0], logits[..., 0])):
+        with pytest.raises(ValueError):
+            head.linear_distill(h, w, *bad)
+        with Mode(), pytest.raises(ValueError):
+            head.linear_distill(h, w, *bad)
+        torch._dynamo.reset()
+        with pytest.raises(Exception, match="teacher"):
+            torch.compile(head.linear_distill, backend="eager")(h, w, *bad)
+    with Mode():
+        seen = head.linear_distill(h, w, ids, logits)
+    assert torch.equal(seen, head.linear_distill(h, w, ids, logits))
