@@ -223,19 +223,27 @@ class LM(nn.Module):
         reduction "none" and no gradient, the scores of a text's tokens.
 
         teacher: (ids (B,T,k), logits (B,T,k)), a teacher's top logits for the same targets; the loss is then (1 - alpha) cross entropy
-        + alpha distillation at `temperature` (head.linear_distill)."""
+        + alpha distillation at `temperature` (head.linear_distill). Tokens that given `targets` mark with ignore_index count in neither
+        term, whatever the teacher holds there; without `targets` a sequence's last token, whose next word only the teacher knows, counts
+        in the distillation alone. alpha 0 leaves the teacher out."""
         B, T = x.shape
         if T < 2 and torch.is_grad_enabled():
             raise ValueError("loss: a sequence of one token has no differentiable pass through the carrier layers (no_grad scores it)")
-        if targets is None:
+        given = targets is not None
+        if given and targets.shape != x.shape:
+            raise ValueError(f"loss: a target per id, got {tuple(targets.shape)} for {tuple(x.shape)}")
+        if not given:
             targets = torch.cat([x[:, 1:], x.new_full((B, 1), ignore_index)], 1)
         plain = type(self.e) is nn.Embedding and self.e.padding_idx is None and self.e.max_norm is None and not self.e.scale_grad_by_freq
         e = head.embedding(x, self.e.weight) if plain and self.e.weight.dtype in (torch.bfloat16, torch.float32) else self.e(x)
         e = e + self.p(torch.arange(T, device=x.device) % self.p.num_embeddings)
         h = self._add_norm(*self._layers(e, [None] * self.layers), self.n)[1]
-        if teacher is None:
+        if teacher is None or alpha == 0.0:
             return head.linear_cross_entropy(h, self.e.weight, targets, ignore_index=ignore_index, reduction=reduction)
-        soft = head.linear_distill(h, self.e.weight, *teacher, temperature=temperature, reduction=reduction)
+        ids, logits = teacher
+        if given:
+            ids = ids.masked_fill((targets == ignore_index).unsqueeze(-1), -1)
+        soft = head.linear_distill(h, self.e.weight, ids, logits, temperature=temperature, reduction=reduction)
         if alpha == 1.0:
             return soft
         return (1.0 - alpha) * head.linear_cross_entropy(h, self.e.weight, targets, ignore_index=ignore_index, reduction=reduction) + alpha * soft

@@ -76,3 +76,69 @@ def test_a_teacher_of_other_axes_is_refused_everywhere():
     with Mode():
         seen = head.linear_distill(h, w, ids, logits)
     assert torch.equal(seen, head.linear_distill(h, w, ids, logits))
+
+
+# ------------------------------------------------------------------------------------------------ the language model's loss
+def masked_batch(g, B=3, T=70, k=5, vocab=333):
+    x = torch.randint(0, vocab, (B, T), device=DEV, generator=g)
+    ids, logits = torch.rand(B, T, vocab, device=DEV, generator=g).argsort(2)[..., :k].contiguous(), 2.0 * torch.randn(B, T, k, device=DEV, generator=g)
+    targets = torch.cat([x[:, 1:], torch.full_like(x[:, :1], -100)], 1)
+    targets[:, :9] = -100                                             # a prompt
+    targets[1, 40:] = -100                                            # padding
+    return x, targets, ids, logits
+
+
+def reference_loss(m, x, targets, ids, logits, tau, alpha):
+    """The formulas in 64 bits on the model's own hidden states, differentiable through its layers and both uses of the table."""
+    z = m.trunk(x).double() @ m.e.weight.double().t()
+    ce = F.cross_entropy(z.flatten(0, 1), targets.flatten(), ignore_index=-100)
+    p = torch.softmax(logits.double() / tau, -1)
+    rows = tau * tau * (p * (p.log() - torch.log_softmax(z / tau, -1).gather(2, ids))).sum(-1)
+    live = targets != -100
+    return (1.0 - alpha) * ce + alpha * torch.where(live, rows, torch.zeros_like(rows)).sum() / live.sum()
+
+
+@pytest.mark.parametrize("mixer,d", [("aspin", 128), ("dspin", 128), ("fspin", 72)])
+@pytest.mark.parametrize("alpha", [0.0, 0.3, 1.0])
+def test_language_model_loss_of_a_masked_batch(mixer, d, alpha):
+    """Tokens without a target count in neither term, and the gradients are those of the formulas on the model's logits. fp32: the head's two gradients are
+    off by some (6 d / 16 + 34) 2^-23 of what they add up, 1e-5, and go through the same layers on either side; a gradient may lose a factor of a hundred to
+    cancellation. The associative layers' backward pass takes the gradient behind it as bf16 (2^-8), whose roundings fall differently for gradients that differ
+    at all: two layers, 2^-7, of which a weight's gradient may lose a factor of four."""
+    m = lm(mixer, F32, d=d)
+    x, targets, ids, logits = masked_batch(torch.Generator(device=DEV).manual_seed(2))
+    params = [(n, p) for n, p in m.named_parameters()]
+    want = reference_loss(m, x, targets, ids, logits, 2.0, alpha)
+    ref = torch.autograd.grad(want, [p for _, p in params], allow_unused=True)
+    loss = m.loss(x, targets, teacher=(ids, logits), temperature=2.0, alpha=alpha)
+    got = torch.autograd.grad(loss, [p for _, p in params], allow_unused=True)
+    assert abs(float(loss) - float(want)) < 1e-4
+    size = math.sqrt(sum(float(r.norm()) ** 2 for r in ref if r is not None))
+    rel, part = (1e-3, 1e-5) if mixer == "fspin" else (2.0 ** -5, 2.0 ** -8)
+    for (n, _), a, b in zip(params, got, ref):
+        assert (a is None) == (b is None), n
+        if a is not None:
+            assert float((a - b).norm()) <= rel * float(b.norm()) + part * size, n
+
+
+def test_masked_tokens_of_a_language_model_may_have_any_teacher():
+    """Lists of masked tokens change nothing, to the bit; int32 lists as int64; the caller's lists stay as they are."""
+    m = lm("aspin", BF)
+    x, targets, ids, logits = masked_batch(torch.Generator(device=DEV).manual_seed(4))
+    dead = targets == -100
+    other = torch.where(dead[..., None], (ids + 7) % 333, ids).int()
+    kept = other.clone()
+    for reduction in ("mean", "sum", "none"):
+        a, b = (m.loss(x, targets, teacher=(t, logits), temperature=1.5, alpha=0.4, reduction=reduction) for t in (ids, other))
+        assert torch.equal(a, b) and (reduction != "none" or not a[dead].any())
+    assert torch.equal(other, kept)
+
+
+def test_a_teacher_of_no_weight_is_left_out():
+    """alpha 0 is the cross entropy, even where no token has an entry (whose mean would be 0 / 0)."""
+    m = lm("aspin", BF)
+    x, targets, ids, logits = masked_batch(torch.Generator(device=DEV).manual_seed(5))
+    with torch.no_grad():
+        assert torch.equal(m.loss(x, targets, teacher=(torch.full_like(ids, -1), logits), alpha=0.0), m.loss(x, targets))
+    with pytest.raises(ValueError):
+        m.loss(x, targets[0], teacher=(ids, logits), alpha=1.0)
