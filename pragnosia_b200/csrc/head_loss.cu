@@ -411,7 +411,7 @@ head_loss_fwd_kernel(const __grid_constant__ HlMaps maps, const __grid_constant_
 // partial sum; the last block to finish adds the partials up in order, so the sum does not depend on who that is.
 struct HlJoin {
     HlTargets t; const float2 *ml; const float *dot; float2 *L; float *row_loss, *loss, *stats; double2 *partial; unsigned *ticket;
-    long long N, Np; int V, tiles; float tau; int reduction;
+    long long N, Np; int V, tiles; float tau, a; int reduction;       // a: as the product's epilogue had it
 };
 template <bool LIST>
 __global__ void __launch_bounds__(256) head_loss_join_kernel(const HlJoin j) {
@@ -468,16 +468,19 @@ __global__ void __launch_bounds__(256) head_loss_join_kernel(const HlJoin j) {
         }
         const float lg = log2f(l), hi = m + lg;                        // hi + lo = m + lg, exactly
         const float back = hi - m, rest = (m - (hi - back)) + (lg - back), lo = rest == rest ? rest : 0.f;
+        // The sum is that of 2^(a s) with a rounded, so over a, not times ln 2, a row's logarithm is the logits' own: for a word that holds all the
+        // probability l tells what a s lost in rounding to m, and L / a - s is 0 to 2^-22, where ln 2 left 1.3e-8 of s.
         const double L = (double)hi + lo;
         j.L[row] = make_float2(hi, lo);
         if (LIST) {
             const float ent = j.t.ent[row];
             live = ent != INFINITY;
-            loss = (double)j.tau * j.tau * (ent + L * 0.693147180559945309) - j.tau * (double)dots[lane];
+            loss = (double)j.tau * j.tau * ent + j.tau * (L / j.a - (double)dots[lane]);
         } else {
             const long long w = j.t.target[row];
             live = w != j.t.ignore;
-            loss = live && w >= 0 && w < j.V ? L * 0.693147180559945309 - j.dot[row] : NAN;
+            loss = live && w >= 0 && w < j.V ? L / j.a - j.dot[row] : NAN;
+            if (loss < 0.0) loss = 0.0;                                // by the rounding of l
         }
         if (!live) {
             loss = 0.0;
@@ -970,7 +973,7 @@ int head_loss_fwd_launch(const HeadLossArgs &x, float *row_loss, float *loss, fl
                   : hl_launch(head_loss_fwd_kernel<false, false>, 3, "head_loss_fwd_kernel", maps, pr, pr.tiles(), f, stream);
     if (rc != PGB_OK) return rc;
     const HlJoin j{t, f.ml, f.dot, reinterpret_cast<float2 *>(L), row_loss, loss, stats, reinterpret_cast<double2 *>(s + pl.off_partial), f.ticket,
-                   x.N, pl.Np, x.V, (int)pl.tiles, x.tau, x.reduction};
+                   x.N, pl.Np, x.V, (int)pl.tiles, x.tau, f.a, x.reduction};
     cudaError_t e = pdl_launch(list ? head_loss_join_kernel<true> : head_loss_join_kernel<false>, dim3((unsigned)(pl.Np / 32)), dim3(256), 0, stream, j);
     if (e != cudaSuccess) { set_cuda_error(e, "head_loss_join launch"); return PGB_ERR_CUDA; }
     return check_launch("head_loss_join_kernel");

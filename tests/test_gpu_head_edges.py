@@ -78,6 +78,19 @@ def test_a_teacher_of_other_axes_is_refused_everywhere():
     assert torch.equal(seen, head.linear_distill(h, w, ids, logits))
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_a_certain_word_loses_nothing(dtype):
+    """Logits of hundreds, the target ahead of all others by 30: its loss is below 700 e^-30, and what is left of it is the rounding of one exponential
+    (two units, 2^-22) and of the sum, not of the logits' own size. No loss is negative."""
+    h, w, _ = operands(400, 700, 64, dtype, 3, spread=120.0)
+    top = (h.double() @ w.double().t()).topk(2, 1)
+    sure = top.values[:, 0] - top.values[:, 1] > 30
+    assert int(sure.sum()) > 100
+    with torch.no_grad():
+        loss = head.linear_cross_entropy(h, w, top.indices[:, 0], reduction="none")
+    assert (loss >= 0).all() and (loss[sure] <= 2.0 ** -21).all(), (float(loss.min()), float(loss[sure].max()))
+
+
 # ------------------------------------------------------------------------------------------------ the language model's loss
 def masked_batch(g, B=3, T=70, k=5, vocab=333):
     x = torch.randint(0, vocab, (B, T), device=DEV, generator=g)
