@@ -114,6 +114,7 @@ __device__ __forceinline__ void hl_body(const HlMaps &maps, const What &what, Ep
     auto bar_empty = [&](int s) { return mb + 64 + 8 * s; };
     auto bar_acc_full = [&](int a) { return mb + 128 + 8 * a; };
     auto bar_acc_empty = [&](int a) { return mb + 144 + 8 * a; };      // used in the first CTA only
+    const uint32_t bar_left = mb + 160;                               // used in the first CTA only, where a wait has run out
     auto bar_quarters = [&](int sub, int a) { return mb + 192 + 32 * sub + 8 * a; };   // three of a row's column quarters are in shared memory
 
     const int tid = threadIdx.x, lane = tid & 31, warp = warp_uniform(tid >> 5);
@@ -123,6 +124,7 @@ __device__ __forceinline__ void hl_body(const HlMaps &maps, const What &what, Ep
         for (int s = 0; s < HL_STAGES; ++s) { mbar_init(bar_full(s), 1); mbar_init(bar_empty(s), 1); }
         for (int a = 0; a < 2; ++a) { mbar_init(bar_acc_full(a), 1); mbar_init(bar_acc_empty(a), 2 * HL_EPI); }
         for (int q = 0; q < 16; ++q) mbar_init(bar_quarters(q >> 2, q & 3), 3);
+        mbar_init(bar_left, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) tmem_alloc_pair(smem_u32(tmem_slot), 512);
@@ -174,6 +176,14 @@ __device__ __forceinline__ void hl_body(const HlMaps &maps, const What &what, Ep
                 __syncwarp();
             }
         }
+        // Nobody leaves with copies into shared memory under way, which a wait that ran out may have left there: the stages written last, both CTAs' halves
+        // (the barriers count both, and the other CTA waits for this one below). All of them have long arrived where every wait was met.
+        if (rank == 0) {
+            const uint32_t issued = ok ? it : it - 1;
+            bool here = true;
+            for (uint32_t j = issued > STAGES ? issued - STAGES : 0; j < issued && here; ++j)
+                here = __all_sync(0xffffffffu, mbar_wait(bar_full(j % STAGES), (j / STAGES) & 1, 91));
+        }
     } else if (warp == 1) {
         // ------------------------------------------------------------------------------------------ MMA issuer (first CTA)
         if (rank == 0) {
@@ -214,6 +224,10 @@ __device__ __forceinline__ void hl_body(const HlMaps &maps, const What &what, Ep
                     if (FINE) done();
                 }
                 if (!FINE && ok) done();
+            }
+            if (!ok) {                                                 // products under way read shared memory and write tensor memory
+                lp_commit_elect(bar_left);
+                __all_sync(0xffffffffu, lp_wait_cluster(bar_left, 0, 93));
             }
         }
     } else {
