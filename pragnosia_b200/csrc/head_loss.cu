@@ -1015,6 +1015,7 @@ struct HlLoad {
     double all() const { return n0 * c0 + (n - n0) * c1; }
 };
 constexpr double HL_DS = 5.0;                                         // what a tile of ds costs beyond its K blocks
+constexpr int HL_LONGEST = 4096;                                      // blocks of a part, 1.4 ms of products: an epilogue's wait for one is bounded by milliseconds
 struct HlSplits { int dh, dw; double cost; };
 // The parts of K with which the pairs finish earliest, `filler` units of short tiles dealt out behind them. fix0, fix1: parts that are given (0: to be chosen).
 static HlSplits hl_splits(long long t0, long long k0, long long t1, long long k1, double filler, int np, int pairs, int fix0, int fix1) {
@@ -1022,8 +1023,10 @@ static HlSplits hl_splits(long long t0, long long k0, long long t1, long long k1
     HlSplits best{1, 1, 1e300};
     for (int a : choice) {
         if (a > 1 && (fix0 || t0 == 0 || k0 / a < 4 * np)) break;
+        if (np == 1 && t0 > 0 && !fix0 && k0 > (long long)HL_LONGEST * a) continue;              // three terms: an accumulator is a block's
         for (int b : choice) {
             if (b > 1 && (fix1 || t1 == 0 || k1 / b < 4 * np)) break;
+            if (np == 1 && t1 > 0 && !fix1 && k1 > (long long)HL_LONGEST * b) continue;
             const int s0 = fix0 ? fix0 : a, s1 = fix1 ? fix1 : b;
             const HlLoad load(t0, k0, s0, t1, k1, s1, pairs);
             const double level = (load.all() + filler) / pairs, most = load.most();

@@ -19,3 +19,13 @@ def test_the_traced_call_refuses_a_teacher_of_other_axes():
             with pytest.raises(ValueError, match="teacher"):
                 head.linear_distill(h, w, e(*ids, dtype=torch.long), e(*logits, dtype=F32))
         assert sig(head.linear_distill(h, w, e(2, 5, 3, dtype=torch.long), e(2, 5, 3, dtype=F32), reduction="none")) == ((2, 5), F32)
+
+
+@pytest.mark.parametrize("N,V,d", [(1 << 23, 1 << 23, 2048), (1 << 22, 1 << 22, 32768), (1 << 24, 3 << 20, 65536), (1 << 21, 1 << 22, 65536)])
+def test_a_long_axis_is_summed_in_parts_that_a_wait_covers(N, V, d):
+    """A gradient's product over millions of columns, whose tiles fill the GPU without a cut: its parts are 4096 blocks of 64 at most, 1.4 ms, since
+    the wait for one that is not finished may end after some. A part's sums are an fp32 plane of the workspace, beside two pieces of 256 rows or columns
+    of the longer axis and a copy of h."""
+    by_rows, shorter = N >= V, min(N, V)
+    n = lib().pgb_head_loss_bwd_scratch_bytes(N, V, d, 1, int(by_rows), int(not by_rows))
+    assert n >= 2 * 2 * 256 * shorter + (0 if by_rows else 2 * N * d) + 4 * (shorter // 64 // 4096) * 256 * d
