@@ -545,7 +545,7 @@ int pgb_linear_act(const void *x, const void *W, const void *bias, void *y, long
  * 64 words they are, and the place of the first; the forward pass alone reads it) and ent [N], the sum of p log p. lists 8-byte, marks 16-byte aligned. kept [N][k]: the entries' logits, which the forward pass
  * leaves to the backward pass. A row's loss is
  * temperature^2 KL(p || softmax(s / temperature)), 0 without gradient for rows without an entry; the same id twice counts twice; an id >= V gives NaN.
- * N, V up to 2^30, d up to 65536, k 1 .. 1024. Bounded waits as in the prefill kernels (pgb_tc_error_flag: 91-95). The same call gives
+ * N, V up to 2^30, d up to 65536, k 1 .. 1024, temperature 1e-37 .. 3e38. Bounded waits as in the prefill kernels (pgb_tc_error_flag: 91-95). The same call gives
  * the same bits.
  * ------------------------------------------------------------------------------------------------------- */
 long long pgb_head_loss_fwd_scratch_bytes(long long N, int V, int d, int dtype);

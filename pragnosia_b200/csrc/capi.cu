@@ -801,6 +801,8 @@ int pgb_linear_act(const void *x, const void *W, const void *bias, void *y, long
 namespace {
 constexpr int HEAD_MOST_K = 1024;
 constexpr long long HEAD_MOST_ROWS = 1LL << 30;
+// neither it nor log2(e) over it leaves fp32
+bool head_temperature(float tau) { return tau >= 1e-37f && tau <= 3e38f; }
 int head_sizes(long long N, int V, int d, int dtype) {
     if (dtype != PGB_F32 && dtype != PGB_BF16) return PGB_ERR_BAD_DTYPE;
     if (N < 1 || V < 1 || d < 8 || (d % 8) != 0) return PGB_ERR_BAD_SHAPE;
@@ -814,7 +816,7 @@ int head_args(HeadLossArgs &x, const void *h, const void *W, int dtype, const lo
     if (target == nullptr && (!lists || !ent || !kept)) return PGB_ERR_NULL_POINTER;
     int rc = head_sizes(N, V, d, dtype);
     if (rc != PGB_OK) return rc;
-    if (reduction < 0 || reduction > 2 || !(tau > 0.f) || tau > 3e38f || (lists && k < 1)) return PGB_ERR_BAD_SHAPE;
+    if (reduction < 0 || reduction > 2 || !head_temperature(tau) || (lists && k < 1)) return PGB_ERR_BAD_SHAPE;
     if (lists && k > HEAD_MOST_K) return PGB_ERR_TOO_LARGE;
     if (!aligned(h, 16) || !aligned(W, 16) || (target && !aligned(target, 8)) || (lists && (!aligned(lists, 8) || !aligned(marks, 16) || !aligned(ent, 4) || !aligned(kept, 4))))
         return PGB_ERR_MISALIGNED;
@@ -858,7 +860,7 @@ int pgb_linear_xent_bwd(const void *h, const void *W, int dtype, const long long
 int pgb_teacher_lists(const long long *teacher_ids, const float *teacher_logits, float temperature, int *lists, unsigned *marks, float *ent, long long N, int V, int k,
                       void *stream) {
     if (!teacher_ids || !teacher_logits || !lists || !marks || !ent) return PGB_ERR_NULL_POINTER;
-    if (N < 1 || V < 1 || k < 1 || !(temperature > 0.f) || temperature > 3e38f) return PGB_ERR_BAD_SHAPE;
+    if (N < 1 || V < 1 || k < 1 || !head_temperature(temperature)) return PGB_ERR_BAD_SHAPE;
     if (N > HEAD_MOST_ROWS || V > HEAD_MOST_ROWS || k > HEAD_MOST_K) return PGB_ERR_TOO_LARGE;
     if (!aligned(teacher_ids, 8) || !aligned(teacher_logits, 4) || !aligned(lists, 8) || !aligned(marks, 16) || !aligned(ent, 4)) return PGB_ERR_MISALIGNED;
     return head_teacher_launch(teacher_ids, teacher_logits, lists, marks, ent, N, V, k, temperature, (cudaStream_t)stream);

@@ -500,7 +500,7 @@ std::tuple<Tensor, Tensor, Tensor> teacher_lists(const Tensor &ids_, const Tenso
     same_device(DISTILL, ids_, logits_);
     TORCH_CHECK_VALUE(ids_.dim() >= 1 && ids_.sizes() == logits_.sizes(), DISTILL, ": a teacher's ids and logits share their shape, got ", ids_.sizes(), " and ",
                       logits_.sizes());
-    TORCH_CHECK_VALUE(tau > 0.0 && tau < 3e38, DISTILL, ": the temperature is positive, got ", tau);
+    TORCH_CHECK_VALUE(tau >= 1e-37 && tau <= 3e38, DISTILL, ": the temperature is positive (1e-37 to 3e38), got ", tau);
     const int64_t k = ids_.size(-1);
     TORCH_CHECK_VALUE(V >= 1 && V <= MOST_WORDS, DISTILL, ": 1 to 2^30 words, got ", V);
     TORCH_CHECK_VALUE(k >= 1 && k <= 1024, DISTILL, ": 1 to 1024 teacher entries a row, got ", k);

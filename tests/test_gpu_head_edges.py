@@ -91,6 +91,16 @@ def test_a_certain_word_loses_nothing(dtype):
     assert (loss >= 0).all() and (loss[sure] <= 2.0 ** -21).all(), (float(loss.min()), float(loss[sure].max()))
 
 
+@pytest.mark.parametrize("tau", [1e-60, 1e-40, 1e-38, -1.0, 1e300, math.inf])
+def test_temperatures_that_fp32_cannot_divide_by_are_refused(tau):
+    h, w, g = operands(6, 70, 16, BF, 3)
+    ids, logits = torch.randint(0, 70, (6, 3), device=DEV, generator=g), torch.randn(6, 3, device=DEV, generator=g)
+    for grad in (False, True):
+        h.requires_grad_(grad)
+        with pytest.raises(ValueError, match="temperature"):
+            head.linear_distill(h, w, ids, logits, temperature=tau)
+
+
 # ------------------------------------------------------------------------------------------------ the language model's loss
 def masked_batch(g, B=3, T=70, k=5, vocab=333):
     x = torch.randint(0, vocab, (B, T), device=DEV, generator=g)

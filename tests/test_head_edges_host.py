@@ -29,3 +29,11 @@ def test_a_long_axis_is_summed_in_parts_that_a_wait_covers(N, V, d):
     by_rows, shorter = N >= V, min(N, V)
     n = lib().pgb_head_loss_bwd_scratch_bytes(N, V, d, 1, int(by_rows), int(not by_rows))
     assert n >= 2 * 2 * 256 * shorter + (0 if by_rows else 2 * N * d) + 4 * (shorter // 64 // 4096) * 256 * d
+
+
+@pytest.mark.parametrize("tau", [1e-38, 1e-40, 1e-45, -1e-40])
+def test_temperatures_whose_reciprocal_is_no_number_are_refused(tau):
+    """log2(e) / temperature is what logits are multiplied with."""
+    assert distill_fwd(tau=tau) == SHAPE
+    assert lib().pgb_teacher_lists(one, one, tau, one, one, one, 4, 9, 3, None) == SHAPE
+    assert lib().pgb_linear_distill_bwd(one, one, 1, one, one, one, 4, tau, one, one, one, one, one, one, 1 << 40, 2, 4, 10, 64, None) == SHAPE
