@@ -101,6 +101,38 @@ def test_temperatures_that_fp32_cannot_divide_by_are_refused(tau):
             head.linear_distill(h, w, ids, logits, temperature=tau)
 
 
+def spread_lists(N, V, k, g, ragged):
+    """k different words a row, evenly apart from a random one on, in an order of their own; ragged: 0 .. k of them."""
+    j = torch.rand(N, k, device=DEV, generator=g).argsort(1)
+    ids = (torch.randint(0, V, (N, 1), device=DEV, generator=g) + j * (V // k)) % V
+    logits = 3.0 * torch.randn(N, k, device=DEV, generator=g)
+    if ragged:
+        ids = torch.where(torch.rand(N, k, device=DEV, generator=g) < torch.rand(N, 1, device=DEV, generator=g), ids, torch.full_like(ids, -1))
+        ids[::11] = -1
+    return ids, logits
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("N,V,d,tau", [(9000, 6200, 64, 3.5), (3000, 17000, 72, 0.7)])
+def test_distillation_in_pieces(N, V, d, tau, dtype):
+    """More logits than the workspace takes at once, pieces along the rows and along the vocabulary: every piece finds its rows' lists and its words."""
+    h, w, g = operands(N, V, d, dtype, N + V)
+    c = torch.rand(N, device=DEV, generator=g) - 0.3
+    ids, logits = spread_lists(N, V, 24, g, True)
+    p, live, _ = teacher(ids, logits, V, tau)
+    # an entry's logit / tau and the largest one are off by two roundings each (the reciprocal, the product), 2^-23 |z|, and so is what they are divided by;
+    # the rest (exponential, sum, quotient) by 2^-20
+    dp = (2.0 ** -20 + 2.0 ** -21 * float(logits.abs().max()) / tau) * p
+    s = (h.double() @ w.double().t()).abs()
+    for reduction in ("mean", "none"):
+        want, off = dense(h, w, p, live, tau, c, reduction)
+        n = max(1, int(live.sum()))
+        cs = (c.abs() if reduction == "none" else torch.full_like(c, 1.0 / n)).double()[:, None] * tau
+        e = tau * tau * ((dp * (s / tau + 20.0)).sum(1) + 2.0 ** -20 * (1 + (p * (p + 1e-300).log().abs()).sum(1)))
+        off = (off[0] + (e if reduction == "none" else e.sum() / n), off[1] + (cs * dp) @ w.double().abs(), off[2] + (cs * dp).t() @ h.double().abs())
+        within(distill(h, w, ids, logits, tau, c, reduction), want, off)
+
+
 # ------------------------------------------------------------------------------------------------ the language model's loss
 def masked_batch(g, B=3, T=70, k=5, vocab=333):
     x = torch.randint(0, vocab, (B, T), device=DEV, generator=g)
