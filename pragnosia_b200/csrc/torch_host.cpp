@@ -674,6 +674,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         return std::make_tuple(r.dq, r.dk, r.dv, r.dla, some(r.dbe), some(r.dS0));
     }, nogil);
     m.def("scan_diff", &scan_diff, nogil);
+    m.def("capture_alone", [](const std::string &what, const Tensor &leaf) { capture_alone(what.c_str(), leaf); }, nogil);
     m.def("linear_xent", &linear_xent, nogil);
     m.def("linear_xent_fwd", [](const Tensor &h, const Tensor &w, const Tensor &target, int64_t ignore, int reduction) {
         const HeadIn x = head_in(XENT, h, w);

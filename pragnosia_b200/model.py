@@ -11,7 +11,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from . import head, ops
-from ._lib import Cached, graph_capture, lib, mark_constants, sm_count, warm_up
+from ._lib import Cached, graph_capture, host, lib, mark_constants, sm_count, warm_up
 from .assoc import AssocCarrier
 from .spin import SpinCarrier
 
@@ -229,6 +229,9 @@ class LM(nn.Module):
         B, T = x.shape
         if T < 2 and torch.is_grad_enabled():
             raise ValueError("loss: a sequence of one token has no differentiable pass through the carrier layers (no_grad scores it)")
+        if not torch.compiler.is_compiling() and torch.is_grad_enabled() and x.is_cuda and torch.cuda.is_current_stream_capturing():
+            for p in self.parameters():                               # of the layers too, should the table be frozen
+                host().capture_alone("LM.loss", p)
         given = targets is not None
         if given and targets.shape != x.shape:
             raise ValueError(f"loss: a target per id, got {tuple(targets.shape)} for {tuple(x.shape)}")

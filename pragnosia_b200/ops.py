@@ -626,6 +626,10 @@ def linear_act(x, W, bias=None, act: Optional[str] = "gelu"):
     if x.dtype != torch.bfloat16 or W.dtype != torch.bfloat16:
         raise ValueError("linear_act: bf16 only")
     K, N = x.shape[-1], W.shape[0]
+    if not _compiling() and _needs_grad(x, W, bias) and torch.cuda.is_current_stream_capturing():
+        for t in (x, W, bias):
+            if t is not None:
+                host().capture_alone("linear_act", t)
     x2 = x.reshape(-1, K).contiguous()
     W = W.contiguous()
     b = None if bias is None else bias.to(x.dtype).contiguous()

@@ -197,3 +197,81 @@ def test_a_teacher_of_no_weight_is_left_out():
         assert torch.equal(m.loss(x, targets, teacher=(torch.full_like(ids, -1), logits), alpha=0.0), m.loss(x, targets))
     with pytest.raises(ValueError):
         m.loss(x, targets[0], teacher=(ids, logits), alpha=1.0)
+
+
+def test_a_captured_training_step_of_the_language_model():
+    """The layers and the three operators as one graph: a replay with other tokens, targets and lists gives what an eager step gives, to the bit."""
+    g = torch.Generator(device=DEV).manual_seed(6)
+    for mixer, dtype, d in (("aspin", BF, 128), ("dspin", BF, 128), ("fspin", F32, 72)):
+        m = lm(mixer, dtype, d=d)
+        x, targets, ids, logits = masked_batch(g)
+        params = [p for n, p in m.named_parameters() if not (".wi." in n and mixer == "dspin")]
+
+        def step():
+            loss = m.loss(x, targets, teacher=(ids, logits), temperature=2.0, alpha=0.3)
+            return [loss.detach(), *torch.autograd.grad(loss, params)]
+        side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step()
+        with torch.cuda.graph(graph, stream=side):
+            out = step()
+        for _ in range(2):
+            for a, b in zip((x, targets, ids, logits), masked_batch(g)):
+                a.copy_(b)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(out, step()))
+
+
+def test_a_capture_beside_an_eager_step_of_the_same_model_is_refused():
+    """Through the tied table, through the layers where the table is frozen, and through the fused up-projection by itself."""
+    from pragnosia_b200 import ops
+    m = lm("aspin", BF)
+    x, targets, _, _ = masked_batch(torch.Generator(device=DEV).manual_seed(7))
+    frozen = lm("aspin", BF)
+    frozen.e.weight.requires_grad_(False)
+    rows, a = torch.randn(130, 128, device=DEV).to(BF), m.mlp[0].a
+    for call in (lambda: m.loss(x, targets), lambda: frozen.loss(x, targets), lambda: ops.linear_act(rows, a.weight, a.bias)):
+        alive = call()
+        side, graph, said = torch.cuda.Stream(), torch.cuda.CUDAGraph(), []
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.graph(graph, stream=side):
+            try:
+                call()
+            except RuntimeError as e:
+                said.append(str(e))
+            with torch.no_grad():
+                seen = call()
+        assert len(said) == 1 and "still alive" in said[0]
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(seen, alive.detach()) or abs(float(seen.float().mean()) - float(alive.float().mean())) < 1e-2     # no_grad fuses the norms
+        del alive
+
+
+def test_threads():
+    """Training steps of two threads at once, each on a stream of its own."""
+    import threading
+    h, w, g = operands(700, 3000, 128, BF, 6)
+    t = torch.randint(0, 3000, (700,), device=DEV, generator=g)
+    ids, logits = torch.randint(0, 3000, (700, 9), device=DEV, generator=g), torch.randn(700, 9, device=DEV, generator=g)
+    want = [xent(h, w, t, None, "mean"), distill(h, w, ids, logits, 2.0, None, "mean")]
+    torch.cuda.synchronize()
+    got, errors = [], []
+
+    def work(kind):
+        try:
+            with torch.enable_grad(), torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    got.append((kind, xent(h, w, t, None, "mean") if kind == 0 else distill(h, w, ids, logits, 2.0, None, "mean")))
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:                                        # noqa: BLE001  (told below)
+            errors.append(e)
+    threads = [threading.Thread(target=work, args=(k,)) for k in (0, 1)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not errors and len(got) == 40
+    assert all(torch.equal(a, b) for k, o in got for a, b in zip(o, want[k]))
