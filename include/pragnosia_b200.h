@@ -538,13 +538,14 @@ int pgb_linear_act(const void *x, const void *W, const void *bias, void *y, long
  *   row_loss may be NULL; 0 / 0 where no row counts). For the backward pass: L [N][2] fp32, log2 of a row's sum of exponentials in two parts, and
  *   stats [2] fp32, the rows that count (reductions 1 and 2) and whether one that does not holds what is no number.
  *   grad: the gradient of row_loss [N] (reduction 0) or of loss (one fp32). dh [N][d], dW [V][d]: dtype; either may be NULL.
- *   scratch: 256-byte aligned, at least what the _scratch_bytes call of the same sizes says (0: bad sizes; k 0: cross entropy).
+ *   scratch: 256-byte aligned, at least what the _scratch_bytes call of the same sizes says (0: bad sizes).
  * Cross entropy: rows whose target is ignore_index lose 0 and have no gradient, whatever h holds there; any other target outside 0 .. V-1 gives NaN, as loss and as gradients of its row and of W.
  * Distillation: pgb_teacher_lists makes of a teacher's k entries per row (ids in any order; an entry with id < 0 or logit -inf is
  * absent) what the losses read: lists [N][k][2] (id, bits of its probability p at the temperature; by id), marks [N][ceil(V / 64)][4] (which of every
  * 64 words they are, and the place of the first; the forward pass alone reads it) and ent [N], the sum of p log p. lists 8-byte, marks 16-byte aligned. kept [N][k]: the entries' logits, which the forward pass
  * leaves to the backward pass. A row's loss is
  * temperature^2 KL(p || softmax(s / temperature)), 0 without gradient for rows without an entry; the same id twice counts twice; an id >= V gives NaN.
+ * marks are N V / 4 bytes, the forward pass's scratch is N V / 32 and more (fp32: split copies of h and W).
  * N, V up to 2^30, d up to 65536, k 1 .. 1024, temperature 1e-37 .. 3e38. Bounded waits as in the prefill kernels (pgb_tc_error_flag: 91-95). The same call gives
  * the same bits.
  * ------------------------------------------------------------------------------------------------------- */

@@ -12,14 +12,17 @@
 //   A row that does not count has zeros in ds, but its h may hold what is no number, and zero times that is none either. The forward pass tells
 // (such a row's sum of exponentials is no number), and the backward pass then multiplies a copy of h with zeros in those rows.
 //   ds holds no upstream scale where that is the same for every row (mean, sum): the scale is applied to the fp32 accumulators.
-//   Rounded to bf16, ds is off by 2^-9 of itself, as the gradients themselves are when they are bf16.
+//   Rounded to bf16, ds is off by at most 2^-8 of itself, as the gradients themselves are when they are bf16. Cross entropy's stay as near to 64 bits
+// as fp32 logits take them (0.0017 in the 2-norm, their own rounding); distillation's, with several large entries a row, are at 0.0023.
+//   What lies in memory beside operands and results. Forward: a tile row's maximum and sum, N V / 32 bytes, and of a teacher's lists the marks, N V / 4 (an
+// eighth of bf16 logits). Backward: two pieces of ds, a clean copy of h, fp32 sums.
 //   fp32 operands: three bf16 terms each (24 bits), six of the nine products (what is left out is below 2^-23 of the sum's terms); ds as
 //   three terms as well. The tensor cores cut off what a partial sum has beyond fp32 instead of rounding it, so sums over a long K axis
 //   drift (gradients were off by 5e-6 to 8e-6): there a block of 64 has an accumulator of its own, small products first, and the
 //   blocks are added in registers.
 // The product: pairs of SMs, 256 x 256 tiles, tcgen05.mma.cta_group::2, six 32 KiB stages a CTA fed by TMA, two accumulators in tensor
 // memory so that a tile's epilogue runs under the next one's products; 16 epilogue warps, a row and a column quarter each.
-//   What bounds it: the tensor pipe (97 % of a forward launch's cycles, 82 % of a backward one's), at the clock that the power limit leaves. 32768 rows, 8192
+//   What bounds it: the tensor pipe (97 % of a forward launch's active cycles and 91 % of its elapsed ones, 82 and 73 % of a backward one's), at the clock that the power limit leaves. 32768 rows, 8192
 // words, 768 wide, bf16: forward 292 us (1.41 PFLOP/s), backward 1.09 ms (1.13 PFLOP/s; a launch's two ends are a tenth of it); fp32, 2000 rows, 704 wide: both 502 us.
 #include <math.h>
 
@@ -38,9 +41,9 @@ static_assert(HL_STAGE % 1024 == 0 && HL_SMEM <= 232448, "shared memory");
 constexpr float LOG2E_F = 1.4426950408889634f;
 
 struct HlMaps { CUtensorMap a[3], b[3], ds, clean; };                 // of the products; ds: the piece of it that is written; clean: b[1] where *dirty is set
-// An epilogue warp's share of a tile: rows row0 .. +31 (a lane each), columns col0 .. +63; block: which of the tile's 32 it is. g, t, sp: the
-// product, its tile, and the part of K that the accumulator holds.
-struct HlTile { int lane, sub, part, block, n, row0, col0, g, t, sp; uint32_t ti; };
+// An epilogue warp's share of a tile: rows row0 .. +31 (a lane each), columns col0 .. +63. g, sp: the product and the part of K that the accumulator
+// holds; ti: how many tiles came before.
+struct HlTile { int lane, sub, part, n, row0, col0, g, sp; uint32_t ti; };
 // One product C[M][N] = A B^T over kb blocks of 64, its K axis in `splits` parts.
 // a_mn / b_mn: the operand lies with its M / N axis contiguous instead of K.
 struct HlProduct {
@@ -237,7 +240,7 @@ __device__ __forceinline__ void hl_body(const HlMaps &maps, const What &what, Ep
         uint8_t *stage = sm + HL_STAGES * HL_STAGE + 1024 + (warp - 2) * HL_OUT_BYTES, *shared = sm + HL_STAGES * HL_STAGE + 1024;
         const int row_in = (int)rank * (HL_B / 2) + 32 * sub, col_in = part * HL_CW;
         HlTile x;
-        x.lane = lane; x.sub = sub; x.part = part; x.block = (int)rank * HL_EPI + (warp - 2);
+        x.lane = lane; x.sub = sub; x.part = part;
         epi.start(tid - 64);
         uint32_t ti = 0, ai = 0;
         bool ok = w.more();
@@ -247,7 +250,7 @@ __device__ __forceinline__ void hl_body(const HlMaps &maps, const What &what, Ep
         }
         for (; ok; ++ti) {
             x.n = n; x.row0 = m * HL_B + row_in; x.col0 = n * HL_B + col_in; x.ti = ti;
-            x.g = w.g; x.t = w.t; x.sp = w.sp;
+            x.g = w.g; x.sp = w.sp;
             epi.begin(x);
             float v[2][32];
             const uint32_t tacc = tmem + lane_base + part * HL_CW;
@@ -537,7 +540,8 @@ __global__ void __launch_bounds__(256) head_loss_join_kernel(const HlJoin j) {
 
 // ------------------------------------------------------------------------------------------------ a teacher's lists
 // A warp per row: probabilities of the entries that are there (id >= 0, logit not -inf) at the temperature, in ascending order of their
-// ids (a rank per entry: k comparisons each), an id that comes again added to the first, and the marks.
+// ids (a rank per entry: k comparisons each), an id that comes again added to the first, and the marks. 4096 rows, 8192 words: 10 us at k 64, 60 at 256, 795 at
+// 1024, where the k^2 comparisons a row are all of it.
 __global__ void __launch_bounds__(128) head_teacher_kernel(const long long *__restrict__ in_ids, const float *__restrict__ in_logits, int2 *__restrict__ lists,
                                                            uint4 *__restrict__ marks, float *__restrict__ ent, long long N, int V, int k, float inv_tau) {
     extern __shared__ __align__(16) int teacher_smem[];

@@ -50,7 +50,11 @@ def linear_distill(h, weight, teacher_ids, teacher_logits, *, temperature: float
 
     h, weight as in linear_cross_entropy; teacher_ids (..., k) int64 or int32, teacher_logits (..., k), k in 1 .. 1024, in any order.
     An entry with id < 0 or logit -inf is absent, so lists may differ in length; a row without any loses 0, has no gradient and
-    does not count in the mean. An id twice counts twice; an id >= V gives nan. No gradient goes to the teacher."""
+    does not count in the mean (nan where all are without). An id twice counts twice; an id >= V gives nan. No gradient goes to the teacher.
+
+    bf16: the gradient of the logits, which has several large entries a row here, is rounded to bf16 on its way into the two products behind it, beside
+    the gradients' own rounding (2-norm against 64 bits: 0.0023, where fp32 logits give 0.0017). Beside the results the call takes V / 4 bytes a row
+    while it runs and keeps 12 k + 16 for the gradient. Sorting lists takes k^2: 4096 of 64 entries 10 us, of 256 60, of 1024 795."""
     r = _reduction(reduction)
     if not torch.compiler.is_compiling():
         out = host().linear_distill(h, weight, teacher_ids, teacher_logits, float(temperature), r)
