@@ -93,9 +93,10 @@ def _levels(w, group, zeros):
     f = torch.nn.functional.pad(w.float(), (0, G * group - K)).view(N, G, group)      # zeros change no group's range
     if zeros:
         lo = f.amin(2).clamp_max(0.0)
-        s = ((f.amax(2).clamp_min(0.0) - lo) / 15.0).to(w.dtype)
+        top = f.amax(2).clamp_min(0.0) - lo
     else:
-        s = (f.abs().amax(2) / 7.0).to(w.dtype)
+        top = f.abs().amax(2)
+    s = (top / torch.full_like(top, 15.0 if zeros else 7.0)).to(w.dtype)              # by a tensor: by a number torch multiplies with its reciprocal
     t = s.float()
     safe = torch.where(t > 0, t, torch.ones_like(t))
     z = torch.round(-lo / safe).clamp(0, 15) if zeros else torch.full_like(t, 8.0)
