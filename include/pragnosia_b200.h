@@ -578,6 +578,47 @@ long long pgb_embedding_bwd_scratch_bytes(long long N, int V, int d);
 int pgb_embedding_bwd(const long long *ids, const void *grad, int dtype, float scale, long long padding_idx, void *dW, void *scratch,
                       long long scratch_bytes, long long N, int V, int d, void *stream);
 
+/* ---------------------------------------------------------------------------------------------------------
+ * Weights in four bits with a scale per group, and the linear layer that reads them. No counterpart in the reference.
+ *   A weight (N, K), K a multiple of 32: q [N][K / 2] (the even column in the low half of a byte), scales [N][G] (scale_dtype) and zeros [N][G]
+ *   (0 .. 127; NULL: 8 everywhere), G = ceil(K / group), group 32, 64 or 128 columns (the last of a row may be shorter). It stands for
+ *   scale (q - zero).
+ * quantize: with zeros, lo = min(0, min w), hi = max(0, max w), scale = (hi - lo) / 15, zero = clamp(rint(-lo / scale), 0, 15); without,
+ *   scale = max|w| / 7, zero 8; q = clamp(rint(w / scale) + zero, 0, 15). scale has w's type and is rounded before it is used; 0 gives q = zero. A group
+ *   that holds an infinity or NaN, or whose range leaves fp32, gets a scale of NaN.
+ * linear: y [M][N] = act(x W^T + bias), x [M][K] and bias [N] (or NULL) of x_dtype, y of out_dtype, act 0 none, 1 erf-GELU.
+ *   Sums in fp32, one rounding at the end. The weight enters as scale times a whole number sum, unrounded -- but for bf16 x and y with more than
+ *   PGB_INT4_ROWS rows, where scale (q - zero) is rounded to bf16 for the tensor cores. flags: PGB_INT4_CONSTANT = q, scales, zeros and bias were
+ *   complete before the kernel ahead on the stream was launched, and may be read while it runs. Bounded waits as in the prefill
+ *   kernels (pgb_tc_error_flag: 61-69).
+ * x, q, w, y 16-byte aligned, scales, zeros, bias to their element. N, K up to 2^24, M below 2^31. The same call gives the same bits.
+ * ------------------------------------------------------------------------------------------------------- */
+enum { PGB_INT4_CONSTANT = 1, PGB_INT4_ROWS = 16 };
+int pgb_int4_quantize(const void *w, int dtype, unsigned char *q, void *scales, unsigned char *zeros, int N, int K, int group, void *stream);
+int pgb_int4_dequantize(const unsigned char *q, const void *scales, int scale_dtype, const unsigned char *zeros, void *w, int dtype, int N,
+                        int K, int group, void *stream);
+int pgb_int4_linear(const void *x, int x_dtype, const unsigned char *q, const void *scales, int scale_dtype, const unsigned char *zeros,
+                    const void *bias, int act, void *y, int out_dtype, long long M, int N, int K, int group, int flags, void *stream);
+
+/* ---------------------------------------------------------------------------------------------------------
+ * Penalties, biases and masks on logits ahead of a draw. No counterpart in the reference. For word v of row b, n times among the generated ids and
+ * m times among those and the prompt's:
+ *   s = l;  m > 0: s = s > 0 ? s / repetition : s repetition;  n > 0: s -= frequency n + presence;  s += its biases;  not allowed: s = -inf
+ *   logits [B] rows of V (dtype; row stride in elements), out [B][V] fp32, dense (may be logits itself, dense and fp32).
+ *   prompt, generated: int64 ids, n a row with a row stride (0: one row for all); lengths int64, how many of them count (clamped to 0 .. n), one per
+ *   row (length_stride 1) or one for all (0); NULL: all. Ids outside 0 .. V-1 count nowhere. n 0: none (NULL).
+ *   repetition, frequency, presence: fp32 [B], or NULL and the value given. bias_ids int64, bias fp32 [nb] a row (bias_stride 0: one row for all), nb up
+ *   to 1024; an id twice counts twice. mask: mask_kind 0 none, 1 bits (32-bit words, bit v mod 32 of word v / 32, set: allowed), 2 bytes (non-zero: allowed);
+ *   mask_stride in words or bytes, 0: one row for all.
+ * V up to 2^30. The same call gives the same bits.
+ * ------------------------------------------------------------------------------------------------------- */
+int pgb_adjust_logits(const void *logits, int dtype, long long row_stride, float *out, const long long *prompt, long long prompt_stride, int prompt_n,
+                      const long long *prompt_lengths, int prompt_length_stride, const long long *generated, long long generated_stride,
+                      int generated_n, const long long *generated_lengths, int generated_length_stride, const float *repetition_rows,
+                      float repetition, const float *frequency_rows, float frequency, const float *presence_rows, float presence,
+                      const long long *bias_ids, const float *bias, long long bias_stride, int nb, const void *mask, int mask_kind,
+                      long long mask_stride, long long B, int V, void *stream);
+
 /* Which kernel pgb_linear_act uses. Bit 0: 0 (default) = one CTA per 128-row tile; 1 = pairs of SMs share one 256-row tile
  * (tcgen05.mma.cta_group::2: each CTA of a two-CTA cluster loads half of either operand, no multicast) whenever the
  * problem has more than 128 rows. Bits 1-2: the tile's width, 0 or 1 = 256 columns (default), 2 = 192. variant in 0..5.

@@ -93,6 +93,11 @@ SIGNATURES = {
     "pgb_embedding_fwd": [_vp, _vp, _i, _f, _vp, _ll, _i, _i, _vp],
     "pgb_embedding_bwd_scratch_bytes": [_ll, _i, _i],
     "pgb_embedding_bwd": [_vp, _vp, _i, _f, _ll, _vp, _vp, _ll, _ll, _i, _i, _vp],
+    "pgb_int4_quantize": [_vp, _i, _vp, _vp, _vp, _i, _i, _i, _vp],
+    "pgb_int4_dequantize": [_vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _vp],
+    "pgb_int4_linear": [_vp, _i, _vp, _vp, _i, _vp, _vp, _i, _vp, _i, _ll, _i, _i, _i, _i, _vp],
+    "pgb_adjust_logits": [_vp, _i, _ll, _vp, _vp, _ll, _i, _vp, _i, _vp, _ll, _i, _vp, _i, _vp, _f, _vp, _f, _vp, _f, _vp, _vp, _ll, _i, _vp, _i, _ll,
+                          _ll, _i, _vp],
     "pgb_skinny_linear": [_vp, _vp, _vp, _vp, _i, _f, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _vp],
     "pgb_tc_error_flag": [_vp],
     "pgb_tc_set_variant": [_i],

@@ -119,6 +119,10 @@ int batch_linear_launch(const void *, const void *, const void *, void *, int, i
 int batch_linear_parts(int N);
 int batch_linear_error_flag(int *);
 int decode_token_wait_selftest_launch(unsigned long long *, unsigned, cudaStream_t);
+int int4_quantize_launch(const void *, int, unsigned char *, void *, unsigned char *, int, int, int, cudaStream_t);
+int int4_dequantize_launch(const Int4Weight &, void *, int, cudaStream_t);
+int int4_linear_launch(const Int4Linear &, cudaStream_t);
+int adjust_logits_launch(const AdjustLogits &, cudaStream_t);
 
 // PGB_PREFILL_AUTO sends bf16 plain-rule work to the tensor-core kernel only once this is on
 static const bool kAutoUsesTensor = true;
@@ -906,6 +910,86 @@ int pgb_embedding_bwd(const long long *ids, const void *grad, int dtype, float s
     if (!aligned(ids, 8) || !aligned(grad, e) || !aligned(dW, e) || !aligned(scratch, 16)) return PGB_ERR_MISALIGNED;
     if (scratch_bytes < bytes) return PGB_ERR_BAD_SHAPE;
     return embedding_bwd_launch(ids, grad, dtype, scale, padding_idx, dW, scratch, N, V, d, (cudaStream_t)stream);
+}
+
+// ---- weights in four bits
+namespace {
+bool io_dtype(int t) { return t == PGB_F32 || t == PGB_BF16; }
+bool aligned_to(const void *p, int dtype) { return aligned(p, dtype == PGB_F32 ? 4 : 2); }
+int int4_sizes(int N, int K, int group) {
+    if (N < 1 || K < 32 || (K % 32) != 0 || (group != 32 && group != 64 && group != 128)) return PGB_ERR_BAD_SHAPE;
+    return N > (1 << 24) || K > (1 << 24) || (long long)N * K > (1LL << 38) ? PGB_ERR_TOO_LARGE : PGB_OK;
+}
+int int4_weight(Int4Weight &w, const unsigned char *q, const void *scales, int scale_dtype, const unsigned char *zeros, int N, int K, int group) {
+    if (!q || !scales) return PGB_ERR_NULL_POINTER;
+    if (!io_dtype(scale_dtype)) return PGB_ERR_BAD_DTYPE;
+    const int rc = int4_sizes(N, K, group);
+    if (rc != PGB_OK) return rc;
+    if (!aligned(q, 16) || !aligned_to(scales, scale_dtype)) return PGB_ERR_MISALIGNED;
+    w = {q, scales, scale_dtype, zeros, N, K, group, (K + group - 1) / group};
+    return PGB_OK;
+}
+}  // namespace
+
+int pgb_int4_quantize(const void *w, int dtype, unsigned char *q, void *scales, unsigned char *zeros, int N, int K, int group, void *stream) {
+    Int4Weight out;
+    if (!w) return PGB_ERR_NULL_POINTER;
+    const int rc = int4_weight(out, q, scales, dtype, zeros, N, K, group);
+    if (rc != PGB_OK) return rc;
+    if (!aligned(w, 16)) return PGB_ERR_MISALIGNED;
+    return int4_quantize_launch(w, dtype, q, scales, zeros, N, K, group, (cudaStream_t)stream);
+}
+
+int pgb_int4_dequantize(const unsigned char *q, const void *scales, int scale_dtype, const unsigned char *zeros, void *w, int dtype, int N, int K,
+                        int group, void *stream) {
+    Int4Weight in;
+    if (!w) return PGB_ERR_NULL_POINTER;
+    if (!io_dtype(dtype)) return PGB_ERR_BAD_DTYPE;
+    const int rc = int4_weight(in, q, scales, scale_dtype, zeros, N, K, group);
+    if (rc != PGB_OK) return rc;
+    if (!aligned(w, 16)) return PGB_ERR_MISALIGNED;
+    return int4_dequantize_launch(in, w, dtype, (cudaStream_t)stream);
+}
+
+int pgb_int4_linear(const void *x, int x_dtype, const unsigned char *q, const void *scales, int scale_dtype, const unsigned char *zeros, const void *bias,
+                    int act, void *y, int out_dtype, long long M, int N, int K, int group, int flags, void *stream) {
+    Int4Linear a;
+    if (!x || !y) return PGB_ERR_NULL_POINTER;
+    if (!io_dtype(x_dtype) || !io_dtype(out_dtype)) return PGB_ERR_BAD_DTYPE;
+    const int rc = int4_weight(a.w, q, scales, scale_dtype, zeros, N, K, group);
+    if (rc != PGB_OK) return rc;
+    if (M < 1 || act < 0 || act > 1 || (flags & ~PGB_INT4_CONSTANT)) return PGB_ERR_BAD_SHAPE;
+    if (M > 0x7fffffffLL) return PGB_ERR_TOO_LARGE;
+    if (!aligned(x, 16) || !aligned(y, 16) || (bias && !aligned_to(bias, x_dtype))) return PGB_ERR_MISALIGNED;
+    a.x = x; a.x_dtype = x_dtype; a.bias = bias; a.act = act; a.y = y; a.out_dtype = out_dtype; a.M = M; a.constant = flags & PGB_INT4_CONSTANT;
+    return int4_linear_launch(a, (cudaStream_t)stream);
+}
+
+// ---- logits ahead of a draw
+int pgb_adjust_logits(const void *logits, int dtype, long long row_stride, float *out, const long long *prompt, long long prompt_stride, int prompt_n,
+                      const long long *prompt_lengths, int prompt_length_stride, const long long *generated, long long generated_stride, int generated_n,
+                      const long long *generated_lengths, int generated_length_stride, const float *repetition_rows, float repetition,
+                      const float *frequency_rows, float frequency, const float *presence_rows, float presence, const long long *bias_ids, const float *bias,
+                      long long bias_stride, int nb, const void *mask, int mask_kind, long long mask_stride, long long B, int V, void *stream) {
+    if (!logits || !out || (prompt_n > 0 && !prompt) || (generated_n > 0 && !generated) || (nb > 0 && (!bias_ids || !bias)) || (mask_kind != 0 && !mask))
+        return PGB_ERR_NULL_POINTER;
+    if (!io_dtype(dtype)) return PGB_ERR_BAD_DTYPE;
+    if (B < 1 || V < 1 || prompt_n < 0 || generated_n < 0 || nb < 0 || mask_kind < 0 || mask_kind > 2 || (prompt_length_stride & ~1) ||
+        (generated_length_stride & ~1) || (!repetition_rows && !(repetition > 0.f)))
+        return PGB_ERR_BAD_SHAPE;
+    if (nb > 1024 || V > (1 << 30) || B > (1LL << 31) / ((V + 2047) / 2048) - 1) return PGB_ERR_TOO_LARGE;
+    if (!aligned_to(logits, dtype) || !aligned(out, 4) || !aligned(prompt, 8) || !aligned(generated, 8) || !aligned(prompt_lengths, 8) ||
+        !aligned(generated_lengths, 8) || !aligned(repetition_rows, 4) || !aligned(frequency_rows, 4) || !aligned(presence_rows, 4) || !aligned(bias_ids, 8) ||
+        !aligned(bias, 4) || (mask_kind == 1 && !aligned(mask, 4)))
+        return PGB_ERR_MISALIGNED;
+    // the rows overlap what is written unless they are the same rows
+    if (logits == (const void *)out && (dtype != PGB_F32 || (row_stride != V && B > 1))) return PGB_ERR_BAD_SHAPE;
+    const AdjustLogits a = {logits, dtype, row_stride, out, B, V,
+                            {prompt, prompt_stride, prompt_n, prompt_lengths, prompt_length_stride},
+                            {generated, generated_stride, generated_n, generated_lengths, generated_length_stride},
+                            {repetition_rows, repetition}, {frequency_rows, frequency}, {presence_rows, presence},
+                            bias_ids, bias, bias_stride, nb, mask, mask_kind, mask_stride};
+    return adjust_logits_launch(a, (cudaStream_t)stream);
 }
 
 int pgb_linear_act_set_variant(int variant) { return linear_gelu_set_variant(variant); }

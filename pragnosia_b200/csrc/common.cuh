@@ -127,6 +127,18 @@ struct HeadLossArgs {
     const void *h, *W; int dtype; const long long *target; long long ignore; const int *lists; const unsigned *marks; const float *ent; float *kept; int k;
     float tau; int reduction; long long N; int V, d;
 };
+// a weight in four bits (int4.cu): q [N][K/2], scales [N][G] in bf16 or fp32, zeros [N][G] or NULL (8); a linear layer of it
+struct Int4Weight { const unsigned char *q; const void *scales; int scale_dtype; const unsigned char *zeros; int N, K, group, G; };
+struct Int4Linear { const void *x; int x_dtype; Int4Weight w; const void *bias; int act; void *y; int out_dtype; long long M; int constant; };
+// what is done to logits ahead of a draw (adjust_logits.cu): ids [rows][n] with a row stride (0: one row for all) and lengths (NULL: all n; stride 0 or 1)
+struct TokenList { const long long *ids; long long stride; int n; const long long *lengths; int length_stride; };
+struct RowValue { const float *at; float all; };                      // one per row, or one for all (at NULL)
+struct AdjustLogits {
+    const void *logits; int dtype; long long stride; float *out; long long B; int V;
+    TokenList prompt, made; RowValue repetition, frequency, presence;
+    const long long *bias_ids; const float *bias; long long bias_stride; int nb;
+    const void *mask; int mask_kind; long long mask_stride;           // 0 none, 1 a bit a word (stride in 32-bit words), 2 a byte a word; stride 0: one row for all
+};
 struct DecodeArgs {
     const void *qp, *kp, *vp; long long in_sb; int normalize;
     const void *gate; long long gate_sb; int gate_is_logit;

@@ -645,6 +645,173 @@ OptTensor embedding(const Tensor &ids, const Tensor &w, double scale, int64_t pa
     }
     return embed_fwd(ids, w, scale);
 }
+
+// ------------------------------------------------------------------------------------------------ weights in four bits
+const char *const INT4 = "int4", *const ADJUST = "adjust_logits";
+void no_gradient(const char *what, const Tensor &t) {
+    if (at::GradMode::is_enabled() && wants_grad(t))
+        throw std::runtime_error(std::string(what) + " has no gradient: call it under torch.no_grad(), or detach what it is given");
+}
+int64_t int4_groups(int64_t K, int64_t group) {
+    TORCH_CHECK_VALUE(group == 32 || group == 64 || group == 128, INT4, ": a group is 32, 64 or 128 columns, got ", group);
+    return (K + group - 1) / group;
+}
+// w (N, K) -> q (N, K / 2), scales (N, G), zeros (N, G) or nothing
+std::tuple<Tensor, Tensor, OptTensor> int4_quantize(const Tensor &w_, int64_t group, bool symmetric) {
+    need_cuda(w_);
+    no_gradient("int4.quantize", w_);
+    TORCH_CHECK_TYPE(io_type(w_.scalar_type()), INT4, ": the weight is float32 or bfloat16, got ", w_.scalar_type());
+    TORCH_CHECK_VALUE(w_.dim() == 2 && w_.size(0) >= 1 && w_.size(1) >= 32 && w_.size(1) % 32 == 0, INT4, ": the weight is (N, K), K a multiple of 32, got ", w_.sizes());
+    const int64_t N = w_.size(0), K = w_.size(1), G = int4_groups(K, group);
+    OnDevice dev(w_);
+    const Tensor w = head_operand(w_), q = alloc(w, {N, K / 2}, at::kByte), s = alloc(w, {N, G}, w.scalar_type());
+    const Tensor z = symmetric ? Tensor() : alloc(w, {N, G}, at::kByte);
+    check(pgb_int4_quantize(vp(w), code(w), static_cast<unsigned char *>(vp(q)), vp(s), static_cast<unsigned char *>(vp(z)), N, K, group, dev.stream), "pgb_int4_quantize");
+    return {q, s, some(z)};
+}
+struct Int4In { Tensor q, s, z; int64_t N, K; };
+Int4In int4_in(const Tensor &q, const Tensor &s, const OptTensor &z_, int64_t group) {
+    const Tensor z = opt(z_);
+    need_cuda(q, s, z);
+    same_device(INT4, q, s);
+    TORCH_CHECK_TYPE(q.scalar_type() == at::kByte && io_type(s.scalar_type()) && (!z.defined() || z.scalar_type() == at::kByte), INT4,
+                     ": q and zeros are uint8, scales float32 or bfloat16, got ", q.scalar_type(), ", ", z.defined() ? z.scalar_type() : at::kByte, ", ", s.scalar_type());
+    TORCH_CHECK_VALUE(q.dim() == 2 && q.size(0) >= 1 && q.size(1) >= 16 && q.size(1) % 16 == 0, INT4, ": q is (N, K / 2), K a multiple of 32, got ", q.sizes());
+    const int64_t N = q.size(0), K = 2 * q.size(1), G = int4_groups(K, group);
+    TORCH_CHECK_VALUE(s.dim() == 2 && s.size(0) == N && s.size(1) == G, INT4, ": a scale per row and group of ", group, ", (", N, ", ", G, "), got ", s.sizes());
+    if (z.defined()) {
+        same_device(INT4, q, z);
+        TORCH_CHECK_VALUE(z.sizes() == s.sizes(), INT4, ": a zero per scale, got ", z.sizes(), " for ", s.sizes());
+    }
+    return {head_operand(q), s.contiguous(), z.defined() ? z.contiguous() : z, N, K};
+}
+unsigned char *u8(const Tensor &t) { return static_cast<unsigned char *>(vp(t)); }
+Tensor int4_dequantize(const Tensor &q, const Tensor &s, const OptTensor &z, int64_t group, bool bf16) {
+    const Int4In w = int4_in(q, s, z, group);
+    OnDevice dev(w.q);
+    const Tensor out = alloc(w.q, {w.N, w.K}, bf16 ? at::kBFloat16 : at::kFloat);
+    check(pgb_int4_dequantize(u8(w.q), vp(w.s), code(w.s), u8(w.z), vp(out), code(out), w.N, w.K, group, dev.stream), "pgb_int4_dequantize");
+    return out;
+}
+Tensor int4_linear_fwd(const Tensor &x_, const Tensor &q, const Tensor &s, const OptTensor &z, int64_t group, const OptTensor &bias_, int act, bool bf16, bool constant) {
+    const Tensor bias = opt(bias_);
+    need_cuda(x_, q, bias);
+    no_gradient("int4.linear", x_);
+    no_gradient("int4.linear", bias);
+    const Int4In w = int4_in(q, s, z, group);
+    same_device(INT4, x_, q);
+    TORCH_CHECK_TYPE(io_type(x_.scalar_type()), INT4, ": x is float32 or bfloat16, got ", x_.scalar_type());
+    TORCH_CHECK_VALUE(x_.dim() >= 1 && x_.size(-1) == w.K, INT4, ": x is (..., K) for a weight of K = ", w.K, ", got ", x_.sizes());
+    if (bias.defined()) {
+        same_device(INT4, x_, bias);
+        TORCH_CHECK_VALUE(bias.dim() == 1 && bias.size(0) == w.N, INT4, ": a bias of (", w.N, "), got ", bias.sizes());
+    }
+    OnDevice dev(x_);
+    const Tensor x = head_operand(x_), b = bias.defined() ? like(bias, x.scalar_type()) : bias;
+    if (constant && b.defined() && b.data_ptr() != bias.data_ptr()) constant = false;         // made by a kernel just now
+    std::vector<int64_t> shape = x_.sizes().vec();
+    shape.back() = w.N;
+    const Tensor y = alloc(x, shape, bf16 ? at::kBFloat16 : at::kFloat);
+    const int64_t M = x.numel() / w.K;
+    if (M > 0)
+        check(pgb_int4_linear(vp(x), code(x), u8(w.q), vp(w.s), code(w.s), u8(w.z), vp(b), act, vp(y), code(y), M, w.N, w.K, group, constant ? PGB_INT4_CONSTANT : 0,
+                              dev.stream), "pgb_int4_linear");
+    return y;
+}
+OptTensor int4_linear(const Tensor &x, const Tensor &q, const Tensor &s, const OptTensor &z, int64_t group, const OptTensor &bias, int act, bool bf16, bool constant) {
+    if (!plain(x, q, s)) return std::nullopt;
+    return int4_linear_fwd(x, q, s, z, group, bias, act, bf16, constant);
+}
+
+// ------------------------------------------------------------------------------------------------ logits ahead of a draw
+// rows of ids or of a mask, one of each row of the logits or one for all: unit stride along a row
+struct Rows { Tensor t; long long stride; int64_t n; };
+Rows rows_of(const char *name, const Tensor &t, const Tensor &logits, int64_t B) {
+    same_device(ADJUST, logits, t);
+    TORCH_CHECK_VALUE(t.dim() == 2 && (t.size(0) == B || t.size(0) == 1) && t.size(1) <= MOST_WORDS, ADJUST, ": ", name, " is (", B, " or 1, n), got ", t.sizes());
+    const Tensor u = t.size(1) > 1 && t.stride(1) != 1 ? t.contiguous() : t;
+    return {u, u.size(0) == 1 ? 0 : u.stride(0), u.size(1)};
+}
+struct IdList { Rows ids; Tensor lengths; int stride; };
+IdList id_list(const char *name, const OptTensor &ids, const OptTensor &lengths, const Tensor &logits, int64_t B) {
+    IdList r{{Tensor(), 0, 0}, Tensor(), 0};
+    TORCH_CHECK_VALUE(ids || !lengths, ADJUST, ": lengths of ", name, " without its ids");
+    if (!ids) return r;
+    r.ids = rows_of(name, *ids, logits, B);
+    if (r.ids.t.scalar_type() != at::kLong) {
+        r.ids.t = whole_numbers(ADJUST, r.ids.t);
+        r.ids.stride = r.ids.t.size(0) == 1 ? 0 : r.ids.n;
+    }
+    if (lengths) {
+        same_device(ADJUST, logits, *lengths);
+        TORCH_CHECK_VALUE(lengths->numel() == 1 || (lengths->dim() == 1 && lengths->size(0) == B), ADJUST, ": a length of ", name, " per row, or one for all, got ", lengths->sizes());
+        r.lengths = whole_numbers(ADJUST, *lengths);
+        r.stride = lengths->numel() == 1 ? 0 : 1;
+    }
+    return r;
+}
+Tensor row_values(const char *name, const OptTensor &t, const Tensor &logits, int64_t B) {
+    if (!t) return Tensor();
+    same_device(ADJUST, logits, *t);
+    TORCH_CHECK_VALUE(t->dim() == 1 && t->size(0) == B && t->is_floating_point(), ADJUST, ": ", name, " is a number or a floating tensor of (", B, "), got ", t->scalar_type(), " ", t->sizes());
+    return f32c(*t);
+}
+Tensor adjust_fwd(const Tensor &l_, const OptTensor &prompt, const OptTensor &prompt_n, const OptTensor &made, const OptTensor &made_n, const OptTensor &rep_t,
+                  double rep, const OptTensor &freq_t, double freq, const OptTensor &pres_t, double pres, const OptTensor &bias_ids, const OptTensor &bias_,
+                  const OptTensor &mask_, const OptTensor &out_) {
+    need_cuda(l_, opt(prompt), opt(prompt_n), opt(made), opt(made_n), opt(rep_t), opt(freq_t), opt(pres_t), opt(bias_ids), opt(bias_), opt(mask_), opt(out_));
+    no_gradient(ADJUST, l_);
+    TORCH_CHECK_TYPE(io_type(l_.scalar_type()), ADJUST, ": logits are float32 or bfloat16, got ", l_.scalar_type());
+    TORCH_CHECK_VALUE(l_.dim() == 2 && l_.size(1) >= 1 && l_.size(1) <= MOST_WORDS, ADJUST, ": logits are (B, V), got ", l_.sizes());
+    const int64_t B = l_.size(0), V = l_.size(1);
+    OnDevice dev(l_);
+    const IdList p = id_list("prompt", prompt, prompt_n, l_, B), g = id_list("generated", made, made_n, l_, B);
+    TORCH_CHECK_VALUE(rep_t || rep > 0, ADJUST, ": repetition is above 0, got ", rep);
+    const Tensor rt = row_values("repetition", rep_t, l_, B), ft = row_values("frequency", freq_t, l_, B), pt = row_values("presence", pres_t, l_, B);
+    TORCH_CHECK_VALUE(bias_ids.has_value() == bias_.has_value(), ADJUST, ": bias_ids and bias come together");
+    Rows bi{Tensor(), 0, 0};
+    Tensor bv;
+    if (bias_) {
+        bi = rows_of("bias_ids", *bias_ids, l_, B);
+        TORCH_CHECK_VALUE(bias_->sizes() == bias_ids->sizes() && bi.n <= 1024 && bias_->is_floating_point(), ADJUST, ": a floating bias per id, up to 1024 a row, got ", bias_->sizes(), " for ",
+                          bias_ids->sizes());
+        same_device(ADJUST, l_, *bias_);
+        bi.t = whole_numbers(ADJUST, bi.t);                           // one stride for both
+        bv = f32c(*bias_);
+        bi.stride = bi.t.size(0) == 1 ? 0 : bi.n;
+    }
+    Rows m{Tensor(), 0, 0};
+    int kind = 0;
+    if (mask_) {
+        kind = mask_->scalar_type() == at::kInt ? 1 : 2;
+        TORCH_CHECK_TYPE(kind == 1 || mask_->scalar_type() == at::kBool, ADJUST, ": the mask is int32 (32 words a number) or bool, got ", mask_->scalar_type());
+        m = rows_of("mask", *mask_, l_, B);
+        TORCH_CHECK_VALUE(m.n == (kind == 1 ? (V + 31) / 32 : V), ADJUST, ": the mask covers V = ", V, " words, got ", mask_->sizes());
+    }
+    Tensor out = opt(out_);
+    if (out.defined()) {
+        same_device(ADJUST, l_, out);
+        TORCH_CHECK_VALUE(out.scalar_type() == at::kFloat && out.is_contiguous() && out.sizes() == l_.sizes() && !wants_grad(out), ADJUST,
+                          ": out is a dense float32 tensor of the logits' shape");
+    }
+    // dense rows as they lie; a row stride of their own only where it does not overlap what is written
+    const bool strided = l_.stride(1) == 1 || V == 1;
+    Tensor l = strided ? l_ : l_.contiguous();
+    if (out.defined() && l.data_ptr() == out.data_ptr() && !(l.scalar_type() == at::kFloat && l.is_contiguous())) l = l.clone();
+    if (!out.defined()) out = alloc(l, {B, V}, at::kFloat);
+    if (B == 0) return out;
+    const auto ll = [](const Tensor &t) { return static_cast<const long long *>(vp(t)); };
+    check(pgb_adjust_logits(vp(l), code(l), l.stride(0), fp(out), ll(p.ids.t), p.ids.stride, p.ids.n, ll(p.lengths), p.stride, ll(g.ids.t), g.ids.stride, g.ids.n,
+                            ll(g.lengths), g.stride, fp(rt), rep, fp(ft), freq, fp(pt), pres, ll(bi.t), fp(bv), bi.stride, bi.n, vp(m.t), kind, m.stride, B, V, dev.stream),
+          "pgb_adjust_logits");
+    return out;
+}
+OptTensor adjust_logits(const Tensor &l, const OptTensor &prompt, const OptTensor &prompt_n, const OptTensor &made, const OptTensor &made_n, const OptTensor &rep_t,
+                        double rep, const OptTensor &freq_t, double freq, const OptTensor &pres_t, double pres, const OptTensor &bias_ids, const OptTensor &bias,
+                        const OptTensor &mask, const OptTensor &out) {
+    if (!plain(l, opt(prompt), opt(made), opt(mask))) return std::nullopt;
+    return adjust_fwd(l, prompt, prompt_n, made, made_n, rep_t, rep, freq_t, freq, pres_t, pres, bias_ids, bias, mask, out);
+}
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -710,4 +877,18 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("embedding", &embedding, nogil);
     m.def("embedding_fwd", &embed_fwd, nogil);
     m.def("embedding_bwd", &embed_bwd, nogil);
+    m.def("int4_quantize", [](const Tensor &w, int64_t group, bool symmetric) -> std::optional<std::tuple<Tensor, Tensor, OptTensor>> {
+        if (!plain(w)) return std::nullopt;
+        return int4_quantize(w, group, symmetric);
+    }, nogil);
+    m.def("int4_quantize_fwd", &int4_quantize, nogil);
+    m.def("int4_dequantize", [](const Tensor &q, const Tensor &s, const OptTensor &z, int64_t group, bool bf16) -> OptTensor {
+        if (!plain(q, s)) return std::nullopt;
+        return int4_dequantize(q, s, z, group, bf16);
+    }, nogil);
+    m.def("int4_dequantize_fwd", &int4_dequantize, nogil);
+    m.def("int4_linear", &int4_linear, nogil);
+    m.def("int4_linear_fwd", &int4_linear_fwd, nogil);
+    m.def("adjust_logits", &adjust_logits, nogil);
+    m.def("adjust_logits_fwd", &adjust_fwd, nogil);
 }

@@ -591,3 +591,50 @@ def _embed_grads(ctx, g):
 
 
 embedding.register_autograd(_embed_grads, setup_context=_embed_ctx)
+
+
+@torch.library.custom_op(f"{NS}::int4_quantize", mutates_args=())
+def int4_quantize(weight: Tensor, group: int, symmetric: bool) -> Tuple[Tensor, Tensor, Tensor]:
+    q, s, z = host().int4_quantize_fwd(weight, group, symmetric)
+    return q, s, (z if z is not None else _none(q))
+
+
+@int4_quantize.register_fake
+def _(weight, group, symmetric):
+    (N, K), G = weight.shape, (weight.shape[1] + group - 1) // group
+    return (_e(weight, N, K // 2, dtype=torch.uint8), _e(weight, N, G),
+            _e(weight, 0, dtype=torch.uint8) if symmetric else _e(weight, N, G, dtype=torch.uint8))
+
+
+@torch.library.custom_op(f"{NS}::int4_dequantize", mutates_args=())
+def int4_dequantize(q: Tensor, scales: Tensor, zeros: Optional[Tensor], group: int, bf16: bool) -> Tensor:
+    return host().int4_dequantize_fwd(q, scales, zeros, group, bf16)
+
+
+@int4_dequantize.register_fake
+def _(q, scales, zeros, group, bf16):
+    return _e(q, q.shape[0], 2 * q.shape[1], dtype=torch.bfloat16 if bf16 else _F32)
+
+
+@torch.library.custom_op(f"{NS}::int4_linear", mutates_args=())
+def int4_linear(x: Tensor, q: Tensor, scales: Tensor, zeros: Optional[Tensor], group: int, bias: Optional[Tensor], act: int, bf16: bool) -> Tensor:
+    return host().int4_linear_fwd(x, q, scales, zeros, group, bias, act, bf16, False)
+
+
+@int4_linear.register_fake
+def _(x, q, scales, zeros, group, bias, act, bf16):
+    return _e(x, *x.shape[:-1], q.shape[0], dtype=torch.bfloat16 if bf16 else _F32)
+
+
+@torch.library.custom_op(f"{NS}::adjust_logits", mutates_args=())
+def adjust_logits(logits: Tensor, prompt: Optional[Tensor], prompt_lengths: Optional[Tensor], generated: Optional[Tensor], generated_lengths: Optional[Tensor],
+                  repetition_rows: Optional[Tensor], repetition: float, frequency_rows: Optional[Tensor], frequency: float, presence_rows: Optional[Tensor],
+                  presence: float, bias_ids: Optional[Tensor], bias: Optional[Tensor], mask: Optional[Tensor]) -> Tensor:
+    return host().adjust_logits_fwd(logits, prompt, prompt_lengths, generated, generated_lengths, repetition_rows, repetition, frequency_rows, frequency,
+                                    presence_rows, presence, bias_ids, bias, mask, None)
+
+
+@adjust_logits.register_fake
+def _(logits, prompt, prompt_lengths, generated, generated_lengths, repetition_rows, repetition, frequency_rows, frequency, presence_rows, presence, bias_ids,
+      bias, mask):
+    return _e(logits, *logits.shape, dtype=_F32)

@@ -1,0 +1,71 @@
+"""Weights held in four bits with a scale per group: made from a weight, read back, and multiplied with -- one token to a whole prompt.
+The reference has none of these.
+
+All take CUDA tensors in float32 or bfloat16, launch on torch's current stream and never synchronise. They have no gradient: a call that would need one
+raises. Eagerly they run through csrc/torch_host.cpp; under torch.compile, a tracer or a dispatch mode as the operators of
+pragnosia_b200.custom_ops.
+"""
+from __future__ import annotations
+
+from typing import NamedTuple, Optional
+
+import torch
+
+from ._lib import BF16, host, type_code
+
+
+class Int4Weight(NamedTuple):
+    """scale (q - zero) for every element of a weight (N, K), K a multiple of 32. A program with levels of its own fills this in itself."""
+    q: torch.Tensor                         # (N, K / 2) uint8, the even column in the low half of a byte
+    scales: torch.Tensor                    # (N, ceil(K / group)) float32 or bfloat16
+    zeros: Optional[torch.Tensor]           # as scales, uint8, 0 .. 127; None: 8 everywhere
+    group: int                              # 32, 64 or 128 columns of a row; its last group may be shorter
+
+    @property
+    def shape(self) -> tuple[int, int]:
+        return self.q.shape[0], 2 * self.q.shape[1]
+
+
+def _operators():
+    from . import custom_ops  # noqa: F401  (registers them)
+    return torch.ops.pragnosia_b200
+
+
+def quantize(weight, group: int = 64, symmetric: bool = False) -> Int4Weight:
+    """The weight (N, K) in four bits. A group's scale is its range (which takes in 0) over 15, with a zero that keeps 0 exact, or (symmetric) its
+    largest magnitude over 7; it has weight's type. Levels are the nearest ones, ties to even, in float32's own arithmetic. A group that holds an
+    infinity or NaN reads back as NaN."""
+    if not torch.compiler.is_compiling():
+        out = host().int4_quantize(weight, int(group), bool(symmetric))
+        if out is not None:
+            return Int4Weight(*out, int(group))
+    q, s, z = _operators().int4_quantize(weight, int(group), bool(symmetric))
+    return Int4Weight(q, s, None if symmetric else z, int(group))
+
+
+def dequantize(w: Int4Weight, dtype: Optional[torch.dtype] = None):
+    """The weight (N, K) that w stands for, rounded once to dtype (default: the scales')."""
+    bf16 = type_code(dtype or w.scales.dtype) == BF16
+    if not torch.compiler.is_compiling():
+        out = host().int4_dequantize(w.q, w.scales, w.zeros, w.group, bf16)
+        if out is not None:
+            return out
+    return _operators().int4_dequantize(w.q, w.scales, w.zeros, w.group, bf16)
+
+
+def linear(x, w: Int4Weight, bias=None, *, act: Optional[str] = None, out_dtype: Optional[torch.dtype] = None, constant: bool = False):
+    """act(x W^T + bias) for x (..., K), bias (N,); act None or "gelu" (erf). Result (..., N) in out_dtype (default: x's).
+
+    Sums in float32, one rounding at the end; a group's whole numbers meet x unrounded and are scaled behind their sum. For bfloat16 in and out from 17 rows up
+    the products run on the tensor cores with scale (q - zero) rounded to bfloat16, an error below that of the result's own rounding. The same
+    call gives the same bits; a row's may differ between calls of up to 16 rows and of more.
+    constant: w and bias were complete before the kernel ahead on the stream was launched (weights of a model in a chain of launches): they are read while it runs."""
+    if act not in (None, "gelu"):
+        raise ValueError(f"act is None or 'gelu', got {act!r}")
+    bf16 = type_code(out_dtype or x.dtype) == BF16
+    code = 0 if act is None else 1
+    if not torch.compiler.is_compiling():
+        out = host().int4_linear(x, w.q, w.scales, w.zeros, w.group, bias, code, bf16, constant)
+        if out is not None:
+            return out
+    return _operators().int4_linear(x, w.q, w.scales, w.zeros, w.group, bias, code, bf16)
