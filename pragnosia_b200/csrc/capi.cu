@@ -122,6 +122,7 @@ int decode_token_wait_selftest_launch(unsigned long long *, unsigned, cudaStream
 int int4_quantize_launch(const void *, int, unsigned char *, void *, unsigned char *, int, int, int, cudaStream_t);
 int int4_dequantize_launch(const Int4Weight &, void *, int, cudaStream_t);
 int int4_linear_launch(const Int4Linear &, cudaStream_t);
+int int4_tile_error_flag(int *);
 int adjust_logits_launch(const AdjustLogits &, cudaStream_t);
 
 // PGB_PREFILL_AUTO sends bf16 plain-rule work to the tensor-core kernel only once this is on
@@ -1089,6 +1090,8 @@ int pgb_tc_error_flag(int *out_host) {
     if (rc == PGB_OK) rc = delta_segments_error_flag(&g);
     f = f > g ? f : g;
     if (rc == PGB_OK) rc = head_loss_error_flag(&g);
+    f = f > g ? f : g;
+    if (rc == PGB_OK) rc = int4_tile_error_flag(&g);
     f = f > g ? f : g;
     e = e > f ? e : f;
     b = b > c ? b : c;

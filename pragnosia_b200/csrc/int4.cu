@@ -10,7 +10,7 @@
 //
 // Every step of the quantisation is one correctly rounded fp32 operation, so the same weights give the same levels anywhere. A group that holds an
 // infinity or NaN has a scale of NaN, and so has one whose range leaves fp32.
-#include "tc_common.cuh"
+#include "int4_linear.cuh"
 
 namespace pgb {
 
@@ -108,193 +108,216 @@ __device__ __forceinline__ float int4_act(float v, int act) { return act == 1 ? 
 // that order and x, whose fragments serve all MT blocks of rows, is reordered by byte permutes. A group's products end in an accumulator of their own that enters the
 // sum times the scale: the weight is never rounded. fp32 rows of x are three terms of eight bits each, cut off (their sum is x to the last bit), three products.
 //   Levels lie in 64-byte rows whose 16-byte pieces are swapped by the row, so that the eight rows of a fragment's word touch every bank once.
-constexpr int RW_WARPS = 8, RW_NT = RW_WARPS * 32;
+constexpr int RW_MOST = 8;                                             // warps of a CTA at most
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, int bytes) {      // bytes 0: zeros
-    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N_> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N_) : "memory"); }
-__device__ __forceinline__ uint32_t lds32(uint32_t a) {
-    uint32_t v;
-    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a));
-    return v;
-}
-__device__ __forceinline__ uint4 lds128(uint32_t a) {
-    uint4 v;
-    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
-    return v;
-}
 __device__ __forceinline__ void mma_bf16_warp(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// the pair of levels in bits 0-3 and 16-19 as bf16 whole numbers less the zero: z2 is 128 + z twice
-__device__ __forceinline__ uint32_t level_pair(uint32_t w, uint32_t z2) {
-    uint32_t v = (w & 0x000f000fu) | 0x43004300u;
-    const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162 *>(&v), *reinterpret_cast<const __nv_bfloat162 *>(&z2));
-    return *reinterpret_cast<const uint32_t *>(&d);
-}
-
 struct RowsArgs {
     const void *x; const unsigned char *q; const void *scales; const unsigned char *zeros; const void *bias; void *y;
-    int act, out_bf16, N, K, G, lg, slots, slot_bytes, constant;
+    int act, out_bf16, N, K, G, lg, warps, each, slots, ahead, slot_bytes, constant;   // each: stretches of a warp; ahead: those on their way
     long long M;
 };
 
-template <int MT, int NB, bool X32, bool S32>
-__global__ void __launch_bounds__(RW_NT) int4_rows_kernel(const RowsArgs a) {
-    constexpr int R = 16 * MT, RP = R + 4, TERMS = X32 ? 3 : 1;
+template <int MT, int NB, int LG, bool X32, bool S32>
+__global__ void __launch_bounds__(RW_MOST * 32) int4_rows_kernel(const RowsArgs a) {
+    constexpr int R = 16 * MT, RP = R + 4, TERMS = X32 ? 3 : 1, XE = X32 ? 4 : 2, GM = (1 << (LG - 5)) - 1;       // GM + 1: pieces of 32 columns a group has
+    constexpr int BL = 1 << (LG - 5);                                 // stretches whose scales a quad of lanes holds: four groups
     extern __shared__ __align__(1024) uint8_t rw_smem[];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-    const int n0 = blockIdx.x * R, rows = a.M - (long long)blockIdx.y * (8 * NB) < 8 * NB ? (int)(a.M - (long long)blockIdx.y * (8 * NB)) : 8 * NB;
+    const int n0 = blockIdx.x * R;
     const long long m0 = (long long)blockIdx.y * (8 * NB);
-    const int C = (a.K + 127) >> 7, mine = C > warp ? (C - warp + RW_WARPS - 1) / RW_WARPS : 0;     // stretches, and this warp's
-    const uint32_t ring = smem_u32(rw_smem) + warp * a.slots * a.slot_bytes;
-    const uint8_t *xg = reinterpret_cast<const uint8_t *>(a.x) + m0 * a.K * (X32 ? 4 : 2);
+    const int rows = a.M - m0 < 8 * NB ? (int)(a.M - m0) : 8 * NB;
+    uint8_t *ring = rw_smem + warp * a.slots * a.slot_bytes;
+    const uint32_t ring_at = smem_u32(ring);
+    const int C = (a.K + 127) >> 7, c0 = warp * a.each, mine = C - c0 < a.each ? C - c0 : a.each;     // this warp's stretches: c0, c0 + 1, ..
+    const int ahead = a.ahead;
 
-    auto fetch_w = [&](int i) {                                       // stretch i of this warp into its slot
-        const int k = (warp + i * RW_WARPS) * 128 + (lane & 3) * 32;
-        const uint32_t dst = ring + (i % a.slots) * a.slot_bytes;
+    // this lane's piece of eight rows at a time (row lane / 4, columns 32 (lane mod 4) ..) of a stretch
+    const int fr = lane >> 2, half = a.K >> 1;
+    uint32_t live = 0;                                                // which of those rows are there
+#pragma unroll
+    for (int u = 0; u < 2 * MT; ++u) live |= (n0 + u * 8 + fr < a.N ? 1u : 0u) << u;
+    int wcol = c0 * 128 + t * 32, xcol = c0 * 128;
+    const unsigned char *wsrc = a.q + (size_t)(n0 + fr) * half + (wcol >> 1);
+    const size_t eight = (size_t)8 * half;
+    const uint32_t wdst = ring_at + fr * 64 + ((t ^ ((fr >> 1) & 3)) << 4);
+    const uint8_t *xsrc = reinterpret_cast<const uint8_t *>(a.x) + (size_t)m0 * a.K * XE;
+
+    auto fetch_w = [&](int slot) {                                    // the next stretch of levels
+        const uint32_t ok = wcol < a.K ? live : 0u, dst = wdst + slot * a.slot_bytes;
+        const unsigned char *p = wsrc;
 #pragma unroll
         for (int u = 0; u < 2 * MT; ++u) {
-            const int r = u * 8 + (lane >> 2);
-            const bool in = n0 + r < a.N && k < a.K;
-            cp_async16(dst + r * 64 + (((lane & 3) ^ ((r >> 1) & 3)) << 4), a.q + (in ? ((size_t)(n0 + r) * a.K + k) / 2 : 0), in ? 16 : 0);
+            const bool in = ok >> u & 1u;
+            cp_async16(dst + u * 512, in ? p : a.q, in ? 16 : 0);
+            p += eight;
         }
+        wcol += 128; wsrc += 64;
     };
-    // x: pieces of 64 B (32 columns of bf16, 16 of fp32), [piece][row]
-    auto fetch_x = [&](int i) {
-        const uint32_t dst = ring + (i % a.slots) * a.slot_bytes + R * 64;
-        constexpr int PIECES = X32 ? 8 : 4, E = X32 ? 4 : 2;
-        const int c0 = (warp + i * RW_WARPS) * 128;
-        for (int u = lane; u < PIECES * rows * 4; u += 32) {
-            const int c = u & 3, pr = u >> 2, p = pr / rows, r = pr - p * rows;
-            const int k = c0 + (p * 64 + c * 16) / E;
+    auto fetch_x = [&](int slot) {                                    // and of x: pieces of 64 B of a row, [piece][row]
+        constexpr int PC = X32 ? 5 : 4;                               // log2 of the 16-byte chunks of a row's stretch
+        const uint32_t dst = ring_at + slot * a.slot_bytes + R * 64;
+        for (int u = lane; u < rows << PC; u += 32) {
+            const int c = u & ((1 << PC) - 1), r = u >> PC, k = xcol + c * (16 / XE);
             const bool in = k < a.K;
-            cp_async16(dst + u * 16, xg + (in ? ((size_t)r * a.K + k) * E : 0), in ? 16 : 0);
+            cp_async16(dst + ((c >> 2) * rows + r) * 64 + (c & 3) * 16, xsrc + (in ? ((size_t)r * a.K + k) * XE : 0), in ? 16 : 0);
         }
+        xcol += 128;
     };
-    // scales and zeros of this lane's rows, group t of the stretch: the scale's bits, or (bf16) those and 128 + z in one word
-    uint32_t sc[2][MT], zr[2][S32 ? MT : 1];
-    auto fetch_s = [&](int i) {
-        const int grp = (((warp + i * RW_WARPS) * 128) >> a.lg) + t;
-        const bool in = i < mine && t < (128 >> a.lg) && grp < a.G;
+    // scales and zeros of this lane's rows (g, g + 8 of every block of 16) for group t of the next four groups: the scale's bits with 128 + z below them
+    // (fp32 scales: in a word of their own)
+    int grp = ((c0 * 128) >> LG) + t;
+    const int last_grp = mine > 0 ? ((c0 + mine) * 128 - 1) >> LG : -1;
+    uint32_t sn[2 * MT], zn[S32 ? 2 * MT : 1];
+    const size_t srow = (size_t)(n0 + g) * a.G, step = (size_t)8 * a.G;
+    auto fetch_s = [&]() {
+        const bool in = grp <= last_grp && grp < a.G;
+        size_t at = srow + grp;
 #pragma unroll
-        for (int u = 0; u < MT; ++u)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int n = n0 + 16 * u + 8 * h + g;
-                const size_t at = (size_t)(n < a.N ? n : a.N - 1) * a.G + grp;
-                const uint32_t z = 0x4300u | (in && a.zeros != nullptr ? a.zeros[at] : 8u);
-                if constexpr (S32) {
-                    sc[h][u] = in ? reinterpret_cast<const uint32_t *>(a.scales)[at] : 0u;
-                    zr[h][u] = z;
-                } else {
-                    sc[h][u] = (in ? (uint32_t)reinterpret_cast<const unsigned short *>(a.scales)[at] << 16 : 0u) | z;
-                }
+        for (int u = 0; u < 2 * MT; ++u) {
+            uint32_t s = 0u, z = 8u;
+            if (in && n0 + g + 8 * u < a.N) {
+                if constexpr (S32) s = __ldg(reinterpret_cast<const uint32_t *>(a.scales) + at);
+                else s = (uint32_t)__ldg(reinterpret_cast<const unsigned short *>(a.scales) + at) << 16;
+                if (a.zeros != nullptr) z = __ldg(a.zeros + at);
             }
+            sn[u] = S32 ? s : s | z;
+            if constexpr (S32) zn[u] = z;
+            at += step;
+        }
+        grp += 4;
     };
 
-    if (!a.constant) { pdl_wait(); pdl_launch_dependents(); }
-    const int ahead = a.slots - 1;
     if (a.constant) {
         for (int i = 0; i < ahead && i < mine; ++i) fetch_w(i);
-        fetch_s(0);
+        fetch_s();
         pdl_launch_dependents();
         pdl_wait();
         for (int i = 0; i < ahead && i < mine; ++i) fetch_x(i);
-        cp_async_commit();                                            // one group for all of them; the empty ones keep the count
-        for (int i = 1; i < ahead; ++i) cp_async_commit();
+        for (int i = 0; i < ahead; ++i) cp_async_commit();            // the first holds them all, the others keep the count
     } else {
+        pdl_wait();
+        pdl_launch_dependents();
         for (int i = 0; i < ahead; ++i) {
             if (i < mine) { fetch_w(i); fetch_x(i); }
             cp_async_commit();
         }
-        fetch_s(0);
+        fetch_s();
     }
+    int woff[4];                                                      // this lane's word of piece j of row g
+#pragma unroll
+    for (int j = 0; j < 4; ++j) woff[j] = g * 64 + ((j ^ ((g >> 1) & 3)) << 4) + 4 * t;
+    float acc[MT][NB][4] = {};
+    uint32_t sc[2 * MT], zc[S32 ? 2 * MT : 1];
 
-    float acc[MT][NB][4] = {}, part[MT][NB][4] = {};
-    const int per = a.lg - 5;                                         // log2 of the 32-column pieces a group has
+    int slot = 0;
     for (int i = 0; i < mine; ++i) {
-        uint32_t s0[2][MT], z0[2][S32 ? MT : 1];
+        if ((i & (BL - 1)) == 0) {                                    // the next four groups' scales: here by now, and those behind them asked for
 #pragma unroll
-        for (int u = 0; u < MT; ++u)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                s0[h][u] = sc[h][u];
-                if constexpr (S32) z0[h][u] = zr[h][u];
+            for (int u = 0; u < 2 * MT; ++u) {
+                sc[u] = sn[u];
+                if constexpr (S32) zc[u] = zn[u];
             }
-        if (i + ahead < mine) { fetch_w(i + ahead); fetch_x(i + ahead); }
+            fetch_s();
+        }
+        if (i + ahead < mine) {                                       // then there is a slot more than stretches ahead: the one read last
+            const int next = slot == 0 ? ahead : slot - 1;
+            fetch_w(next);
+            fetch_x(next);
+        }
         cp_async_commit();
-        fetch_s(i + 1);
-        if (a.slots == 2) cp_async_wait<1>(); else if (a.slots == 3) cp_async_wait<2>(); else if (a.slots == 4) cp_async_wait<3>();
-        else if (a.slots == 5) cp_async_wait<4>(); else cp_async_wait<5>();
+        if (ahead == 1) cp_async_wait<1>(); else if (ahead == 2) cp_async_wait<2>(); else if (ahead == 3) cp_async_wait<3>(); else cp_async_wait<4>();
         __syncwarp();
-        const uint32_t ws = ring + (i % a.slots) * a.slot_bytes, xs = ws + R * 64;
+        const uint8_t *ws = ring + slot * a.slot_bytes, *xs = ws + R * 64;
+        slot = slot + 1 == a.slots ? 0 : slot + 1;
+        // x: columns 32 j + 8 t .. + 7 of row 8 b + g, as (0,4) (1,5) (2,6) (3,7)
+        uint32_t bx[4][TERMS][NB][4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            // x: columns 32 j + 8 t .. + 7 of row 8 b + g, as (0,4) (1,5) (2,6) (3,7)
-            uint32_t bx[TERMS][NB][4];
+        for (int b = 0; b < NB; ++b) {
+            const int r = 8 * b + g;
 #pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                const int r = 8 * b + g;
+            for (int j = 0; j < 4; ++j) {
                 if constexpr (!X32) {
                     uint4 v = make_uint4(0u, 0u, 0u, 0u);
-                    if (r < rows) v = lds128(xs + (j * rows + r) * 64 + t * 16);
-                    bx[0][b][0] = __byte_perm(v.x, v.z, 0x5410); bx[0][b][1] = __byte_perm(v.x, v.z, 0x7632);
-                    bx[0][b][2] = __byte_perm(v.y, v.w, 0x5410); bx[0][b][3] = __byte_perm(v.y, v.w, 0x7632);
+                    if (r < rows) v = *reinterpret_cast<const uint4 *>(xs + (j * rows + r) * 64 + t * 16);
+                    bx[j][0][b][0] = __byte_perm(v.x, v.z, 0x5410); bx[j][0][b][1] = __byte_perm(v.x, v.z, 0x7632);
+                    bx[j][0][b][2] = __byte_perm(v.y, v.w, 0x5410); bx[j][0][b][3] = __byte_perm(v.y, v.w, 0x7632);
                 } else {
                     uint4 lo = make_uint4(0u, 0u, 0u, 0u), hi = lo;
                     if (r < rows) {
-                        const uint32_t at = xs + ((2 * j + (t >> 1)) * rows + r) * 64 + (t & 1) * 32;
-                        lo = lds128(at); hi = lds128(at + 16);
+                        const uint4 *at = reinterpret_cast<const uint4 *>(xs + ((2 * j + (t >> 1)) * rows + r) * 64 + (t & 1) * 32);
+                        lo = at[0]; hi = at[1];
                     }
-                    const uint32_t first[4] = {lo.x, lo.y, lo.z, lo.w}, second[4] = {hi.x, hi.y, hi.z, hi.w};
+                    const uint32_t one[4] = {lo.x, lo.y, lo.z, lo.w}, two[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         uint32_t u[2][3];
 #pragma unroll
                         for (int p = 0; p < 2; ++p) {                 // x = head + middle + rest, eight bits each
-                            const uint32_t bits = p == 0 ? first[e] : second[e];
+                            const uint32_t bits = p == 0 ? one[e] : two[e];
                             const bool fin = (bits & 0x7f800000u) != 0x7f800000u;
                             const float f = __uint_as_float(bits);
                             const float r1 = fin ? f - __uint_as_float(bits & 0xffff0000u) : 0.f;
                             const float r2 = r1 - __uint_as_float(__float_as_uint(r1) & 0xffff0000u);
-                            u[p][0] = fin ? bits : (bits & 0x007fffffu) != 0u ? 0x7fc00000u : bits;
+                            u[p][0] = fin || (bits & 0x007fffffu) == 0u ? bits : 0x7fc00000u;
                             u[p][1] = __float_as_uint(r1); u[p][2] = __float_as_uint(r2);
                         }
 #pragma unroll
-                        for (int q3 = 0; q3 < 3; ++q3) bx[q3][b][e] = __byte_perm(u[0][q3], u[1][q3], 0x7632);
+                        for (int q3 = 0; q3 < 3; ++q3) bx[j][q3][b][e] = __byte_perm(u[0][q3], u[1][q3], 0x7632);
                     }
                 }
             }
-            const int src = (lane & ~3) + (j >> per);
+        }
+        const uint32_t *wp[4];
 #pragma unroll
-            for (int u = 0; u < MT; ++u) {
-                const int r = 16 * u + g;
-                const uint32_t wa = lds32(ws + r * 64 + ((j ^ ((r >> 1) & 3)) << 4) + 4 * t), wb = lds32(ws + (r + 8) * 64 + ((j ^ (((r + 8) >> 1) & 3)) << 4) + 4 * t);
-                const uint32_t sa = __shfl_sync(0xffffffffu, s0[0][u], src), sb = __shfl_sync(0xffffffffu, s0[1][u], src);
-                uint32_t za, zb;
-                if constexpr (S32) { za = __shfl_sync(0xffffffffu, z0[0][u], src); zb = __shfl_sync(0xffffffffu, z0[1][u], src); }
-                else { za = sa; zb = sb; }
-                za = __byte_perm(za, za, 0x1010); zb = __byte_perm(zb, zb, 0x1010);
+        for (int j = 0; j < 4; ++j) wp[j] = reinterpret_cast<const uint32_t *>(ws + woff[j]);
+        const int quad = (lane & ~3) + (LG == 7 ? i & 3 : LG == 6 ? (i & 1) * 2 : 0);     // the lane that has the stretch's first group
+        // Pieces outside, blocks of rows inside: products of different blocks (and, for one block, of a word's halves) do not wait for one another.
+        constexpr int CH = MT == 1 ? 2 : 1;
+        float part[MT][CH][NB][4];
+        uint32_t sa[MT], sb[MT], za[MT], zb[MT];
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const uint32_t a0 = level_pair(wa >> (8 * h), za), a1 = level_pair(wb >> (8 * h), zb), a2 = level_pair(wa >> (8 * h + 4), za),
-                                   a3 = level_pair(wb >> (8 * h + 4), zb);
+        for (int j = 0; j < 4; ++j) {
+            if ((j & GM) == 0) {                                      // a group begins here
+                const int src = quad + j / (GM + 1);
+#pragma unroll
+                for (int u = 0; u < MT; ++u) {
+                    sa[u] = __shfl_sync(0xffffffffu, sc[2 * u], src); sb[u] = __shfl_sync(0xffffffffu, sc[2 * u + 1], src);
+                    if constexpr (S32) { za[u] = __shfl_sync(0xffffffffu, zc[2 * u], src); zb[u] = __shfl_sync(0xffffffffu, zc[2 * u + 1], src); }
+                    else { za[u] = sa[u]; zb[u] = sb[u]; }
+                    za[u] = __byte_perm(za[u], 0x43u, 0x4040); zb[u] = __byte_perm(zb[u], 0x43u, 0x4040);       // 128 + z, twice
+#pragma unroll
+                    for (int c = 0; c < CH; ++c)
+#pragma unroll
+                        for (int b = 0; b < NB; ++b) part[u][c][b][0] = part[u][c][b][1] = part[u][c][b][2] = part[u][c][b][3] = 0.f;
+                }
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int u = 0; u < MT; ++u) {
+                    const uint32_t wa = wp[j][u * 256], wb = wp[j][u * 256 + 128];
+                    const uint32_t a0 = level_pair(wa >> (8 * h), za[u]), a1 = level_pair(wb >> (8 * h), zb[u]), a2 = level_pair(wa >> (8 * h + 4), za[u]),
+                                   a3 = level_pair(wb >> (8 * h + 4), zb[u]);
 #pragma unroll
                     for (int b = 0; b < NB; ++b)
 #pragma unroll
-                        for (int q3 = TERMS - 1; q3 >= 0; --q3) mma_bf16_warp(part[u][b], a0, a1, a2, a3, bx[q3][b][2 * h], bx[q3][b][2 * h + 1]);
+                        for (int q3 = TERMS - 1; q3 >= 0; --q3) mma_bf16_warp(part[u][h % CH][b], a0, a1, a2, a3, bx[j][q3][b][2 * h], bx[j][q3][b][2 * h + 1]);
                 }
-                if (((j + 1) & ((1 << per) - 1)) == 0) {              // the group ends here
-                    const float fa = __uint_as_float(S32 ? sa : sa & 0xffff0000u), fb = __uint_as_float(S32 ? sb : sb & 0xffff0000u);
+            if ((j & GM) == GM) {                                     // and ends here
+#pragma unroll
+                for (int u = 0; u < MT; ++u) {
+                    const float fa = __uint_as_float(S32 ? sa[u] : sa[u] & 0xffff0000u), fb = __uint_as_float(S32 ? sb[u] : sb[u] & 0xffff0000u);
 #pragma unroll
                     for (int b = 0; b < NB; ++b) {
-                        acc[u][b][0] = fmaf(fa, part[u][b][0], acc[u][b][0]); acc[u][b][1] = fmaf(fa, part[u][b][1], acc[u][b][1]);
-                        acc[u][b][2] = fmaf(fb, part[u][b][2], acc[u][b][2]); acc[u][b][3] = fmaf(fb, part[u][b][3], acc[u][b][3]);
-                        part[u][b][0] = part[u][b][1] = part[u][b][2] = part[u][b][3] = 0.f;
+                        if constexpr (CH == 2) {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) part[u][0][b][e] += part[u][1][b][e];
+                        }
+                        acc[u][b][0] = fmaf(fa, part[u][0][b][0], acc[u][b][0]); acc[u][b][1] = fmaf(fa, part[u][0][b][1], acc[u][b][1]);
+                        acc[u][b][2] = fmaf(fb, part[u][0][b][2], acc[u][b][2]); acc[u][b][3] = fmaf(fb, part[u][0][b][3], acc[u][b][3]);
                     }
                 }
             }
@@ -302,25 +325,21 @@ __global__ void __launch_bounds__(RW_NT) int4_rows_kernel(const RowsArgs a) {
         __syncwarp();                                                 // the slot is read: the next copy may take it
     }
     cp_async_wait<0>();
-    if (a.constant) pdl_wait();
     __syncthreads();                                                  // the slots become the sums' meeting place
     float *red = reinterpret_cast<float *>(rw_smem);                  // [warp][row of x][row of W]
-    const int busy = C < RW_WARPS ? C : RW_WARPS;
-    if (warp < busy) {
 #pragma unroll
-        for (int u = 0; u < MT; ++u)
+    for (int u = 0; u < MT; ++u)
 #pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                float *p = red + (warp * 8 * NB + 8 * b + 2 * t) * RP + 16 * u + g;
-                p[0] = acc[u][b][0]; p[RP] = acc[u][b][1]; p[8] = acc[u][b][2]; p[RP + 8] = acc[u][b][3];
-            }
-    }
+        for (int b = 0; b < NB; ++b) {
+            float *p = red + (warp * 8 * NB + 8 * b + 2 * t) * RP + 16 * u + g;
+            p[0] = acc[u][b][0]; p[RP] = acc[u][b][1]; p[8] = acc[u][b][2]; p[RP + 8] = acc[u][b][3];
+        }
     __syncthreads();
-    for (int i = tid; i < R * rows; i += RW_NT) {
+    for (int i = tid; i < R * rows; i += a.warps * 32) {
         const int n = i % R, m = i / R;
         if (n0 + n >= a.N) continue;
         float s = 0.f;
-        for (int w = 0; w < busy; ++w) s += red[(w * 8 * NB + m) * RP + n];
+        for (int w = 0; w < a.warps; ++w) s += red[(w * 8 * NB + m) * RP + n];
         if (a.bias != nullptr) s += X32 ? reinterpret_cast<const float *>(a.bias)[n0 + n] : __bfloat162float(reinterpret_cast<const __nv_bfloat16 *>(a.bias)[n0 + n]);
         s = int4_act(s, a.act);
         const size_t at = (size_t)(m0 + m) * a.N + n0 + n;
@@ -361,39 +380,56 @@ int int4_dequantize_launch(const Int4Weight &w, void *out, int out_dtype, cudaSt
     return check_launch("int4_dequantize_kernel");
 }
 
-template <int MT, int NB, bool X32, bool S32>
-static cudaError_t rows_go(RowsArgs a, cudaStream_t stream) {
-    constexpr int R = 16 * MT, RED = RW_WARPS * 8 * NB * (R + 4) * 4, MOST = 104 * 1024;     // two CTAs an SM
-    const int rows = a.M < 8 * NB ? (int)a.M : 8 * NB;
+template <int MT, int NB, int LG, bool X32, bool S32>
+static cudaError_t rows_go_group(RowsArgs a, cudaStream_t stream) {
+    constexpr int R = 16 * MT, RP = R + 4;
+    const int rows = a.M < 8 * NB ? (int)a.M : 8 * NB, C = (a.K + 127) / 128;
+    a.each = (C + a.warps - 1) / a.warps;
+    a.warps = (C + a.each - 1) / a.each;
     a.slot_bytes = R * 64 + rows * (X32 ? 512 : 256);
-    const int mine = ((a.K + 127) / 128 + RW_WARPS - 1) / RW_WARPS;
-    a.slots = MOST / (RW_WARPS * a.slot_bytes);
-    if (a.slots > mine + 1) a.slots = mine + 1;
-    a.slots = a.slots < 2 ? 2 : a.slots > 6 ? 6 : a.slots;
-    int smem = RW_WARPS * a.slots * a.slot_bytes;
-    if (smem < RED) smem = RED;
+    // stretches ahead: what keeps an SM's memory busy, four at most; either all of a warp's at once, or one slot more than are ahead
+    a.ahead = a.each < 4 ? a.each : 4;
+    while (a.ahead > 1 && a.warps * (a.ahead + (a.ahead < a.each ? 1 : 0)) * a.slot_bytes > 100 * 1024) --a.ahead;
+    a.slots = a.ahead + (a.ahead < a.each ? 1 : 0);
+    int smem = a.warps * a.slots * a.slot_bytes;
+    const int red = a.warps * 8 * NB * RP * 4;
+    if (smem < red) smem = red;
     cudaError_t e = cudaSuccess;
-    if (smem > 48 * 1024) e = cudaFuncSetAttribute(int4_rows_kernel<MT, NB, X32, S32>, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+    if (smem > 48 * 1024) e = cudaFuncSetAttribute(int4_rows_kernel<MT, NB, LG, X32, S32>, cudaFuncAttributeMaxDynamicSharedMemorySize, 136 * 1024);
     for (; e == cudaSuccess && a.M > 0; ) {                           // a grid's second axis ends at 65535
         const long long most = 65535LL * 8 * NB, M = a.M < most ? a.M : most, rest = a.M - M;
         a.M = M;
-        e = pdl_launch(int4_rows_kernel<MT, NB, X32, S32>, dim3((unsigned)((a.N + R - 1) / R), (unsigned)((M + 8 * NB - 1) / (8 * NB))), dim3(RW_NT), (size_t)smem, stream, a);
+        e = pdl_launch(int4_rows_kernel<MT, NB, LG, X32, S32>, dim3((unsigned)((a.N + R - 1) / R), (unsigned)((M + 8 * NB - 1) / (8 * NB))),
+                       dim3((unsigned)a.warps * 32), (size_t)smem, stream, a);
         a.x = (const uint8_t *)a.x + (size_t)M * a.K * (X32 ? 4 : 2);
         a.y = (uint8_t *)a.y + (size_t)M * a.N * (a.out_bf16 ? 2 : 4);
         a.M = rest;
     }
     return e;
 }
+template <int MT, int NB, bool X32, bool S32>
+static cudaError_t rows_go(RowsArgs a, cudaStream_t stream) {
+    if (a.lg == 5) return rows_go_group<MT, NB, 5, X32, S32>(a, stream);
+    if (a.lg == 6) return rows_go_group<MT, NB, 6, X32, S32>(a, stream);
+    return rows_go_group<MT, NB, 7, X32, S32>(a, stream);
+}
 template <int NB, bool X32, bool S32>
-static cudaError_t rows_blocks(const RowsArgs &a, cudaStream_t stream) {
+static cudaError_t rows_blocks(RowsArgs a, cudaStream_t stream) {
+    // 16 warps an SM, of as many rows as that leaves (us, one row of x): N 16384 K 4096 with 32 rows and 4 warps a CTA 17.1, 64 and 8 18.5, 16 and 8 20.0; N 8192 K 2048 32 and 8 8.0,
+    // 16 and 8 9.1; N 2048 K 2048 16 and 8 3.3, 32 and 8 4.3; K 16384 N 4096 32 and 8 22, 16 and 8 28, 64 and 8 33. Several rows: N 16384 K 4096, 8 rows, 64 and 8 20.9, 32 and 8 22.9.
     const long long tiles = (a.M + 8 * NB - 1) / (8 * NB), sms = sm_count();
-    if ((a.N + 63) / 64 * tiles >= sms) return rows_go<4, NB, X32, S32>(a, stream);
-    if ((a.N + 31) / 32 * tiles >= sms) return rows_go<2, NB, X32, S32>(a, stream);
+    const long long by64 = (a.N + 63) / 64 * tiles, by32 = (a.N + 31) / 32 * tiles, by16 = (a.N + 15) / 16 * tiles;
+    const int MT = a.M > 4 && by64 * 10 >= 17 * sms ? 4 : by32 * 10 >= 7 * sms ? 2 : 1;
+    const long long ctas = MT == 4 ? by64 : MT == 2 ? by32 : by16;
+    a.warps = ctas * 8 <= 17 * sms ? 8 : ctas * 4 <= 17 * sms ? 4 : 2;
+    if (MT == 4) return rows_go<4, NB, X32, S32>(a, stream);
+    if (MT == 2) return rows_go<2, NB, X32, S32>(a, stream);
     return rows_go<1, NB, X32, S32>(a, stream);
 }
 int int4_linear_launch(const Int4Linear &l, cudaStream_t stream) {
     const Int4Weight &w = l.w;
-    const RowsArgs a{l.x, w.q, w.scales, w.zeros, l.bias, l.y, l.act, l.out_dtype == PGB_BF16, w.N, w.K, w.G, log2_group(w.group), 0, 0, l.constant, l.M};
+    if (l.M > PGB_INT4_ROWS && l.x_dtype == PGB_BF16 && l.out_dtype == PGB_BF16) return int4_tile_launch(l, stream);
+    const RowsArgs a{l.x, w.q, w.scales, w.zeros, l.bias, l.y, l.act, l.out_dtype == PGB_BF16, w.N, w.K, w.G, log2_group(w.group), 0, 0, 0, 0, 0, l.constant, l.M};
     const bool x32 = l.x_dtype == PGB_F32, s32 = w.scale_dtype == PGB_F32;
     cudaError_t e;
     if (x32) e = s32 ? rows_blocks<1, true, true>(a, stream) : rows_blocks<1, true, false>(a, stream);

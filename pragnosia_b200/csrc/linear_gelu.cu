@@ -14,6 +14,7 @@
 //   per element decides the kernel's speed: see lg_gelu.
 //   One CTA per SM walks tiles blockIdx.x, blockIdx.x + gridDim.x, ... (column blocks fastest, so the CTAs running together
 //   share rows of x in L2). Every mbarrier wait is bounded; a wait that runs out sets the error flag and the CTA winds down.
+#include "gelu.cuh"
 #include "tc_pair.cuh"
 
 namespace pgb {
@@ -43,21 +44,6 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap *map
 }
 __device__ __forceinline__ void lg_arrive(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-// GELU(x) = x Phi(x) with Phi(x) = 0.5 (1 + erf(x / sqrt 2)) written as a logistic function of an odd polynomial,
-// Phi(x) ~= 1 / (1 + exp(-2 x p(x^2))): p fitted (minimax, |x| <= 6, beyond which Phi is 0 or 1 to 1e-9) so that the result
-// is within 3.3e-5 of the erf form everywhere -- a sixtieth of the bf16 rounding of a value near 1. The logistic form has
-// no cancellation in either tail (1 + tanh would), and costs a dozen instructions with two special-function issues
-// against about twenty for an erf polynomial.
-__device__ __forceinline__ float lg_gelu(float x) {
-    // the coefficients carry the factor -2 log2(e); the square is clamped, so beyond |x| = 6 the exponent keeps growing with
-    // x and the result goes to x or to -0 as it should
-    const float z2 = fminf(x * x, 36.0f);
-    float p = fmaf(4.6257928e-05f, z2, 4.6197393e-04f);
-    p = fmaf(p, z2, -1.0517757e-01f);
-    p = fmaf(p, z2, -2.3021175e+00f);
-    const float e = fast_exp2(x * p);                                 // exp(-2 x p(x^2))
-    return __fdividef(x, 1.0f + e);
 }
 // columns of its block an epilogue warp stages at a time: half of a 64-column block, the whole of a 48-column one
 template <int CW> struct LgStage { static constexpr int cols = CW == 64 ? 32 : CW; };
