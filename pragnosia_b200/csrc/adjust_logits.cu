@@ -20,102 +20,168 @@ __device__ __forceinline__ int list_length(const TokenList &t, long long b) {
     return n < 0 ? 0 : n > t.n ? t.n : (int)n;
 }
 
-// NT threads, VPT words each: slices of NT VPT words. SEEN: 0x80000000 marks a word of the prompt, the rest counts the generated ones.
-template <typename T_, int NT, int VPT>
-__global__ void __launch_bounds__(NT) adjust_logits_kernel(AdjustLogits a, int slices) {
-    constexpr int S = NT * VPT;
+// NT threads, QT quads of words each: slices of 4 NT QT words that begin where the row's address is a multiple of four words, so that a quad is one load and one store (a
+// row's ends, and rows whose result lies otherwise than they do, go word by word). In a word's count IN_PROMPT marks one of the prompt, the rest counts the
+// generated ones. Everything that hangs on no other load is asked for first: logits, mask, lengths, and the ids up to HEAD a thread whether they count or not.
+template <typename T_, int NT, int QT, int PER_SM>
+__global__ void __launch_bounds__(NT, PER_SM) adjust_logits_kernel(const AdjustLogits a, const int slices) {
+    constexpr int S = 4 * NT * QT, HEAD = 2;
     constexpr uint32_t IN_PROMPT = 0x80000000u;
-    extern __shared__ uint32_t adj_smem[];
-    uint32_t *count = adj_smem;                                       // [S]
-    float *sbias = reinterpret_cast<float *>(adj_smem + S);           // [S] with biases
-    int *bid = reinterpret_cast<int *>(adj_smem + 2 * S);             // [nb]: place in the slice, -1 outside
+    extern __shared__ uint4 adj_smem[];
+    uint32_t *count = reinterpret_cast<uint32_t *>(adj_smem);         // [S]
+    float *sbias = reinterpret_cast<float *>(count + S);              // [S] with biases
+    int *bid = reinterpret_cast<int *>(count + 2 * S);                // [nb]: place in the slice, -1 outside
     float *bval = reinterpret_cast<float *>(bid + a.nb);
-    const int tid = threadIdx.x;
-    const long long b = blockIdx.x / slices;
-    const int v0 = (int)(blockIdx.x % slices) * S;
-    pdl_launch_dependents();
+    const int tid = threadIdx.x, lane = tid & 31;
+    const unsigned b = blockIdx.x / (unsigned)slices;
     pdl_wait();
+    pdl_launch_dependents();
 
-    const T_ *row = reinterpret_cast<const T_ *>(a.logits) + b * a.stride;
-    float l[VPT];
+    const long long *pid = a.prompt.ids + b * a.prompt.stride, *gid = a.made.ids + b * a.made.stride;
+    long long ph[HEAD], gh[HEAD];
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-        const int v = v0 + tid + i * NT;
-        l[i] = v < a.V ? to_f32(row[v]) : 0.f;
+    for (int i = 0; i < HEAD; ++i) {
+        ph[i] = tid + i * NT < a.prompt.n ? pid[tid + i * NT] : -1;
+        gh[i] = tid + i * NT < a.made.n ? gid[tid + i * NT] : -1;
     }
     const int np = list_length(a.prompt, b), ng = list_length(a.made, b);
+    const T_ *row = reinterpret_cast<const T_ *>(a.logits) + b * a.stride;
+    float *out = a.out + b * (long long)a.V;
+    const int shift = (int)(reinterpret_cast<uintptr_t>(row) / sizeof(T_) & 3);
+    const bool alike = shift == (int)(reinterpret_cast<uintptr_t>(out) / 4 & 3);
+    const int v0 = (int)(blockIdx.x - b * slices) * S - shift;        // below 0 in a row's first slice
+    T_ l[QT][4];
+    uint32_t banned = 0;
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) count[tid + i * NT] = 0u;
-    if (a.nb > 0) {
+    for (int q = 0; q < QT; ++q) {
+        const int v = v0 + 4 * (tid + q * NT);
+        const bool whole = v >= 0 && v + 4 <= a.V;
+        if (whole && alike) {
+            if constexpr (sizeof(T_) == 2) *reinterpret_cast<uint2 *>(l[q]) = *reinterpret_cast<const uint2 *>(row + v);
+            else *reinterpret_cast<uint4 *>(l[q]) = *reinterpret_cast<const uint4 *>(row + v);
+        } else {
 #pragma unroll
-        for (int i = 0; i < VPT; ++i) sbias[tid + i * NT] = 0.f;
-        for (int j = tid; j < a.nb; j += NT) {
-            const long long at = a.bias_ids[b * a.bias_stride + j] - v0;
-            const bool in = at >= 0 && at < S && at + v0 < a.V;
-            bid[j] = in ? (int)at : -1;
-            bval[j] = a.bias[b * a.bias_stride + j];
+            for (int e = 0; e < 4; ++e)
+                if (v + e >= 0 && v + e < a.V) l[q][e] = row[v + e];
+        }
+        if (a.mask_kind == 1) {
+            const uint32_t *m = reinterpret_cast<const uint32_t *>(a.mask) + b * a.mask_stride;
+            if (whole) banned |= (~__funnelshift_r(m[v >> 5], m[(v + 3) >> 5], v & 31) & 15u) << (4 * q);
+            else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (v + e >= 0 && v + e < a.V) banned |= (~m[(v + e) >> 5] >> ((v + e) & 31) & 1u) << (4 * q + e);
+            }
+        } else if (a.mask_kind == 2) {
+            const unsigned char *m = reinterpret_cast<const unsigned char *>(a.mask) + b * a.mask_stride;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (v + e >= 0 && v + e < a.V) banned |= (m[v + e] == 0 ? 1u : 0u) << (4 * q + e);
         }
     }
-    __syncthreads();
-    const long long *ids = a.prompt.ids + b * a.prompt.stride;
-#pragma unroll 8
-    for (int j = tid; j < np; j += NT) {
-        const long long at = ids[j] - v0;
-        if (at >= 0 && at < S && !(count[at] & IN_PROMPT)) atomicOr(&count[at], IN_PROMPT);
-    }
-    ids = a.made.ids + b * a.made.stride;
-#pragma unroll 8
-    for (int j = tid; j < ng; j += NT) {
-        const long long at = ids[j] - v0;
-        if (at >= 0 && at < S) atomicAdd(&count[at], 1u);
-    }
-    for (int j = tid; j < a.nb; j += NT) {
-        const int at = bid[j];
-        if (at < 0) continue;
-        bool first = true;
-        for (int i = 0; i < j; ++i) first = first && bid[i] != at;
-        if (!first) continue;
-        float s = bval[j];
-        for (int i = j + 1; i < a.nb; ++i)
-            if (bid[i] == at) s += bval[i];
-        sbias[at] = s;
-    }
-    __syncthreads();
-
     const float r = a.repetition.at ? a.repetition.at[b] : a.repetition.all, f = a.frequency.at ? a.frequency.at[b] : a.frequency.all,
                 p = a.presence.at ? a.presence.at[b] : a.presence.all;
-    float *out = a.out + b * (long long)a.V;
+    // an id's place in the slice; one that is not there (below 0, in another slice, past 32 bits) at S or beyond. Places past V are counted and not read.
+    auto place = [&](long long id) { return (uint32_t)(id >> 31) == 0u ? (uint32_t)((int)id - v0) : 0xffffffffu; };
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-        const int at = tid + i * NT, v = v0 + at;
-        if (v >= a.V) break;
-        float s = l[i];
-        const uint32_t c = count[at];
-        if (c != 0u) {
-            s = s > 0.f ? __fdiv_rn(s, r) : __fmul_rn(s, r);
-            const uint32_t n = c & ~IN_PROMPT;
-            if (n != 0u) s = __fsub_rn(__fsub_rn(s, __fmul_rn(f, (float)n)), p);
+    for (int q = 0; q < QT; ++q) {
+        reinterpret_cast<uint4 *>(count)[tid + q * NT] = make_uint4(0u, 0u, 0u, 0u);
+        if (a.nb > 0) reinterpret_cast<uint4 *>(sbias)[tid + q * NT] = make_uint4(0u, 0u, 0u, 0u);
+    }
+    for (int j = tid; j < a.nb; j += NT) {
+        const uint32_t at = place(a.bias_ids[b * a.bias_stride + j]);
+        bid[j] = at < S ? (int)at : -1;
+        bval[j] = a.bias[b * a.bias_stride + j];
+    }
+    __syncthreads();
+    auto prompt_id = [&](long long id) {
+        const uint32_t at = place(id);
+        if (at < S && !(count[at] & IN_PROMPT)) atomicOr(&count[at], IN_PROMPT);
+    };
+    auto made_id = [&](long long id) {
+        const uint32_t at = place(id);
+        if (at < S) atomicAdd(&count[at], 1u);
+    };
+#pragma unroll
+    for (int i = 0; i < HEAD; ++i) {
+        if (tid + i * NT < np) prompt_id(ph[i]);
+        if (tid + i * NT < ng) made_id(gh[i]);
+    }
+#pragma unroll 8
+    for (int j = tid + HEAD * NT; j < np; j += NT) prompt_id(pid[j]);
+#pragma unroll 8
+    for (int j = tid + HEAD * NT; j < ng; j += NT) made_id(gid[j]);
+    // A warp an entry: the first one that names a word adds up all that do, in their order.
+    for (int j = tid >> 5; j < a.nb; j += NT / 32) {
+        const int at = bid[j];
+        if (at < 0) continue;
+        float s = 0.f;
+        bool begun = false, mine = true;
+        for (int c = 0; c < a.nb && mine; c += 32) {
+            uint32_t same = __ballot_sync(0xffffffffu, c + lane < a.nb && bid[c + lane] == at);
+            if (!begun && same != 0u) {
+                begun = true;
+                mine = c + __ffs(same) - 1 == j;
+            }
+            for (; same != 0u && mine; same &= same - 1u) {
+                const float v = bval[c + __ffs(same) - 1];
+                s = c + __ffs(same) - 1 == j ? v : __fadd_rn(s, v);
+            }
         }
-        if (a.nb > 0) s = __fadd_rn(s, sbias[at]);
-        bool ok = true;
-        if (a.mask_kind == 1) ok = (reinterpret_cast<const uint32_t *>(a.mask)[b * a.mask_stride + (v >> 5)] >> (v & 31)) & 1u;
-        else if (a.mask_kind == 2) ok = reinterpret_cast<const unsigned char *>(a.mask)[b * a.mask_stride + v] != 0;
-        out[v] = ok ? s : -INFINITY;
+        if (mine && lane == 0) sbias[at] = s;
+    }
+    __syncthreads();
+
+#pragma unroll
+    for (int q = 0; q < QT; ++q) {
+        const int at = tid + q * NT, v = v0 + 4 * at;
+        float s[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[e] = to_f32(l[q][e]);
+        const uint4 c4 = reinterpret_cast<const uint4 *>(count)[at];
+        // A lane has few words that were seen, so a lane's words take turns: as many as the lane with the most has, not four.
+        uint32_t seen = (c4.x != 0u ? 1u : 0u) | (c4.y != 0u ? 2u : 0u) | (c4.z != 0u ? 4u : 0u) | (c4.w != 0u ? 8u : 0u);
+        while (seen != 0u) {
+            const int e = __ffs(seen) - 1;
+            seen &= seen - 1u;
+            const uint32_t n = (e < 2 ? (e == 0 ? c4.x : c4.y) : (e == 2 ? c4.z : c4.w)) & ~IN_PROMPT;
+            float x = e < 2 ? (e == 0 ? s[0] : s[1]) : (e == 2 ? s[2] : s[3]);
+            x = x > 0.f ? __fdiv_rn(x, r) : __fmul_rn(x, r);
+            if (n != 0u) x = __fsub_rn(__fsub_rn(x, __fmul_rn(f, (float)n)), p);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[i] = e == i ? x : s[i];
+        }
+        if (a.nb > 0) {
+            const float4 add = reinterpret_cast<const float4 *>(sbias)[at];
+            s[0] = __fadd_rn(s[0], add.x); s[1] = __fadd_rn(s[1], add.y); s[2] = __fadd_rn(s[2], add.z); s[3] = __fadd_rn(s[3], add.w);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (banned >> (4 * q + e) & 1u) s[e] = -INFINITY;
+        if (v >= 0 && v + 4 <= a.V && alike) *reinterpret_cast<float4 *>(out + v) = make_float4(s[0], s[1], s[2], s[3]);
+        else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (v + e >= 0 && v + e < a.V) out[v + e] = s[e];
+        }
     }
 }
 
-template <typename T_, int NT, int VPT>
+template <typename T_, int NT, int QT, int PER_SM>
 static cudaError_t adjust_go(const AdjustLogits &a, cudaStream_t stream) {
-    constexpr int S = NT * VPT;
-    const int slices = (a.V + S - 1) / S;
+    constexpr int S = 4 * NT * QT;
+    const int slices = (int)(((long long)a.V + 3 + S - 1) / S);       // a row's first slice may begin up to three words ahead of it
     const size_t smem = (size_t)S * 4 * (a.nb > 0 ? 2 : 1) + (size_t)a.nb * 8;
-    return pdl_launch(adjust_logits_kernel<T_, NT, VPT>, dim3((unsigned)(a.B * slices)), dim3(NT), smem, stream, a, slices);
+    return pdl_launch(adjust_logits_kernel<T_, NT, QT, PER_SM>, dim3((unsigned)(a.B * slices)), dim3(NT), smem, stream, a, slices);
+}
+template <typename T_>
+static cudaError_t adjust_types(const AdjustLogits &a, cudaStream_t stream) {
+    if (a.prompt.n + (long long)a.made.n > 4096) return adjust_go<T_, 1024, 1, 2>(a, stream);
+    if (a.B * ((a.V + 4095) / 4096) >= 2 * sm_count()) return adjust_go<T_, 512, 2, 3>(a, stream);
+    return adjust_go<T_, 256, 1, 6>(a, stream);
 }
 int adjust_logits_launch(const AdjustLogits &a, cudaStream_t stream) {
-    const bool many = a.prompt.n + a.made.n > 4096;
-    cudaError_t e;
-    if (a.dtype == PGB_BF16) e = many ? adjust_go<__nv_bfloat16, 1024, 4>(a, stream) : adjust_go<__nv_bfloat16, 256, 8>(a, stream);
-    else e = many ? adjust_go<float, 1024, 4>(a, stream) : adjust_go<float, 256, 8>(a, stream);
+    const cudaError_t e = a.dtype == PGB_BF16 ? adjust_types<__nv_bfloat16>(a, stream) : adjust_types<float>(a, stream);
     if (e != cudaSuccess) { set_cuda_error(e, "adjust_logits launch"); return PGB_ERR_CUDA; }
     return check_launch("adjust_logits_kernel");
 }

@@ -978,7 +978,7 @@ int pgb_adjust_logits(const void *logits, int dtype, long long row_stride, float
     if (B < 1 || V < 1 || prompt_n < 0 || generated_n < 0 || nb < 0 || mask_kind < 0 || mask_kind > 2 || (prompt_length_stride & ~1) ||
         (generated_length_stride & ~1) || (!repetition_rows && !(repetition > 0.f)))
         return PGB_ERR_BAD_SHAPE;
-    if (nb > 1024 || V > (1 << 30) || B > (1LL << 31) / ((V + 2047) / 2048) - 1) return PGB_ERR_TOO_LARGE;
+    if (nb > 1024 || V > (1 << 30) || B > (1LL << 31) / ((V + 1026) / 1024) - 1) return PGB_ERR_TOO_LARGE;
     if (!aligned_to(logits, dtype) || !aligned(out, 4) || !aligned(prompt, 8) || !aligned(generated, 8) || !aligned(prompt_lengths, 8) ||
         !aligned(generated_lengths, 8) || !aligned(repetition_rows, 4) || !aligned(frequency_rows, 4) || !aligned(presence_rows, 4) || !aligned(bias_ids, 8) ||
         !aligned(bias, 4) || (mask_kind == 1 && !aligned(mask, 4)))

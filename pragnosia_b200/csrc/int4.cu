@@ -40,61 +40,156 @@ template <typename T_> __device__ __forceinline__ void store8(T_ *p, const float
     }
 }
 
-template <typename T_, int GROUP>
+// QU pieces of eight columns a thread, 256 apart: what a thread has on its way. A CTA takes the whole rows that fit into its 256 QU pieces (magic = ceil(2^32 / per)
+// finds a piece's row; exact, both being below 2^11), or a part of one (magic 0), so nothing is divided on the device.
+constexpr int QU = 4, CTA_PIECES = 256 * QU;
+struct Pieces { int per, rows; unsigned magic; };                     // pieces of a row; rows of a CTA
+static inline Pieces pieces_of(int per) {
+    if (per > CTA_PIECES) return {per, 1, 0u};
+    return {per, CTA_PIECES / per, per == 1 ? 0xffffffffu : (unsigned)(((1ULL << 32) + per - 1) / per)};
+}
+static inline dim3 pieces_grid(const Pieces &p, int N) { return dim3((unsigned)((N + p.rows - 1) / p.rows), (unsigned)((p.per + CTA_PIECES - 1) / CTA_PIECES)); }
+// the thread's piece u: false where there is none
+__device__ __forceinline__ bool piece_at(const Pieces &p, int u, int N, int &n, int &piece) {
+    const unsigned j = blockIdx.y * CTA_PIECES + threadIdx.x + 256 * u, r = p.per == 1 ? j : __umulhi(j, p.magic);
+    n = blockIdx.x * p.rows + r;
+    piece = j - r * p.per;
+    return r < p.rows && n < N && piece < p.per;
+}
+
+// What bounds it: the arithmetic of a level, before the bytes. A level is the nearest whole number to the correctly rounded quotient w / s. The product with
+// an approximate 1 / s is within 3e-6 of the quotient (15 at most), so away from a tie both round alike: 1.5 2^23 added and taken off again rounds to even in two
+// additions, the distance to the result says how near a tie was, and where one of a thread's eight came close all eight are divided. Four levels are one fp32 number (16 bits)
+// before they become integers. At N 16384, K 4096 bf16 division, rounding and conversion a value took 109 us.
+template <typename T_, int GROUP, bool SYM>
 __global__ void __launch_bounds__(256) int4_quantize_kernel(const T_ *__restrict__ w, unsigned char *__restrict__ q, T_ *__restrict__ scales,
-                                                            unsigned char *__restrict__ zeros, int N, int K, int G) {
+                                                            unsigned char *__restrict__ zeros, int N, int K, int G, const Pieces pieces) {
     constexpr int PER = GROUP / 8;                                    // threads of a group
-    const long long idx = (long long)blockIdx.x * 256 + threadIdx.x;
-    const long long grp = idx / PER;                                  // row-major over (N, G)
-    const int part = (int)(idx % PER);
-    const bool row_live = grp < (long long)N * G;
-    const int n = row_live ? (int)(grp / G) : 0, col = row_live ? (int)(grp % G) * GROUP + part * 8 : K;
-    const bool live = row_live && col < K;
-    float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};            // zeros change no group's range
-    if (live) load8(w + (size_t)n * K + col, f);
-    float lo = 0.f, hi = 0.f, bad = 0.f;                              // bad: NaN where a value is not finite (x - x), else 0
+    constexpr float ROUND = 12582912.f;
+    constexpr int RAW = (int)sizeof(T_) * 2;                          // 32-bit registers of a piece
+    uint32_t v[QU][RAW];
+    int n[QU], piece[QU];
+    bool live[QU];
+    auto value = [&](int u, int i) {                                  // bf16: the even ones in the low halves
+        if constexpr (sizeof(T_) == 4) return __uint_as_float(v[u][i]);
+        else return __uint_as_float(i & 1 ? v[u][i / 2] & 0xffff0000u : v[u][i / 2] << 16);
+    };
 #pragma unroll
-    for (int i = 0; i < 8; ++i) { lo = fminf(lo, f[i]); hi = fmaxf(hi, f[i]); bad += f[i] - f[i]; }
+    for (int u = 0; u < QU; ++u) {
+        live[u] = piece_at(pieces, u, N, n[u], piece[u]) && piece[u] * 8 < K;
 #pragma unroll
-    for (int o = PER / 2; o > 0; o >>= 1) {
-        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-        bad += __shfl_xor_sync(0xffffffffu, bad, o);
+        for (int i = 0; i < RAW; ++i) v[u][i] = 0u;                   // zeros change no group's range
+        const uint4 *src = reinterpret_cast<const uint4 *>(w + (size_t)n[u] * K + piece[u] * 8);
+        if (live[u]) {
+#pragma unroll
+            for (int i = 0; i < RAW / 4; ++i) {
+                const uint4 x = __ldg(src + i);
+                v[u][4 * i] = x.x; v[u][4 * i + 1] = x.y; v[u][4 * i + 2] = x.z; v[u][4 * i + 3] = x.w;
+            }
+        }
     }
-    const bool sym = zeros == nullptr;
-    T_ st;
-    from_f32(st, sym ? __fdiv_rn(fmaxf(-lo, hi), 7.f) : __fdiv_rn(__fsub_rn(hi, lo), 15.f));
-    float s = to_f32(st);
-    if (bad != 0.f || !(s < INFINITY)) { s = nanf(""); from_f32(st, s); }
-    const bool flat = !(s > 0.f);                                     // no range, or NaN
-    const float z = sym ? 8.f : flat ? 0.f : fminf(fmaxf(rintf(__fdiv_rn(-lo, s)), 0.f), 15.f);
-    if (!live) return;
-    uint32_t packed = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float r = flat ? z : fminf(fmaxf(rintf(__fdiv_rn(f[i], s)) + z, 0.f), 15.f);
-        packed |= (uint32_t)r << (4 * i);
-    }
-    *reinterpret_cast<uint32_t *>(q + ((size_t)n * K + col) / 2) = packed;
-    if (part == 0) {
-        scales[grp] = st;
-        if (!sym) zeros[grp] = (unsigned char)z;
+    for (int u = 0; u < QU; ++u) {
+        float lo = 0.f, hi = 0.f;                                     // hi is NaN where a value is, and infinite where one is
+        if constexpr (sizeof(T_) == 2) {                              // two at a time, and both ends of the range in one register: (hi, -lo)
+            __nv_bfloat162 x[4], m;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const __nv_bfloat162 *>(&v[u][i]);
+            if constexpr (SYM) m = __hmax2_nan(__hmax2_nan(__habs2(x[0]), __habs2(x[1])), __hmax2_nan(__habs2(x[2]), __habs2(x[3])));
+            else {
+                const __nv_bfloat162 top = __hmax2_nan(__hmax2_nan(x[0], x[1]), __hmax2_nan(x[2], x[3])), low = __hmin2_nan(__hmin2_nan(x[0], x[1]), __hmin2_nan(x[2], x[3]));
+                m = __hmax2_nan(__lows2bfloat162(top, __hneg2(low)), __highs2bfloat162(top, __hneg2(low)));
+            }
+#pragma unroll
+            for (int o = PER / 2; o > 0; o >>= 1) m = __hmax2_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+            if constexpr (SYM) m = __hmax2_nan(m, __lowhigh2highlow(m));
+            else m = __hmax2_nan(m, __floats2bfloat162_rn(0.f, 0.f));
+            hi = __low2float(m);
+            if constexpr (!SYM) lo = -__high2float(m);
+        } else {
+            float bad = 0.f;                                          // NaN where a value is not finite, else 0
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float f = value(u, i);
+                if constexpr (SYM) hi = fmaxf(hi, fabsf(f));
+                else { lo = fminf(lo, f); hi = fmaxf(hi, f); }
+                bad = fmaf(f, 0.f, bad);
+            }
+            if (bad != 0.f) hi = INFINITY;
+#pragma unroll
+            for (int o = PER / 2; o > 0; o >>= 1) {
+                if constexpr (!SYM) lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+                hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+            }
+        }
+        T_ st;
+        from_f32(st, SYM ? __fdiv_rn(hi, 7.f) : __fdiv_rn(__fsub_rn(hi, lo), 15.f));
+        float s = to_f32(st);
+        if (!(s < INFINITY)) { s = nanf(""); from_f32(st, s); }
+        const bool flat = !(s > 0.f);                                 // no range, or NaN
+        const float z = SYM ? 8.f : flat ? 0.f : fminf(rintf(__fdiv_rn(-lo, s)), 15.f), inv = flat ? 0.f : __fdividef(1.f, s);
+        if (!live[u]) continue;
+        float r[8], far = s < 1e-30f && !flat ? 1.f : 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float t = value(u, i) * inv;
+            r[i] = __fadd_rn(__fadd_rn(t, ROUND), -ROUND);
+            far = fmaxf(far, fabsf(t - r[i]));
+        }
+        if (far > 0.49998f) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) r[i] = rintf(__fdiv_rn(value(u, i), s));
+        }
+        // levels below 0 cannot come up: the lowest value's quotient is the zero's with the sign changed
+#pragma unroll
+        for (int i = 0; i < 8; ++i) r[i] = SYM ? r[i] + z : fminf(r[i] + z, 15.f);
+        const float half0 = fmaf(fmaf(fmaf(r[3], 16.f, r[2]), 16.f, r[1]), 16.f, r[0]), half1 = fmaf(fmaf(fmaf(r[7], 16.f, r[6]), 16.f, r[5]), 16.f, r[4]);
+        *reinterpret_cast<uint32_t *>(q + (size_t)n[u] * (K / 2) + piece[u] * 4) =
+            __byte_perm(__float_as_uint(half0 + 8388608.f), __float_as_uint(half1 + 8388608.f), 0x5410);
+        if (piece[u] % PER == 0) {
+            const size_t grp = (size_t)n[u] * G + piece[u] / PER;
+            scales[grp] = st;
+            if constexpr (!SYM) zeros[grp] = (unsigned char)z;
+        }
     }
 }
 
+// q - z without a conversion: 0x4b000000 | q is 2^23 + q, less 2^23 + z; bf16 from bf16 scales two at a time, 128 + q less 128 + z, times the scale in its one rounding.
 template <typename T_, typename O_>
 __global__ void __launch_bounds__(256) int4_dequantize_kernel(const unsigned char *__restrict__ q, const T_ *__restrict__ scales,
-                                                              const unsigned char *__restrict__ zeros, O_ *__restrict__ w, int N, int K, int G, int lg) {
-    const long long i8 = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (i8 >= (long long)N * K / 8) return;
-    const int per = K / 8, n = (int)(i8 / per), col = (int)(i8 % per) * 8;
-    const size_t at = (size_t)n * G + (col >> lg);
-    const uint32_t p = reinterpret_cast<const uint32_t *>(q)[i8];
-    const float s = to_f32(scales[at]), z = zeros != nullptr ? (float)zeros[at] : 8.f;
-    float f[8];
+                                                              const unsigned char *__restrict__ zeros, O_ *__restrict__ w, int N, int K, int G, int lg, const Pieces pieces) {
+    uint32_t p[QU], z[QU];
+    T_ s[QU];
+    int n[QU], piece[QU];
+    bool live[QU];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = s * ((float)((p >> (4 * i)) & 15u) - z);
-    store8(w + (size_t)i8 * 8, f);
+    for (int u = 0; u < QU; ++u) {
+        live[u] = piece_at(pieces, u, N, n[u], piece[u]);
+        if (!live[u]) continue;
+        const size_t at = (size_t)n[u] * G + (piece[u] * 8 >> lg);
+        p[u] = *reinterpret_cast<const uint32_t *>(q + (size_t)n[u] * (K / 2) + piece[u] * 4);
+        s[u] = scales[at];
+        z[u] = zeros != nullptr ? zeros[at] : 8u;
+    }
+#pragma unroll
+    for (int u = 0; u < QU; ++u) {
+        if (!live[u]) continue;
+        O_ *out = w + (size_t)n[u] * K + piece[u] * 8;
+        if constexpr (sizeof(T_) == 2 && sizeof(O_) == 2) {
+            const uint32_t z2 = __byte_perm(z[u], 0x43u, 0x4040), s2 = (uint32_t)__bfloat16_as_ushort(s[u]) * 0x10001u;
+            uint32_t v[4];
+#pragma unroll
+            for (int h = 0; h < 4; ++h) v[h] = mul_bf16x2(level_pair(p[u] >> (4 * h), z2), s2);       // (0,4) (1,5) (2,6) (3,7)
+            *reinterpret_cast<uint4 *>(out) = make_uint4(__byte_perm(v[0], v[1], 0x5410), __byte_perm(v[2], v[3], 0x5410), __byte_perm(v[0], v[1], 0x7632),
+                                                         __byte_perm(v[2], v[3], 0x7632));
+        } else {
+            const float sf = to_f32(s[u]), zf = 8388608.f + (float)z[u];
+            float f[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] = sf * (__uint_as_float(((p[u] >> (4 * i)) & 15u) | 0x4b000000u) - zf);
+            store8(out, f);
+        }
+    }
 }
 
 // ------------------------------------------------------------------------------------------------ linear
@@ -354,12 +449,14 @@ static inline int log2_group(int group) { return group == 32 ? 5 : group == 64 ?
 template <typename T_>
 static void quantize_go(const void *w, unsigned char *q, void *scales, unsigned char *zeros, int N, int K, int group, cudaStream_t stream) {
     const int G = (K + group - 1) / group;
-    const unsigned grid = (unsigned)(((long long)N * G * (group / 8) + 255) / 256);
-    const T_ *wp = (const T_ *)w;
-    T_ *sp = (T_ *)scales;
-    if (group == 32) int4_quantize_kernel<T_, 32><<<grid, 256, 0, stream>>>(wp, q, sp, zeros, N, K, G);
-    else if (group == 64) int4_quantize_kernel<T_, 64><<<grid, 256, 0, stream>>>(wp, q, sp, zeros, N, K, G);
-    else int4_quantize_kernel<T_, 128><<<grid, 256, 0, stream>>>(wp, q, sp, zeros, N, K, G);
+    const Pieces pieces = pieces_of(G * (group / 8));
+    const dim3 grid = pieces_grid(pieces, N);
+    auto go = [&](auto *kernel) { kernel<<<grid, 256, 0, stream>>>((const T_ *)w, q, (T_ *)scales, zeros, N, K, G, pieces); };
+    if (zeros != nullptr) {
+        if (group == 32) go(int4_quantize_kernel<T_, 32, false>); else if (group == 64) go(int4_quantize_kernel<T_, 64, false>); else go(int4_quantize_kernel<T_, 128, false>);
+    } else {
+        if (group == 32) go(int4_quantize_kernel<T_, 32, true>); else if (group == 64) go(int4_quantize_kernel<T_, 64, true>); else go(int4_quantize_kernel<T_, 128, true>);
+    }
 }
 int int4_quantize_launch(const void *w, int dtype, unsigned char *q, void *scales, unsigned char *zeros, int N, int K, int group, cudaStream_t stream) {
     if (dtype == PGB_BF16) quantize_go<__nv_bfloat16>(w, q, scales, zeros, N, K, group, stream);
@@ -368,15 +465,16 @@ int int4_quantize_launch(const void *w, int dtype, unsigned char *q, void *scale
 }
 
 int int4_dequantize_launch(const Int4Weight &w, void *out, int out_dtype, cudaStream_t stream) {
-    const unsigned grid = (unsigned)(((long long)w.N * w.K / 8 + 255) / 256);
+    const Pieces pieces = pieces_of(w.K / 8);
+    const dim3 grid = pieces_grid(pieces, w.N);
     const int lg = log2_group(w.group);
     const bool sb = w.scale_dtype == PGB_BF16, ob = out_dtype == PGB_BF16;
     const __nv_bfloat16 *s16 = (const __nv_bfloat16 *)w.scales;
     const float *s32 = (const float *)w.scales;
-    if (sb && ob) int4_dequantize_kernel<<<grid, 256, 0, stream>>>(w.q, s16, w.zeros, (__nv_bfloat16 *)out, w.N, w.K, w.G, lg);
-    else if (sb) int4_dequantize_kernel<<<grid, 256, 0, stream>>>(w.q, s16, w.zeros, (float *)out, w.N, w.K, w.G, lg);
-    else if (ob) int4_dequantize_kernel<<<grid, 256, 0, stream>>>(w.q, s32, w.zeros, (__nv_bfloat16 *)out, w.N, w.K, w.G, lg);
-    else int4_dequantize_kernel<<<grid, 256, 0, stream>>>(w.q, s32, w.zeros, (float *)out, w.N, w.K, w.G, lg);
+    if (sb && ob) int4_dequantize_kernel<<<grid, 256, 0, stream>>>(w.q, s16, w.zeros, (__nv_bfloat16 *)out, w.N, w.K, w.G, lg, pieces);
+    else if (sb) int4_dequantize_kernel<<<grid, 256, 0, stream>>>(w.q, s16, w.zeros, (float *)out, w.N, w.K, w.G, lg, pieces);
+    else if (ob) int4_dequantize_kernel<<<grid, 256, 0, stream>>>(w.q, s32, w.zeros, (__nv_bfloat16 *)out, w.N, w.K, w.G, lg, pieces);
+    else int4_dequantize_kernel<<<grid, 256, 0, stream>>>(w.q, s32, w.zeros, (float *)out, w.N, w.K, w.G, lg, pieces);
     return check_launch("int4_dequantize_kernel");
 }
 
