@@ -13,14 +13,16 @@ import numpy as np
 import torch
 import torch.nn.functional as F
 
-from . import ops
+from . import int4 as int4_ops, ops, sampling
 from ._lib import warm_up
 from .assoc import AssocCarrier
 
 
 class Decoder:
     def __init__(self, model, batch: int, use_graph: bool = True, fused: bool = True, min_p: float = 0.0,
-                 token_kernel: bool = True, folded: bool = False):
+                 token_kernel: bool = True, folded: bool = False, int4: Optional[int] = None, controls: Optional[sampling.Controls] = None):
+        """int4: tokens are stepped with the layers' linear weights in four bits, a scale and a zero per group of so many columns (32, 64 or 128); prompts and
+        the head keep the model's own. controls: what is done to the logits ahead of each draw of generate()."""
         self.m = model.eval()
         self.min_p = float(min_p)                            # drop ids below min_p x the most likely one's probability (src/bench.py:38)
         self.B = batch
@@ -28,7 +30,11 @@ class Decoder:
         self.fused = fused                                   # small-batch bf16 step through the fused linear kernel
         self.token_kernel = token_kernel                     # ... and, where it applies, the whole step as one launch
         self.folded = folded                                 # batches 5..128: this library's tensor-core linear with the norms folded in
+        self.int4, self.controls = int4, controls
         self._plan = None
+        self._four = None
+        if int4 is not None:
+            self._check_int4()
         self.dev = next(model.parameters()).device
         self.w = model.ctx
         self.states = None
@@ -92,7 +98,7 @@ class Decoder:
         0.30 / 0.33 / 0.37 ms per token at batch 1 / 2 / 4 against 0.45-0.48 through the library GEMMs; from batch 8 on
         the library path wins)."""
         m = self.m
-        return (self.fused and self.B <= 4 and m.e.weight.dtype == torch.bfloat16 and m.d % 8 == 0 and
+        return (self.fused and self.int4 is None and self.B <= 4 and m.e.weight.dtype == torch.bfloat16 and m.d % 8 == 0 and
                 all(isinstance(mx, AssocCarrier) and mx.plain_step for mx in m.mix))
 
     def _token_ok(self):
@@ -181,6 +187,8 @@ class Decoder:
             return 1 + 1 + 5 * L + 1 + 1                      # draw, embedding, five per layer, head, logits copy
         if self._chain_ok():
             return 1 + 1 + 5 * L + 1                          # draw, embedding, five per layer, head
+        if self.int4 is not None:
+            return 1 + 1 + 7 * L + 3                          # draw, embedding, seven per layer (two add + norm, four linear, state), add + norm, head, logits copy
         per_layer = 2 + 1 + 1 + 1 + 1 + 1 + 1            # two add+norm, projection, state step, output projection, MLP up (+GELU) and down
         return 1 + 3 + per_layer * L + 2 + 1               # draw; embedding gather x2 + add; layers; final add+norm, head; logits copy
 
@@ -208,7 +216,7 @@ class Decoder:
         is never rounded to bf16 where a separate norm is. The default rounds after every linear layer, norm, activation and add,
         as the oracle's bf16 mode does; only the order of fp32 sums inside a product differs between its kernels."""
         m = self.m
-        return (self.fused and self.folded and 4 < self.B <= 128 and m.e.weight.dtype == torch.bfloat16 and m.d % 8 == 0 and
+        return (self.fused and self.int4 is None and self.folded and 4 < self.B <= 128 and m.e.weight.dtype == torch.bfloat16 and m.d % 8 == 0 and
                 m.e.weight.shape[0] % 8 == 0 and all(isinstance(mx, AssocCarrier) and mx.plain_step for mx in m.mix) and
                 all(mp.a.weight.shape[0] % 8 == 0 for mp in m.mlp))
 
@@ -248,7 +256,7 @@ class Decoder:
         exactly these types (a carrier's subclass may have a mix of its own; a parametrized weight would be formed between two links, the second of which
         reads it ahead of its wait); else the separate kernels."""
         m = self.m
-        if not (self.fused and not self.folded and 4 < self.B <= 64 and m.e.weight.is_cuda and m.e.weight.dtype == m.p.weight.dtype == torch.bfloat16 and
+        if not (self.fused and self.int4 is None and not self.folded and 4 < self.B <= 64 and m.e.weight.is_cuda and m.e.weight.dtype == m.p.weight.dtype == torch.bfloat16 and
                 type(m.e) is type(m.p) is torch.nn.Embedding and all(type(mx) is AssocCarrier and mx.plain_step for mx in m.mix) and
                 all(mp.fused_up and type(mp.a) is type(mp.b) is torch.nn.Linear for mp in m.mlp)):
             return False
@@ -285,7 +293,60 @@ class Decoder:
             out = torch.empty(self.B, m.e.weight.shape[0], dtype=torch.float32, device=self.dev)
         return ops.decode_linear(xw, m.e.weight, None, sq, eps(m.n), logits=out, pos=self.pos, shift=self.shift, window=self.w if advance else 0)
 
+    def _check_int4(self):
+        m, group = self.m, self.int4
+        if group not in (32, 64, 128):
+            raise ValueError(f"Decoder: int4 is a group of 32, 64 or 128 columns, got {group}")
+        if not all(isinstance(mx, AssocCarrier) and mx.plain_step for mx in m.mix) or not all(type(mp.a) is type(mp.b) is torch.nn.Linear for mp in m.mlp):
+            raise ValueError("Decoder: int4 takes associative carrier layers without options and plain nn.Linear feed-forward layers")
+        widths = [m.d, *(mp.b.weight.shape[1] for mp in m.mlp)]
+        if any(w % 32 for w in widths):
+            raise ValueError(f"Decoder: int4 takes widths that are multiples of 32, got {sorted(set(widths))}")
+
+    def _int4_weights(self):
+        """Per layer, the fused projection, the gated output weight and the feed-forward weights in four bits; rebuilt with the weights' stamp."""
+        if self._four is None or self._four[0] != self._stamp:
+            with torch.no_grad():
+                four = lambda W: int4_ops.quantize(W.detach(), self.int4)
+                per = [(four(mx._consts()["W"]), four(mx._consts()["ow"]), four(mp.a.weight), four(mp.b.weight)) for mx, mp in zip(self.m.mix, self.m.mlp)]
+            self._four = (self._stamp, per)
+        return self._four[1]
+
+    def _step_int4(self, advance: bool = True):
+        """The separate kernels with the four linear layers of each block reading four-bit weights (int4.linear; behind the embedding's kernel everything ahead of the token
+        is complete, so they are read early). It pays where a token's time is its weights' bytes: twelve layers with MLP 4 d, us a token, default / four bits with groups of 64:
+        d 2048 batch 1 460 / 554, 4 796 / 537, 8 844 / 596, 16 853 / 738, 64 945 / 867; d 768 batch 1 155 / 223, 64 319 / 553."""
+        m = self.m
+        per = self._int4_weights()
+        if m.e.weight.dtype == torch.bfloat16 and m.d % 8 == 0:
+            x = ops.decode_embed(self.tok, self.pos, m.e.weight, m.p.weight)
+        else:
+            x = (m.e(self.tok) + m.p(self.pos)).view(self.B, m.d)
+        delta = None
+        for i, (mx, mp, (W, ow, a, b)) in enumerate(zip(m.mix, m.mlp, per)):
+            x, z = m._add_norm(x, delta, mx.ln)
+            y = int4_ops.linear(z, W, mx._consts()["b"], constant=True)
+            o, _ = mx.step_from_projection(y, self.states[i][0], self.shift, inplace=True)
+            delta = int4_ops.linear(o, ow, constant=True)
+            x, z = m._add_norm(x, delta, mp.n)
+            h = int4_ops.linear(z, a, mp.a.bias, act="gelu", constant=True)
+            delta = int4_ops.linear(h, b, mp.b.bias, constant=True)
+        if advance:
+            self._advance()
+        return self._head(m._add_norm(x, delta, m.n)[1])
+
+    def _head(self, z):
+        """Logits of the final norm's rows."""
+        m = self.m
+        if self.B <= 128 and z.dtype == torch.bfloat16 and m.e.weight.dtype == torch.bfloat16 and m.d % 8 == 0 and m.e.weight.shape[0] % 8 == 0:
+            # the tied head for up to 128 rows on this library's tensor-core kernel: for 64 rows by 8192 columns the
+            # library's heuristic picked a kernel that took 78 us, a sixth of the whole step
+            return ops.batch_linear(z.reshape(self.B, m.d), m.e.weight).float()
+        return F.linear(z.reshape(self.B, m.d), m.e.weight).float()
+
     def _step(self, advance: bool = True):
+        if self.int4 is not None:
+            return self._step_int4(advance)
         if self._token_ok():
             return self._step_token(advance)
         if self._fused_ok():
@@ -314,12 +375,7 @@ class Decoder:
             delta = self._ff_rows(mp, z)
         if advance:
             self._advance()
-        z = m._add_norm(x, delta, m.n)[1]
-        if self.B <= 128 and z.dtype == torch.bfloat16 and m.e.weight.dtype == torch.bfloat16 and m.d % 8 == 0 and m.e.weight.shape[0] % 8 == 0:
-            # the tied head for up to 128 rows on this library's tensor-core kernel: for 64 rows by 8192 columns the
-            # library's heuristic picked a kernel that took 78 us, a sixth of the whole step
-            return ops.batch_linear(z.reshape(self.B, m.d), m.e.weight).float()
-        return F.linear(z, m.e.weight)[:, -1].float()
+        return self._head(m._add_norm(x, delta, m.n)[1])
 
     @torch.no_grad()
     def step(self, tok: torch.Tensor):
@@ -334,7 +390,7 @@ class Decoder:
             with warm_up(s):
                 for _ in range(2): self._step()
                 self._graph, self.logits, held = self.m.capture(s, self._step)
-            self._held = (held, getattr(self, "_wide", None), self._plan)     # what the graph reads, for as long as it lives
+            self._held = (held, getattr(self, "_wide", None), self._plan, self._four)     # what the graph reads, for as long as it lives
             for st, sv in zip(self.states, saved):           # warm-up and capture advanced the state: restore it
                 for a, b in zip(st, sv):
                     if torch.is_tensor(a): a.copy_(b)
@@ -354,22 +410,50 @@ class Decoder:
         """prompt_ids (B,Tp) -> sampled ids (B,n). With use_graph the draw, the bookkeeping and the model step of one token
         are a single CUDA-graph replay (no per-token work on the host besides the replay itself)."""
         lg = self.prefill(prompt_ids)
+        key = self._set_controls(prompt_ids)
         if self.use_graph:
-            return self._generate_graphed(lg, n, temp, seed)
+            return self._generate_graphed(lg, n, temp, seed, key)
         out = torch.zeros(self.B, max(n, 1), dtype=torch.long, device=self.dev)
         cnt = torch.zeros(1, dtype=torch.long, device=self.dev)
         ticket = torch.zeros(1, dtype=torch.int32, device=self.dev)
         nxt = torch.empty(self.B, dtype=torch.long, device=self.dev)
         for _ in range(n):                                   # the same draws as the graphed loop, launched one by one
-            ops.decode_sample(lg, temp, seed, nxt, cnt, ticket, hist=out, min_p=self.min_p)
+            ops.decode_sample(self._adjusted(lg, out, cnt), temp, seed, nxt, cnt, ticket, hist=out, min_p=self.min_p)
             lg = self.step(nxt)
         return out[:, :n]
+
+    def _set_controls(self, prompt_ids):
+        """The controls' tensors and the prompt in buffers of this decoder's own, which a captured loop reads; returns what tells such loops apart: numbers,
+        shapes, and the room for the prompt (a power of two, so that prompts of many lengths share a loop)."""
+        c = self.controls
+        if c is None or c.idle:
+            self._ctl, self._ctl_key = None, None
+            return None
+        given = dict(c.tensors())
+        if c.sees_prompt:
+            room = 1 << max(6, (prompt_ids.shape[1] - 1).bit_length())
+            given["prompt"] = F.pad(prompt_ids.to(torch.long), (0, room - prompt_ids.shape[1]), value=-1)
+        if any(not t.is_cuda or t.device != prompt_ids.device for t in given.values()):
+            raise ValueError("Decoder: the controls' tensors are on the prompt's device")
+        key = (tuple(sorted(c.numbers().items())), tuple(sorted((k, tuple(t.shape), t.dtype) for k, t in given.items())))
+        if getattr(self, "_ctl_key", None) != key:
+            self._ctl, self._ctl_key = {k: torch.empty(t.shape, dtype=t.dtype, device=t.device) for k, t in given.items()}, key
+            self._ctl_numbers = c.numbers()
+        for k, t in given.items():
+            self._ctl[k].copy_(t)
+        return key
+
+    def _adjusted(self, lg, hist, cnt):
+        """The logits as the draw takes them: with the controls applied, history from the prompt and the tokens drawn so far."""
+        if self._ctl is None:
+            return lg
+        return sampling.adjust_logits(lg, generated=hist, generated_lengths=cnt, **self._ctl_numbers, **self._ctl)
 
     def _token_body(self, temp: float, seed: int):
         """Draw from the waiting logits, record the token at the running index, run the model on the token, leave the next
         logits waiting: a fixed kernel sequence, nothing on the host. The position and the rebase shift belong to the token
         being fed, so the draw kernel advances them for the PREVIOUS token (from the second token on) before the step."""
-        ops.decode_sample(self._lg_in, temp, seed, self.tok, self._cnt, self._ticket, hist=self._hist, pos=self.pos,
+        ops.decode_sample(self._adjusted(self._lg_in, self._hist, self._cnt), temp, seed, self.tok, self._cnt, self._ticket, hist=self._hist, pos=self.pos,
                           shift=self.shift, ctx=self.w, min_p=self.min_p)
         if self._token_ok():
             self._step_token(advance=False, out=self._lg_in)  # the step writes the waiting logits itself
@@ -378,8 +462,8 @@ class Decoder:
         else:
             self._lg_in.copy_(self._step(advance=False))
 
-    def _generate_graphed(self, lg, n: int, temp: float, seed: int):
-        key = (n, float(temp), int(seed), self.min_p)
+    def _generate_graphed(self, lg, n: int, temp: float, seed: int, controls=None):
+        key = (n, float(temp), int(seed), self.min_p, controls)
         if getattr(self, "_gen_key", None) != key:
             V = lg.shape[-1]
             self._lg_in = torch.empty(self.B, V, dtype=torch.float32, device=self.dev)
@@ -393,7 +477,7 @@ class Decoder:
             with warm_up(s):
                 for _ in range(2): self._token_body(temp, seed)
                 self._gen_graph, _, held = self.m.capture(s, lambda: self._token_body(temp, seed))
-            self._gen_held = (held, getattr(self, "_wide", None), self._plan)
+            self._gen_held = (held, self._ctl, getattr(self, "_wide", None), self._plan, self._four)
             for st, sv in zip(self.states, saved):           # warm-up and capture advanced the state: restore it
                 for a, b in zip(st, sv):
                     if torch.is_tensor(a): a.copy_(b)

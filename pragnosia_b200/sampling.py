@@ -5,6 +5,9 @@ CUDA tensors, torch's current stream, no synchronisation; no gradient (a call th
 """
 from __future__ import annotations
 
+from dataclasses import dataclass
+from typing import Optional, Union
+
 import torch
 
 from ._lib import host
@@ -36,3 +39,33 @@ def adjust_logits(logits, *, prompt=None, prompt_lengths=None, generated=None, g
     from . import custom_ops  # noqa: F401  (registers the operator)
     done = torch.ops.pragnosia_b200.adjust_logits(logits, prompt, prompt_lengths, generated, generated_lengths, rt, r, ft, f, pt, p, bias_ids, bias, mask)
     return done if out is None else out.copy_(done)
+
+
+@dataclass
+class Controls:
+    """What a decoder does to logits ahead of each draw (adjust_logits' settings): numbers, or tensors with a value per sequence; bias (ids, values); mask as
+    there, the same for every token. The prompt counts for the repetition, the generated tokens for all three."""
+    repetition: Union[float, torch.Tensor] = 1.0
+    frequency: Union[float, torch.Tensor] = 0.0
+    presence: Union[float, torch.Tensor] = 0.0
+    bias: Optional[tuple] = None
+    mask: Optional[torch.Tensor] = None
+
+    def tensors(self) -> dict:
+        """The settings that are tensors, by adjust_logits' names."""
+        named = dict(repetition=self.repetition, frequency=self.frequency, presence=self.presence, mask=self.mask)
+        if self.bias is not None:
+            named["bias_ids"], named["bias"] = self.bias
+        return {k: t for k, t in named.items() if torch.is_tensor(t)}
+
+    def numbers(self) -> dict:
+        return {k: float(v) for k, v in (("repetition", self.repetition), ("frequency", self.frequency), ("presence", self.presence)) if not torch.is_tensor(v)}
+
+    @property
+    def sees_prompt(self) -> bool:
+        return torch.is_tensor(self.repetition) or self.repetition != 1.0
+
+    @property
+    def idle(self) -> bool:
+        """Whether logits leave as they came."""
+        return not self.tensors() and not self.sees_prompt and self.frequency == 0.0 and self.presence == 0.0
