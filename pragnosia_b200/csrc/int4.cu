@@ -226,40 +226,48 @@ __global__ void __launch_bounds__(RW_MOST * 32) int4_rows_kernel(const RowsArgs 
     const int rows = a.M - m0 < 8 * NB ? (int)(a.M - m0) : 8 * NB;
     uint8_t *ring = rw_smem + warp * a.slots * a.slot_bytes;
     const uint32_t ring_at = smem_u32(ring);
+    // what rows of x that are not there are read as: 32 bytes of zeros behind the slots; an offset either way, so that lanes with and without a row load together
+    const int nothing = a.warps * a.slots * a.slot_bytes;
     const int C = (a.K + 127) >> 7, c0 = warp * a.each, mine = C - c0 < a.each ? C - c0 : a.each;     // this warp's stretches: c0, c0 + 1, ..
     const int ahead = a.ahead;
 
-    // this lane's piece of eight rows at a time (row lane / 4, columns 32 (lane mod 4) ..) of a stretch
+    // this lane's piece of eight rows at a time (row lane / 4, columns 32 (lane mod 4) ..) of a stretch. Rows past the last one are read as that one: what comes of them is not stored.
     const int fr = lane >> 2, half = a.K >> 1;
-    uint32_t live = 0;                                                // which of those rows are there
+    int wcol = c0 * 128 + t * 32;
+    const unsigned char *wsrc = a.q + (size_t)n0 * half + (wcol >> 1);
+    uint32_t woff_g[2 * MT];                                          // below 64 rows of 2^23 bytes
 #pragma unroll
-    for (int u = 0; u < 2 * MT; ++u) live |= (n0 + u * 8 + fr < a.N ? 1u : 0u) << u;
-    int wcol = c0 * 128 + t * 32, xcol = c0 * 128;
-    const unsigned char *wsrc = a.q + (size_t)(n0 + fr) * half + (wcol >> 1);
-    const size_t eight = (size_t)8 * half;
+    for (int u = 0; u < 2 * MT; ++u) {
+        const int r = 8 * u + fr;
+        woff_g[u] = (uint32_t)(n0 + r < a.N ? r : a.N - 1 - n0) * (uint32_t)half;
+    }
     const uint32_t wdst = ring_at + fr * 64 + ((t ^ ((fr >> 1) & 3)) << 4);
-    const uint8_t *xsrc = reinterpret_cast<const uint8_t *>(a.x) + (size_t)m0 * a.K * XE;
+    // x: pieces of 64 B of a row, [piece][row]; this lane's 16-byte chunk xc of every XR-th row from xr on
+    constexpr int CHUNKS = X32 ? 32 : 16, XR = 32 / CHUNKS;
+    const int xc = lane & (CHUNKS - 1), xr = lane / CHUNKS;
+    int xcol = c0 * 128 + xc * (16 / XE);
+    const uint8_t *xsrc = reinterpret_cast<const uint8_t *>(a.x) + ((size_t)(m0 + xr) * a.K + xcol) * XE;
+    const size_t xstep = (size_t)XR * a.K * XE;
+    const uint32_t xdst = ring_at + R * 64 + ((xc >> 2) * rows + xr) * 64 + (xc & 3) * 16;
 
     auto fetch_w = [&](int slot) {                                    // the next stretch of levels
-        const uint32_t ok = wcol < a.K ? live : 0u, dst = wdst + slot * a.slot_bytes;
-        const unsigned char *p = wsrc;
+        const bool in = wcol < a.K;
+        const unsigned char *p = in ? wsrc : a.q;
+        const uint32_t dst = wdst + slot * a.slot_bytes;
 #pragma unroll
-        for (int u = 0; u < 2 * MT; ++u) {
-            const bool in = ok >> u & 1u;
-            cp_async16(dst + u * 512, in ? p : a.q, in ? 16 : 0);
-            p += eight;
-        }
+        for (int u = 0; u < 2 * MT; ++u) cp_async16(dst + u * 512, p + (in ? woff_g[u] : 0u), in ? 16 : 0);
         wcol += 128; wsrc += 64;
     };
-    auto fetch_x = [&](int slot) {                                    // and of x: pieces of 64 B of a row, [piece][row]
-        constexpr int PC = X32 ? 5 : 4;                               // log2 of the 16-byte chunks of a row's stretch
-        const uint32_t dst = ring_at + slot * a.slot_bytes + R * 64;
-        for (int u = lane; u < rows << PC; u += 32) {
-            const int c = u & ((1 << PC) - 1), r = u >> PC, k = xcol + c * (16 / XE);
-            const bool in = k < a.K;
-            cp_async16(dst + ((c >> 2) * rows + r) * 64 + (c & 3) * 16, xsrc + (in ? ((size_t)r * a.K + k) * XE : 0), in ? 16 : 0);
+    auto fetch_x = [&](int slot) {                                    // and of x
+        const bool in = xcol < a.K;
+        const uint8_t *p = xsrc;
+        uint32_t dst = xdst + slot * a.slot_bytes;
+        for (int r = xr; r < rows; r += XR) {
+            cp_async16(dst, in ? p : reinterpret_cast<const uint8_t *>(a.x), in ? 16 : 0);
+            p += xstep;
+            dst += XR * 64;
         }
-        xcol += 128;
+        xcol += 128; xsrc += 128 * XE;
     };
     // scales and zeros of this lane's rows (g, g + 8 of every block of 16) for group t of the next four groups: the scale's bits with 128 + z below them
     // (fp32 scales: in a word of their own)
@@ -288,11 +296,16 @@ __global__ void __launch_bounds__(RW_MOST * 32) int4_rows_kernel(const RowsArgs 
     if (a.constant) {
         for (int i = 0; i < ahead && i < mine; ++i) fetch_w(i);
         fetch_s();
-        pdl_launch_dependents();
         pdl_wait();
+        pdl_launch_dependents();
         for (int i = 0; i < ahead && i < mine; ++i) fetch_x(i);
         for (int i = 0; i < ahead; ++i) cp_async_commit();            // the first holds them all, the others keep the count
     } else {
+        // the levels on their way to the L2 while the kernel ahead ends: a row's stretches of this warp are one piece of memory
+        if (blockIdx.y == 0 && mine > 0) {
+            const int from = c0 * 64, bytes = half - from < a.each * 64 ? half - from : a.each * 64;
+            for (int r = lane; r < R && n0 + r < a.N; r += 32) l2_prefetch(a.q + (size_t)(n0 + r) * half + from, (uint32_t)bytes);
+        }
         pdl_wait();
         pdl_launch_dependents();
         for (int i = 0; i < ahead; ++i) {
@@ -304,6 +317,7 @@ __global__ void __launch_bounds__(RW_MOST * 32) int4_rows_kernel(const RowsArgs 
     int woff[4];                                                      // this lane's word of piece j of row g
 #pragma unroll
     for (int j = 0; j < 4; ++j) woff[j] = g * 64 + ((j ^ ((g >> 1) & 3)) << 4) + 4 * t;
+    if (lane < 2) reinterpret_cast<uint4 *>(rw_smem + nothing)[lane] = make_uint4(0u, 0u, 0u, 0u);      // every warp for itself
     float acc[MT][NB][4] = {};
     uint32_t sc[2 * MT], zc[S32 ? 2 * MT : 1];
 
@@ -325,7 +339,8 @@ __global__ void __launch_bounds__(RW_MOST * 32) int4_rows_kernel(const RowsArgs 
         cp_async_commit();
         if (ahead == 1) cp_async_wait<1>(); else if (ahead == 2) cp_async_wait<2>(); else if (ahead == 3) cp_async_wait<3>(); else cp_async_wait<4>();
         __syncwarp();
-        const uint8_t *ws = ring + slot * a.slot_bytes, *xs = ws + R * 64;
+        const uint8_t *ws = ring + slot * a.slot_bytes;
+        const int xs = (warp * a.slots + slot) * a.slot_bytes + R * 64;
         slot = slot + 1 == a.slots ? 0 : slot + 1;
         // x: columns 32 j + 8 t .. + 7 of row 8 b + g, as (0,4) (1,5) (2,6) (3,7)
         uint32_t bx[4][TERMS][NB][4];
@@ -335,16 +350,12 @@ __global__ void __launch_bounds__(RW_MOST * 32) int4_rows_kernel(const RowsArgs 
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 if constexpr (!X32) {
-                    uint4 v = make_uint4(0u, 0u, 0u, 0u);
-                    if (r < rows) v = *reinterpret_cast<const uint4 *>(xs + (j * rows + r) * 64 + t * 16);
+                    const uint4 v = *reinterpret_cast<const uint4 *>(rw_smem + (r < rows ? xs + (j * rows + r) * 64 + t * 16 : nothing));
                     bx[j][0][b][0] = __byte_perm(v.x, v.z, 0x5410); bx[j][0][b][1] = __byte_perm(v.x, v.z, 0x7632);
                     bx[j][0][b][2] = __byte_perm(v.y, v.w, 0x5410); bx[j][0][b][3] = __byte_perm(v.y, v.w, 0x7632);
                 } else {
-                    uint4 lo = make_uint4(0u, 0u, 0u, 0u), hi = lo;
-                    if (r < rows) {
-                        const uint4 *at = reinterpret_cast<const uint4 *>(xs + ((2 * j + (t >> 1)) * rows + r) * 64 + (t & 1) * 32);
-                        lo = at[0]; hi = at[1];
-                    }
+                    const uint4 *at = reinterpret_cast<const uint4 *>(rw_smem + (r < rows ? xs + ((2 * j + (t >> 1)) * rows + r) * 64 + (t & 1) * 32 : nothing));
+                    const uint4 lo = at[0], hi = at[1];
                     const uint32_t one[4] = {lo.x, lo.y, lo.z, lo.w}, two[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
@@ -389,13 +400,15 @@ __global__ void __launch_bounds__(RW_MOST * 32) int4_rows_kernel(const RowsArgs 
                         for (int b = 0; b < NB; ++b) part[u][c][b][0] = part[u][c][b][1] = part[u][c][b][2] = part[u][c][b][3] = 0.f;
                 }
             }
+            uint32_t wa[MT], wb[MT];
+#pragma unroll
+            for (int u = 0; u < MT; ++u) { wa[u] = wp[j][u * 256]; wb[u] = wp[j][u * 256 + 128]; }
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
                 for (int u = 0; u < MT; ++u) {
-                    const uint32_t wa = wp[j][u * 256], wb = wp[j][u * 256 + 128];
-                    const uint32_t a0 = level_pair(wa >> (8 * h), za[u]), a1 = level_pair(wb >> (8 * h), zb[u]), a2 = level_pair(wa >> (8 * h + 4), za[u]),
-                                   a3 = level_pair(wb >> (8 * h + 4), zb[u]);
+                    const uint32_t a0 = level_pair(wa[u] >> (8 * h), za[u]), a1 = level_pair(wb[u] >> (8 * h), zb[u]), a2 = level_pair(wa[u] >> (8 * h + 4), za[u]),
+                                   a3 = level_pair(wb[u] >> (8 * h + 4), zb[u]);
 #pragma unroll
                     for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -489,7 +502,7 @@ static cudaError_t rows_go_group(RowsArgs a, cudaStream_t stream) {
     a.ahead = a.each < 4 ? a.each : 4;
     while (a.ahead > 1 && a.warps * (a.ahead + (a.ahead < a.each ? 1 : 0)) * a.slot_bytes > 100 * 1024) --a.ahead;
     a.slots = a.ahead + (a.ahead < a.each ? 1 : 0);
-    int smem = a.warps * a.slots * a.slot_bytes;
+    int smem = a.warps * a.slots * a.slot_bytes + 32;
     const int red = a.warps * 8 * NB * RP * 4;
     if (smem < red) smem = red;
     cudaError_t e = cudaSuccess;

@@ -9,6 +9,11 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, int by
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N_> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N_) : "memory"); }
+// Asks for memory to be brought into the L2: 16-byte aligned, a multiple of 16 bytes. It reads nothing that anyone sees, so it may come ahead of the wait for the kernel
+// that writes there.
+__device__ __forceinline__ void l2_prefetch(const void *p, uint32_t bytes) {
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory");
+}
 // the pair of levels in bits 0-3 and 16-19 as bf16 whole numbers less the zero: 0x4300 | q is 128 + q, z2 is 128 + z twice
 __device__ __forceinline__ uint32_t level_pair(uint32_t w, uint32_t z2) {
     uint32_t v, d;

@@ -8,13 +8,14 @@
 // result's own; kept exact, each group's products would have to be read back from tensor memory and scaled, as long as the products themselves take.
 //   Few rows: the columns of W are shared out over a cluster of CTAs, whose sums meet in shared memory and are added in the order of their rank.
 // Every wait is bounded; one that runs out sets the error flag and the CTA winds down.
+#include <cstdlib>
 #include "gelu.cuh"
 #include "int4_linear.cuh"
 #include "tc_pair.cuh"
 
 namespace pgb {
 
-constexpr int IT_DQ = 8, IT_NT = (IT_DQ + 2) * 32, IT_XS = 4;         // dequantising warps, threads, stages of x
+constexpr int IT_DQ = 8, IT_NT = (IT_DQ + 2) * 32, IT_XS = 4, IT_SPLITS = 8;     // dequantising warps, threads, stages of x; shares of K at most
 
 struct TileArgs {
     const unsigned char *q; const void *scales; const unsigned char *zeros; const __nv_bfloat16 *bias; __nv_bfloat16 *y;
@@ -31,6 +32,86 @@ struct ItCfg {
     static_assert(NT * ROW * 4 <= BARS, "the sums lie where x and the levels were");
     static_assert(2 * (SMEM + 1024) <= 227 * 1024 && SMEM > 76 * 1024, "two CTAs an SM, and no third, whose tensor memory would not be there");
 };
+
+// the scales (bf16 ones two a register) and zeros of the four groups that a row's stretch lies in; those behind the last one 0
+template <int LG, bool S32>
+__device__ __forceinline__ void it_groups(const TileArgs &a, int row, int stretch, bool live, uint32_t (&s)[S32 ? 4 : 2], uint32_t &z) {
+    const int g0 = ((stretch * 128) >> LG) & ~3;
+    z = 0x08080808u;
+#pragma unroll
+    for (int e = 0; e < (S32 ? 4 : 2); ++e) s[e] = 0u;
+    if (row >= a.N || !live) return;
+    const size_t at = (size_t)row * a.G + g0;
+    if (a.wide) {
+        if constexpr (S32) {
+            const uint4 v = __ldg(reinterpret_cast<const uint4 *>(reinterpret_cast<const float *>(a.scales) + at));
+            s[0] = v.x; s[1] = v.y; s[2] = v.z; s[3] = v.w;
+        } else {
+            const uint2 v = __ldg(reinterpret_cast<const uint2 *>(reinterpret_cast<const __nv_bfloat16 *>(a.scales) + at));
+            s[0] = v.x; s[1] = v.y;
+        }
+        if (a.zeros != nullptr) z = __ldg(reinterpret_cast<const uint32_t *>(a.zeros + at));
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (g0 + e < a.G) {
+            if constexpr (S32) s[e] = __ldg(reinterpret_cast<const uint32_t *>(a.scales) + at + e);
+            else s[e >> 1] |= (uint32_t)__ldg(reinterpret_cast<const unsigned short *>(a.scales) + at + e) << (16 * (e & 1));
+            if (a.zeros != nullptr) z = (z & ~(255u << (8 * e))) | (uint32_t)__ldg(a.zeros + at + e) << (8 * e);
+        }
+}
+// 32 levels of group e of those four as bf16 pairs in their order: scale (q - z), rounded once
+template <bool S32>
+__device__ __forceinline__ void it_values(const uint4 &levels, const uint32_t (&s)[S32 ? 4 : 2], uint32_t z, int e, uint32_t (&out)[16]) {
+    const uint32_t z2 = __byte_perm(z, 0x43u, 0x4040 | e | e << 8);
+    uint32_t s2 = 0u;
+    float sf = 0.f;
+    if constexpr (S32) sf = __uint_as_float(e < 2 ? (e == 0 ? s[0] : s[1]) : (e == 2 ? s[2] : s[3]));
+    else s2 = __byte_perm(e >> 1 ? s[1] : s[0], 0u, e & 1 ? 0x3232 : 0x1010);
+    const uint32_t w[4] = {levels.x, levels.y, levels.z, levels.w};
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+        uint32_t p[4];
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {                                 // (0,4) (1,5) (2,6) (3,7)
+            p[h] = level_pair(w[v] >> (4 * h), z2);
+            if constexpr (!S32) p[h] = mul_bf16x2(p[h], s2);
+            else {
+                const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&p[h]));
+                const __nv_bfloat162 r = __floats2bfloat162_rn(f.x * sf, f.y * sf);
+                p[h] = *reinterpret_cast<const uint32_t *>(&r);
+            }
+        }
+        out[4 * v] = __byte_perm(p[0], p[1], 0x5410); out[4 * v + 1] = __byte_perm(p[2], p[3], 0x5410);
+        out[4 * v + 2] = __byte_perm(p[0], p[1], 0x7632); out[4 * v + 3] = __byte_perm(p[2], p[3], 0x7632);
+    }
+}
+// the first of those four groups that a stretch has
+template <int LG> __device__ __forceinline__ int it_first(int stretch) { return LG == 7 ? stretch & 3 : LG == 6 ? (stretch & 1) * 2 : 0; }
+// 16 columns of D (rows m, m + 1, .. of x) of this lane's row n of W: + bias, the activation, rounded and stored; a row's 32 lanes are 64 bytes
+__device__ __forceinline__ void it_store16(const TileArgs &a, const float (&v)[16], float bias, long long m, int n, int count) {
+    __nv_bfloat16 *row = a.y + (size_t)m * a.N;                       // uniform
+    if (m + count <= a.M) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            if (e >= count) break;
+            float s = v[e] + bias;
+            if (a.act == 1) s = lg_gelu(s);
+            if (n < a.N) row[n] = __float2bfloat16_rn(s);
+            row += a.N;
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            if (e >= count) break;
+            float s = v[e] + bias;
+            if (a.act == 1) s = lg_gelu(s);
+            if (m + e < a.M && n < a.N) row[n] = __float2bfloat16_rn(s);
+            row += a.N;
+        }
+    }
+}
 
 template <int NT, int LG, bool S32>
 __global__ void __launch_bounds__(IT_NT, 2) int4_tile_kernel(const __grid_constant__ CUtensorMap mx, const TileArgs a) {
@@ -63,7 +144,15 @@ __global__ void __launch_bounds__(IT_NT, 2) int4_tile_kernel(const __grid_consta
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = warp_uniform(*tmem_slot), tA = tmem + NT;    // D: NT columns; A: two stretches of 64
-    if (!a.constant) { pdl_wait(); pdl_launch_dependents(); }
+    if (!a.constant) {
+        // few rows: the levels on their way to the L2 while the kernel ahead ends
+        if (NT < 128 && blockIdx.y == 0 && tid < 128 && n0 + tid < a.N) {
+            const int half = a.K >> 1, from = c0 * 64, bytes = half - from < mine * 64 ? half - from : mine * 64;
+            l2_prefetch(a.q + (size_t)(n0 + tid) * half + from, (uint32_t)bytes);
+        }
+        pdl_wait();
+        pdl_launch_dependents();
+    }
     bool ok = true;
 
     if (warp < IT_DQ) {
@@ -88,37 +177,11 @@ __global__ void __launch_bounds__(IT_NT, 2) int4_tile_kernel(const __grid_consta
             }
             wcol += 256; wsrc += 128;
         };
-        // scales and zeros of the four groups that stretch i lies in; those behind the last one 0
         uint32_t sn[S32 ? 4 : 2], zn;
-        auto fetch_s = [&](int i) {
-            const int g0 = (((c0 + i) * 128) >> LG) & ~3;
-            zn = 0x08080808u;
-#pragma unroll
-            for (int e = 0; e < (S32 ? 4 : 2); ++e) sn[e] = 0u;
-            if (row >= a.N || i >= mine) return;
-            const size_t at = (size_t)row * a.G + g0;
-            if (a.wide) {
-                if constexpr (S32) {
-                    const uint4 v = __ldg(reinterpret_cast<const uint4 *>(reinterpret_cast<const float *>(a.scales) + at));
-                    sn[0] = v.x; sn[1] = v.y; sn[2] = v.z; sn[3] = v.w;
-                } else {
-                    const uint2 v = __ldg(reinterpret_cast<const uint2 *>(reinterpret_cast<const __nv_bfloat16 *>(a.scales) + at));
-                    sn[0] = v.x; sn[1] = v.y;
-                }
-                if (a.zeros != nullptr) zn = __ldg(reinterpret_cast<const uint32_t *>(a.zeros + at));
-                return;
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (g0 + e < a.G) {
-                    if constexpr (S32) sn[e] = __ldg(reinterpret_cast<const uint32_t *>(a.scales) + at + e);
-                    else sn[e >> 1] |= (uint32_t)__ldg(reinterpret_cast<const unsigned short *>(a.scales) + at + e) << (16 * (e & 1));
-                    if (a.zeros != nullptr) zn = (zn & ~(255u << (8 * e))) | (uint32_t)__ldg(a.zeros + at + e) << (8 * e);
-                }
-        };
+        auto fetch_s = [&](int i) { it_groups<LG, S32>(a, row, c0 + i, i < mine, sn, zn); };
         for (int i = 0; i < a.ahead; ++i) { if (par + 2 * i < mine) fetch(i); cp_async_commit(); }
         fetch_s(par);
-        if (a.constant) { pdl_launch_dependents(); pdl_wait(); }
+        if (a.constant) { pdl_wait(); pdl_launch_dependents(); }
         const uint32_t mine_row = lane * 64, sw = (lane >> 1) & 3;
         int slot = 0;
         uint32_t round = 0;                                           // of this warp's stage: stretch i goes to stage i mod 2 = par
@@ -134,36 +197,14 @@ __global__ void __launch_bounds__(IT_NT, 2) int4_tile_kernel(const __grid_consta
             const uint8_t *ws = sm + (ring - base) + slot * CF::SLOT + mine_row;
             slot = slot + 1 == slots ? 0 : slot + 1;
             const uint32_t dst = tA + ((uint32_t)(32 * sub) << 16) + par * 64;
-            const int first = LG == 7 ? (c0 + i) & 3 : LG == 6 ? ((c0 + i) & 1) * 2 : 0;      // of the four groups, the stretch's first
+            const int first = it_first<LG>(c0 + i);
             if (round >= 1) ok = mbar_wait_warp(a_empty(par), (round + 1) & 1, 61);
             if (!ok) break;
             tc_fence_after();
 #pragma unroll
             for (int j = 0; j < 4; ++j) {                             // 32 columns
-                const int e = first + (j >> (LG - 5));
-                uint32_t z2 = __byte_perm(zc, 0x43u, 0x4040 | e | e << 8), s2 = 0u;
-                float sf = 0.f;
-                if constexpr (S32) sf = __uint_as_float(e == 0 ? sc[0] : e == 1 ? sc[1] : e == 2 ? sc[2] : sc[3]);
-                else s2 = __byte_perm(e >> 1 ? sc[1] : sc[0], 0u, e & 1 ? 0x3232 : 0x1010);
-                const uint4 lv = *reinterpret_cast<const uint4 *>(ws + ((j ^ sw) << 4));
-                const uint32_t wv[4] = {lv.x, lv.y, lv.z, lv.w};
                 uint32_t out[16];
-#pragma unroll
-                for (int v = 0; v < 4; ++v) {
-                    uint32_t p[4];
-#pragma unroll
-                    for (int h = 0; h < 4; ++h) {                     // (0,4) (1,5) (2,6) (3,7)
-                        p[h] = level_pair(wv[v] >> (4 * h), z2);
-                        if constexpr (!S32) p[h] = mul_bf16x2(p[h], s2);
-                        else {
-                            const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&p[h]));
-                            const __nv_bfloat162 r = __floats2bfloat162_rn(f.x * sf, f.y * sf);
-                            p[h] = *reinterpret_cast<const uint32_t *>(&r);
-                        }
-                    }
-                    out[4 * v] = __byte_perm(p[0], p[1], 0x5410); out[4 * v + 1] = __byte_perm(p[2], p[3], 0x5410);
-                    out[4 * v + 2] = __byte_perm(p[0], p[1], 0x7632); out[4 * v + 3] = __byte_perm(p[2], p[3], 0x7632);
-                }
+                it_values<S32>(*reinterpret_cast<const uint4 *>(ws + ((j ^ sw) << 4)), sc, zc, first + (j >> (LG - 5)), out);
                 tmem_st16(dst + 16 * j, out);
             }
             tmem_st_wait();
@@ -238,17 +279,27 @@ __global__ void __launch_bounds__(IT_NT, 2) int4_tile_kernel(const __grid_consta
         }
         cluster_sync_all();                                           // every CTA's sums are there
         const uint32_t rank = cluster_rank();
-        for (int i = (int)rank * IT_NT + tid; i < 128 * NT; i += a.splits * IT_NT) {
-            const int n = n0 + (i & 127), m = i >> 7;
+        for (int i = (int)rank * IT_NT + tid; i < 32 * NT; i += a.splits * IT_NT) {       // four rows of W a thread, all ranks' sums asked for at once
+            const int n = n0 + 4 * (i & 31), m = i >> 5;
             if (n >= a.N || m0 + m >= a.M) continue;
-            float s = 0.f;
-            for (int r = 0; r < a.splits; ++r) {
-                float v;
-                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr(base + (m * CF::ROW + (i & 127)) * 4, r)));
-                s += v;
+            const uint32_t at = base + (m * CF::ROW + 4 * (i & 31)) * 4;
+            float4 v[IT_SPLITS];
+#pragma unroll
+            for (int r = 0; r < IT_SPLITS; ++r) {
+                v[r] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (r < a.splits)
+                    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[r].x), "=f"(v[r].y), "=f"(v[r].z), "=f"(v[r].w) : "r"(cluster_addr(at, r)));
             }
-            if (a.bias != nullptr) s += __bfloat162float(a.bias[n]);
-            a.y[(size_t)(m0 + m) * a.N + n] = __float2bfloat16_rn(a.act == 1 ? lg_gelu(s) : s);
+            float s[4] = {v[0].x, v[0].y, v[0].z, v[0].w};
+#pragma unroll
+            for (int r = 1; r < IT_SPLITS; ++r) { s[0] += v[r].x; s[1] += v[r].y; s[2] += v[r].z; s[3] += v[r].w; }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (n + e >= a.N) break;
+                float x = s[e] + (a.bias != nullptr ? __bfloat162float(a.bias[n + e]) : 0.f);
+                if (a.act == 1) x = lg_gelu(x);
+                a.y[(size_t)(m0 + m) * a.N + n + e] = __float2bfloat16_rn(x);
+            }
         }
         cluster_sync_all();                                           // nobody leaves while its sums are read
     } else if (warp < IT_DQ && ok) {
@@ -259,18 +310,220 @@ __global__ void __launch_bounds__(IT_NT, 2) int4_tile_kernel(const __grid_consta
             float v[16];
             tmem_ld16_nowait(tD + c, v);
             tmem_ld_wait();
-#pragma unroll
-            for (int e = 0; e < STEP; ++e) {
-                const long long m = m0 + mh + c + e;
-                float s = v[e] + bias;
-                if (a.act == 1) s = lg_gelu(s);
-                if (m < a.M && n < a.N) a.y[(size_t)m * a.N + n] = __float2bfloat16_rn(s);
-            }
+            it_store16(a, v, bias, m0 + mh + c, n, STEP);
         }
     }
     tc_fence_before();
     __syncthreads();
     if (warp == 9) tmem_dealloc(tmem, 256);
+}
+
+// ------------------------------------------------------------------------------------------------ very many rows
+// The same for tiles of 256 rows of x: twice the products for a tile's dequantisation, which is what the smaller tiles are bound by (issue slots: 128 rows of W and 128 of x
+// take 630 instructions and an epilogue as long for 256 cycles of the tensor pipe). One CTA an SM walks tiles: eight warps dequantise into four stages of shared memory
+// (A, 64 columns, 128-byte swizzle: D, twice 256 columns, takes all of tensor memory), eight store the tile before, 128 columns of D each.
+constexpr int IW_NT = 18 * 32, IW_XS = 3, IW_AS = 4, IW_AHEAD = 1;
+constexpr int IW_XSTAGE = 256 * 128, IW_ASTAGE = 128 * 128, IW_SLOT = 32 * 64;
+constexpr int IW_A = IW_XS * IW_XSTAGE, IW_RING = IW_A + IW_AS * IW_ASTAGE, IW_BARS = IW_RING + IT_DQ * (IW_AHEAD + 1) * IW_SLOT, IW_SMEM = IW_BARS + 256 + 1024;
+static_assert(IW_SMEM <= 227 * 1024, "shared memory");
+
+template <int LG, bool S32>
+__global__ void __launch_bounds__(IW_NT, 1) int4_wide_kernel(const __grid_constant__ CUtensorMap mx, const TileArgs a) {
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t *sm = smem_raw + (base - smem_u32(smem_raw));
+    const uint32_t mb = base + IW_BARS;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(sm + IW_BARS + 192);
+    auto x_full = [&](int s) { return mb + 8 * s; };
+    auto x_empty = [&](int s) { return mb + 32 + 8 * s; };
+    auto a_full = [&](int s) { return mb + 64 + 8 * s; };
+    auto a_empty = [&](int s) { return mb + 96 + 8 * s; };
+    auto acc_full = [&](int d) { return mb + 128 + 8 * d; };
+    auto acc_empty = [&](int d) { return mb + 144 + 8 * d; };
+    const uint32_t drained = mb + 160;
+
+    const int tid = threadIdx.x, lane = tid & 31, warp = warp_uniform(tid >> 5);
+    const int C = (a.K + 127) >> 7, tiles_n = (a.N + 127) >> 7;
+    const long long tiles = (long long)tiles_n * ((a.M + 255) / 256);
+    // tile t: the CTAs that run together share rows of x
+    auto n_of = [&](long long t) { return (int)(t % tiles_n) * 128; };
+    auto m_of = [&](long long t) { return t / tiles_n * 256; };
+
+    if (tid == 0) {
+        for (int s = 0; s < IW_XS; ++s) { mbar_init(x_full(s), 1); mbar_init(x_empty(s), 1); }
+        for (int s = 0; s < IW_AS; ++s) { mbar_init(a_full(s), 4); mbar_init(a_empty(s), 1); }
+        for (int d = 0; d < 2; ++d) { mbar_init(acc_full(d), 1); mbar_init(acc_empty(d), 8); }
+        mbar_init(drained, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 17) tmem_alloc(smem_u32(tmem_slot), 512);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = warp_uniform(*tmem_slot);
+    pdl_wait();
+    pdl_launch_dependents();
+    bool ok = true;
+
+    if (warp < IT_DQ) {
+        // ------------------------------------------------------------------------------------------ levels -> A
+        // This warp's stretches of all the CTA's tiles in a row are every second one; a fetch iterator runs IW_AHEAD of them ahead.
+        const int sub = warp & 3, par = warp >> 2, fr = lane >> 2, ft = lane & 3, half = a.K >> 1;
+        const uint32_t ring = base + IW_RING + warp * (IW_AHEAD + 1) * IW_SLOT;
+        const uint32_t wdst = ring + fr * 64 + ((ft ^ ((fr >> 1) & 3)) << 4);
+        long long tile = blockIdx.x, ftile = blockIdx.x;
+        int i = par, fi = par;
+        auto step = [&](long long &t, int &k) { for (; k >= C && t < tiles; k -= C) t += gridDim.x; };
+        step(tile, i);
+        ftile = tile; fi = i;
+        uint32_t sn[S32 ? 4 : 2], zn;
+        auto fetch = [&](int slot) {                                  // the fetch iterator's stretch, and on
+            if (ftile < tiles) {
+                const int r0 = n_of(ftile) + 32 * sub + fr, col = fi * 128 + ft * 32;
+                const unsigned char *p = a.q + (size_t)r0 * half + (col >> 1);
+                const bool in = col < a.K;
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const bool here = in && r0 + 8 * u < a.N;
+                    cp_async16(wdst + slot * IW_SLOT + u * 512, here ? p : a.q, here ? 16 : 0);
+                    p += (size_t)8 * half;
+                }
+                fi += 2;
+                step(ftile, fi);
+            }
+            cp_async_commit();
+        };
+        for (int k = 0; k < IW_AHEAD; ++k) fetch(k);
+        it_groups<LG, S32>(a, tile < tiles ? n_of(tile) + 32 * sub + lane : a.N, i, true, sn, zn);
+        const uint32_t sw = (lane >> 1) & 3;
+        int slot = 0;
+        for (uint32_t round = 0; tile < tiles; ++round) {
+            uint32_t sc[S32 ? 4 : 2], zc = zn;
+#pragma unroll
+            for (int e = 0; e < (S32 ? 4 : 2); ++e) sc[e] = sn[e];
+            const int first = it_first<LG>(i);
+            fetch(slot == 0 ? IW_AHEAD : slot - 1);
+            i += 2;
+            step(tile, i);
+            it_groups<LG, S32>(a, tile < tiles ? n_of(tile) + 32 * sub + lane : a.N, i, true, sn, zn);
+            cp_async_wait<IW_AHEAD>();
+            __syncwarp();
+            const uint8_t *ws = sm + IW_RING + (warp * (IW_AHEAD + 1) + slot) * IW_SLOT + lane * 64;
+            slot = slot == IW_AHEAD ? 0 : slot + 1;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {                             // 64 columns: a stage
+                const int st = 2 * par + h;
+                if (round >= 1) ok = mbar_wait_warp(a_empty(st), (round + 1) & 1, 66);
+                if (!ok) break;
+                uint8_t *dst = sm + IW_A + st * IW_ASTAGE;
+#pragma unroll
+                for (int j = 2 * h; j < 2 * h + 2; ++j) {
+                    uint32_t out[16];
+                    it_values<S32>(*reinterpret_cast<const uint4 *>(ws + ((j ^ sw) << 4)), sc, zc, first + (j >> (LG - 5)), out);
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        *reinterpret_cast<uint4 *>(dst + swz(32 * sub + lane, 4 * (j & 1) + q)) = make_uint4(out[4 * q], out[4 * q + 1], out[4 * q + 2], out[4 * q + 3]);
+                }
+                warp_arrive(a_full(st), lane);
+            }
+            if (!ok) break;
+        }
+        cp_async_wait<0>();
+    } else if (warp < 16) {
+        // ------------------------------------------------------------------------------------------ D -> y
+        const int sub = warp & 3, mh = ((warp >> 2) & 1) * 128;
+        uint32_t ti = 0;
+        for (long long t = blockIdx.x; t < tiles; t += gridDim.x, ++ti) {
+            const int d = ti & 1, n = n_of(t) + 32 * sub + lane;
+            const long long m = m_of(t) + mh;
+            const float bias = a.bias != nullptr && n < a.N ? __bfloat162float(a.bias[n]) : 0.f;
+            ok = mbar_wait_warp(acc_full(d), (ti >> 1) & 1, 67);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t tD = tmem + ((uint32_t)(32 * sub) << 16) + d * 256 + mh;
+            float v[2][16];
+            tmem_ld16_nowait(tD, v[0]);
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+                tmem_ld_wait();
+                if (c < 7) tmem_ld16_nowait(tD + 16 * (c + 1), v[(c + 1) & 1]);
+                else {                                                // all of D is in registers
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(acc_empty(d));
+                }
+                it_store16(a, v[c & 1], bias, m + 16 * c, n, 16);
+            }
+        }
+    } else if (warp == 16) {
+        // ------------------------------------------------------------------------------------------ x
+        const bool leader = elect_one();
+        long long it = 0;
+        for (long long t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+            const int m = (int)m_of(t);
+            for (int kb = 0; kb < 2 * C && ok; ++kb, ++it) {
+                const int s = (int)(it % IW_XS);
+                if (it >= IW_XS) ok = mbar_wait_warp(x_empty(s), (uint32_t)((it / IW_XS) + 1) & 1, 68);
+                if (ok && leader) {
+                    mbar_expect_tx(x_full(s), IW_XSTAGE);
+                    tma_load_3d(base + s * IW_XSTAGE, &mx, x_full(s), kb * 64, m, 0);
+                }
+                __syncwarp();
+            }
+        }
+        if (!ok)                                                      // the copies under way land before shared memory goes
+            for (long long k = it - 1 - IW_XS < 0 ? 0 : it - 1 - IW_XS; k < it - 1; ++k) mbar_wait_tries(x_full((int)(k % IW_XS)), (uint32_t)(k / IW_XS) & 1);
+    } else {
+        // ------------------------------------------------------------------------------------------ products
+        constexpr uint32_t IDESC = idesc_bf16(128, 256, 0, 0);
+        uint32_t ti = 0, ai = 0;                                      // tiles; stretches
+        int xs = 0;
+        uint32_t xp = 0;
+        for (long long t = blockIdx.x; t < tiles && ok; t += gridDim.x, ++ti) {
+            const uint32_t d = ti & 1;
+            if (ti >= 2) ok = mbar_wait_warp(acc_empty(d), ((ti >> 1) + 1) & 1, 69);
+            tc_fence_after();
+            for (int i = 0; i < C && ok; ++i, ++ai) {
+                for (int h = 0; h < 2 && ok; ++h) {
+                    const int st = 2 * (ai & 1) + h;
+                    ok = mbar_wait_warp(a_full(st), (ai >> 1) & 1, 63);
+                    if (ok) ok = mbar_wait_warp(x_full(xs), xp, 64);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint64_t da = smem_desc(base + IW_A + st * IW_ASTAGE, 16, 1024), db = smem_desc(base + xs * IW_XSTAGE, 16, 1024);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) mma_bf16_elect(tmem + d * 256, da + k * 2, db + k * 2, IDESC, (i | h | k) != 0);
+                    mma_commit_elect(x_empty(xs));
+                    mma_commit_elect(a_empty(st));
+                    if (++xs == IW_XS) { xs = 0; xp ^= 1; }
+                }
+            }
+            if (ok) mma_commit_elect(acc_full(d));
+        }
+        if (!ok) {                                                    // products under way end before tensor memory goes
+            mma_commit_elect(drained);
+            mbar_wait_tries(drained, 0);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 17) tmem_dealloc(tmem, 512);
+}
+
+template <int LG, bool S32>
+static cudaError_t wide_go(const Int4Linear &l, const TileArgs &a, cudaStream_t stream) {
+    CUtensorMap mx;
+    if (!tc_make_map(&mx, l.x, 1, l.M, l.w.K, l.w.K, l.M * l.w.K, 256)) return cudaErrorUnknown;
+    cudaError_t e = cudaFuncSetAttribute(int4_wide_kernel<LG, S32>, cudaFuncAttributeMaxDynamicSharedMemorySize, IW_SMEM);
+    if (e != cudaSuccess) return e;
+    const long long tiles = (long long)((l.w.N + 127) / 128) * ((l.M + 255) / 256), sms = sm_count();
+    return pdl_launch(int4_wide_kernel<LG, S32>, dim3((unsigned)(tiles < sms ? tiles : sms)), dim3(IW_NT), (size_t)IW_SMEM, stream, mx, a);
+}
+static cudaError_t wide_group(const Int4Linear &l, const TileArgs &a, cudaStream_t stream) {
+    const bool s32 = l.w.scale_dtype == PGB_F32;
+    if (l.w.group == 32) return s32 ? wide_go<5, true>(l, a, stream) : wide_go<5, false>(l, a, stream);
+    if (l.w.group == 64) return s32 ? wide_go<6, true>(l, a, stream) : wide_go<6, false>(l, a, stream);
+    return s32 ? wide_go<7, true>(l, a, stream) : wide_go<7, false>(l, a, stream);
 }
 
 template <int NT, int LG, bool S32>
@@ -313,9 +566,16 @@ int int4_tile_launch(const Int4Linear &l, cudaStream_t stream) {
     const int NT = l.M <= 32 ? 32 : l.M <= 64 ? 64 : 128, C = (w.K + 127) / 128;
     const long long tiles = (long long)((w.N + 127) / 128) * ((l.M + NT - 1) / NT);
     int splits = 1;                                                   // as many as give every SM a CTA, of two stretches or more
-    while (NT < 128 && splits < 8 && tiles * splits * 2 <= sm_count() * 2 && C >= 4 * splits) splits *= 2;
+    while (NT < 128 && splits < IT_SPLITS && tiles * splits * 2 <= sm_count() * 2 && C >= 4 * splits) splits *= 2;
+    if (const char *f = getenv("SPL")) { if (NT < 128 && atoi(f)) splits = atoi(f); }
     Int4Linear part = l;
     cudaError_t e = cudaSuccess;
+    // From four rounds over the chip on the larger tiles are ahead (us, N 8192 K 2048: 4096 rows 120 against 135; 1.7 rounds, N 2048 K 8192: 130 against 125).
+    if ((long long)((w.N + 127) / 128) * ((l.M + 255) / 256) >= 4LL * sm_count()) {
+        e = wide_group(l, a, stream);
+        if (e != cudaSuccess) { set_cuda_error(e, "int4_wide launch"); return PGB_ERR_CUDA; }
+        return check_launch("int4_wide_kernel");
+    }
     for (long long m = 0; m < l.M && e == cudaSuccess; m += 65535LL * NT) {
         part.M = l.M - m < 65535LL * NT ? l.M - m : 65535LL * NT;
         part.x = (const __nv_bfloat16 *)l.x + (size_t)m * w.K;
