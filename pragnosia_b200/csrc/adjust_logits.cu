@@ -82,7 +82,7 @@ __global__ void __launch_bounds__(NT, PER_SM) adjust_logits_kernel(const AdjustL
     const float r = a.repetition.at ? a.repetition.at[b] : a.repetition.all, f = a.frequency.at ? a.frequency.at[b] : a.frequency.all,
                 p = a.presence.at ? a.presence.at[b] : a.presence.all;
     // an id's place in the slice; one that is not there (below 0, in another slice, past 32 bits) at S or beyond. Places past V are counted and not read.
-    auto place = [&](long long id) { return (uint32_t)(id >> 31) == 0u ? (uint32_t)((int)id - v0) : 0xffffffffu; };
+    auto place = [&](long long id) { return (uint32_t)(id >> 31) == 0u ? (uint32_t)id - (uint32_t)v0 : 0xffffffffu; };
 #pragma unroll
     for (int q = 0; q < QT; ++q) {
         reinterpret_cast<uint4 *>(count)[tid + q * NT] = make_uint4(0u, 0u, 0u, 0u);

@@ -530,7 +530,8 @@ static cudaError_t rows_blocks(RowsArgs a, cudaStream_t stream) {
     // 16 and 8 9.1; N 2048 K 2048 16 and 8 3.3, 32 and 8 4.3; K 16384 N 4096 32 and 8 22, 16 and 8 28, 64 and 8 33. Several rows: N 16384 K 4096, 8 rows, 64 and 8 20.9, 32 and 8 22.9.
     const long long tiles = (a.M + 8 * NB - 1) / (8 * NB), sms = sm_count();
     const long long by64 = (a.N + 63) / 64 * tiles, by32 = (a.N + 31) / 32 * tiles, by16 = (a.N + 15) / 16 * tiles;
-    const int MT = a.M > 4 && by64 * 10 >= 17 * sms ? 4 : by32 * 10 >= 7 * sms ? 2 : 1;
+    // few columns and very many rows of W, whose CTAs are short: N 50257 K 768 16 and 2 13.8, 32 and 2 16.0
+    const int MT = a.M > 4 && by64 * 10 >= 17 * sms ? 4 : by32 * 10 < 7 * sms || (a.K <= 1024 && by16 >= 10 * sms) ? 1 : 2;
     const long long ctas = MT == 4 ? by64 : MT == 2 ? by32 : by16;
     a.warps = ctas * 8 <= 17 * sms ? 8 : ctas * 4 <= 17 * sms ? 4 : 2;
     if (MT == 4) return rows_go<4, NB, X32, S32>(a, stream);

@@ -8,7 +8,6 @@
 // result's own; kept exact, each group's products would have to be read back from tensor memory and scaled, as long as the products themselves take.
 //   Few rows: the columns of W are shared out over a cluster of CTAs, whose sums meet in shared memory and are added in the order of their rank.
 // Every wait is bounded; one that runs out sets the error flag and the CTA winds down.
-#include <cstdlib>
 #include "gelu.cuh"
 #include "int4_linear.cuh"
 #include "tc_pair.cuh"
@@ -567,7 +566,6 @@ int int4_tile_launch(const Int4Linear &l, cudaStream_t stream) {
     const long long tiles = (long long)((w.N + 127) / 128) * ((l.M + NT - 1) / NT);
     int splits = 1;                                                   // as many as give every SM a CTA, of two stretches or more
     while (NT < 128 && splits < IT_SPLITS && tiles * splits * 2 <= sm_count() * 2 && C >= 4 * splits) splits *= 2;
-    if (const char *f = getenv("SPL")) { if (NT < 128 && atoi(f)) splits = atoi(f); }
     Int4Linear part = l;
     cudaError_t e = cudaSuccess;
     // From four rounds over the chip on the larger tiles are ahead (us, N 8192 K 2048: 4096 rows 120 against 135; 1.7 rounds, N 2048 K 8192: 130 against 125).

@@ -708,7 +708,8 @@ Tensor int4_linear_fwd(const Tensor &x_, const Tensor &q, const Tensor &s, const
     }
     OnDevice dev(x_);
     const Tensor x = head_operand(x_), b = bias.defined() ? like(bias, x.scalar_type()) : bias;
-    if (constant && b.defined() && b.data_ptr() != bias.data_ptr()) constant = false;         // made by a kernel just now
+    const auto moved = [](const Tensor &to, const Tensor &from) { return to.defined() && to.data_ptr() != from.data_ptr(); };
+    if (moved(b, bias) || moved(w.q, q) || moved(w.s, s) || moved(w.z, opt(z))) constant = false;      // made by a kernel just now
     std::vector<int64_t> shape = x_.sizes().vec();
     shape.back() = w.N;
     const Tensor y = alloc(x, shape, bf16 ? at::kBFloat16 : at::kFloat);
@@ -797,7 +798,7 @@ Tensor adjust_fwd(const Tensor &l_, const OptTensor &prompt, const OptTensor &pr
     // dense rows as they lie; a row stride of their own only where it does not overlap what is written
     const bool strided = l_.stride(1) == 1 || V == 1;
     Tensor l = strided ? l_ : l_.contiguous();
-    if (out.defined() && l.data_ptr() == out.data_ptr() && !(l.scalar_type() == at::kFloat && l.is_contiguous())) l = l.clone();
+    if (out.defined() && out.is_alias_of(l) && !(l.data_ptr() == out.data_ptr() && l.scalar_type() == at::kFloat && l.is_contiguous())) l = l.clone();
     if (!out.defined()) out = alloc(l, {B, V}, at::kFloat);
     if (B == 0) return out;
     const auto ll = [](const Tensor &t) { return static_cast<const long long *>(vp(t)); };

@@ -145,6 +145,10 @@ def test_rows_with_a_stride_and_in_place():
     assert sampling.adjust_logits(l, **kw, out=out) is not None and torch.equal(out, ref)
     got = sampling.adjust_logits(l, **kw, out=l)
     assert got.data_ptr() == l.data_ptr() and torch.equal(l, ref)
+    both = torch.randn(2 * 3 * V, device="cuda")                      # rows that overlap where the result goes
+    l, out = both[:3 * V].view(3, V), both[V:4 * V].view(3, V)
+    ref = sampling.adjust_logits(l, **kw)
+    assert torch.equal(sampling.adjust_logits(l, **kw, out=out), ref) and torch.equal(out, ref)
     one = big[0:1, :V]
     ref = sampling.adjust_logits(one, frequency=0.0, bias_ids=torch.zeros(1, 1, dtype=torch.long, device="cuda"), bias=torch.ones(1, 1, device="cuda"))
     assert torch.equal(sampling.adjust_logits(one, bias_ids=torch.zeros(1, 1, dtype=torch.long, device="cuda"), bias=torch.ones(1, 1, device="cuda"), out=one), ref)

@@ -169,6 +169,9 @@ def test_linear_views_strides_and_empty():
             check_linear(x, w, None, None, BF, y)
     part = int4.Int4Weight(w.q[8:40], w.scales[8:40], w.zeros[8:40], 64)       # rows of a held weight are a held weight
     assert torch.equal(int4.linear(whole[:4], part), int4.linear(whole[:4], w)[:, 8:40])
+    wide = torch.zeros(N, K, dtype=torch.uint8, device="cuda")                  # levels, scales and zeros in every second column of something, made dense just ahead of the kernel
+    wide[:, ::2] = w.q
+    assert torch.equal(int4.linear(whole[:4], w._replace(q=wide[:, ::2], scales=w.scales.t().contiguous().t()), constant=True), int4.linear(whole[:4], w))
     odd = torch.empty(N * K // 2 + 1, dtype=torch.uint8, device="cuda")[1:].view(N, K // 2).copy_(w.q)      # levels that begin at an odd address
     assert torch.equal(int4.linear(whole[:4], w._replace(q=odd)), int4.linear(whole[:4], w))
 
