@@ -59,13 +59,13 @@ __device__ __forceinline__ bool piece_at(const Pieces &p, int u, int N, int &n, 
 
 // What bounds it: the arithmetic of a level, before the bytes. A level is the nearest whole number to the correctly rounded quotient w / s. The product with
 // an approximate 1 / s is within 3e-6 of the quotient (15 at most), so away from a tie both round alike: 1.5 2^23 added and taken off again rounds to even in two
-// additions, the distance to the result says how near a tie was, and where one of a thread's eight came close all eight are divided. Four levels are one fp32 number (16 bits)
-// before they become integers. At N 16384, K 4096 bf16 division, rounding and conversion a value took 109 us.
+// additions. Where fp32 values come near a tie all eight of a thread are divided. Four levels are one fp32 number (16 bits) before they become integers.
+// N 16384, K 4096 bf16: 109 us with a division, a rounding and a conversion a value.
 template <typename T_, int GROUP, bool SYM>
 __global__ void __launch_bounds__(256) int4_quantize_kernel(const T_ *__restrict__ w, unsigned char *__restrict__ q, T_ *__restrict__ scales,
                                                             unsigned char *__restrict__ zeros, int N, int K, int G, const Pieces pieces) {
     constexpr int PER = GROUP / 8;                                    // threads of a group
-    constexpr float ROUND = 12582912.f;
+    constexpr float ROUND = 12582912.f, GRID = 768.f;                 // 1.5 2^23: to whole numbers; 1.5 2^9: to multiples of 2^-14 (for up to 256 of them)
     constexpr int RAW = (int)sizeof(T_) * 2;                          // 32-bit registers of a piece
     uint32_t v[QU][RAW];
     int n[QU], piece[QU];
@@ -129,20 +129,30 @@ __global__ void __launch_bounds__(256) int4_quantize_kernel(const T_ *__restrict
         const bool flat = !(s > 0.f);                                 // no range, or NaN
         const float z = SYM ? 8.f : flat ? 0.f : fminf(rintf(__fdiv_rn(-lo, s)), 15.f), inv = flat ? 0.f : __fdividef(1.f, s);
         if (!live[u]) continue;
-        float r[8], far = s < 1e-30f && !flat ? 1.f : 0.f;
+        float r[8];                                                   // levels, as whole numbers of fp32
+        bool divide = s < 1e-30f && !flat;                            // no 1 / s to speak of; and the scale's own rounding may put levels outside 0 .. 15
+        if constexpr (sizeof(T_) == 2) {
+            // Quotients of two bf16 numbers that are no tie are 1/512 or more away from one: taken to a multiple of 2^-14 first, what the approximation missed is gone.
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float t = value(u, i) * inv;
-            r[i] = __fadd_rn(__fadd_rn(t, ROUND), -ROUND);
-            far = fmaxf(far, fabsf(t - r[i]));
+            for (int i = 0; i < 8; ++i) r[i] = __fadd_rn(__fadd_rn(__fadd_rn(value(u, i) * inv, GRID), -GRID), ROUND);
+        } else {
+            float far = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float t = value(u, i) * inv;
+                r[i] = __fadd_rn(t, ROUND);
+                far = fmaxf(far, fabsf(t - __fadd_rn(r[i], -ROUND)));
+            }
+            divide |= far > 0.49998f;
         }
-        if (far > 0.49998f) {
+        // otherwise levels below 0 cannot come up: the lowest value's quotient is the zero's with the sign changed
+        const float shift = z - ROUND;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) r[i] = rintf(__fdiv_rn(value(u, i), s));
+        for (int i = 0; i < 8; ++i) r[i] = SYM ? r[i] + shift : fminf(r[i] + shift, 15.f);
+        if (divide) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) r[i] = fminf(fmaxf(rintf(__fdiv_rn(value(u, i), s)) + z, 0.f), 15.f);
         }
-        // levels below 0 cannot come up: the lowest value's quotient is the zero's with the sign changed
-#pragma unroll
-        for (int i = 0; i < 8; ++i) r[i] = SYM ? r[i] + z : fminf(r[i] + z, 15.f);
         const float half0 = fmaf(fmaf(fmaf(r[3], 16.f, r[2]), 16.f, r[1]), 16.f, r[0]), half1 = fmaf(fmaf(fmaf(r[7], 16.f, r[6]), 16.f, r[5]), 16.f, r[4]);
         *reinterpret_cast<uint32_t *>(q + (size_t)n[u] * (K / 2) + piece[u] * 4) =
             __byte_perm(__float_as_uint(half0 + 8388608.f), __float_as_uint(half1 + 8388608.f), 0x5410);

@@ -82,6 +82,24 @@ def test_quantize(N, K, group, zeros, dtype):
     assert torch.all((value(got) - w.double()).abs() <= (0.5 + (16 * 2.0 ** -8 if dtype == BF else 32 * U) + 1e-6) * step + (0 if zeros else 0))
 
 
+@pytest.mark.parametrize("zeros", [True, False])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_quantize_ties_and_extremes(dtype, zeros):
+    """Quotients that are ties, next to ties, huge and subnormal: the formulas' own levels."""
+    g = torch.Generator(device="cuda").manual_seed(1)
+    rows = [torch.arange(128, device="cuda") % 31 - 15.0]             # ends at +-15: quotients of halves and wholes
+    rows[0] = rows[0] / 2
+    rows += [torch.where(torch.rand(128, device="cuda", generator=g) < 0.5, 7.0, 3.5) * s for s in (1.0, 2.0 ** -130, 2.0 ** 100, 3e-45)]
+    rows += [torch.randint(-40, 41, (128,), device="cuda", generator=g).float() * s for s in (2.0 ** -149, 2.0 ** -133, 2.0 ** -126, 1e-30, 1e37 / 4)]
+    rows += [(torch.randint(-64, 65, (128,), device="cuda", generator=g).float() + 0.5) / 9.0, torch.randn(128, device="cuda", generator=g).to(BF).float()]
+    w = torch.stack(rows).repeat(64, 1)
+    w[::7] *= torch.randint(1, 256, (w[::7].shape[0], 1), device="cuda", generator=g)
+    w = w.clamp(-1e37, 1e37).to(dtype)
+    for group in (32, 128):
+        got, (q, s, z) = int4.quantize(w, group, not zeros), levels(w, group, zeros)
+        assert torch.equal(got.scales, s) and torch.equal(got.q, packed(q)) and (not zeros or torch.equal(got.zeros, z))
+
+
 def test_quantize_what_is_no_number():
     w = torch.randn(4, 128, device="cuda")
     w[0, 3], w[1, 70], w[2, 127] = math.inf, math.nan, -math.inf
