@@ -6,7 +6,7 @@
 //   Warp w < 8 takes tensor-memory lanes 32 (w mod 4) .. and every second stretch of 128 columns; warp 8 loads x (64 columns a stage, 128-byte swizzle), warp 9 issues
 // the products. Two CTAs share an SM, so one's epilogue runs under the other's products. The rounding of the weight (2^-8 of it at most) costs less than the
 // result's own; kept exact, each group's products would have to be read back from tensor memory and scaled, as long as the products themselves take.
-//   Few rows: the columns of W are shared out over a cluster of CTAs, whose sums meet in shared memory and are added in the order of their rank.
+//   Few rows: the columns of W are shared out over a cluster of CTAs, which send one another their sums; those are added in the order of their ranks.
 // Every wait is bounded; one that runs out sets the error flag and the CTA winds down.
 #include "gelu.cuh"
 #include "int4_linear.cuh"
@@ -24,11 +24,11 @@ struct TileArgs {
 template <int NT>
 struct ItCfg {
     static constexpr int XSTAGE = NT * 128, SLOT = 32 * 64;
-    static constexpr int most_ahead = NT == 128 ? 1 : NT == 64 ? 3 : 4;      // of a warp's own stretches, every second one
-    static constexpr int BARS = IT_XS * XSTAGE + IT_DQ * (most_ahead + 1) * SLOT;
+    static constexpr int most_ahead = NT == 32 ? 2 : 1;               // of a warp's own stretches, every second one (the L2 has been asked for them all)
+    static constexpr int MEET = IT_XS * XSTAGE + IT_DQ * (most_ahead + 1) * SLOT;
+    // where a cluster's sums meet: [rank they come from][row of x][row of W] fp32, of the rows of x that this CTA finishes (shares rounded up)
+    static constexpr int BARS = MEET + (NT < 128 ? (NT + IT_SPLITS - 1) * 512 : 0);
     static constexpr int SMEM = BARS + 256 + 1024;
-    static constexpr int ROW = 128 + 4;                               // of the sums' meeting place: [row of x][row of W] fp32
-    static_assert(NT * ROW * 4 <= BARS, "the sums lie where x and the levels were");
     static_assert(2 * (SMEM + 1024) <= 227 * 1024 && SMEM > 76 * 1024, "two CTAs an SM, and no third, whose tensor memory would not be there");
 };
 
@@ -142,6 +142,7 @@ __global__ void __launch_bounds__(IT_NT, 2) int4_tile_kernel(const __grid_consta
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    if (a.splits > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");      // here: this CTA runs, and may be written to
     const uint32_t tmem = warp_uniform(*tmem_slot), tA = tmem + NT;    // D: NT columns; A: two stretches of 64
     if (!a.constant) {
         // few rows: the levels on their way to the L2 while the kernel ahead ends
@@ -264,43 +265,60 @@ __global__ void __launch_bounds__(IT_NT, 2) int4_tile_kernel(const __grid_consta
     constexpr int HALF = NT / 2, STEP = HALF < 16 ? HALF : 16;
     const int sub = warp & 3, mh = (warp >> 2) * HALF;
     const uint32_t tD = tmem + ((uint32_t)(32 * sub) << 16) + mh;
-    float *sums = reinterpret_cast<float *>(sm);
     if (a.splits > 1) {
+        // A CTA finishes `share` rows of x: every other one's sums of them are sent there, and added in the order of the ranks once all have met.
+        const int share = (NT + a.splits - 1) / a.splits;
+        const uint32_t rank = cluster_rank();
+        asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
         if (warp < IT_DQ && ok) {
+            int owner = mh / share, left = (owner + 1) * share - mh;  // of the next column, and how many more are its
+            uint32_t to = cluster_addr(base + CF::MEET + ((rank * share + mh - owner * share) * 128 + 32 * sub + lane) * 4, owner);
 #pragma unroll
             for (int c = 0; c < HALF; c += STEP) {
                 float v[16];
                 tmem_ld16_nowait(tD + c, v);
                 tmem_ld_wait();
 #pragma unroll
-                for (int e = 0; e < STEP; ++e) sums[(mh + c + e) * CF::ROW + 32 * sub + lane] = v[e];
+                for (int e = 0; e < STEP; ++e) {
+                    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(v[e]) : "memory");
+                    to += 512;
+                    if (--left == 0) {
+                        left = share;
+                        ++owner;
+                        if (mh + c + e + 1 < NT) to = cluster_addr(base + CF::MEET + (rank * share * 128 + 32 * sub + lane) * 4, owner);
+                    }
+                }
             }
         }
-        cluster_sync_all();                                           // every CTA's sums are there
-        const uint32_t rank = cluster_rank();
-        for (int i = (int)rank * IT_NT + tid; i < 32 * NT; i += a.splits * IT_NT) {       // four rows of W a thread, all ranks' sums asked for at once
-            const int n = n0 + 4 * (i & 31), m = i >> 5;
-            if (n >= a.N || m0 + m >= a.M) continue;
-            const uint32_t at = base + (m * CF::ROW + 4 * (i & 31)) * 4;
-            float4 v[IT_SPLITS];
-#pragma unroll
-            for (int r = 0; r < IT_SPLITS; ++r) {
-                v[r] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (r < a.splits)
-                    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[r].x), "=f"(v[r].y), "=f"(v[r].z), "=f"(v[r].w) : "r"(cluster_addr(at, r)));
+        cluster_sync_all();                                           // and nobody writes to anyone from here on
+        const float4 *sums = reinterpret_cast<const float4 *>(sm + CF::MEET);
+        const bool whole = a.N % 4 == 0;
+        for (int i = tid; i < 32 * share; i += IT_NT) {               // four rows of W a thread
+            const int n = n0 + 4 * (i & 31), m = (int)rank * share + (i >> 5);
+            if (n >= a.N || m >= NT || m0 + m >= a.M) continue;
+            float4 v = sums[i];
+            for (int r = 1; r < a.splits; ++r) {
+                const float4 w = sums[r * share * 32 + i];
+                v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
             }
-            float s[4] = {v[0].x, v[0].y, v[0].z, v[0].w};
-#pragma unroll
-            for (int r = 1; r < IT_SPLITS; ++r) { s[0] += v[r].x; s[1] += v[r].y; s[2] += v[r].z; s[3] += v[r].w; }
+            float x[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                if (n + e >= a.N) break;
-                float x = s[e] + (a.bias != nullptr ? __bfloat162float(a.bias[n + e]) : 0.f);
-                if (a.act == 1) x = lg_gelu(x);
-                a.y[(size_t)(m0 + m) * a.N + n + e] = __float2bfloat16_rn(x);
+                if (a.bias != nullptr && n + e < a.N) x[e] += __bfloat162float(a.bias[n + e]);
+                if (a.act == 1) x[e] = lg_gelu(x[e]);
+            }
+            __nv_bfloat16 *at = a.y + (size_t)(m0 + m) * a.N + n;
+            if (whole) {
+                uint2 out;
+                reinterpret_cast<__nv_bfloat162 *>(&out)[0] = __floats2bfloat162_rn(x[0], x[1]);
+                reinterpret_cast<__nv_bfloat162 *>(&out)[1] = __floats2bfloat162_rn(x[2], x[3]);
+                *reinterpret_cast<uint2 *>(at) = out;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (n + e < a.N) at[e] = __float2bfloat16_rn(x[e]);
             }
         }
-        cluster_sync_all();                                           // nobody leaves while its sums are read
     } else if (warp < IT_DQ && ok) {
         const int n = n0 + 32 * sub + lane;
         const float bias = a.bias != nullptr && n < a.N ? __bfloat162float(a.bias[n]) : 0.f;
@@ -564,8 +582,10 @@ int int4_tile_launch(const Int4Linear &l, cudaStream_t stream) {
     a.wide = w.G % 4 == 0 && aligned(w.scales, 4 * es) && (w.zeros == nullptr || aligned(w.zeros, 4));
     const int NT = l.M <= 32 ? 32 : l.M <= 64 ? 64 : 128, C = (w.K + 127) / 128;
     const long long tiles = (long long)((w.N + 127) / 128) * ((l.M + NT - 1) / NT);
-    int splits = 1;                                                   // as many as give every SM a CTA, of two stretches or more
-    while (NT < 128 && splits < IT_SPLITS && tiles * splits * 2 <= sm_count() * 2 && C >= 4 * splits) splits *= 2;
+    // Shares of K while CTAs are no more than the SMs hold, and a share a stretch (us, 64 rows of x, 1 / 2 / 4 / 8: N 8192 K 2048 12.8 / 10.4 / 10.0 / 16.7, N 2048 K 8192 38 / 22 / 14 / 13.5,
+    // N 2328 K 768 6.4 / 6.2 / 5.5 / 5.5, N 50257 K 768 16 / 27 / 37 / 69).
+    int splits = 1;
+    while (NT < 128 && splits < IT_SPLITS && tiles * splits <= sm_count() && C >= 2 * splits) splits *= 2;
     Int4Linear part = l;
     cudaError_t e = cudaSuccess;
     // From four rounds over the chip on the larger tiles are ahead (us, N 8192 K 2048: 4096 rows 120 against 135; 1.7 rounds, N 2048 K 8192: 130 against 125).
