@@ -213,6 +213,7 @@ __device__ __forceinline__ float int4_act(float v, int act) { return act == 1 ? 
 // that order and x, whose fragments serve all MT blocks of rows, is reordered by byte permutes. A group's products end in an accumulator of their own that enters the
 // sum times the scale: the weight is never rounded. fp32 rows of x are three terms of eight bits each, cut off (their sum is x to the last bit), three products.
 //   Levels lie in 64-byte rows whose 16-byte pieces are swapped by the row, so that the eight rows of a fragment's word touch every bank once.
+constexpr long long PREFETCH = 48LL << 20;                            // of the L2's 126 MB, which the kernel ahead uses as well
 constexpr int RW_MOST = 8;                                             // warps of a CTA at most
 
 __device__ __forceinline__ void mma_bf16_warp(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -221,7 +222,7 @@ __device__ __forceinline__ void mma_bf16_warp(float (&c)[4], uint32_t a0, uint32
 }
 struct RowsArgs {
     const void *x; const unsigned char *q; const void *scales; const unsigned char *zeros; const void *bias; void *y;
-    int act, out_bf16, N, K, G, lg, warps, each, slots, ahead, slot_bytes, constant;   // each: stretches of a warp; ahead: those on their way
+    int act, out_bf16, N, K, G, lg, sms, warps, each, slots, ahead, slot_bytes, constant;   // each: stretches of a warp; ahead: those on their way
     long long M;
 };
 
@@ -311,10 +312,18 @@ __global__ void __launch_bounds__(RW_MOST * 32) int4_rows_kernel(const RowsArgs 
         for (int i = 0; i < ahead && i < mine; ++i) fetch_x(i);
         for (int i = 0; i < ahead; ++i) cp_async_commit();            // the first holds them all, the others keep the count
     } else {
-        // the levels on their way to the L2 while the kernel ahead ends: a row's stretches of this warp are one piece of memory
-        if (blockIdx.y == 0 && mine > 0) {
-            const int from = c0 * 64, bytes = half - from < a.each * 64 ? half - from : a.each * 64;
-            for (int r = lane; r < R && n0 + r < a.N; r += 32) l2_prefetch(a.q + (size_t)(n0 + r) * half + from, (uint32_t)bytes);
+        // Levels, scales and zeros on their way to the L2 while the kernel ahead runs. Where the SMs will not hold all CTAs beside it, the first ones ask for those of the CTAs
+        // behind them as well, up to PREFETCH bytes (N 16384 K 4096, one row: 16.6 -> 15.4 us a pass); many short ones ask for themselves (N 50257 K 768: 13.8 against 15.8).
+        const bool few = gridDim.x <= 4u * a.sms;
+        if (blockIdx.y == 0 && (!few || blockIdx.x < (unsigned)a.sms)) {
+            for (int n1 = n0; n1 < a.N && (long long)n1 * half < PREFETCH; n1 += few ? a.sms * R : a.N) {
+                const int count = a.N - n1 < R ? a.N - n1 : R;
+                for (int r = tid; r < count; r += a.warps * 32) l2_prefetch(a.q + (size_t)(n1 + r) * half, (uint32_t)half);
+                if (tid == 0) {
+                    l2_prefetch_around(reinterpret_cast<const uint8_t *>(a.scales) + (size_t)n1 * a.G * (S32 ? 4 : 2), (size_t)count * a.G * (S32 ? 4 : 2));
+                    if (a.zeros != nullptr) l2_prefetch_around(a.zeros + (size_t)n1 * a.G, (size_t)count * a.G);
+                }
+            }
         }
         pdl_wait();
         pdl_launch_dependents();
@@ -508,8 +517,9 @@ static cudaError_t rows_go_group(RowsArgs a, cudaStream_t stream) {
     a.each = (C + a.warps - 1) / a.warps;
     a.warps = (C + a.each - 1) / a.each;
     a.slot_bytes = R * 64 + rows * (X32 ? 512 : 256);
-    // stretches ahead: what keeps an SM's memory busy, four at most; either all of a warp's at once, or one slot more than are ahead
-    a.ahead = a.each < 4 ? a.each : 4;
+    // two stretches ahead: the levels come from the L2 as a rule, and more at once keep every warp's first one waiting (N 16384 K 4096, one row: 4 ahead 15.3 us, 2 14.6, 1 14.9).
+    // Either all of a warp's at once, or one slot more than are ahead.
+    a.ahead = a.each < 2 ? a.each : 2;
     while (a.ahead > 1 && a.warps * (a.ahead + (a.ahead < a.each ? 1 : 0)) * a.slot_bytes > 100 * 1024) --a.ahead;
     a.slots = a.ahead + (a.ahead < a.each ? 1 : 0);
     int smem = a.warps * a.slots * a.slot_bytes + 32;
@@ -536,14 +546,14 @@ static cudaError_t rows_go(RowsArgs a, cudaStream_t stream) {
 }
 template <int NB, bool X32, bool S32>
 static cudaError_t rows_blocks(RowsArgs a, cudaStream_t stream) {
-    // 16 warps an SM, of as many rows as that leaves (us, one row of x): N 16384 K 4096 with 32 rows and 4 warps a CTA 17.1, 64 and 8 18.5, 16 and 8 20.0; N 8192 K 2048 32 and 8 8.0,
-    // 16 and 8 9.1; N 2048 K 2048 16 and 8 3.3, 32 and 8 4.3; K 16384 N 4096 32 and 8 22, 16 and 8 28, 64 and 8 33. Several rows: N 16384 K 4096, 8 rows, 64 and 8 20.9, 32 and 8 22.9.
-    const long long tiles = (a.M + 8 * NB - 1) / (8 * NB), sms = sm_count();
+    // 16 warps an SM, of as many rows as that leaves (us; rows of W a CTA / warps): one row of x, N 16384 K 4096 32 / 4 15.3, 64 / 8 16.4, 16 / 8 18.3; N 8192 K 8192 32 / 8 16.7,
+    // 16 / 8 19.7, 64 / 8 21.9; N 2048 K 8192 16 / 8 8.1, 32 / 8 11.0. 8 rows, N 16384 K 4096: 64 / 8 18.9, 32 / 8 19.7; 16 rows: 32 / 8 24.6, 64 / 4 25.1, 64 / 8 30.
+    const long long tiles = (a.M + 8 * NB - 1) / (8 * NB), sms = a.sms;
     const long long by64 = (a.N + 63) / 64 * tiles, by32 = (a.N + 31) / 32 * tiles, by16 = (a.N + 15) / 16 * tiles;
-    // few columns and very many rows of W, whose CTAs are short: N 50257 K 768 16 and 2 13.8, 32 and 2 16.0
-    const int MT = a.M > 4 && by64 * 10 >= 17 * sms ? 4 : by32 * 10 < 7 * sms || (a.K <= 1024 && by16 >= 10 * sms) ? 1 : 2;
+    // few columns and very many rows of W, whose CTAs are short: N 50257 K 768 16 / 2 13.3, 32 / 2 13.6, 32 / 4 14.3
+    const int MT = a.M > 4 && NB == 1 && by64 * 10 >= 17 * sms ? 4 : by32 * 10 < 7 * sms || (a.K <= 1024 && by16 >= 10 * sms) ? 1 : 2;
     const long long ctas = MT == 4 ? by64 : MT == 2 ? by32 : by16;
-    a.warps = ctas * 8 <= 17 * sms ? 8 : ctas * 4 <= 17 * sms ? 4 : 2;
+    a.warps = ctas * 8 <= 17 * sms || NB > 1 ? 8 : ctas * 4 <= 17 * sms ? 4 : 2;
     if (MT == 4) return rows_go<4, NB, X32, S32>(a, stream);
     if (MT == 2) return rows_go<2, NB, X32, S32>(a, stream);
     return rows_go<1, NB, X32, S32>(a, stream);
@@ -551,7 +561,7 @@ static cudaError_t rows_blocks(RowsArgs a, cudaStream_t stream) {
 int int4_linear_launch(const Int4Linear &l, cudaStream_t stream) {
     const Int4Weight &w = l.w;
     if (l.M > PGB_INT4_ROWS && l.x_dtype == PGB_BF16 && l.out_dtype == PGB_BF16) return int4_tile_launch(l, stream);
-    const RowsArgs a{l.x, w.q, w.scales, w.zeros, l.bias, l.y, l.act, l.out_dtype == PGB_BF16, w.N, w.K, w.G, log2_group(w.group), 0, 0, 0, 0, 0, l.constant, l.M};
+    const RowsArgs a{l.x, w.q, w.scales, w.zeros, l.bias, l.y, l.act, l.out_dtype == PGB_BF16, w.N, w.K, w.G, log2_group(w.group), sm_count(), 0, 0, 0, 0, 0, l.constant, l.M};
     const bool x32 = l.x_dtype == PGB_F32, s32 = w.scale_dtype == PGB_F32;
     cudaError_t e;
     if (x32) e = s32 ? rows_blocks<1, true, true>(a, stream) : rows_blocks<1, true, false>(a, stream);

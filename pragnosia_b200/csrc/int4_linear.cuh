@@ -14,6 +14,11 @@ template <int N_> __device__ __forceinline__ void cp_async_wait() { asm volatile
 __device__ __forceinline__ void l2_prefetch(const void *p, uint32_t bytes) {
     asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory");
 }
+// the same for any address and size: the 16-byte pieces that hold any of it
+__device__ __forceinline__ void l2_prefetch_around(const void *p, size_t bytes) {
+    const uintptr_t from = reinterpret_cast<uintptr_t>(p) & ~(uintptr_t)15, to = (reinterpret_cast<uintptr_t>(p) + bytes + 15) & ~(uintptr_t)15;
+    l2_prefetch(reinterpret_cast<const void *>(from), (uint32_t)(to - from));
+}
 // the pair of levels in bits 0-3 and 16-19 as bf16 whole numbers less the zero: 0x4300 | q is 128 + q, z2 is 128 + z twice
 __device__ __forceinline__ uint32_t level_pair(uint32_t w, uint32_t z2) {
     uint32_t v, d;
