@@ -88,27 +88,16 @@ __device__ __forceinline__ void it_values(const uint4 &levels, const uint32_t (&
 }
 // the first of those four groups that a stretch has
 template <int LG> __device__ __forceinline__ int it_first(int stretch) { return LG == 7 ? stretch & 3 : LG == 6 ? (stretch & 1) * 2 : 0; }
-// 16 columns of D (rows m, m + 1, .. of x) of this lane's row n of W: + bias, the activation, rounded and stored; a row's 32 lanes are 64 bytes
-__device__ __forceinline__ void it_store16(const TileArgs &a, const float (&v)[16], float bias, long long m, int n, int count) {
+// 16 columns of D (rows m, m + 1, .. of x, `left` of them there) of this lane's row n of W: + bias, the activation, rounded and stored; a row's 32 lanes are 64 bytes
+__device__ __forceinline__ void it_store16(const TileArgs &a, const float (&v)[16], float bias, long long m, long long left, int n) {
     __nv_bfloat16 *row = a.y + (size_t)m * a.N;                       // uniform
-    if (m + count <= a.M) {
+    const bool there = n < a.N;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            if (e >= count) break;
-            float s = v[e] + bias;
-            if (a.act == 1) s = lg_gelu(s);
-            if (n < a.N) row[n] = __float2bfloat16_rn(s);
-            row += a.N;
-        }
-    } else {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            if (e >= count) break;
-            float s = v[e] + bias;
-            if (a.act == 1) s = lg_gelu(s);
-            if (m + e < a.M && n < a.N) row[n] = __float2bfloat16_rn(s);
-            row += a.N;
-        }
+    for (int e = 0; e < 16; ++e) {
+        float s = v[e] + bias;
+        if (a.act == 1) s = lg_gelu(s);
+        if (e < left && there) row[n] = __float2bfloat16_rn(s);
+        row += a.N;
     }
 }
 
@@ -262,7 +251,7 @@ __global__ void __launch_bounds__(IT_NT, 2) int4_tile_kernel(const __grid_consta
         ok = mbar_wait_warp(acc_full, 0, 65);
         tc_fence_after();
     }
-    constexpr int HALF = NT / 2, STEP = HALF < 16 ? HALF : 16;
+    constexpr int HALF = NT / 2, STEP = 16;
     const int sub = warp & 3, mh = (warp >> 2) * HALF;
     const uint32_t tD = tmem + ((uint32_t)(32 * sub) << 16) + mh;
     if (a.splits > 1) {
@@ -322,12 +311,12 @@ __global__ void __launch_bounds__(IT_NT, 2) int4_tile_kernel(const __grid_consta
     } else if (warp < IT_DQ && ok) {
         const int n = n0 + 32 * sub + lane;
         const float bias = a.bias != nullptr && n < a.N ? __bfloat162float(a.bias[n]) : 0.f;
-#pragma unroll
-        for (int c = 0; c < HALF; c += STEP) {
+#pragma unroll 1                                                      // unrolled, the epilogue's code evicts the other warps'
+        for (int c = 0; c < HALF; c += 16) {
             float v[16];
             tmem_ld16_nowait(tD + c, v);
             tmem_ld_wait();
-            it_store16(a, v, bias, m0 + mh + c, n, STEP);
+            it_store16(a, v, bias, m0 + mh + c, a.M - (m0 + mh + c), n);
         }
     }
     tc_fence_before();
@@ -339,7 +328,7 @@ __global__ void __launch_bounds__(IT_NT, 2) int4_tile_kernel(const __grid_consta
 // The same for tiles of 256 rows of x: twice the products for a tile's dequantisation, which is what the smaller tiles are bound by (issue slots: 128 rows of W and 128 of x
 // take 630 instructions and an epilogue as long for 256 cycles of the tensor pipe). One CTA an SM walks tiles: eight warps dequantise into four stages of shared memory
 // (A, 64 columns, 128-byte swizzle: D, twice 256 columns, takes all of tensor memory), eight store the tile before, 128 columns of D each.
-constexpr int IW_NT = 18 * 32, IW_XS = 3, IW_AS = 4, IW_AHEAD = 1;
+constexpr int IW_NT = 18 * 32, IW_XS = 4, IW_AS = 4, IW_AHEAD = 1;
 constexpr int IW_XSTAGE = 256 * 128, IW_ASTAGE = 128 * 128, IW_SLOT = 32 * 64;
 constexpr int IW_A = IW_XS * IW_XSTAGE, IW_RING = IW_A + IW_AS * IW_ASTAGE, IW_BARS = IW_RING + IT_DQ * (IW_AHEAD + 1) * IW_SLOT, IW_SMEM = IW_BARS + 256 + 1024;
 static_assert(IW_SMEM <= 227 * 1024, "shared memory");
@@ -390,13 +379,19 @@ __global__ void __launch_bounds__(IW_NT, 1) int4_wide_kernel(const __grid_consta
         const uint32_t wdst = ring + fr * 64 + ((ft ^ ((fr >> 1) & 3)) << 4);
         long long tile = blockIdx.x, ftile = blockIdx.x;
         int i = par, fi = par;
-        auto step = [&](long long &t, int &k) { for (; k >= C && t < tiles; k -= C) t += gridDim.x; };
-        step(tile, i);
-        ftile = tile; fi = i;
+        int row = 0, frow = 0;                                        // the first rows of W of the two iterators' tiles
+        auto step = [&](long long &t, int &k, int &r) {
+            if (k < C) return;
+            for (; k >= C && t < tiles; k -= C) t += gridDim.x;
+            r = n_of(t) + 32 * sub;
+        };
+        row = n_of(tile) + 32 * sub;
+        step(tile, i, row);
+        ftile = tile; fi = i; frow = row;
         uint32_t sn[S32 ? 4 : 2], zn;
         auto fetch = [&](int slot) {                                  // the fetch iterator's stretch, and on
             if (ftile < tiles) {
-                const int r0 = n_of(ftile) + 32 * sub + fr, col = fi * 128 + ft * 32;
+                const int r0 = frow + fr, col = fi * 128 + ft * 32;
                 const unsigned char *p = a.q + (size_t)r0 * half + (col >> 1);
                 const bool in = col < a.K;
 #pragma unroll
@@ -406,12 +401,12 @@ __global__ void __launch_bounds__(IW_NT, 1) int4_wide_kernel(const __grid_consta
                     p += (size_t)8 * half;
                 }
                 fi += 2;
-                step(ftile, fi);
+                step(ftile, fi, frow);
             }
             cp_async_commit();
         };
         for (int k = 0; k < IW_AHEAD; ++k) fetch(k);
-        it_groups<LG, S32>(a, tile < tiles ? n_of(tile) + 32 * sub + lane : a.N, i, true, sn, zn);
+        it_groups<LG, S32>(a, row + lane, i, tile < tiles, sn, zn);
         const uint32_t sw = (lane >> 1) & 3;
         int slot = 0;
         for (uint32_t round = 0; tile < tiles; ++round) {
@@ -421,8 +416,8 @@ __global__ void __launch_bounds__(IW_NT, 1) int4_wide_kernel(const __grid_consta
             const int first = it_first<LG>(i);
             fetch(slot == 0 ? IW_AHEAD : slot - 1);
             i += 2;
-            step(tile, i);
-            it_groups<LG, S32>(a, tile < tiles ? n_of(tile) + 32 * sub + lane : a.N, i, true, sn, zn);
+            step(tile, i, row);
+            it_groups<LG, S32>(a, row + lane, i, tile < tiles, sn, zn);
             cp_async_wait<IW_AHEAD>();
             __syncwarp();
             const uint8_t *ws = sm + IW_RING + (warp * (IW_AHEAD + 1) + slot) * IW_SLOT + lane * 64;
@@ -460,16 +455,19 @@ __global__ void __launch_bounds__(IW_NT, 1) int4_wide_kernel(const __grid_consta
             const uint32_t tD = tmem + ((uint32_t)(32 * sub) << 16) + d * 256 + mh;
             float v[2][16];
             tmem_ld16_nowait(tD, v[0]);
-#pragma unroll
-            for (int c = 0; c < 8; ++c) {
+#pragma unroll 1                                                      // unrolled, the epilogue's code evicts the other warps'
+            for (int c = 0; c < 8; c += 2) {
                 tmem_ld_wait();
-                if (c < 7) tmem_ld16_nowait(tD + 16 * (c + 1), v[(c + 1) & 1]);
+                tmem_ld16_nowait(tD + 16 * (c + 1), v[1]);
+                it_store16(a, v[0], bias, m + 16 * c, a.M - (m + 16 * c), n);
+                tmem_ld_wait();
+                if (c < 6) tmem_ld16_nowait(tD + 16 * (c + 2), v[0]);
                 else {                                                // all of D is in registers
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(acc_empty(d));
                 }
-                it_store16(a, v[c & 1], bias, m + 16 * c, n, 16);
+                it_store16(a, v[1], bias, m + 16 * (c + 1), a.M - (m + 16 * (c + 1)), n);
             }
         }
     } else if (warp == 16) {
