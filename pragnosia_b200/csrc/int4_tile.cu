@@ -586,8 +586,9 @@ int int4_tile_launch(const Int4Linear &l, cudaStream_t stream) {
     while (NT < 128 && splits < IT_SPLITS && tiles * splits <= sm_count() && C >= 2 * splits) splits *= 2;
     Int4Linear part = l;
     cudaError_t e = cudaSuccess;
-    // From four rounds over the chip on the larger tiles are ahead (us, N 8192 K 2048: 4096 rows 120 against 135; 1.7 rounds, N 2048 K 8192: 130 against 125).
-    if ((long long)((w.N + 127) / 128) * ((l.M + 255) / 256) >= 4LL * sm_count()) {
+    // From one and a half rounds over the chip on the larger tiles are ahead (us, theirs / the smaller ones': 4096 rows, N 2048 K 8192 113 / 136, N 2328 K 768 24 / 27, N 50257 K 768 323 / 431;
+    // a round: 2048 rows, N 2048 K 2048 19.4 / 19.2, N 2328 K 768 23.8 / 20.5; half a one: 512 rows, N 4096 K 4096 31 / 23).
+    if ((long long)((w.N + 127) / 128) * ((l.M + 255) / 256) * 2 >= 3LL * sm_count()) {
         e = wide_group(l, a, stream);
         if (e != cudaSuccess) { set_cuda_error(e, "int4_wide launch"); return PGB_ERR_CUDA; }
         return check_launch("int4_wide_kernel");
