@@ -572,7 +572,7 @@ static cudaError_t tile_group(const Int4Linear &l, const TileArgs &a, int splits
     return s32 ? tile_go<NT, 7, true>(l, a, splits, stream) : tile_go<NT, 7, false>(l, a, splits, stream);
 }
 
-// bf16 x and y. A grid's second axis ends at 65535, so very many rows go in several launches.
+// bf16 x and y.
 int int4_tile_launch(const Int4Linear &l, cudaStream_t stream) {
     const Int4Weight &w = l.w;
     const int es = w.scale_dtype == PGB_F32 ? 4 : 2;
@@ -584,22 +584,17 @@ int int4_tile_launch(const Int4Linear &l, cudaStream_t stream) {
     // N 2328 K 768 6.4 / 6.2 / 5.5 / 5.5, N 50257 K 768 16 / 27 / 37 / 69).
     int splits = 1;
     while (NT < 128 && splits < IT_SPLITS && tiles * splits <= sm_count() && C >= 2 * splits) splits *= 2;
-    Int4Linear part = l;
-    cudaError_t e = cudaSuccess;
-    // From one and a half rounds over the chip on the larger tiles are ahead (us, theirs / the smaller ones': 4096 rows, N 2048 K 8192 113 / 136, N 2328 K 768 24 / 27, N 50257 K 768 323 / 431;
+    // The larger tiles from one and a half rounds over the chip on, where x fills them well: one of 256 rows takes 1.6 times as long as one of 128 (us, theirs / the smaller ones':
+    // 4096 rows, N 2048 K 8192 113 / 136, N 2328 K 768 24 / 27, N 50257 K 768 323 / 431; 256 rows, N 32768 K 4096 64 / 72, 384 115 / 107, 128 59 / 39;
     // a round: 2048 rows, N 2048 K 2048 19.4 / 19.2, N 2328 K 768 23.8 / 20.5; half a one: 512 rows, N 4096 K 4096 31 / 23).
-    if ((long long)((w.N + 127) / 128) * ((l.M + 255) / 256) * 2 >= 3LL * sm_count()) {
-        e = wide_group(l, a, stream);
+    const long long halves = (l.M + 127) / 128, wide_rows = (l.M + 255) / 256;
+    if (8 * wide_rows < 5 * halves && (long long)((w.N + 127) / 128) * wide_rows * 2 >= 3LL * sm_count()) {
+        const cudaError_t e = wide_group(l, a, stream);
         if (e != cudaSuccess) { set_cuda_error(e, "int4_wide launch"); return PGB_ERR_CUDA; }
         return check_launch("int4_wide_kernel");
     }
-    for (long long m = 0; m < l.M && e == cudaSuccess; m += 65535LL * NT) {
-        part.M = l.M - m < 65535LL * NT ? l.M - m : 65535LL * NT;
-        part.x = (const __nv_bfloat16 *)l.x + (size_t)m * w.K;
-        a.M = part.M;
-        a.y = (__nv_bfloat16 *)l.y + (size_t)m * w.N;
-        e = NT == 32 ? tile_group<32>(part, a, splits, stream) : NT == 64 ? tile_group<64>(part, a, splits, stream) : tile_group<128>(part, a, splits, stream);
-    }
+    // so x has few enough tiles for a grid's second axis
+    const cudaError_t e = NT == 32 ? tile_group<32>(l, a, splits, stream) : NT == 64 ? tile_group<64>(l, a, splits, stream) : tile_group<128>(l, a, splits, stream);
     if (e != cudaSuccess) { set_cuda_error(e, "int4_tile launch"); return PGB_ERR_CUDA; }
     return check_launch("int4_tile_kernel");
 }

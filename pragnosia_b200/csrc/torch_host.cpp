@@ -676,6 +676,7 @@ struct Int4In { Tensor q, s, z; int64_t N, K; };
 Int4In int4_in(const Tensor &q, const Tensor &s, const OptTensor &z_, int64_t group) {
     const Tensor z = opt(z_);
     need_cuda(q, s, z);
+    no_gradient("an int4 weight", s);
     same_device(INT4, q, s);
     TORCH_CHECK_TYPE(q.scalar_type() == at::kByte && io_type(s.scalar_type()) && (!z.defined() || z.scalar_type() == at::kByte), INT4,
                      ": q and zeros are uint8, scales float32 or bfloat16, got ", q.scalar_type(), ", ", z.defined() ? z.scalar_type() : at::kByte, ", ", s.scalar_type());
@@ -723,7 +724,7 @@ Tensor int4_linear_fwd(const Tensor &x_, const Tensor &q, const Tensor &s, const
     return y;
 }
 OptTensor int4_linear(const Tensor &x, const Tensor &q, const Tensor &s, const OptTensor &z, int64_t group, const OptTensor &bias, int act, bool bf16, bool constant) {
-    if (!plain(x, q, s)) return std::nullopt;
+    if (!plain(x, q, s, opt(bias))) return std::nullopt;
     return int4_linear_fwd(x, q, s, z, group, bias, act, bf16, constant);
 }
 
@@ -764,7 +765,8 @@ Tensor adjust_fwd(const Tensor &l_, const OptTensor &prompt, const OptTensor &pr
                   double rep, const OptTensor &freq_t, double freq, const OptTensor &pres_t, double pres, const OptTensor &bias_ids, const OptTensor &bias_,
                   const OptTensor &mask_, const OptTensor &out_) {
     need_cuda(l_, opt(prompt), opt(prompt_n), opt(made), opt(made_n), opt(rep_t), opt(freq_t), opt(pres_t), opt(bias_ids), opt(bias_), opt(mask_), opt(out_));
-    no_gradient(ADJUST, l_);
+    for (const OptTensor &t : {OptTensor(l_), rep_t, freq_t, pres_t, bias_})
+        if (t) no_gradient(ADJUST, *t);
     TORCH_CHECK_TYPE(io_type(l_.scalar_type()), ADJUST, ": logits are float32 or bfloat16, got ", l_.scalar_type());
     TORCH_CHECK_VALUE(l_.dim() == 2 && l_.size(1) >= 1 && l_.size(1) <= MOST_WORDS, ADJUST, ": logits are (B, V), got ", l_.sizes());
     const int64_t B = l_.size(0), V = l_.size(1);
@@ -813,7 +815,7 @@ Tensor adjust_fwd(const Tensor &l_, const OptTensor &prompt, const OptTensor &pr
 OptTensor adjust_logits(const Tensor &l, const OptTensor &prompt, const OptTensor &prompt_n, const OptTensor &made, const OptTensor &made_n, const OptTensor &rep_t,
                         double rep, const OptTensor &freq_t, double freq, const OptTensor &pres_t, double pres, const OptTensor &bias_ids, const OptTensor &bias,
                         const OptTensor &mask, const OptTensor &out) {
-    if (!plain(l, opt(prompt), opt(made), opt(mask))) return std::nullopt;
+    if (!plain(l, opt(prompt), opt(made), opt(mask), opt(rep_t), opt(freq_t), opt(pres_t), opt(bias))) return std::nullopt;
     return adjust_fwd(l, prompt, prompt_n, made, made_n, rep_t, rep, freq_t, freq, pres_t, pres, bias_ids, bias, mask, out);
 }
 }  // namespace

@@ -38,7 +38,11 @@ def adjust_logits(logits, *, prompt=None, prompt_lengths=None, generated=None, g
             return done
     from . import custom_ops  # noqa: F401  (registers the operator)
     done = torch.ops.pragnosia_b200.adjust_logits(logits, prompt, prompt_lengths, generated, generated_lengths, rt, r, ft, f, pt, p, bias_ids, bias, mask)
-    return done if out is None else out.copy_(done)
+    if out is None:
+        return done
+    if out.dtype != done.dtype or out.shape != done.shape:
+        raise ValueError("adjust_logits: out is a dense float32 tensor of the logits' shape")
+    return out.copy_(done)
 
 
 @dataclass

@@ -172,6 +172,12 @@ def test_refusals():
             bad()
     with torch.enable_grad(), pytest.raises(RuntimeError, match="no gradient"):
         f(l.clone().requires_grad_())
+    leaf = torch.ones(l.shape[0], device=l.device, requires_grad=True)
+    for kw in (dict(repetition=leaf), dict(frequency=leaf), dict(presence=leaf), dict(bias_ids=torch.zeros(1, 1, dtype=torch.long, device=l.device), bias=leaf[:1, None])):
+        with torch.enable_grad(), pytest.raises(RuntimeError, match="no gradient"):
+            f(l, **kw)
+        with torch.no_grad():
+            assert f(l, **kw).shape == l.shape
 
 
 def test_in_a_graph_with_a_counter_on_the_device():

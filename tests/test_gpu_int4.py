@@ -159,6 +159,36 @@ def test_linear(M, K, N, x_dtype, scale_dtype, out):
     assert torch.equal(y, int4.linear(x, w, bias, act=act, out_dtype=out))
 
 
+LARGE = [(4096, 160, 1900), (129, 96, 28500), (8197, 416, 1000), (16384, 32, 1001), (256, 704, 50257), (2000, 2048, 4099), (896, 128, 16384)]
+
+
+@pytest.mark.parametrize("M,K,N", LARGE)
+@pytest.mark.parametrize("scale_dtype", [BF, F32])
+def test_linear_of_many_tiles(M, K, N, scale_dtype):
+    """From one to several tiles a CTA, ends that fill no tile, one stretch of columns and many."""
+    i = LARGE.index((M, K, N))
+    w = random_weight(N, K, (64, 32, 128)[i % 3], i % 2 == 0, scale_dtype, i)
+    g = torch.Generator(device="cuda").manual_seed(200 + i)
+    x = torch.randn(M, K, device="cuda", generator=g).to(BF)
+    bias = torch.randn(N, device="cuda", generator=g).to(BF) if i % 3 != 1 else None
+    act = "gelu" if i % 2 else None
+    y = int4.linear(x, w, bias, act=act)
+    check_linear(x, w, bias, act, BF, y)
+    assert torch.equal(y, int4.linear(x, w, bias, act=act))
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("zeros", [True, False])
+def test_linear_groups_of_many_tiles(group, zeros):
+    K, N, M = 416, 4000, 2000
+    w = random_weight(N, K, group, zeros, BF, 3)
+    x = torch.zeros(M, K, device="cuda", dtype=BF)
+    cols = (torch.arange(M, device="cuda") * 7) % K
+    x[torch.arange(M, device="cuda"), cols] = 1.0
+    v = value(w).t()[cols]
+    assert torch.all((int4.linear(x, w).double() - v).abs() <= 2.0 ** -8 * v.abs())
+
+
 @pytest.mark.parametrize("group", [32, 64, 128])
 @pytest.mark.parametrize("zeros", [True, False])
 @pytest.mark.parametrize("M", [1, 5, 12, 40, 200])
@@ -219,14 +249,15 @@ def test_linear_refusals():
             bad()
     with torch.enable_grad():
         for call in (lambda: int4.linear(x.clone().requires_grad_(), w), lambda: int4.linear(x, w, torch.zeros(40, device="cuda", requires_grad=True)),
-                     lambda: int4.quantize(x.clone().requires_grad_())):
+                     lambda: int4.quantize(x.clone().requires_grad_()), lambda: int4.linear(x, w._replace(scales=w.scales.clone().requires_grad_())),
+                     lambda: int4.dequantize(w._replace(scales=w.scales.clone().requires_grad_()))):
             with pytest.raises(RuntimeError, match="no gradient"):
                 call()
     with torch.no_grad():
         assert int4.linear(x.clone().requires_grad_(), w).shape == (3, 40)
 
 
-@pytest.mark.parametrize("M", [1, 12, 40, 300])
+@pytest.mark.parametrize("M", [1, 12, 40, 300, 10000])
 def test_linear_in_a_graph_and_on_another_stream(M):
     K, N = 768, 776
     w = random_weight(N, K, 64, True, BF, 8)
@@ -249,7 +280,7 @@ def test_linear_in_a_graph_and_on_another_stream(M):
     assert torch.equal(other, want)
 
 
-@pytest.mark.parametrize("M", [1, 40])
+@pytest.mark.parametrize("M", [1, 40, 2000])
 def test_a_weight_made_just_ahead(M):
     """Levels, scales and activations that the kernels right ahead on the stream write: read behind them."""
     K, N = 2048, 4096
