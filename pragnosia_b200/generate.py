@@ -438,7 +438,7 @@ class Decoder:
         key = (tuple(sorted(c.numbers().items())), tuple(sorted((k, tuple(t.shape), t.dtype) for k, t in given.items())))
         if getattr(self, "_ctl_key", None) != key:
             self._ctl, self._ctl_key = {k: torch.empty(t.shape, dtype=t.dtype, device=t.device) for k, t in given.items()}, key
-            self._ctl_numbers = c.numbers()
+            self._ctl_numbers, self._gen_key = c.numbers(), None      # a captured loop reads the buffers it was captured with
         for k, t in given.items():
             self._ctl[k].copy_(t)
         return key

@@ -134,6 +134,23 @@ def test_generated_tokens_under_controls(kind, B, dtype):
     assert torch.equal(dec.generate(ids, 24), Decoder(m, batch=B).generate(ids, 24))
 
 
+def test_a_captured_loop_reads_the_settings_of_its_own_call():
+    """Settings that were others in between, while the loop was not in use."""
+    V = 500
+    m = model(dtype=BF, vocab=V)
+    ids = synth.token_ids(2, 20, V, seed=7).to(DEV)
+    one, other = sampling.Controls(frequency=torch.full((2,), 0.5, device=DEV)), sampling.Controls(mask=torch.arange(V, device=DEV)[None] < 50)
+    dec = Decoder(m, batch=2, controls=one)
+    first = dec.generate(ids, 24)
+    for between in (other, None):
+        dec.use_graph, dec.controls = False, between
+        dec.generate(ids, 24)
+        dec.use_graph, dec.controls = True, sampling.Controls(frequency=torch.full((2,), 3.0, device=DEV))
+        assert torch.equal(dec.generate(ids, 24), Decoder(m, batch=2, controls=dec.controls).generate(ids, 24))
+        dec.controls = one
+        assert torch.equal(dec.generate(ids, 24), first)
+
+
 def test_a_sampled_loop_keeps_to_its_mask():
     V, B = 500, 3
     m = model(dtype=BF, vocab=V)
