@@ -590,15 +590,18 @@ int pgb_embedding_bwd(const long long *ids, const void *grad, int dtype, float s
  *   Sums in fp32, one rounding at the end. The weight enters as scale times a whole number sum, unrounded -- but for bf16 x and y with more than
  *   PGB_INT4_ROWS rows, where scale (q - zero) is rounded to bf16 for the tensor cores. flags: PGB_INT4_CONSTANT = q, scales, zeros and bias were
  *   complete before the kernel ahead on the stream was launched, and may be read while it runs. Bounded waits as in the prefill
- *   kernels (pgb_tc_error_flag: 61-69).
+ *   kernels (pgb_tc_error_flag: 61-69). scratch, 16-byte aligned, of pgb_int4_linear_scratch_bytes (0: none, NULL) holds what fp32 rows of x become for the
+ *   tensor cores; a call's own until the call is over. Sums of x (q - zero) over a group have to stay within fp32.
  * x, q, w, y 16-byte aligned, scales, zeros, bias to their element. N, K up to 2^24, M below 2^31. The same call gives the same bits.
  * ------------------------------------------------------------------------------------------------------- */
 enum { PGB_INT4_CONSTANT = 1, PGB_INT4_ROWS = 16 };
 int pgb_int4_quantize(const void *w, int dtype, unsigned char *q, void *scales, unsigned char *zeros, int N, int K, int group, void *stream);
 int pgb_int4_dequantize(const unsigned char *q, const void *scales, int scale_dtype, const unsigned char *zeros, void *w, int dtype, int N,
                         int K, int group, void *stream);
+long long pgb_int4_linear_scratch_bytes(int x_dtype, int out_dtype, long long M, int N, int K);
 int pgb_int4_linear(const void *x, int x_dtype, const unsigned char *q, const void *scales, int scale_dtype, const unsigned char *zeros,
-                    const void *bias, int act, void *y, int out_dtype, long long M, int N, int K, int group, int flags, void *stream);
+                    const void *bias, int act, void *y, int out_dtype, void *scratch, long long scratch_bytes, long long M, int N, int K, int group,
+                    int flags, void *stream);
 
 /* ---------------------------------------------------------------------------------------------------------
  * Penalties, biases and masks on logits ahead of a draw. No counterpart in the reference. For word v of row b, n times among the generated ids and

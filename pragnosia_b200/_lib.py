@@ -95,7 +95,8 @@ SIGNATURES = {
     "pgb_embedding_bwd": [_vp, _vp, _i, _f, _ll, _vp, _vp, _ll, _ll, _i, _i, _vp],
     "pgb_int4_quantize": [_vp, _i, _vp, _vp, _vp, _i, _i, _i, _vp],
     "pgb_int4_dequantize": [_vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _vp],
-    "pgb_int4_linear": [_vp, _i, _vp, _vp, _i, _vp, _vp, _i, _vp, _i, _ll, _i, _i, _i, _i, _vp],
+    "pgb_int4_linear": [_vp, _i, _vp, _vp, _i, _vp, _vp, _i, _vp, _i, _vp, _ll, _ll, _i, _i, _i, _i, _vp],
+    "pgb_int4_linear_scratch_bytes": [_i, _i, _ll, _i, _i],
     "pgb_adjust_logits": [_vp, _i, _ll, _vp, _vp, _ll, _i, _vp, _i, _vp, _ll, _i, _vp, _i, _vp, _f, _vp, _f, _vp, _f, _vp, _vp, _ll, _i, _vp, _i, _ll,
                           _ll, _i, _vp],
     "pgb_skinny_linear": [_vp, _vp, _vp, _vp, _i, _f, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _vp],

@@ -122,7 +122,9 @@ int decode_token_wait_selftest_launch(unsigned long long *, unsigned, cudaStream
 int int4_quantize_launch(const void *, int, unsigned char *, void *, unsigned char *, int, int, int, cudaStream_t);
 int int4_dequantize_launch(const Int4Weight &, void *, int, cudaStream_t);
 int int4_linear_launch(const Int4Linear &, cudaStream_t);
+bool int4_exact_tiles(const Int4Linear &);
 int int4_tile_error_flag(int *);
+int int4_exact_error_flag(int *);
 int adjust_logits_launch(const AdjustLogits &, cudaStream_t);
 
 // PGB_PREFILL_AUTO sends bf16 plain-rule work to the tensor-core kernel only once this is on
@@ -952,8 +954,15 @@ int pgb_int4_dequantize(const unsigned char *q, const void *scales, int scale_dt
     return int4_dequantize_launch(in, w, dtype, (cudaStream_t)stream);
 }
 
+long long pgb_int4_linear_scratch_bytes(int x_dtype, int out_dtype, long long M, int N, int K) {
+    if (M < 1 || M > 0x7fffffffLL || int4_sizes(N, K, 32) != PGB_OK || x_dtype != PGB_F32) return 0;
+    Int4Linear a;
+    a.x_dtype = x_dtype; a.out_dtype = out_dtype; a.M = M; a.w.N = N; a.w.K = K;
+    return int4_exact_tiles(a) ? 6 * M * K : 0;
+}
+
 int pgb_int4_linear(const void *x, int x_dtype, const unsigned char *q, const void *scales, int scale_dtype, const unsigned char *zeros, const void *bias,
-                    int act, void *y, int out_dtype, long long M, int N, int K, int group, int flags, void *stream) {
+                    int act, void *y, int out_dtype, void *scratch, long long scratch_bytes, long long M, int N, int K, int group, int flags, void *stream) {
     Int4Linear a;
     if (!x || !y) return PGB_ERR_NULL_POINTER;
     if (!io_dtype(x_dtype) || !io_dtype(out_dtype)) return PGB_ERR_BAD_DTYPE;
@@ -963,6 +972,11 @@ int pgb_int4_linear(const void *x, int x_dtype, const unsigned char *q, const vo
     if (M > 0x7fffffffLL) return PGB_ERR_TOO_LARGE;
     if (!aligned(x, 16) || !aligned(y, 16) || (bias && !aligned_to(bias, x_dtype))) return PGB_ERR_MISALIGNED;
     a.x = x; a.x_dtype = x_dtype; a.bias = bias; a.act = act; a.y = y; a.out_dtype = out_dtype; a.M = M; a.constant = flags & PGB_INT4_CONSTANT;
+    a.scratch = scratch;
+    const long long need = pgb_int4_linear_scratch_bytes(x_dtype, out_dtype, M, N, K);
+    if (need > 0 && !scratch) return PGB_ERR_NULL_POINTER;
+    if (need > scratch_bytes && need > 0) return PGB_ERR_BAD_SHAPE;
+    if (need > 0 && !aligned(scratch, 16)) return PGB_ERR_MISALIGNED;
     return int4_linear_launch(a, (cudaStream_t)stream);
 }
 
@@ -1092,6 +1106,8 @@ int pgb_tc_error_flag(int *out_host) {
     if (rc == PGB_OK) rc = head_loss_error_flag(&g);
     f = f > g ? f : g;
     if (rc == PGB_OK) rc = int4_tile_error_flag(&g);
+    f = f > g ? f : g;
+    if (rc == PGB_OK) rc = int4_exact_error_flag(&g);
     f = f > g ? f : g;
     e = e > f ? e : f;
     b = b > c ? b : c;

@@ -129,7 +129,7 @@ struct HeadLossArgs {
 };
 // a weight in four bits (int4.cu): q [N][K/2], scales [N][G] in bf16 or fp32, zeros [N][G] or NULL (8); a linear layer of it
 struct Int4Weight { const unsigned char *q; const void *scales; int scale_dtype; const unsigned char *zeros; int N, K, group, G; };
-struct Int4Linear { const void *x; int x_dtype; Int4Weight w; const void *bias; int act; void *y; int out_dtype; long long M; int constant; };
+struct Int4Linear { const void *x; int x_dtype; Int4Weight w; const void *bias; int act; void *y; int out_dtype; long long M; int constant; void *scratch; };
 // what is done to logits ahead of a draw (adjust_logits.cu): ids [rows][n] with a row stride (0: one row for all) and lengths (NULL: all n; stride 0 or 1)
 struct TokenList { const long long *ids; long long stride; int n; const long long *lengths; int length_stride; };
 struct RowValue { const float *at; float all; };                      // one per row, or one for all (at NULL)

@@ -203,8 +203,6 @@ __global__ void __launch_bounds__(256) int4_dequantize_kernel(const unsigned cha
 }
 
 // ------------------------------------------------------------------------------------------------ linear
-__device__ __forceinline__ float int4_act(float v, int act) { return act == 1 ? 0.5f * v * (1.0f + erff(v * 0.70710678118654752f)) : v; }
-
 // Few rows of x: the time is the weight's bytes, and what stands in their way is the arithmetic that makes operands of them. One CTA owns 16 MT rows of W, its
 // eight warps every eighth stretch of 128 columns each. A warp streams its stretches through slots of shared memory of its own by asynchronous copies (nothing
 // is held in registers while they fly, no barrier between warps), so a CTA reads 512 B of each row at a time, and the warps' sums meet once at the end, in order.
@@ -380,15 +378,7 @@ __global__ void __launch_bounds__(RW_MOST * 32) int4_rows_kernel(const RowsArgs 
                     for (int e = 0; e < 4; ++e) {
                         uint32_t u[2][3];
 #pragma unroll
-                        for (int p = 0; p < 2; ++p) {                 // x = head + middle + rest, eight bits each
-                            const uint32_t bits = p == 0 ? one[e] : two[e];
-                            const bool fin = (bits & 0x7f800000u) != 0x7f800000u;
-                            const float f = __uint_as_float(bits);
-                            const float r1 = fin ? f - __uint_as_float(bits & 0xffff0000u) : 0.f;
-                            const float r2 = r1 - __uint_as_float(__float_as_uint(r1) & 0xffff0000u);
-                            u[p][0] = fin || (bits & 0x007fffffu) == 0u ? bits : 0x7fc00000u;
-                            u[p][1] = __float_as_uint(r1); u[p][2] = __float_as_uint(r2);
-                        }
+                        for (int p = 0; p < 2; ++p) fp32_terms(p == 0 ? one[e] : two[e], u[p]);
 #pragma unroll
                         for (int q3 = 0; q3 < 3; ++q3) bx[j][q3][b][e] = __byte_perm(u[0][q3], u[1][q3], 0x7632);
                     }
@@ -562,6 +552,7 @@ static cudaError_t rows_blocks(RowsArgs a, cudaStream_t stream) {
 int int4_linear_launch(const Int4Linear &l, cudaStream_t stream) {
     const Int4Weight &w = l.w;
     if (l.M > PGB_INT4_ROWS && l.x_dtype == PGB_BF16 && l.out_dtype == PGB_BF16) return int4_tile_launch(l, stream);
+    if (int4_exact_tiles(l)) return int4_exact_launch(l, stream);
     const RowsArgs a{l.x, w.q, w.scales, w.zeros, l.bias, l.y, l.act, l.out_dtype == PGB_BF16, w.N, w.K, w.G, log2_group(w.group), sm_count(), 0, 0, 0, 0, 0, l.constant, l.M};
     const bool x32 = l.x_dtype == PGB_F32, s32 = w.scale_dtype == PGB_F32;
     cudaError_t e;

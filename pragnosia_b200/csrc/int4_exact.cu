@@ -1,0 +1,388 @@
+// The four-bit linear layer for many rows of x where x or y is fp32: the weight is not rounded. y^T = sum over groups of s (q - z) x^T on the tensor cores.
+//
+//   A is the whole numbers q - z, exact in bf16; x its own bf16 or, for fp32, three bf16 terms of eight bits each, cut off, whose sum is x to the last bit. So a group's
+// products are exact and its sum an fp32 one, in an accumulator D of its own; the scale, one per row of W and group, meets it in registers: acc += s D.
+//   A CTA owns 128 rows of W and NT rows of x. Four warps make A in tensor memory (two stretches of 128 columns; lane = row of W), one loads x by TMA (64 columns of each
+// term a stage, 128-byte swizzle), one issues the products, and eight take the groups' sums: D has two halves, so the next group's products run under them. Two
+// CTAs share an SM. For 64 columns of three terms the tensor pipe takes 384 cycles, the reading and scaling of a group of 64 about 130, one of 32 twice that.
+//   The columns of W are shared out over a cluster of CTAs where tiles are few; their sums meet in shared memory and are added in the order of the ranks.
+// Every wait is bounded; one that runs out sets the error flag and the CTA winds down.
+#include "int4_linear.cuh"
+#include "tc_pair.cuh"
+
+namespace pgb {
+
+constexpr int IE_DQ = 4, IE_ACC = 8, IE_NT = (IE_DQ + IE_ACC + 2) * 32, IE_AHEAD = 2, IE_SPLITS = 8;     // warps that make A, that add up; stretches of levels on their way; shares of K
+
+struct ExactArgs {
+    const unsigned char *q; const void *scales; const unsigned char *zeros; const void *bias; void *y;
+    long long M; int act, out_bf16, N, K, G, wide, each, splits, constant;      // wide: scales of four groups at once; each: a share's stretches
+};
+
+template <int NT, int XT>
+struct IeCfg {
+    static constexpr int XS = XT == 3 ? 3 : 6, XPLANE = NT * 128, XSTAGE = XT * XPLANE, SLOT = 32 * 64, RING = XS * XSTAGE;
+    static constexpr int USED = RING + IE_DQ * (IE_AHEAD + 1) * SLOT;
+    // the sums' meeting place [rank they come from][row of x][row of W] fp32 takes the stages' room
+    static constexpr int MEET = (NT + IE_SPLITS - 1) * 512, LEAST = 77 * 1024 - 1280, BODY = USED > MEET ? USED : MEET;
+    static constexpr int BARS = (BODY > LEAST ? BODY : LEAST), SMEM = BARS + 256 + 1024;
+    static_assert(2 * (SMEM + 1024) <= 227 * 1024 && SMEM > 76 * 1024, "two CTAs an SM, and no third, whose tensor memory would not be there");
+};
+
+// 32 levels as whole numbers q - z in bf16, in their order; z2: 128 + z twice
+__device__ __forceinline__ void ie_levels(const uint4 &levels, uint32_t z2, uint32_t (&out)[16]) {
+    const uint32_t w[4] = {levels.x, levels.y, levels.z, levels.w};
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+        uint32_t p[4];
+#pragma unroll
+        for (int h = 0; h < 4; ++h) p[h] = level_pair(w[v] >> (4 * h), z2);      // (0,4) (1,5) (2,6) (3,7)
+        out[4 * v] = __byte_perm(p[0], p[1], 0x5410); out[4 * v + 1] = __byte_perm(p[2], p[3], 0x5410);
+        out[4 * v + 2] = __byte_perm(p[0], p[1], 0x7632); out[4 * v + 3] = __byte_perm(p[2], p[3], 0x7632);
+    }
+}
+
+template <int NT, int XT, int LG, bool S32>
+__global__ void __launch_bounds__(IE_NT, 2) int4_exact_kernel(const __grid_constant__ CUtensorMap mx, const ExactArgs a) {
+    using CF = IeCfg<NT, XT>;
+    constexpr int XS = CF::XS, COLS = NT / 2, PER = 128 >> LG;        // columns of D a warp adds up; groups of a stretch
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t *sm = smem_raw + (base - smem_u32(smem_raw));
+    const uint32_t mb = base + CF::BARS;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(sm + CF::BARS + 192);
+    auto x_full = [&](int s) { return mb + 8 * s; };
+    auto x_empty = [&](int s) { return mb + 48 + 8 * s; };
+    auto a_full = [&](int s) { return mb + 96 + 8 * s; };
+    auto a_empty = [&](int s) { return mb + 112 + 8 * s; };
+    auto d_full = [&](int d) { return mb + 128 + 8 * d; };
+    auto d_empty = [&](int d) { return mb + 144 + 8 * d; };
+    const uint32_t drained = mb + 160;
+
+    const int tid = threadIdx.x, lane = tid & 31, warp = warp_uniform(tid >> 5);
+    const int n0 = blockIdx.x * 128;
+    const long long m0 = (long long)blockIdx.y * NT;
+    const int C = (a.K + 127) >> 7, c0 = (int)blockIdx.z * a.each, mine = C - c0 < a.each ? C - c0 : a.each;     // this CTA's stretches (one at least)
+
+    if (tid == 0) {
+        for (int s = 0; s < XS; ++s) { mbar_init(x_full(s), 1); mbar_init(x_empty(s), 1); }
+        for (int s = 0; s < 2; ++s) { mbar_init(a_full(s), IE_DQ); mbar_init(a_empty(s), 1); mbar_init(d_full(s), 1); mbar_init(d_empty(s), IE_ACC); }
+        mbar_init(drained, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 13) tmem_alloc(smem_u32(tmem_slot), 256);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = warp_uniform(*tmem_slot), tA = tmem + 2 * NT;        // D: two times NT columns; A: two stretches of 64
+    if (!a.constant) { pdl_wait(); pdl_launch_dependents(); }
+    bool ok = true;
+    float acc[COLS];
+#pragma unroll
+    for (int e = 0; e < COLS; ++e) acc[e] = 0.f;
+    const int sub = warp & 3, row = n0 + 32 * sub + lane;              // tensor memory's lanes 32 sub .. are this warp's
+
+    if (warp < IE_DQ) {
+        // ------------------------------------------------------------------------------------------ levels -> A
+        const uint32_t ring = base + CF::RING + warp * (IE_AHEAD + 1) * CF::SLOT;
+        const int half = a.K >> 1, fr = lane >> 2, ft = lane & 3;
+        int wcol = c0 * 128 + ft * 32;
+        const unsigned char *wsrc = a.q + (size_t)(n0 + 32 * sub + fr) * half + (wcol >> 1);
+        uint32_t live = 0;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) live |= (n0 + 32 * sub + 8 * u + fr < a.N ? 1u : 0u) << u;
+        const uint32_t wdst = ring + fr * 64 + ((ft ^ ((fr >> 1) & 3)) << 4);
+        auto fetch = [&](int slot) {
+            const uint32_t in = wcol < a.K ? live : 0u, dst = wdst + slot * CF::SLOT;
+            const unsigned char *p = wsrc;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const bool here = in >> u & 1u;
+                cp_async16(dst + u * 512, here ? p : a.q, here ? 16 : 0);
+                p += (size_t)8 * half;
+            }
+            wcol += 128; wsrc += 64;
+        };
+        uint32_t unused[S32 ? 4 : 2], zn;
+        for (int i = 0; i < IE_AHEAD; ++i) { if (i < mine) fetch(i); cp_async_commit(); }
+        it_groups<LG, S32>(a, row, c0, true, unused, zn);
+        if (a.constant) { pdl_wait(); pdl_launch_dependents(); }
+        const uint32_t mine_row = lane * 64, sw = (lane >> 1) & 3;
+        int slot = 0;
+        for (int i = 0; i < mine; ++i) {
+            const uint32_t zc = zn;
+            it_groups<LG, S32>(a, row, c0 + i + 1, i + 1 < mine, unused, zn);
+            if (i + IE_AHEAD < mine) fetch(slot == 0 ? IE_AHEAD : slot - 1);
+            cp_async_commit();
+            cp_async_wait<IE_AHEAD>();
+            __syncwarp();
+            const uint8_t *ws = sm + (ring - base) + slot * CF::SLOT + mine_row;
+            slot = slot == IE_AHEAD ? 0 : slot + 1;
+            const int st = i & 1, first = it_first<LG>(c0 + i);
+            const uint32_t dst = tA + ((uint32_t)(32 * sub) << 16) + st * 64;
+            if (i >= 2) ok = mbar_wait_warp(a_empty(st), ((i >> 1) + 1) & 1, 61);
+            if (!ok) break;
+            tc_fence_after();
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {                             // 32 columns
+                uint32_t out[16];
+                const int e = first + (j >> (LG - 5));
+                ie_levels(*reinterpret_cast<const uint4 *>(ws + ((j ^ sw) << 4)), __byte_perm(zc, 0x43u, 0x4040 | e | e << 8), out);
+                tmem_st16(dst + 16 * j, out);
+            }
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(a_full(st));
+        }
+        cp_async_wait<0>();
+    } else if (warp < IE_DQ + IE_ACC) {
+        // ------------------------------------------------------------------------------------------ acc += s D
+        uint32_t sn[S32 ? 4 : 2], zn;
+        it_groups<LG, S32>(a, row, c0, true, sn, zn);
+        if (a.constant) pdl_wait();
+        const uint32_t tD = tmem + ((uint32_t)(32 * sub) << 16) + ((warp - IE_DQ) >> 2) * COLS;
+        uint32_t group = 0;
+        for (int i = 0; i < mine && ok; ++i) {
+            uint32_t sc[S32 ? 4 : 2];
+#pragma unroll
+            for (int e = 0; e < (S32 ? 4 : 2); ++e) sc[e] = sn[e];
+            it_groups<LG, S32>(a, row, c0 + i + 1, i + 1 < mine, sn, zn);
+            const int first = it_first<LG>(c0 + i);
+#pragma unroll 1
+            for (int j = 0; j < PER; ++j, ++group) {
+                const int d = group & 1, e = first + j;
+                float s;
+                if constexpr (S32) s = __uint_as_float(e < 2 ? (e == 0 ? sc[0] : sc[1]) : (e == 2 ? sc[2] : sc[3]));
+                else {
+                    const uint32_t two = e >> 1 ? sc[1] : sc[0];
+                    s = __uint_as_float(e & 1 ? two & 0xffff0000u : two << 16);
+                }
+                ok = mbar_wait_warp(d_full(d), (group >> 1) & 1, 65);
+                if (!ok) break;
+                tc_fence_after();
+#pragma unroll
+                for (int c = 0; c < COLS; c += 16) {
+                    float v[16];
+                    tmem_ld16_nowait(tD + d * NT + c, v);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) acc[c + k] = fmaf(s, v[k], acc[c + k]);
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(d_empty(d));
+            }
+        }
+    } else if (warp == 12) {
+        // ------------------------------------------------------------------------------------------ x
+        if (a.constant) pdl_wait();
+        const bool leader = elect_one();
+        int it = 0;
+        for (; it < 2 * mine && ok; ++it) {
+            const int s = it % XS;
+            if (it >= XS) ok = mbar_wait_warp(x_empty(s), ((it / XS) + 1) & 1, 62);
+            if (ok && leader) {
+                mbar_expect_tx(x_full(s), CF::XSTAGE);
+#pragma unroll
+                for (int t = 0; t < XT; ++t) tma_load_3d(base + s * CF::XSTAGE + t * CF::XPLANE, &mx, x_full(s), c0 * 128 + it * 64, (int)m0, t);
+            }
+            __syncwarp();
+        }
+        if (!ok)                                                      // the copies under way land before shared memory goes
+            for (int k = it - 1 - XS < 0 ? 0 : it - 1 - XS; k < it - 1; ++k) mbar_wait_tries(x_full(k % XS), (k / XS) & 1);
+    } else {
+        // ------------------------------------------------------------------------------------------ products
+        if (a.constant) pdl_wait();
+        constexpr uint32_t IDESC = idesc_bf16(128, NT, 0, 0);
+        constexpr int WITHIN = (1 << LG) - 1;
+        int it = 0;
+        uint32_t group = 0;
+        for (int i = 0; i < mine && ok; ++i) {
+            const int st = i & 1;
+            ok = mbar_wait_warp(a_full(st), (i >> 1) & 1, 63);
+            for (int kb = 0; kb < 2 && ok; ++kb, ++it) {
+                const int s = it % XS;
+                ok = mbar_wait_warp(x_full(s), (it / XS) & 1, 64);
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t xs = base + s * CF::XSTAGE;
+#pragma unroll
+                for (int h = 0; h < 2 && ok; ++h) {                   // 32 columns
+                    const int col = kb * 64 + h * 32, d = group & 1;
+                    if ((col & WITHIN) == 0 && group >= 2) {          // a group begins
+                        ok = mbar_wait_warp(d_empty(d), ((group >> 1) + 1) & 1, 66);
+                        tc_fence_after();
+                        if (!ok) break;
+                    }
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+#pragma unroll
+                        for (int t = XT - 1; t >= 0; --t)
+                            mma_bf16_ts_elect(tmem + d * NT, tA + st * 64 + kb * 32 + h * 16 + k * 8, smem_desc(xs + t * CF::XPLANE, 16, 1024) + h * 4 + k * 2, IDESC,
+                                              (col & WITHIN) != 0 || k != 0 || t != XT - 1);
+                    if (((col + 32) & WITHIN) == 0) { mma_commit_elect(d_full(d)); ++group; }
+                }
+                if (ok) mma_commit_elect(x_empty(s));
+            }
+            if (ok) mma_commit_elect(a_empty(st));
+        }
+        if (!ok) {                                                    // products under way end before tensor memory goes
+            mma_commit_elect(drained);
+            mbar_wait_tries(drained, 0);
+        }
+    }
+
+    // ---------------------------------------------------------------------------------------------- sums -> y
+    // A CTA finishes `share` rows of x: every one's sums of them are sent there, into the room of stages that nobody needs any more.
+    const int share = (NT + a.splits - 1) / a.splits;
+    const uint32_t rank = a.splits > 1 ? cluster_rank() : 0u;
+    if (a.splits > 1) cluster_sync_all(); else __syncthreads();
+    if (warp >= IE_DQ && warp < IE_DQ + IE_ACC && ok) {
+        const int mh = ((warp - IE_DQ) >> 2) * COLS;
+        int owner = mh / share, left = (owner + 1) * share - mh;      // of the next column, and how many more are its
+        uint32_t to = cluster_addr(base + ((rank * share + mh - owner * share) * 128 + 32 * sub + lane) * 4, owner);
+#pragma unroll
+        for (int e = 0; e < COLS; ++e) {
+            asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(acc[e]) : "memory");
+            to += 512;
+            if (--left == 0) {
+                left = share;
+                ++owner;
+                if (mh + e + 1 < NT) to = cluster_addr(base + (rank * share * 128 + 32 * sub + lane) * 4, owner);
+            }
+        }
+    }
+    if (a.splits > 1) cluster_sync_all(); else __syncthreads();       // and nobody writes to anyone from here on
+    const float4 *sums = reinterpret_cast<const float4 *>(sm);
+    const bool whole = a.N % 4 == 0;
+    for (int i = tid; i < 32 * share; i += IE_NT) {                   // four rows of W a thread
+        const int n = n0 + 4 * (i & 31), m = (int)rank * share + (i >> 5);
+        if (n >= a.N || m >= NT || m0 + m >= a.M) continue;
+        float4 v = sums[i];
+        for (int r = 1; r < a.splits; ++r) {
+            const float4 w = sums[r * share * 32 + i];
+            v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
+        }
+        float x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (a.bias != nullptr && n + e < a.N)
+                x[e] += XT == 3 ? reinterpret_cast<const float *>(a.bias)[n + e] : __bfloat162float(reinterpret_cast<const __nv_bfloat16 *>(a.bias)[n + e]);
+            x[e] = int4_act(x[e], a.act);
+        }
+        const size_t at = (size_t)(m0 + m) * a.N + n;
+        if (a.out_bf16) {
+            __nv_bfloat16 *y = reinterpret_cast<__nv_bfloat16 *>(a.y) + at;
+            if (whole) {
+                uint2 out;
+                reinterpret_cast<__nv_bfloat162 *>(&out)[0] = __floats2bfloat162_rn(x[0], x[1]);
+                reinterpret_cast<__nv_bfloat162 *>(&out)[1] = __floats2bfloat162_rn(x[2], x[3]);
+                *reinterpret_cast<uint2 *>(y) = out;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (n + e < a.N) y[e] = __float2bfloat16_rn(x[e]);
+            }
+        } else {
+            float *y = reinterpret_cast<float *>(a.y) + at;
+            if (whole) *reinterpret_cast<float4 *>(y) = make_float4(x[0], x[1], x[2], x[3]);
+            else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (n + e < a.N) y[e] = x[e];
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 13) tmem_dealloc(tmem, 256);
+}
+
+// x as three bf16 terms, [3][n]: eight bits each, cut off, so that they add up to x; an infinity or NaN is the first one's. Eight values a thread.
+__global__ void __launch_bounds__(256) int4_terms_kernel(const float *__restrict__ x, __nv_bfloat16 *__restrict__ out, long long n) {
+    pdl_wait();
+    pdl_launch_dependents();
+    const long long i = 8 * ((long long)blockIdx.x * 256 + threadIdx.x);
+    if (i >= n) return;
+    uint32_t v[8], t[3][4];
+    *reinterpret_cast<uint4 *>(v) = *reinterpret_cast<const uint4 *>(x + i);
+    *reinterpret_cast<uint4 *>(v + 4) = *reinterpret_cast<const uint4 *>(x + i + 4);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        uint32_t u[2][3];
+#pragma unroll
+        for (int p = 0; p < 2; ++p) fp32_terms(v[2 * e + p], u[p]);
+#pragma unroll
+        for (int q = 0; q < 3; ++q) t[q][e] = __byte_perm(u[0][q], u[1][q], 0x7632);
+    }
+#pragma unroll
+    for (int q = 0; q < 3; ++q) *reinterpret_cast<uint4 *>(out + q * n + i) = make_uint4(t[q][0], t[q][1], t[q][2], t[q][3]);
+}
+
+// ------------------------------------------------------------------------------------------------ host
+template <int NT, int XT, int LG, bool S32>
+static cudaError_t exact_go(const void *x, const ExactArgs &a, cudaStream_t stream) {
+    CUtensorMap mx;
+    if (!tc_make_map(&mx, x, XT, a.M, a.K, a.K, a.M * a.K, NT)) return cudaErrorUnknown;
+    cudaError_t e = cudaFuncSetAttribute(int4_exact_kernel<NT, XT, LG, S32>, cudaFuncAttributeMaxDynamicSharedMemorySize, IeCfg<NT, XT>::SMEM);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((a.N + 127) / 128), (unsigned)((a.M + NT - 1) / NT), (unsigned)a.splits);
+    cfg.blockDim = dim3(IE_NT); cfg.dynamicSmemBytes = IeCfg<NT, XT>::SMEM; cfg.stream = stream;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = 1; at[1].val.clusterDim.y = 1; at[1].val.clusterDim.z = (unsigned)a.splits;
+    cfg.attrs = at; cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, int4_exact_kernel<NT, XT, LG, S32>, mx, a);
+}
+template <int NT, int XT>
+static cudaError_t exact_group(const Int4Linear &l, const void *x, const ExactArgs &a, cudaStream_t stream) {
+    const bool s32 = l.w.scale_dtype == PGB_F32;
+    if (l.w.group == 32) return s32 ? exact_go<NT, XT, 5, true>(x, a, stream) : exact_go<NT, XT, 5, false>(x, a, stream);
+    if (l.w.group == 64) return s32 ? exact_go<NT, XT, 6, true>(x, a, stream) : exact_go<NT, XT, 6, false>(x, a, stream);
+    return s32 ? exact_go<NT, XT, 7, true>(x, a, stream) : exact_go<NT, XT, 7, false>(x, a, stream);
+}
+
+// More rows than the kernel for few takes at a time (8 of fp32, 16 of bf16), and work enough for what this one's start costs: 2^24 weights times eights of rows. us here / there,
+// groups of 64, fp32: 9 rows, N 2328 K 768 6.5 / 4.0, N 2048 K 8192 16.8 / 17.3, N 50257 K 768 21.7 / 31.9; 64 rows, N 2328 K 768 7.7 / 7.0; 227, N 9636 K 64 13.1 / 25.4; 680, N 6 K 14432
+// 33.8 / 24.4; 2000, N 2048 K 1024 38.7 / 173. bf16 rows, fp32 out: 17, N 768 K 768 4.9 / 3.1; 256, N 768 K 768 5.9 / 9.1; 25, N 1929 K 14048 19.9 / 24.1; 64, N 8192 K 2048 12.1 / 27.0.
+bool int4_exact_tiles(const Int4Linear &l) {
+    if (l.x_dtype == PGB_BF16 && (l.out_dtype == PGB_BF16 || l.M <= PGB_INT4_ROWS)) return false;
+    return l.M > 8 && (l.M + 7) / 8 * l.w.N * l.w.K >= 1LL << 24;
+}
+
+// l.scratch: room for x's terms where it is fp32. A grid's second axis ends at 65535, so very many rows go in several launches.
+int int4_exact_launch(const Int4Linear &l, cudaStream_t stream) {
+    const Int4Weight &w = l.w;
+    const bool x32 = l.x_dtype == PGB_F32;
+    const int es = w.scale_dtype == PGB_F32 ? 4 : 2, NT = l.M <= 32 ? 32 : 64, C = (w.K + 127) / 128;
+    const long long tiles = (long long)((w.N + 127) / 128) * ((l.M + NT - 1) / NT);
+    int splits = 1;
+    while (splits < IE_SPLITS && tiles * splits <= sm_count() && C >= 2 * splits) splits *= 2;
+    const int each = (C + splits - 1) / splits;
+    ExactArgs a{w.q, w.scales, w.zeros, l.bias, l.y, l.M, l.act, l.out_dtype == PGB_BF16, w.N, w.K, w.G, 0, each, (C + each - 1) / each, l.constant};
+    a.wide = w.G % 4 == 0 && aligned(w.scales, 4 * es) && (w.zeros == nullptr || aligned(w.zeros, 4));
+    cudaError_t e = cudaSuccess;
+    for (long long m = 0; m < l.M && e == cudaSuccess; m += 65535LL * NT) {
+        a.M = l.M - m < 65535LL * NT ? l.M - m : 65535LL * NT;
+        a.y = (uint8_t *)l.y + (size_t)m * w.N * (a.out_bf16 ? 2 : 4);
+        const void *x = (const uint8_t *)l.x + (size_t)m * w.K * (x32 ? 4 : 2);
+        if (x32) {
+            const long long n = a.M * w.K;
+            e = pdl_launch(int4_terms_kernel, dim3((unsigned)((n + 2047) / 2048)), dim3(256), 0, stream, (const float *)x, (__nv_bfloat16 *)l.scratch, n);
+            if (e != cudaSuccess) break;
+            x = l.scratch;
+        }
+        if (NT == 32) e = x32 ? exact_group<32, 3>(l, x, a, stream) : exact_group<32, 1>(l, x, a, stream);
+        else e = x32 ? exact_group<64, 3>(l, x, a, stream) : exact_group<64, 1>(l, x, a, stream);
+    }
+    if (e != cudaSuccess) { set_cuda_error(e, "int4_exact launch"); return PGB_ERR_CUDA; }
+    return check_launch("int4_exact_kernel");
+}
+
+int int4_exact_error_flag(int *out) { return tc_read_error_flag(out); }
+
+}  // namespace pgb

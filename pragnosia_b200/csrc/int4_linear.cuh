@@ -32,6 +32,51 @@ __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
     return d;
 }
 
-int int4_tile_launch(const Int4Linear &a, cudaStream_t stream);
+
+// the scales (bf16 ones two a register) and zeros of the four groups that a row's stretch of 128 columns lies in; those behind the last one 0
+template <int LG, bool S32, class Args>
+__device__ __forceinline__ void it_groups(const Args &a, int row, int stretch, bool live, uint32_t (&s)[S32 ? 4 : 2], uint32_t &z) {
+    const int g0 = ((stretch * 128) >> LG) & ~3;
+    z = 0x08080808u;
+#pragma unroll
+    for (int e = 0; e < (S32 ? 4 : 2); ++e) s[e] = 0u;
+    if (row >= a.N || !live) return;
+    const size_t at = (size_t)row * a.G + g0;
+    if (a.wide) {
+        if constexpr (S32) {
+            const uint4 v = __ldg(reinterpret_cast<const uint4 *>(reinterpret_cast<const float *>(a.scales) + at));
+            s[0] = v.x; s[1] = v.y; s[2] = v.z; s[3] = v.w;
+        } else {
+            const uint2 v = __ldg(reinterpret_cast<const uint2 *>(reinterpret_cast<const __nv_bfloat16 *>(a.scales) + at));
+            s[0] = v.x; s[1] = v.y;
+        }
+        if (a.zeros != nullptr) z = __ldg(reinterpret_cast<const uint32_t *>(a.zeros + at));
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (g0 + e < a.G) {
+            if constexpr (S32) s[e] = __ldg(reinterpret_cast<const uint32_t *>(a.scales) + at + e);
+            else s[e >> 1] |= (uint32_t)__ldg(reinterpret_cast<const unsigned short *>(a.scales) + at + e) << (16 * (e & 1));
+            if (a.zeros != nullptr) z = (z & ~(255u << (8 * e))) | (uint32_t)__ldg(a.zeros + at + e) << (8 * e);
+        }
+}
+// the first of those four groups that a stretch has
+template <int LG> __device__ __forceinline__ int it_first(int stretch) { return LG == 7 ? stretch & 3 : LG == 6 ? (stretch & 1) * 2 : 0; }
+__device__ __forceinline__ float int4_act(float v, int act) { return act == 1 ? 0.5f * v * (1.0f + erff(v * 0.70710678118654752f)) : v; }
+
+// fp32 as three bf16 terms in the upper halves: eight bits each, cut off, so that they add up to it (but for what lies below 2^-133, bf16's
+// least). An infinity or NaN is the first one's.
+__device__ __forceinline__ void fp32_terms(uint32_t bits, uint32_t (&u)[3]) {
+    const bool fin = (bits & 0x7f800000u) != 0x7f800000u;
+    const float r1 = fin ? __uint_as_float(bits) - __uint_as_float(bits & 0xffff0000u) : 0.f, r2 = r1 - __uint_as_float(__float_as_uint(r1) & 0xffff0000u);
+    u[0] = fin || (bits & 0x007fffffu) == 0u ? bits : 0x7fc00000u;
+    u[1] = __float_as_uint(r1); u[2] = __float_as_uint(r2);
+}
+
+// the kernels for many rows (int4_tile.cu, int4_exact.cu)
+int int4_tile_launch(const Int4Linear &l, cudaStream_t stream);
+bool int4_exact_tiles(const Int4Linear &l);                           // whether a call with fp32 in or out takes int4_exact_launch
+int int4_exact_launch(const Int4Linear &l, cudaStream_t stream);
 
 }  // namespace pgb

@@ -32,35 +32,7 @@ struct ItCfg {
     static_assert(2 * (SMEM + 1024) <= 227 * 1024 && SMEM > 76 * 1024, "two CTAs an SM, and no third, whose tensor memory would not be there");
 };
 
-// the scales (bf16 ones two a register) and zeros of the four groups that a row's stretch lies in; those behind the last one 0
-template <int LG, bool S32>
-__device__ __forceinline__ void it_groups(const TileArgs &a, int row, int stretch, bool live, uint32_t (&s)[S32 ? 4 : 2], uint32_t &z) {
-    const int g0 = ((stretch * 128) >> LG) & ~3;
-    z = 0x08080808u;
-#pragma unroll
-    for (int e = 0; e < (S32 ? 4 : 2); ++e) s[e] = 0u;
-    if (row >= a.N || !live) return;
-    const size_t at = (size_t)row * a.G + g0;
-    if (a.wide) {
-        if constexpr (S32) {
-            const uint4 v = __ldg(reinterpret_cast<const uint4 *>(reinterpret_cast<const float *>(a.scales) + at));
-            s[0] = v.x; s[1] = v.y; s[2] = v.z; s[3] = v.w;
-        } else {
-            const uint2 v = __ldg(reinterpret_cast<const uint2 *>(reinterpret_cast<const __nv_bfloat16 *>(a.scales) + at));
-            s[0] = v.x; s[1] = v.y;
-        }
-        if (a.zeros != nullptr) z = __ldg(reinterpret_cast<const uint32_t *>(a.zeros + at));
-        return;
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-        if (g0 + e < a.G) {
-            if constexpr (S32) s[e] = __ldg(reinterpret_cast<const uint32_t *>(a.scales) + at + e);
-            else s[e >> 1] |= (uint32_t)__ldg(reinterpret_cast<const unsigned short *>(a.scales) + at + e) << (16 * (e & 1));
-            if (a.zeros != nullptr) z = (z & ~(255u << (8 * e))) | (uint32_t)__ldg(a.zeros + at + e) << (8 * e);
-        }
-}
-// 32 levels of group e of those four as bf16 pairs in their order: scale (q - z), rounded once
+// 32 levels of group e of four (it_groups) as bf16 pairs in their order: scale (q - z), rounded once
 template <bool S32>
 __device__ __forceinline__ void it_values(const uint4 &levels, const uint32_t (&s)[S32 ? 4 : 2], uint32_t z, int e, uint32_t (&out)[16]) {
     const uint32_t z2 = __byte_perm(z, 0x43u, 0x4040 | e | e << 8);
@@ -86,8 +58,6 @@ __device__ __forceinline__ void it_values(const uint4 &levels, const uint32_t (&
         out[4 * v + 2] = __byte_perm(p[0], p[1], 0x7632); out[4 * v + 3] = __byte_perm(p[2], p[3], 0x7632);
     }
 }
-// the first of those four groups that a stretch has
-template <int LG> __device__ __forceinline__ int it_first(int stretch) { return LG == 7 ? stretch & 3 : LG == 6 ? (stretch & 1) * 2 : 0; }
 // 16 columns of D (rows m, m + 1, .. of x, `left` of them there) of this lane's row n of W: + bias, the activation, rounded and stored; a row's 32 lanes are 64 bytes
 __device__ __forceinline__ void it_store16(const TileArgs &a, const float (&v)[16], float bias, long long m, long long left, int n) {
     __nv_bfloat16 *row = a.y + (size_t)m * a.N;                       // uniform

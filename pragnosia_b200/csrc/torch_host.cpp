@@ -718,8 +718,10 @@ Tensor int4_linear_fwd(const Tensor &x_, const Tensor &q, const Tensor &s, const
     shape.back() = w.N;
     const Tensor y = result(x, shape, bf16 ? at::kBFloat16 : at::kFloat);
     const int64_t M = x.numel() / w.K;
+    const int64_t room = M > 0 ? pgb_int4_linear_scratch_bytes(code(x), code(y), M, w.N, w.K) : 0;
+    const Tensor scratch = room > 0 ? result(x, {room}, at::kByte) : Tensor();
     if (M > 0)
-        check(pgb_int4_linear(vp(x), code(x), u8(w.q), vp(w.s), code(w.s), u8(w.z), vp(b), act, vp(y), code(y), M, w.N, w.K, group, constant ? PGB_INT4_CONSTANT : 0,
+        check(pgb_int4_linear(vp(x), code(x), u8(w.q), vp(w.s), code(w.s), u8(w.z), vp(b), act, vp(y), code(y), vp(scratch), room, M, w.N, w.K, group, constant ? PGB_INT4_CONSTANT : 0,
                               dev.stream), "pgb_int4_linear");
     return y;
 }

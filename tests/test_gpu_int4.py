@@ -177,6 +177,65 @@ def test_linear_of_many_tiles(M, K, N, scale_dtype):
     assert torch.equal(y, int4.linear(x, w, bias, act=act))
 
 
+EXACT = [(9, 2048, 4100), (17, 96, 60001), (20, 14048, 410), (33, 1024, 5000), (200, 416, 2003), (2000, 32, 4099), (129, 160, 8190), (64, 768, 50257), (1000, 4096, 130), (4100, 704, 704)]
+
+
+@pytest.mark.parametrize("M,K,N", EXACT)
+@pytest.mark.parametrize("x_dtype,scale_dtype,out", [(BF, BF, F32), (F32, BF, F32), (F32, F32, F32), (BF, F32, F32), (F32, BF, BF)])
+def test_linear_in_full_precision(M, K, N, x_dtype, scale_dtype, out):
+    """Many rows, x or the result in float32: no weight is rounded. From one share of K to eight, ends that fill no tile."""
+    i = EXACT.index((M, K, N))
+    w = random_weight(N, K, (64, 32, 128)[(i + (scale_dtype == F32)) % 3], i % 2 == 0, scale_dtype, i)
+    g = torch.Generator(device="cuda").manual_seed(300 + i)
+    x = torch.randn(M, K, device="cuda", generator=g).to(x_dtype)
+    bias = torch.randn(N, device="cuda", generator=g).to(x_dtype) if i % 3 != 1 else None
+    act = "gelu" if i % 2 else None
+    y = int4.linear(x, w, bias, act=act, out_dtype=out)
+    check_linear(x, w, bias, act, out, y)
+    assert torch.equal(y, int4.linear(x, w, bias, act=act, out_dtype=out))
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("zeros", [True, False])
+@pytest.mark.parametrize("dtype", [F32, BF])
+def test_linear_groups_in_full_precision(group, zeros, dtype):
+    K, N, M = 416, 1000, 2000
+    w = random_weight(N, K, group, zeros, dtype, 3)
+    rows = torch.arange(M, device="cuda")
+    cols, f = rows * 7 % K, (1.0 + rows * 2.0 ** -13)                 # in float32 twelve bits and more, which only the sum of a value's terms has
+    for x_dtype in (F32, BF):
+        x = torch.zeros(M, K, device="cuda", dtype=x_dtype)
+        x[rows, cols] = f.to(x_dtype)
+        want = value(w).t()[cols] * x[rows, cols].double()[:, None]
+        y = int4.linear(x, w, out_dtype=F32).double()
+        assert torch.all((y - want).abs() <= 2.0 ** -23 * want.abs())     # the product of x and the whole number, and that by the scale, are rounded
+
+
+def test_full_precision_carries_what_is_no_number():
+    M, K, N = 100, 704, 3000
+    w = random_weight(N, K, 64, False, BF, 5)
+    x = torch.randn(M, K, device="cuda")
+    x[3, 7], x[50, 700], x[99, 0] = math.inf, math.nan, -math.inf
+    x[7] *= 1e-30
+    w.scales[5, 2] = math.nan
+    q = w.q.clone()
+    q[:, 3] |= 0x90                                                   # no weight of column 7 is 0
+    w = w._replace(q=q)
+    y, v = int4.linear(x, w), value(w)
+    bad = torch.zeros(M, N, dtype=torch.bool, device="cuda")
+    bad[50], bad[:, 5] = True, True
+    bad[99] |= v[:, 0] == 0
+    want = x.double() @ v.t()
+    assert torch.equal(y.isnan(), bad)
+    inf = torch.zeros_like(bad)
+    inf[3] = inf[99] = True
+    inf &= ~bad
+    assert torch.equal(y.isinf(), inf) and torch.equal(y[inf].double(), want[inf])
+    rest = ~(bad | inf)
+    A = x.double().abs().nan_to_num(0, 0, 0) @ v.abs().nan_to_num(0).t()
+    assert torch.all((y.double() - want).abs()[rest] <= (2 * U * (K + 2 * 11 + 4) * A + 2.0 ** -22 * A)[rest])
+
+
 @pytest.mark.parametrize("group", [32, 64, 128])
 @pytest.mark.parametrize("zeros", [True, False])
 def test_linear_groups_of_many_tiles(group, zeros):
@@ -258,10 +317,11 @@ def test_linear_refusals():
 
 
 @pytest.mark.parametrize("M", [1, 12, 40, 300, 10000])
-def test_linear_in_a_graph_and_on_another_stream(M):
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_linear_in_a_graph_and_on_another_stream(M, dtype):
     K, N = 768, 776
     w = random_weight(N, K, 64, True, BF, 8)
-    x = torch.randn(M, K, device="cuda").to(BF)
+    x = torch.randn(M, K, device="cuda").to(dtype)
     want = int4.linear(x, w)
     side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
     held = torch.zeros_like(x)

@@ -24,8 +24,8 @@ def dequantize(q=one, s=one, sd=1, z=one, w=one, dtype=1, N=4, K=64, group=64):
     return lib().pgb_int4_dequantize(q, s, sd, z, w, dtype, N, K, group, None)
 
 
-def linear(x=one, xd=1, q=one, s=one, sd=1, z=None, b=None, act=0, y=one, od=1, M=1, N=4, K=64, group=64, flags=0):
-    return lib().pgb_int4_linear(x, xd, q, s, sd, z, b, act, y, od, M, N, K, group, flags, None)
+def linear(x=one, xd=1, q=one, s=one, sd=1, z=None, b=None, act=0, y=one, od=1, sc=None, n=0, M=1, N=4, K=64, group=64, flags=0):
+    return lib().pgb_int4_linear(x, xd, q, s, sd, z, b, act, y, od, sc, n, M, N, K, group, flags, None)
 
 
 def adjust(l=one, dtype=0, stride=10, out=at(0x9000), p=None, ps=0, pn=0, pl=None, pls=0, g=None, gs=0, gn=0, gl=None, gls=0, rt=None, r=1.0, ft=None, pt=None,
@@ -44,6 +44,7 @@ SIZES = [(dict(N=0), SHAPE), (dict(K=0), SHAPE), (dict(K=40), SHAPE), (dict(K=16
     *[(dequantize, {n: None}, NULL) for n in ("w", "q", "s")], (dequantize, dict(dtype=2), DTYPE), (dequantize, dict(sd=-1), DTYPE), (dequantize, dict(w=off8), ALIGN),
     *[(linear, {n: None}, NULL) for n in ("x", "q", "s", "y")], (linear, dict(xd=2), DTYPE), (linear, dict(sd=2), DTYPE), (linear, dict(od=2), DTYPE),
     (linear, dict(M=0), SHAPE), (linear, dict(M=1 << 31), LARGE), (linear, dict(act=2), SHAPE), (linear, dict(act=-1), SHAPE), (linear, dict(flags=2), SHAPE),
+    *[(linear, dict(xd=0, M=64, N=4096, K=768, **kw), code) for kw, code in ((dict(), NULL), (dict(sc=one, n=6 * 64 * 768 - 1), SHAPE), (dict(sc=off8, n=1 << 20), ALIGN))],
     (linear, dict(x=off8), ALIGN), (linear, dict(q=off8), ALIGN), (linear, dict(y=off8), ALIGN), (linear, dict(b=off1), ALIGN), (linear, dict(b=off2, xd=0), ALIGN),
     (adjust, dict(l=None), NULL), (adjust, dict(out=None), NULL), (adjust, dict(pn=3), NULL), (adjust, dict(gn=3), NULL), (adjust, dict(nb=3), NULL),
     (adjust, dict(nb=3, bi=one), NULL), (adjust, dict(kind=1), NULL), (adjust, dict(dtype=3), DTYPE), (adjust, dict(B=0), SHAPE), (adjust, dict(V=0), SHAPE),
@@ -54,6 +55,13 @@ SIZES = [(dict(N=0), SHAPE), (dict(K=0), SHAPE), (dict(K=40), SHAPE), (dict(K=16
     (adjust, dict(bi=off4, bv=one, nb=1), ALIGN), (adjust, dict(mask=off2, kind=1), ALIGN), (adjust, dict(out=one, dtype=1), SHAPE), (adjust, dict(out=one, stride=12), SHAPE)])
 def test_bad_calls(call, kw, code):
     assert call(**kw) == code
+
+
+def test_scratch_of_the_linear_layer():
+    n = lib().pgb_int4_linear_scratch_bytes
+    assert n(0, 0, 64, 4096, 768) == n(0, 1, 64, 4096, 768) == 6 * 64 * 768 and n(0, 0, 1 << 20, 64, 4096) == 6 << 32
+    assert n(0, 0, 64, 1024, 768) == n(0, 0, 8, 1 << 20, 768) == n(1, 0, 64, 4096, 768) == n(1, 1, 64, 4096, 768) == 0     # few, or bf16
+    assert n(0, 0, 0, 4096, 768) == n(0, 0, 1 << 31, 4096, 768) == n(0, 0, 64, 0, 768) == n(0, 0, 64, 4096, 100) == 0
 
 
 def held(N=5, K=96, group=64, zeros=True, **kw):
