@@ -548,17 +548,21 @@ int int4_tile_launch(const Int4Linear &l, cudaStream_t stream) {
     const int es = w.scale_dtype == PGB_F32 ? 4 : 2;
     TileArgs a{w.q, w.scales, w.zeros, (const __nv_bfloat16 *)l.bias, (__nv_bfloat16 *)l.y, l.M, l.act, w.N, w.K, w.G, 0, 0, 0, 1, l.constant};
     a.wide = w.G % 4 == 0 && aligned(w.scales, 4 * es) && (w.zeros == nullptr || aligned(w.zeros, 4));
-    const int NT = l.M <= 32 ? 32 : l.M <= 64 ? 64 : 128, C = (w.K + 127) / 128;
-    const long long tiles = (long long)((w.N + 127) / 128) * ((l.M + NT - 1) / NT);
+    // Rows of x a tile, with its shares of K below: 128 once those tiles are more than half the SMs; where even tiles of 64 in eight shares leave SMs idle, 32 (us, 32 / 64 / 128:
+    // 128 rows, N 768 K 768 4.7 / 5.5 / 7.4; 452, N 1 K 15424 13 / 14 / 74; 64, N 2048 K 8192 12.0 / 13.6 / -; 256, N 2048 K 2048 11.2 / 9.1 / 13.7; 349, N 2785 K 14784 133 / 106 / 131;
+    // 128, N 8192 K 2048 16.6 / 12.9 / 14.0; 1000, N 2048 K 2048 31 / 17.4 / 14.2).
+    const long long sms = sm_count(), tiles_n = (w.N + 127) / 128, halves = (l.M + 127) / 128, by64 = tiles_n * ((l.M + 63) / 64);
+    const int NT = l.M <= 32 || 7 * by64 <= sms ? 32 : l.M <= 64 || 2 * tiles_n * halves <= sms ? 64 : 128, C = (w.K + 127) / 128;
+    const long long tiles = tiles_n * ((l.M + NT - 1) / NT);
     // Shares of K while CTAs are no more than the SMs hold, and a share a stretch (us, 64 rows of x, 1 / 2 / 4 / 8: N 8192 K 2048 12.8 / 10.4 / 10.0 / 16.7, N 2048 K 8192 38 / 22 / 14 / 13.5,
     // N 2328 K 768 6.4 / 6.2 / 5.5 / 5.5, N 50257 K 768 16 / 27 / 37 / 69).
     int splits = 1;
-    while (NT < 128 && splits < IT_SPLITS && tiles * splits <= sm_count() && C >= 2 * splits) splits *= 2;
+    while (NT < 128 && splits < IT_SPLITS && tiles * splits <= sms && C >= 2 * splits) splits *= 2;
     // The larger tiles from one and a half rounds over the chip on, where x fills them well: one of 256 rows takes 1.6 times as long as one of 128 (us, theirs / the smaller ones':
     // 4096 rows, N 2048 K 8192 113 / 136, N 2328 K 768 24 / 27, N 50257 K 768 323 / 431; 256 rows, N 32768 K 4096 64 / 72, 384 115 / 107, 128 59 / 39;
     // a round: 2048 rows, N 2048 K 2048 19.4 / 19.2, N 2328 K 768 23.8 / 20.5; half a one: 512 rows, N 4096 K 4096 31 / 23).
-    const long long halves = (l.M + 127) / 128, wide_rows = (l.M + 255) / 256;
-    if (8 * wide_rows < 5 * halves && (long long)((w.N + 127) / 128) * wide_rows * 2 >= 3LL * sm_count()) {
+    const long long wide_rows = (l.M + 255) / 256;
+    if (8 * wide_rows < 5 * halves && tiles_n * wide_rows * 2 >= 3 * sms) {
         const cudaError_t e = wide_group(l, a, stream);
         if (e != cudaSuccess) { set_cuda_error(e, "int4_wide launch"); return PGB_ERR_CUDA; }
         return check_launch("int4_wide_kernel");
