@@ -26,12 +26,14 @@ __device__ __forceinline__ int list_length(const TokenList &t, long long b) {
 template <typename T_, int NT, int QT, int PER_SM>
 __global__ void __launch_bounds__(NT, PER_SM) adjust_logits_kernel(const AdjustLogits a, const int slices) {
     constexpr int S = 4 * NT * QT, HEAD = 2;
-    constexpr uint32_t IN_PROMPT = 0x80000000u;
+    constexpr uint32_t IN_PROMPT = 0x80000000u, NONE = 0xffffffffu;
     extern __shared__ uint4 adj_smem[];
     uint32_t *count = reinterpret_cast<uint32_t *>(adj_smem);         // [S]
-    float *sbias = reinterpret_cast<float *>(count + S);              // [S] with biases
-    int *bid = reinterpret_cast<int *>(count + 2 * S);                // [nb]: place in the slice, -1 outside
-    float *bval = reinterpret_cast<float *>(bid + a.nb);
+    uint32_t *first = count + S;                                      // [S] with biases: the first entry that names the word, NONE
+    const int nb4 = (a.nb + 3) & ~3;
+    int *bid = reinterpret_cast<int *>(count + 2 * S);                // [nb4]: place in the slice, -1 outside
+    int *again = bid + nb4;                                           // [nb]: whether later entries name the word as well
+    float *bval = reinterpret_cast<float *>(again + nb4);            // [nb]: the value; then, at a word's first entry, the sum
     const int tid = threadIdx.x, lane = tid & 31;
     const unsigned b = blockIdx.x / (unsigned)slices;
     pdl_wait();
@@ -86,12 +88,13 @@ __global__ void __launch_bounds__(NT, PER_SM) adjust_logits_kernel(const AdjustL
 #pragma unroll
     for (int q = 0; q < QT; ++q) {
         reinterpret_cast<uint4 *>(count)[tid + q * NT] = make_uint4(0u, 0u, 0u, 0u);
-        if (a.nb > 0) reinterpret_cast<uint4 *>(sbias)[tid + q * NT] = make_uint4(0u, 0u, 0u, 0u);
+        if (a.nb > 0) reinterpret_cast<uint4 *>(first)[tid + q * NT] = make_uint4(NONE, NONE, NONE, NONE);
     }
-    for (int j = tid; j < a.nb; j += NT) {
-        const uint32_t at = place(a.bias_ids[b * a.bias_stride + j]);
+    for (int j = tid; j < nb4; j += NT) {
+        const uint32_t at = j < a.nb ? place(a.bias_ids[b * a.bias_stride + j]) : NONE;
         bid[j] = at < S ? (int)at : -1;
-        bval[j] = a.bias[b * a.bias_stride + j];
+        again[j] = 0;
+        if (j < a.nb) bval[j] = a.bias[b * a.bias_stride + j];
     }
     __syncthreads();
     auto prompt_id = [&](long long id) {
@@ -111,24 +114,28 @@ __global__ void __launch_bounds__(NT, PER_SM) adjust_logits_kernel(const AdjustL
     for (int j = tid + HEAD * NT; j < np; j += NT) prompt_id(pid[j]);
 #pragma unroll 8
     for (int j = tid + HEAD * NT; j < ng; j += NT) made_id(gid[j]);
-    // A warp an entry: the first one that names a word adds up all that do, in their order.
-    for (int j = tid >> 5; j < a.nb; j += NT / 32) {
-        const int at = bid[j];
-        if (at < 0) continue;
-        float s = 0.f;
-        bool begun = false, mine = true;
-        for (int c = 0; c < a.nb && mine; c += 32) {
-            uint32_t same = __ballot_sync(0xffffffffu, c + lane < a.nb && bid[c + lane] == at);
-            if (!begun && same != 0u) {
-                begun = true;
-                mine = c + __ffs(same) - 1 == j;
+    // A thread an entry: the first one that names a word adds up all that do, in their order (it looks for them only where there are any).
+    for (int j = tid; j < a.nb; j += NT)
+        if (bid[j] >= 0) atomicMin(&first[bid[j]], (uint32_t)j);
+    if (a.nb > 0) {
+        __syncthreads();
+        for (int j = tid; j < a.nb; j += NT)
+            if (bid[j] >= 0 && first[bid[j]] != (uint32_t)j) again[first[bid[j]]] = 1;
+        __syncthreads();
+        for (int j = tid; j < a.nb; j += NT)
+            if (again[j]) {
+                const int at = bid[j];
+                float s = bval[j];
+#pragma unroll 4
+                for (int c = j & ~3; c < nb4; c += 4) {
+                    const int4 v = *reinterpret_cast<const int4 *>(bid + c);
+                    if (v.x == at && c > j) s = __fadd_rn(s, bval[c]);
+                    if (v.y == at && c + 1 > j) s = __fadd_rn(s, bval[c + 1]);
+                    if (v.z == at && c + 2 > j) s = __fadd_rn(s, bval[c + 2]);
+                    if (v.w == at && c + 3 > j) s = __fadd_rn(s, bval[c + 3]);
+                }
+                bval[j] = s;                                          // read by nobody else: entry j is the first of its word
             }
-            for (; same != 0u && mine; same &= same - 1u) {
-                const float v = bval[c + __ffs(same) - 1];
-                s = c + __ffs(same) - 1 == j ? v : __fadd_rn(s, v);
-            }
-        }
-        if (mine && lane == 0) sbias[at] = s;
     }
     __syncthreads();
 
@@ -152,8 +159,11 @@ __global__ void __launch_bounds__(NT, PER_SM) adjust_logits_kernel(const AdjustL
             for (int i = 0; i < 4; ++i) s[i] = e == i ? x : s[i];
         }
         if (a.nb > 0) {
-            const float4 add = reinterpret_cast<const float4 *>(sbias)[at];
-            s[0] = __fadd_rn(s[0], add.x); s[1] = __fadd_rn(s[1], add.y); s[2] = __fadd_rn(s[2], add.z); s[3] = __fadd_rn(s[3], add.w);
+            const uint4 f4 = reinterpret_cast<const uint4 *>(first)[at];
+            const uint32_t from[4] = {f4.x, f4.y, f4.z, f4.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (from[e] != NONE) s[e] = __fadd_rn(s[e], bval[from[e]]);
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e)
@@ -171,7 +181,7 @@ template <typename T_, int NT, int QT, int PER_SM>
 static cudaError_t adjust_go(const AdjustLogits &a, cudaStream_t stream) {
     constexpr int S = 4 * NT * QT;
     const int slices = (int)(((long long)a.V + 3 + S - 1) / S);       // a row's first slice may begin up to three words ahead of it
-    const size_t smem = (size_t)S * 4 * (a.nb > 0 ? 2 : 1) + (size_t)a.nb * 8;
+    const size_t smem = (size_t)S * 4 * (a.nb > 0 ? 2 : 1) + (size_t)((a.nb + 3) & ~3) * 12;
     return pdl_launch(adjust_logits_kernel<T_, NT, QT, PER_SM>, dim3((unsigned)(a.B * slices)), dim3(NT), smem, stream, a, slices);
 }
 template <typename T_>
