@@ -541,10 +541,11 @@ static cudaError_t rows_blocks(RowsArgs a, cudaStream_t stream) {
     const long long tiles = (a.M + 8 * NB - 1) / (8 * NB), sms = a.sms;
     const long long by64 = (a.N + 63) / 64 * tiles, by32 = (a.N + 31) / 32 * tiles, by16 = (a.N + 15) / 16 * tiles;
     // few columns and very many rows of W, whose CTAs are short: N 50257 K 768 16 / 2 13.3, 32 / 2 13.6, 32 / 4 14.3
-    const int MT = a.M > 4 && NB == 1 && by64 * 10 >= 17 * sms ? 4 : by32 * 10 < 7 * sms || (a.M <= 4 && a.K <= 1024 && by16 >= 10 * sms) ? 1 : 2;
+    // fp32 rows cost more to take apart than levels: many rows of W a CTA (4 rows, N 50257 K 768 64 / 4 18.9, 16 / 2 26.1; 3 rows, N 10490 K 4960 32 / 8 29, 32 / 4 37)
+    const int MT = (X32 || a.M > 4) && NB == 1 && by64 * 10 >= 17 * sms ? 4 : by32 * 10 < 7 * sms || (!X32 && a.M <= 4 && a.K <= 1024 && by16 >= 10 * sms) ? 1 : 2;
     const long long ctas = MT == 4 ? by64 : MT == 2 ? by32 : by16;
-    // 16 rows of x at a time: 8 warps, 4 where those would have a stretch each and CTAs abound (64 rows in fp32, N 50257 K 768: 99 -> 63)
-    a.warps = NB > 1 ? (ctas > 4 * sms && a.K < 2048 ? 4 : 8) : ctas * 8 <= 17 * sms ? 8 : ctas * 4 <= 17 * sms ? 4 : 2;
+    // 16 rows of x at a time: 8 warps, 4 where those would have a stretch each and CTAs abound (16 rows, N 50257 K 768: 32 -> 23.6)
+    a.warps = NB > 1 ? (ctas > 4 * sms && a.K < 2048 ? 4 : 8) : X32 ? (MT == 4 && ctas * 8 > 17 * sms ? 4 : 8) : ctas * 8 <= 17 * sms ? 8 : ctas * 4 <= 17 * sms ? 4 : 2;
     if (MT == 4) return rows_go<4, NB, X32, S32>(a, stream);
     if (MT == 2) return rows_go<2, NB, X32, S32>(a, stream);
     return rows_go<1, NB, X32, S32>(a, stream);
