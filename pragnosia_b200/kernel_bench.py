@@ -1,9 +1,9 @@
 """Each hand-written kernel alone on a fixed synthetic case: what bench.py times for its roofline entries and what the
 ncu captures summarised under profiles/ run.
 
-    python -m pragnosia_b200.kernel_bench NAME [--launches N] [--time]
+    python -m pragnosia_b200.kernel_bench NAME.. [--launches N] [--time]
 
-NAME is one of CASES. Without --time it just launches the kernel N times (the form to put under ncu); with --time it
+NAME is one of CASES (or several, one after the other). Without --time it just launches the kernel N times (the form to put under ncu); with --time it
 prints the CUDA-event time per launch (L2 flushed before each) and the achieved algorithmic GB/s.
 """
 from __future__ import annotations
@@ -13,7 +13,7 @@ import sys
 
 import torch
 
-from . import _lib, ops, synth
+from . import _lib, int4, ops, sampling, synth
 
 
 def _prefill(B, H, T, D, fused=False):
@@ -122,6 +122,29 @@ def _embed(N, V, d, backward=False):
     return (lambda: _lib.host().embedding_fwd(ids, W, 1.0)), 2 * (N + min(N, V)) * d + 8 * N
 
 
+def _int4(M, K, N, dtype=torch.bfloat16, out=None, act=None):
+    dev = "cuda"
+    w = int4.quantize((torch.randn(N, K, device=dev) * K ** -0.5).to(dtype))
+    x, b = torch.randn(M, K, device=dev).to(dtype), torch.randn(N, device=dev).to(dtype)
+    e, o = x.element_size(), torch.empty((), dtype=out or dtype).element_size()
+    return (lambda: int4.linear(x, w, b, act=act, out_dtype=out)), N * K // 2 + N * w.scales.shape[1] * (e + 1) + M * K * e + M * N * o + N * e
+
+
+def _int4_quantize(N, K):
+    w = torch.randn(N, K, device="cuda").to(torch.bfloat16)
+    return (lambda: int4.quantize(w)), N * K * 5 // 2 + N * K // 64 * 3
+
+
+def _adjust(B, V, prompt=512, made=512):
+    dev = "cuda"
+    l = torch.randn(B, V, device=dev)
+    ids = [torch.randint(0, V, (B, n), device=dev) for n in (prompt, made)]
+    bias_ids, bias = torch.randint(0, V, (B, 16), device=dev), torch.randn(B, 16, device=dev)
+    mask = torch.randint(-(1 << 31), (1 << 31) - 1, (B, (V + 31) // 32), device=dev, dtype=torch.int32)
+    return (lambda: sampling.adjust_logits(l, prompt=ids[0], generated=ids[1], repetition=1.1, frequency=0.1, presence=0.2, bias_ids=bias_ids, bias=bias,
+                                           mask=mask)), 8 * B * V + 8 * B * (prompt + made) + mask.numel() * 4
+
+
 CASES = {
     # name: (builder, what it is)
     "prefill": (lambda: _prefill(64, 12, 1024, 64), "aspin chunked prefill, plain rule, tensor cores: B64 H12 T1024 D64 bf16"),
@@ -149,12 +172,18 @@ CASES = {
     "embed_bwd": (lambda: _embed(32768, 8192, 768, True), "its gradient by sorted tokens"),
     "skinny": (lambda: _skinny(1, 768, 3072), "decode-step linear (add + RMS norm + linear + GELU) at batch 1: K768 N3072 bf16"),
     "batch_linear": (lambda: _batch_linear(64, 768, 2328), "decode-step linear for 64 rows on the tensor cores (bias): K768 N2328 bf16"),
+    "int4_token": (lambda: _int4(1, 4096, 16384), "linear layer with four-bit weights, one row: K4096 N16384, groups of 64, bf16"),
+    "int4_batch": (lambda: _int4(64, 2048, 8192, act="gelu"), "the same for 64 rows: K2048 N8192, GELU"),
+    "int4_prompt": (lambda: _int4(4096, 2048, 8192, act="gelu"), "the same for 4096 rows"),
+    "int4_prompt_fp32": (lambda: _int4(1024, 2048, 2048, torch.float32), "the same in fp32, no weight rounded: M1024 K2048 N2048"),
+    "int4_quantize": (lambda: _int4_quantize(16384, 4096), "a weight into four bits: N16384 K4096 bf16"),
+    "adjust_logits": (lambda: _adjust(64, 50257), "penalties, biases and a mask on logits: B64 V50257 fp32, 512 + 512 ids a row"),
     "decode_token": (lambda: _decode_token(1), "the whole decode step of the configuration-2 model as one launch, batch 1 (12 layers, d768, vocabulary 8192)"),
     "decode_token_b4": (lambda: _decode_token(4), "the same at batch 4"),
 }
 
 # floating-point operations per launch of the cases that are bound by the tensor pipe rather than by HBM
-FLOPS = {"mlp_up": 2 * 8192 * 768 * 3072, "mlp_up_pair": 2 * 8192 * 768 * 3072}
+FLOPS = {"mlp_up": 2 * 8192 * 768 * 3072, "mlp_up_pair": 2 * 8192 * 768 * 3072, "int4_prompt": 2 * 4096 * 2048 * 8192, "int4_prompt_fp32": 2 * 1024 * 2048 * 2048}
 
 
 def _linear_act(M, K, N, variant=0):
@@ -226,11 +255,11 @@ def time_case(name: str, iters: int = 20, flush_mb: int = 256):
 
 def main(argv=None):
     ap = argparse.ArgumentParser()
-    ap.add_argument("name", choices=sorted(CASES) + ["all"])
+    ap.add_argument("name", nargs="+", choices=sorted(CASES) + ["all"])
     ap.add_argument("--launches", type=int, default=2)
     ap.add_argument("--time", action="store_true")
     a = ap.parse_args(argv)
-    names = sorted(CASES) if a.name == "all" else [a.name]
+    names = sorted(CASES) if "all" in a.name else a.name
     with torch.no_grad():
         for n in names:
             if a.time:
