@@ -58,11 +58,11 @@ __device__ __forceinline__ bool piece_at(const Pieces &p, int u, int N, int &n, 
 }
 
 // What bounds it: the arithmetic of a level, before the bytes. A level is the nearest whole number to the correctly rounded quotient w / s. The product with
-// an approximate 1 / s is within 3e-6 of the quotient (15 at most), so away from a tie both round alike: 1.5 2^23 added and taken off again rounds to even in two
-// additions. Where fp32 values come near a tie all eight of a thread are divided. Four levels are one fp32 number (16 bits) before they become integers.
-// N 16384, K 4096 bf16: 109 us with a division, a rounding and a conversion a value.
+// an approximate 1 / s is within 3e-6 of the quotient (15 at most), so away from a tie both round alike: 1.5 2^23 added rounds to even, one operation. Where fp32
+// values come near a tie all eight of a thread are divided. Three operations take a bf16 value to its clamped level; four levels are one fp32 number (16 bits)
+// before they become integers. N 16384, K 4096 bf16: 109 us with a division, a rounding and a conversion a value, 48 with the products, 36 so (a copy of as many bytes: 26).
 template <typename T_, int GROUP, bool SYM>
-__global__ void __launch_bounds__(256) int4_quantize_kernel(const T_ *__restrict__ w, unsigned char *__restrict__ q, T_ *__restrict__ scales,
+__global__ void __launch_bounds__(256, sizeof(T_) == 2 ? 5 : 4) int4_quantize_kernel(const T_ *__restrict__ w, unsigned char *__restrict__ q, T_ *__restrict__ scales,
                                                             unsigned char *__restrict__ zeros, int N, int K, int G, const Pieces pieces) {
     constexpr int PER = GROUP / 8;                                    // threads of a group
     constexpr float ROUND = 12582912.f, GRID = 768.f;                 // 1.5 2^23: to whole numbers; 1.5 2^9: to multiples of 2^-14 (for up to 256 of them)
@@ -88,6 +88,7 @@ __global__ void __launch_bounds__(256) int4_quantize_kernel(const T_ *__restrict
             }
         }
     }
+    float los[QU], his[QU];
 #pragma unroll
     for (int u = 0; u < QU; ++u) {
         float lo = 0.f, hi = 0.f;                                     // hi is NaN where a value is, and infinite where one is
@@ -122,45 +123,60 @@ __global__ void __launch_bounds__(256) int4_quantize_kernel(const T_ *__restrict
                 hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
             }
         }
-        T_ st;
+        los[u] = lo; his[u] = hi;
+    }
+    // The lanes of a group share out its scale's divisions: the first QU of them take a group each (the others repeat them), and hand on what they got.
+    static_assert(QU == 4 && PER >= QU, "a lane for each piece");
+    const int own = threadIdx.x & (QU - 1);
+    auto mine = [&](auto &t) { return own < 2 ? (own == 0 ? t[0] : t[1]) : (own == 2 ? t[2] : t[3]); };
+    T_ st;
+    {
+        const float lo = mine(los), hi = mine(his);
         from_f32(st, SYM ? __fdiv_rn(hi, 7.f) : __fdiv_rn(__fsub_rn(hi, lo), 15.f));
-        float s = to_f32(st);
-        if (!(s < INFINITY)) { s = nanf(""); from_f32(st, s); }
+        if (!(to_f32(st) < INFINITY)) from_f32(st, nanf(""));
+        los[0] = lo;
+    }
+    const float s_own = to_f32(st), z_own = SYM ? 8.f : s_own > 0.f ? fminf(rintf(__fdiv_rn(-los[0], s_own)), 15.f) : 0.f;
+    if ((threadIdx.x & (PER - 1)) < QU && mine(live)) {
+        const size_t grp = (size_t)mine(n) * G + mine(piece) / PER;
+        scales[grp] = st;
+        if constexpr (!SYM) zeros[grp] = (unsigned char)z_own;
+    }
+#pragma unroll
+    for (int u = 0; u < QU; ++u) {
+        const int from = (threadIdx.x & 31 & ~(PER - 1)) + u;
+        const float s = __shfl_sync(0xffffffffu, s_own, from), z = SYM ? 8.f : __shfl_sync(0xffffffffu, z_own, from);
         const bool flat = !(s > 0.f);                                 // no range, or NaN
-        const float z = SYM ? 8.f : flat ? 0.f : fminf(rintf(__fdiv_rn(-lo, s)), 15.f), inv = flat ? 0.f : __fdividef(1.f, s);
+        const float inv = flat ? 0.f : __fdividef(1.f, s);
         if (!live[u]) continue;
-        float r[8];                                                   // levels, as whole numbers of fp32
+        float r[8];                                                   // a level and one more, over 16: its clamp to 0 .. 15 is a saturating operation's
         bool divide = s < 1e-30f && !flat;                            // no 1 / s to speak of; and the scale's own rounding may put levels outside 0 .. 15
+        const float shift = (z + 1.f - ROUND) * 0.0625f;              // exact
         if constexpr (sizeof(T_) == 2) {
             // Quotients of two bf16 numbers that are no tie are 1/512 or more away from one: taken to a multiple of 2^-14 first, what the approximation missed is gone.
 #pragma unroll
-            for (int i = 0; i < 8; ++i) r[i] = __fadd_rn(__fadd_rn(__fadd_rn(value(u, i) * inv, GRID), -GRID), ROUND);
+            for (int i = 0; i < 8; ++i) r[i] = __saturatef(fmaf(__fadd_rn(fmaf(value(u, i), inv, GRID), ROUND - GRID), 0.0625f, shift));
         } else {
             float far = 0.f;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float t = value(u, i) * inv;
-                r[i] = __fadd_rn(t, ROUND);
-                far = fmaxf(far, fabsf(t - __fadd_rn(r[i], -ROUND)));
+                const float t = value(u, i) * inv, whole = __fadd_rn(t, ROUND);
+                far = fmaxf(far, fabsf(t - __fadd_rn(whole, -ROUND)));
+                r[i] = __saturatef(fmaf(whole, 0.0625f, shift));
             }
             divide |= far > 0.49998f;
         }
-        // otherwise levels below 0 cannot come up: the lowest value's quotient is the zero's with the sign changed
-        const float shift = z - ROUND;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) r[i] = SYM ? r[i] + shift : fminf(r[i] + shift, 15.f);
+        // levels below 0 cannot come up: the lowest value's quotient is the zero's with the sign changed
         if (divide) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) r[i] = fminf(fmaxf(rintf(__fdiv_rn(value(u, i), s)) + z, 0.f), 15.f);
+            for (int i = 0; i < 8; ++i) r[i] = (fminf(fmaxf(rintf(__fdiv_rn(value(u, i), s)) + z, 0.f), 15.f) + 1.f) * 0.0625f;
         }
-        const float half0 = fmaf(fmaf(fmaf(r[3], 16.f, r[2]), 16.f, r[1]), 16.f, r[0]), half1 = fmaf(fmaf(fmaf(r[7], 16.f, r[6]), 16.f, r[5]), 16.f, r[4]);
+        // four of them in a whole number of 16 bits, behind 2^23: the ones taken off again
+        constexpr float ONES = 8388608.f - 4369.f;
+        const float half0 = fmaf(fmaf(fmaf(fmaf(r[3], 16.f, r[2]), 16.f, r[1]), 16.f, r[0]), 16.f, ONES),
+                    half1 = fmaf(fmaf(fmaf(fmaf(r[7], 16.f, r[6]), 16.f, r[5]), 16.f, r[4]), 16.f, ONES);
         *reinterpret_cast<uint32_t *>(q + (size_t)n[u] * (K / 2) + piece[u] * 4) =
-            __byte_perm(__float_as_uint(half0 + 8388608.f), __float_as_uint(half1 + 8388608.f), 0x5410);
-        if (piece[u] % PER == 0) {
-            const size_t grp = (size_t)n[u] * G + piece[u] / PER;
-            scales[grp] = st;
-            if constexpr (!SYM) zeros[grp] = (unsigned char)z;
-        }
+            __byte_perm(__float_as_uint(half0), __float_as_uint(half1), 0x5410);
     }
 }
 
