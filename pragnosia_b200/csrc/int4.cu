@@ -524,8 +524,10 @@ static cudaError_t rows_go_group(RowsArgs a, cudaStream_t stream) {
     a.warps = (C + a.each - 1) / a.each;
     a.slot_bytes = R * 64 + rows * (X32 ? 512 : 256);
     // two stretches ahead: the levels come from the L2 as a rule, and more at once keep every warp's first one waiting (N 16384 K 4096, one row: 4 ahead 15.3 us, 2 14.6, 1 14.9).
-    // Either all of a warp's at once, or one slot more than are ahead.
-    a.ahead = a.each < 2 ? a.each : 2;
+    // Behind a kernel that constant weights need not wait for, they come from memory meanwhile: four (twelve layers of four such calls, d 2048, us a token, 4 / 2 ahead: 4 rows 537 / 575,
+    // 8 rows 595 / 632; one row 552 / 544). Either all of a warp's at once, or one slot more than are ahead.
+    const int most = a.constant && a.M > 1 ? 4 : 2;
+    a.ahead = a.each < most ? a.each : most;
     while (a.ahead > 1 && a.warps * (a.ahead + (a.ahead < a.each ? 1 : 0)) * a.slot_bytes > 100 * 1024) --a.ahead;
     a.slots = a.ahead + (a.ahead < a.each ? 1 : 0);
     int smem = a.warps * a.slots * a.slot_bytes + 32;

@@ -550,9 +550,10 @@ int int4_tile_launch(const Int4Linear &l, cudaStream_t stream) {
     a.wide = w.G % 4 == 0 && aligned(w.scales, 4 * es) && (w.zeros == nullptr || aligned(w.zeros, 4));
     // Rows of x a tile, with its shares of K below: 128 once those tiles are more than half the SMs; where even tiles of 64 in eight shares leave SMs idle, 32 (us, 32 / 64 / 128:
     // 128 rows, N 768 K 768 4.7 / 5.5 / 7.4; 452, N 1 K 15424 13 / 14 / 74; 64, N 2048 K 8192 12.0 / 13.6 / -; 256, N 2048 K 2048 11.2 / 9.1 / 13.7; 349, N 2785 K 14784 133 / 106 / 131;
-    // 128, N 8192 K 2048 16.6 / 12.9 / 14.0; 1000, N 2048 K 2048 31 / 17.4 / 14.2).
+    // 128, N 8192 K 2048 16.6 / 12.9 / 14.0; 1000, N 2048 K 2048 31 / 17.4 / 14.2). Not 32 for constant weights, whose CTAs start under the kernel ahead: twice as many are in its way
+    // (twelve layers of four such calls, d 2048, 64 rows: 837 us a token against 813).
     const long long sms = sm_count(), tiles_n = (w.N + 127) / 128, halves = (l.M + 127) / 128, by64 = tiles_n * ((l.M + 63) / 64);
-    const int NT = l.M <= 32 || 7 * by64 <= sms ? 32 : l.M <= 64 || 2 * tiles_n * halves <= sms ? 64 : 128, C = (w.K + 127) / 128;
+    const int NT = l.M <= 32 || (!l.constant && 7 * by64 <= sms) ? 32 : l.M <= 64 || 2 * tiles_n * halves <= sms ? 64 : 128, C = (w.K + 127) / 128;
     const long long tiles = tiles_n * ((l.M + NT - 1) / NT);
     // Shares of K while CTAs are no more than the SMs hold, and a share a stretch (us, 64 rows of x, 1 / 2 / 4 / 8: N 8192 K 2048 12.8 / 10.4 / 10.0 / 16.7, N 2048 K 8192 38 / 22 / 14 / 13.5,
     // N 2328 K 768 6.4 / 6.2 / 5.5 / 5.5, N 50257 K 768 16 / 27 / 37 / 69).

@@ -315,7 +315,7 @@ class Decoder:
     def _step_int4(self, advance: bool = True):
         """The separate kernels with the four linear layers of each block reading four-bit weights (int4.linear; behind the embedding's kernel everything ahead of the token
         is complete, so they are read early). It pays where a token's time is its weights' bytes: twelve layers with MLP 4 d, us a token, default / four bits with groups of 64:
-        d 2048 batch 1 460 / 554, 4 796 / 537, 8 844 / 596, 16 853 / 738, 64 945 / 867; d 768 batch 1 155 / 223, 64 319 / 553."""
+        d 2048 batch 1 456 / 544, 4 795 / 537, 8 860 / 595, 16 860 / 695, 64 955 / 813; d 768 batch 1 160 / 216, 64 320 / 420."""
         m = self.m
         per = self._int4_weights()
         if m.e.weight.dtype == torch.bfloat16 and m.d % 8 == 0:
