@@ -590,8 +590,8 @@ int pgb_embedding_bwd(const long long *ids, const void *grad, int dtype, float s
  *   Sums in fp32, one rounding at the end. The weight enters as scale times a whole number sum, unrounded -- but for bf16 x and y with more than
  *   PGB_INT4_ROWS rows, where scale (q - zero) is rounded to bf16 for the tensor cores. flags: PGB_INT4_CONSTANT = q, scales, zeros and bias were
  *   complete before the kernel ahead on the stream was launched, and may be read while it runs. Bounded waits as in the prefill
- *   kernels (pgb_tc_error_flag: 61-69). scratch, 16-byte aligned, of pgb_int4_linear_scratch_bytes (0: none, NULL) holds what fp32 rows of x become for the
- *   tensor cores; a call's own until the call is over. Sums of x (q - zero) over a group have to stay within fp32.
+ *   kernels (pgb_tc_error_flag: 61-69). scratch, 16-byte aligned, of pgb_int4_linear_scratch_bytes (0: none, NULL; never above 256 MiB, or 64 rows' share) holds what
+ *   fp32 rows of x become for the tensor cores; a call's own until the call is over. Sums of x (q - zero) over a group have to stay within fp32.
  * x, q, w, y 16-byte aligned, scales, zeros, bias to their element. N, K up to 2^24, M below 2^31. The same call gives the same bits.
  * ------------------------------------------------------------------------------------------------------- */
 enum { PGB_INT4_CONSTANT = 1, PGB_INT4_ROWS = 16 };

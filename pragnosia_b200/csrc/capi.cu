@@ -122,7 +122,7 @@ int decode_token_wait_selftest_launch(unsigned long long *, unsigned, cudaStream
 int int4_quantize_launch(const void *, int, unsigned char *, void *, unsigned char *, int, int, int, cudaStream_t);
 int int4_dequantize_launch(const Int4Weight &, void *, int, cudaStream_t);
 int int4_linear_launch(const Int4Linear &, cudaStream_t);
-bool int4_exact_tiles(const Int4Linear &);
+long long int4_exact_scratch(const Int4Linear &);
 int int4_tile_error_flag(int *);
 int int4_exact_error_flag(int *);
 int adjust_logits_launch(const AdjustLogits &, cudaStream_t);
@@ -958,7 +958,7 @@ long long pgb_int4_linear_scratch_bytes(int x_dtype, int out_dtype, long long M,
     if (M < 1 || M > 0x7fffffffLL || int4_sizes(N, K, 32) != PGB_OK || x_dtype != PGB_F32) return 0;
     Int4Linear a;
     a.x_dtype = x_dtype; a.out_dtype = out_dtype; a.M = M; a.w.N = N; a.w.K = K;
-    return int4_exact_tiles(a) ? 6 * M * K : 0;
+    return int4_exact_scratch(a);
 }
 
 int pgb_int4_linear(const void *x, int x_dtype, const unsigned char *q, const void *scales, int scale_dtype, const unsigned char *zeros, const void *bias,

@@ -355,11 +355,24 @@ bool int4_exact_tiles(const Int4Linear &l) {
     return l.M > 8 && (l.M + 7) / 8 * l.w.N * l.w.K >= 1LL << 24;
 }
 
-// l.scratch: room for x's terms where it is fp32. A grid's second axis ends at 65535, so very many rows go in several launches.
+// Rows of x a launch takes: those whose terms fit in 256 MiB (64 at least) where it is fp32; a grid's second axis ends at 65535.
+static long long exact_rows(const Int4Linear &l, int NT) {
+    if (l.x_dtype == PGB_BF16) return 65535LL * NT;
+    const long long fit = (1LL << 28) / (6LL * l.w.K) / 64 * 64;
+    return fit < 64 ? 64 : fit < 65535LL * NT ? fit : 65535LL * NT;
+}
+static int exact_tile(const Int4Linear &l) { return l.M <= 32 ? 32 : 64; }
+long long int4_exact_scratch(const Int4Linear &l) {
+    if (l.x_dtype != PGB_F32 || !int4_exact_tiles(l)) return 0;
+    const long long rows = exact_rows(l, exact_tile(l));
+    return 6 * (l.M < rows ? l.M : rows) * l.w.K;
+}
+
+// l.scratch: room for the terms of as many rows of x where it is fp32
 int int4_exact_launch(const Int4Linear &l, cudaStream_t stream) {
     const Int4Weight &w = l.w;
     const bool x32 = l.x_dtype == PGB_F32;
-    const int es = w.scale_dtype == PGB_F32 ? 4 : 2, NT = l.M <= 32 ? 32 : 64, C = (w.K + 127) / 128;
+    const int es = w.scale_dtype == PGB_F32 ? 4 : 2, NT = exact_tile(l), C = (w.K + 127) / 128;
     const long long tiles = (long long)((w.N + 127) / 128) * ((l.M + NT - 1) / NT);
     int splits = 1;
     while (splits < IE_SPLITS && tiles * splits <= sm_count() && C >= 2 * splits) splits *= 2;
@@ -367,8 +380,9 @@ int int4_exact_launch(const Int4Linear &l, cudaStream_t stream) {
     ExactArgs a{w.q, w.scales, w.zeros, l.bias, l.y, l.M, l.act, l.out_dtype == PGB_BF16, w.N, w.K, w.G, 0, each, (C + each - 1) / each, l.constant};
     a.wide = w.G % 4 == 0 && aligned(w.scales, 4 * es) && (w.zeros == nullptr || aligned(w.zeros, 4));
     cudaError_t e = cudaSuccess;
-    for (long long m = 0; m < l.M && e == cudaSuccess; m += 65535LL * NT) {
-        a.M = l.M - m < 65535LL * NT ? l.M - m : 65535LL * NT;
+    const long long rows = exact_rows(l, NT);
+    for (long long m = 0; m < l.M && e == cudaSuccess; m += rows) {
+        a.M = l.M - m < rows ? l.M - m : rows;
         a.y = (uint8_t *)l.y + (size_t)m * w.N * (a.out_bf16 ? 2 : 4);
         const void *x = (const uint8_t *)l.x + (size_t)m * w.K * (x32 ? 4 : 2);
         if (x32) {

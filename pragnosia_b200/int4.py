@@ -57,8 +57,9 @@ def linear(x, w: Int4Weight, bias=None, *, act: Optional[str] = None, out_dtype:
     """act(x W^T + bias) for x (..., K), bias (N,); act None or "gelu" (erf). Result (..., N) in out_dtype (default: x's).
 
     Sums in float32, one rounding at the end; a group's whole numbers meet x unrounded and are scaled behind their sum. For bfloat16 in and out from 17 rows up
-    the products run on the tensor cores with scale (q - zero) rounded to bfloat16, an error below that of the result's own rounding. The same
-    call gives the same bits; a row's may differ between calls of up to 16 rows and of more.
+    the products run on the tensor cores with scale (q - zero) rounded to bfloat16, an error below that of the result's own rounding; with
+    float32 in or out no weight is rounded however many rows there are (many of them want up to 256 MiB while the call runs). The same
+    call gives the same bits; a row's last ones may differ between calls of few rows and of many.
     constant: w and bias were complete before the kernel ahead on the stream was launched (weights of a model in a chain of launches): they are read while it runs."""
     if act not in (None, "gelu"):
         raise ValueError(f"act is None or 'gelu', got {act!r}")

@@ -177,7 +177,7 @@ def test_linear_of_many_tiles(M, K, N, scale_dtype):
     assert torch.equal(y, int4.linear(x, w, bias, act=act))
 
 
-EXACT = [(9, 2048, 4100), (17, 96, 60001), (20, 14048, 410), (33, 1024, 5000), (200, 416, 2003), (2000, 32, 4099), (129, 160, 8190), (64, 768, 50257), (1000, 4096, 130), (4100, 704, 704)]
+EXACT = [(9, 2048, 4100), (17, 96, 60001), (20, 14048, 410), (33, 1024, 5000), (200, 416, 2003), (2000, 32, 4099), (129, 160, 8190), (64, 768, 50257), (1000, 4096, 130), (4100, 704, 704), (11000, 4096, 40)]
 
 
 @pytest.mark.parametrize("M,K,N", EXACT)

@@ -59,7 +59,7 @@ def test_bad_calls(call, kw, code):
 
 def test_scratch_of_the_linear_layer():
     n = lib().pgb_int4_linear_scratch_bytes
-    assert n(0, 0, 64, 4096, 768) == n(0, 1, 64, 4096, 768) == 6 * 64 * 768 and n(0, 0, 1 << 20, 64, 4096) == 6 << 32
+    assert n(0, 0, 64, 4096, 768) == n(0, 1, 64, 4096, 768) == 6 * 64 * 768 and n(0, 0, 1 << 20, 64, 4096) == 6 * 4096 * 10880 and n(0, 0, 1 << 20, 64, 1 << 24) == 6 * 64 << 24
     assert n(0, 0, 64, 1024, 768) == n(0, 0, 8, 1 << 20, 768) == n(1, 0, 64, 4096, 768) == n(1, 1, 64, 4096, 768) == 0     # few, or bf16
     assert n(0, 0, 0, 4096, 768) == n(0, 0, 1 << 31, 4096, 768) == n(0, 0, 64, 0, 768) == n(0, 0, 64, 4096, 100) == 0
 
