@@ -238,7 +238,11 @@ __global__ void __launch_bounds__(IE_NT, 2) int4_exact_kernel(const __grid_const
     // A CTA finishes `share` rows of x: every one's sums of them are sent there, into the room of stages that nobody needs any more.
     const int share = (NT + a.splits - 1) / a.splits;
     const uint32_t rank = a.splits > 1 ? cluster_rank() : 0u;
-    if (a.splits > 1) cluster_sync_all(); else __syncthreads();
+    // Tensor memory goes back first: no CTA holds any while it waits for one of its cluster that may be kept from its own by another stream's kernel.
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 13) tmem_dealloc(tmem, 256);
+    if (a.splits > 1) cluster_sync_all();
     if (warp >= IE_DQ && warp < IE_DQ + IE_ACC && ok) {
         const int mh = ((warp - IE_DQ) >> 2) * COLS;
         int owner = mh / share, left = (owner + 1) * share - mh;      // of the next column, and how many more are its
@@ -295,9 +299,6 @@ __global__ void __launch_bounds__(IE_NT, 2) int4_exact_kernel(const __grid_const
             }
         }
     }
-    tc_fence_before();
-    __syncthreads();
-    if (warp == 13) tmem_dealloc(tmem, 256);
 }
 
 // x as three bf16 terms, [3][n]: eight bits each, cut off, so that they add up to x; an infinity or NaN is the first one's. Eight values a thread.

@@ -99,11 +99,13 @@ __global__ void __launch_bounds__(IT_NT, 2) int4_tile_kernel(const __grid_consta
         mbar_init(drained, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    // This CTA runs, and may be written to. Said before it asks for tensor memory, and tensor memory goes back before it waits for the others' sums: no CTA of a cluster
+    // holds any while it waits for one that may be kept from its own by another stream's kernel.
+    if (a.splits > 1) { __syncwarp(); asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
     if (warp == 9) tmem_alloc(smem_u32(tmem_slot), 256);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (a.splits > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");      // here: this CTA runs, and may be written to
     const uint32_t tmem = warp_uniform(*tmem_slot), tA = tmem + NT;    // D: NT columns; A: two stretches of 64
     if (!a.constant) {
         // few rows: the levels on their way to the L2 while the kernel ahead ends
@@ -251,6 +253,9 @@ __global__ void __launch_bounds__(IT_NT, 2) int4_tile_kernel(const __grid_consta
                 }
             }
         }
+        tc_fence_before();
+        __syncthreads();
+        if (warp == 9) tmem_dealloc(tmem, 256);
         cluster_sync_all();                                           // and nobody writes to anyone from here on
         const float4 *sums = reinterpret_cast<const float4 *>(sm + CF::MEET);
         const bool whole = a.N % 4 == 0;
@@ -291,9 +296,11 @@ __global__ void __launch_bounds__(IT_NT, 2) int4_tile_kernel(const __grid_consta
             it_store16(a, v, bias, m0 + mh + c, a.M - (m0 + mh + c), n);
         }
     }
-    tc_fence_before();
-    __syncthreads();
-    if (warp == 9) tmem_dealloc(tmem, 256);
+    if (a.splits == 1) {
+        tc_fence_before();
+        __syncthreads();
+        if (warp == 9) tmem_dealloc(tmem, 256);
+    }
 }
 
 // ------------------------------------------------------------------------------------------------ very many rows

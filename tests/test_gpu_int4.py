@@ -12,7 +12,7 @@ import math
 import pytest
 import torch
 
-from pragnosia_b200 import int4
+from pragnosia_b200 import int4, ops
 from pragnosia_b200._lib import graph_capture, warm_up
 
 pytestmark = pytest.mark.gpu
@@ -338,6 +338,27 @@ def test_linear_in_a_graph_and_on_another_stream(M, dtype):
         other = int4.linear(x, w)
     torch.cuda.current_stream().wait_stream(side)
     assert torch.equal(other, want)
+
+
+def test_streams_side_by_side():
+    """Clusters that exchange sums, on two streams at once and beside another kernel's with tensor memory of their own."""
+    K, N = 2048, 1000
+    w = random_weight(N, K, 64, True, BF, 12)
+    g = torch.Generator(device="cuda").manual_seed(5)
+    a, b = torch.randn(64, K, device="cuda", generator=g).to(BF), torch.randn(120, K, device="cuda", generator=g)
+    W = (torch.randn(N, K, device="cuda", generator=g) * 0.02).to(BF)
+    calls = (lambda: int4.linear(a, w, act="gelu"), lambda: int4.linear(b, w), lambda: ops.batch_linear(a[:16], W), lambda: int4.linear(a, w, out_dtype=F32))
+    want = [f() for f in calls]
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    out = [[] for _ in streams]
+    for i in range(20):
+        for j, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                k = (i + j) % len(calls)
+                out[j].append((k, calls[k]()))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want[k]) for o in out for k, y in o)
 
 
 @pytest.mark.parametrize("M", [1, 40, 2000])
