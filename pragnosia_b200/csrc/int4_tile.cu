@@ -8,7 +8,7 @@
 // result's own; kept exact, each group's products would have to be read back from tensor memory and scaled, as long as the products themselves take.
 //   Few rows: the columns of W are shared out over a cluster of CTAs, which send one another their sums; those are added in the order of their ranks.
 //   What bounds it, 64 rows, N 8192 K 2048: a chain of latencies, 10.0 us -- the launch 2, two stretches' levels made operands 2.5, the products' tail 1.2, sums exchanged and stored 2;
-// the tensor pipe is active a tenth of the time. 1000 rows, N 2048 K 2048: 14.2 us, 590 TFLOP/s.
+// the tensor pipe is active a tenth of the time. 1000 rows, N 2048 K 2048: 13.2 us, 640 TFLOP/s.
 // Every wait is bounded; one that runs out sets the error flag and the CTA winds down.
 #include "gelu.cuh"
 #include "int4_linear.cuh"
@@ -60,8 +60,26 @@ __device__ __forceinline__ void it_values(const uint4 &levels, const uint32_t (&
         out[4 * v + 2] = __byte_perm(p[0], p[1], 0x7632); out[4 * v + 3] = __byte_perm(p[2], p[3], 0x7632);
     }
 }
-// 16 columns of D (rows m, m + 1, .. of x, `left` of them there) of this lane's row n of W: + bias, the activation, rounded and stored; a row's 32 lanes are 64 bytes
+// 16 columns of D (rows m, m + 1, .. of x, `left` of them there) of this lane's row n of W: + bias, the activation, rounded and stored; a row's 32 lanes are 64 bytes. Where a row
+// has an even number, two lanes exchange halves, and each stores both their values of every other row
+// (4096 rows, N 8192 K 128: 35.6 us with two bytes a lane, 21.9 so).
 __device__ __forceinline__ void it_store16(const TileArgs &a, const float (&v)[16], float bias, long long m, long long left, int n) {
+    if (a.N % 2 == 0) {
+        const int odd = n & 1;
+        const uint32_t halves = odd ? 0x3276u : 0x5410u;
+        __nv_bfloat16 *row = a.y + (size_t)(m + odd) * a.N + (n - odd);
+        const long long mine = n < a.N ? left - odd : 0;
+#pragma unroll
+        for (int e = 0; e < 16; e += 2) {
+            float s0 = v[e] + bias, s1 = v[e + 1] + bias;
+            if (a.act == 1) { s0 = lg_gelu(s0); s1 = lg_gelu(s1); }
+            const __nv_bfloat162 own = __floats2bfloat162_rn(s0, s1);
+            const uint32_t p = *reinterpret_cast<const uint32_t *>(&own), q = __shfl_xor_sync(0xffffffffu, p, 1);
+            if (e < mine) *reinterpret_cast<uint32_t *>(row) = __byte_perm(p, q, halves);
+            row += 2 * (size_t)a.N;
+        }
+        return;
+    }
     __nv_bfloat16 *row = a.y + (size_t)m * a.N;                       // uniform
     const bool there = n < a.N;
 #pragma unroll
@@ -307,7 +325,7 @@ __global__ void __launch_bounds__(IT_NT, 2) int4_tile_kernel(const __grid_consta
 // The same for tiles of 256 rows of x: twice the products for a tile's dequantisation, which is what the smaller tiles are bound by (issue slots: 128 rows of W and 128 of x
 // take 630 instructions and an epilogue as long for 256 cycles of the tensor pipe). One CTA an SM walks tiles: eight warps dequantise into four stages of shared memory
 // (A, 64 columns, 128-byte swizzle: D, twice 256 columns, takes all of tensor memory), eight store the tile before, 128 columns of D each.
-//   What bounds it: issue slots (62 % busy) of warps that feed the tensor pipe (65 % active). 4096 rows, N 8192 K 2048 with GELU: 112-116 us, 1.19-1.23 PFLOP/s, 105 without the GELU (the
+//   What bounds it: issue slots (62 % busy) of warps that feed the tensor pipe (65 % active). 4096 rows, N 8192 K 2048 with GELU: 109 us, 1.25 PFLOP/s, 104 without the GELU (the
 // library's bf16 product of that size at its sustained rate: 98); the smaller tiles 135.
 constexpr int IW_NT = 18 * 32, IW_XS = 4, IW_AS = 4, IW_AHEAD = 1;
 constexpr int IW_XSTAGE = 256 * 128, IW_ASTAGE = 128 * 128, IW_SLOT = 32 * 64;
@@ -571,7 +589,7 @@ int int4_tile_launch(const Int4Linear &l, cudaStream_t stream) {
     int splits = 1;
     while (NT < 128 && splits < IT_SPLITS && tiles * splits <= sms && C >= 2 * splits) splits *= 2;
     // The larger tiles from one and a half rounds over the chip on, where x fills them well: one of 256 rows takes 1.6 times as long as one of 128 (us, theirs / the smaller ones':
-    // 4096 rows, N 2048 K 8192 113 / 136, N 2328 K 768 24 / 27, N 50257 K 768 323 / 431; 256 rows, N 32768 K 4096 64 / 72, 384 115 / 107, 128 59 / 39;
+    // two-byte stores, 4096 rows: N 2048 K 8192 113 / 136, N 2328 K 768 24 / 27, N 50257 K 768 323 / 431; 256 rows, N 32768 K 4096 64 / 72, 384 115 / 107, 128 59 / 39;
     // a round: 2048 rows, N 2048 K 2048 19.4 / 19.2, N 2328 K 768 23.8 / 20.5; half a one: 512 rows, N 4096 K 4096 31 / 23).
     const long long wide_rows = (l.M + 255) / 256;
     if (8 * wide_rows < 5 * halves && tiles_n * wide_rows * 2 >= 3 * sms) {
